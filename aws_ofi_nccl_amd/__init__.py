@@ -561,6 +561,18 @@ PROTOTYPES = {
     "ofi_amd_tuner_query": (ctypes.c_int, [c_vp, c_u32, c_vp]),
     "ofi_amd_tuner_query_prepare": (ctypes.c_int, [c_u32]),
     "ofi_amd_tuner_ctx_stats": (ctypes.c_int, [c_vp, ctypes.POINTER(TunerCtxStats)]),
+    "ofi_amd_rms_norm": (ctypes.c_int, [c_vp, c_u64, c_vp, c_u64, c_vp, c_i32, c_u32, c_u32, c_i32, ctypes.c_float,
+                                        c_vp, c_u64, c_vp, c_u64, c_vp, c_u64, c_vp, c_u64, c_u32, c_vp, c_vp]),
+    "ofi_amd_rms_norm_grad_work_bytes": (c_u64, [c_u32, c_u32]),
+    "ofi_amd_rms_norm_grad": (ctypes.c_int, [c_vp, c_u64, c_vp, c_u64, c_vp, c_vp, c_i32, c_u32, c_u32, c_i32, c_vp,
+                                             c_u64, c_vp, c_u64, c_vp, c_vp, c_u64, c_vp]),
+    "ofi_amd_token_dispatch_work_bytes": (c_u64, [c_u32, c_u32, c_u32]),
+    "ofi_amd_token_dispatch": (ctypes.c_int, [c_vp, c_i32, c_u32, c_u32, c_u32, c_u32, c_vp, c_vp, c_vp, c_vp, c_u64,
+                                              c_vp, c_u64, c_u32, c_vp, c_u64, c_vp, c_u64, c_u32, c_vp, c_u64, c_vp]),
+    "ofi_amd_token_combine": (ctypes.c_int, [c_vp, c_u64, c_u32, c_vp, c_vp, c_u32, c_u32, c_u32, c_i32, c_vp, c_u64,
+                                             c_vp, c_u64, c_vp]),
+    "ofi_amd_token_combine_grad": (ctypes.c_int, [c_vp, c_u64, c_vp, c_u64, c_u32, c_vp, c_vp, c_u32, c_u32, c_u32,
+                                                  c_i32, c_vp, c_u64, c_vp, c_vp]),
 }
 
 
@@ -581,6 +593,10 @@ def load(path=None):
     if path is None:
         _lib = lib
     return lib
+
+
+# ncclDataType_t numbers of the types that ofi_amd_rms_norm and ofi_amd_token_* take
+INT32, INT64, FLOAT16, FLOAT32, BFLOAT16 = 2, 4, 6, 7, 9
 
 
 def check(rc, what="call"):

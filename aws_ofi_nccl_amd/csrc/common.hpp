@@ -97,6 +97,7 @@ enum : uint32_t {
 	ASYNC_ERR_GIN_TIMEOUT = 1u << 1,  /* producer gave up on a full ring */
 	ASYNC_ERR_SCHED_STATE = 1u << 2,  /* scheduler state unusable (rails, stripe size) */
 	ASYNC_ERR_COPY_LENGTH = 1u << 3,  /* a copy-table entry longer than the stated maximum */
+	ASYNC_ERR_TOKEN_ROWS = 1u << 4,   /* more sorted tokens than rows for them */
 };
 
 /* The device side of a flush read for the first 64 lanes of a workgroup: one lane per 8-byte

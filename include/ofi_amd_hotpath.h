@@ -81,7 +81,8 @@ int ofi_amd_gpu_stream_synchronize(void *stream);
  * bit 0 = bounce destination out of range / misaligned, bit 1 = GIN producer
  * timed out, bit 2 = scheduler state unusable (num_rails outside 1..4 or a zero
  * min_stripe_size; the batch is then left unwritten), bit 3 = an entry of
- * ofi_amd_copy_table_pieces longer than max_len (its bytes beyond are not copied). */
+ * ofi_amd_copy_table_pieces longer than max_len (its bytes beyond are not copied), bit 4 = more
+ * pairs in ofi_amd_token_dispatch than max_rows (those beyond have no row). */
 int ofi_amd_async_error_fetch(uint32_t *bits);
 
 /* ======================================================================
@@ -938,6 +939,107 @@ int ofi_amd_tuner_ctx_stats(const void *context, ofi_amd_tuner_ctx_stats_t *out)
  * They are data symbols of this library; their types are declared in
  * aws_ofi_nccl_amd/csrc/nccl_tuner_abi.h.
  */
+
+/* ======================================================================
+ * 6. Tokens between experts: what an expert-parallel layer computes around its puts.
+ *    A layer's rows are normalised into 8-bit rows with scales (rms_norm), sorted by expert, so
+ *    that what goes to a peer is one piece of memory and one put (token_dispatch), and what comes
+ *    back is weighted and summed per token (token_combine).  The gradients go the same way back.
+ *    The reference has none of these; its users do (the GIN interface of section 4 is what their
+ *    exchange runs over).
+ *
+ *    Rows are `pitch` bytes apart (any multiple of the element's size that is not less than a row;
+ *    less than 2^40), and need no alignment beyond their element's.  Rows, pitches and tables that
+ *    lie on 16 bytes are faster.  Sums, statistics and products are held in 32 bits; each output is
+ *    rounded once, to nearest even.  Results do not depend on the order in which the GPU runs things:
+ *    the same call gives the same bits.  Nothing is allocated; calls may be captured into a graph
+ *    (after ofi_amd_gpu_init()).  -EINVAL: a missing or misaligned argument, a type or group not
+ *    named here, a pitch below a row; -E2BIG: beyond the stated limits.
+ * ====================================================================== */
+
+/* Types, by their numbers in ncclDataType_t */
+#define OFI_AMD_INT32 2
+#define OFI_AMD_INT64 4
+#define OFI_AMD_FLOAT16 6
+#define OFI_AMD_FLOAT32 7
+#define OFI_AMD_BFLOAT16 9
+
+/*
+ * For each of n_rows rows of `width` values (1..32768) of `type` (float16, bfloat16, float32):
+ *   s = x + residual          (d_residual NULL: s = x)
+ *   rstd = 1 / sqrt(mean(s^2) + eps)
+ *   n = s * rstd * gain       (gain: `width` values of `type` or of float32)
+ * and writes what is asked for (at least one, the others NULL): s to d_sum, n to d_out, both in
+ * `type`; rstd to d_rstd[row]; and to d_q the values n / scale as OCP e4m3, one byte each, with
+ * d_scale[row][j] = max(largest |n| of columns [j*group, (j+1)*group) / 448, 2^-126).  group is 32,
+ * 64, 128 or 256, or 0 for one scale per row; d_scale rows are scale_pitch bytes apart.  n is made
+ * from the unrounded s.  A row that holds a NaN or an infinity has NaN where the formulas have, and
+ * the scale of a group with a NaN in it is NaN.  d_sum may be d_x or d_residual, with the same pitch.
+ */
+int ofi_amd_rms_norm(const void *d_x, uint64_t x_pitch, const void *d_residual, uint64_t residual_pitch, const void *d_gain,
+		     int gain_type, uint32_t n_rows, uint32_t width, int type, float eps, void *d_sum, uint64_t sum_pitch,
+		     void *d_out, uint64_t out_pitch, void *d_q, uint64_t q_pitch, float *d_scale, uint64_t scale_pitch,
+		     uint32_t group, float *d_rstd, void *stream);
+
+/*
+ * The gradient.  d_s and d_rstd are the forward call's, d_dout the gradient of n, d_dsum (or NULL)
+ * what reaches s past the norm.  With h = s * rstd:
+ *   dx = dsum + rstd * (gain * dout - h * mean(gain * dout * h))   in `type`: of x and of residual
+ *   dgain[i] = sum over rows of dout * h                           in float32
+ * d_dgain may be NULL; otherwise d_work holds ofi_amd_rms_norm_grad_work_bytes bytes on a 16-byte
+ * boundary, free again when the call's work has ended.  No rows: dgain is zeros.  d_dx may be d_dout
+ * or d_dsum, with the same pitch.  The 8-bit rounding is passed through as if it were not there.
+ */
+uint64_t ofi_amd_rms_norm_grad_work_bytes(uint32_t n_rows, uint32_t width);
+int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d_s, uint64_t s_pitch, const float *d_rstd,
+			  const void *d_gain, int gain_type, uint32_t n_rows, uint32_t width, int type, const void *d_dsum,
+			  uint64_t dsum_pitch, void *d_dx, uint64_t dx_pitch, float *d_dgain, void *d_work, uint64_t work_bytes,
+			  void *stream);
+
+/*
+ * Sorts n_tokens * top_k pairs (a token and one of its choices; pair = token * top_k + choice) by
+ * d_expert[pair] (int32 or int64), pairs of one expert in their own order.  A value outside
+ * [0, n_experts) is a pair without a row: a choice that is not taken, or an expert that is elsewhere.
+ *   d_offset[0..n_experts]   the first row of each expert and the rows in all
+ *   d_row_of[pair]           the pair's row or -1
+ *   d_pair_of[0..max_rows)   (optional) the row's pair, or -1 behind the last
+ * and copies row_bytes of token t's row of d_x to the row of each of its pairs in d_rows, and
+ * scale_bytes of its row of d_scale to d_scale_rows; either copy may be left out (NULL; no scales
+ * without rows).  Rows behind the last pair's are not written.  Pairs whose row would be max_rows or
+ * more have none: d_row_of is -1, d_offset ends at max_rows, and bit 4 of ofi_amd_async_error_fetch is set.
+ * Rows of e4m3 with scales go as they are: the copy is of bytes, at any alignment.
+ * n_experts <= 1024, top_k <= 64, row_bytes and scale_bytes <= 2^24, pairs and max_rows < 2^31.
+ * d_work: ofi_amd_token_dispatch_work_bytes bytes on a 16-byte boundary (NULL where that is 0), free
+ * again when the call's work has ended.
+ * The gradient of d_x is ofi_amd_token_combine of the gradient of d_rows without weights.
+ */
+uint64_t ofi_amd_token_dispatch_work_bytes(uint32_t n_tokens, uint32_t top_k, uint32_t n_experts);
+int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tokens, uint32_t top_k, uint32_t n_experts,
+			   uint32_t max_rows, int32_t *d_offset, int32_t *d_row_of, int32_t *d_pair_of, const void *d_x,
+			   uint64_t x_pitch, void *d_rows, uint64_t rows_pitch, uint32_t row_bytes, const void *d_scale,
+			   uint64_t scale_pitch, void *d_scale_rows, uint64_t scale_rows_pitch, uint32_t scale_bytes, void *d_work,
+			   uint64_t work_bytes, void *stream);
+
+/*
+ * out[t] = add[t] + sum over k of weight[t][k] * rows[row_of[t][k]], in the order of k, `width` values
+ * (1..2^20) of `type`.  d_add NULL: 0; d_weight (float32) NULL: 1.  A pair whose d_row_of is outside
+ * [0, max_rows) is passed over, whatever its weight.  d_out may be d_add, with the same pitch.
+ */
+int ofi_amd_token_combine(const void *d_rows, uint64_t rows_pitch, uint32_t max_rows, const int32_t *d_row_of,
+			  const float *d_weight, uint32_t n_tokens, uint32_t top_k, uint32_t width, int type, const void *d_add,
+			  uint64_t add_pitch, void *d_out, uint64_t out_pitch, void *stream);
+
+/*
+ * The gradient of the sum above with respect to rows and weights:
+ *   drows[row_of[t][k]] = weight[t][k] * dout[t]      (the gradient of add is dout itself)
+ *   dweight[t][k] = <dout[t], rows[row_of[t][k]]>     float32; 0 for a pair without a row
+ * Either may be NULL (d_rows is then not looked at for d_dweight NULL).  Rows that no pair names are not
+ * written; d_row_of names a row once, as ofi_amd_token_dispatch leaves it.  d_drows may be d_rows, with
+ * the same pitch.
+ */
+int ofi_amd_token_combine_grad(const void *d_dout, uint64_t dout_pitch, const void *d_rows, uint64_t rows_pitch,
+			       uint32_t max_rows, const int32_t *d_row_of, const float *d_weight, uint32_t n_tokens, uint32_t top_k,
+			       uint32_t width, int type, void *d_drows, uint64_t drows_pitch, float *d_dweight, void *stream);
 
 #ifdef __cplusplus
 }
