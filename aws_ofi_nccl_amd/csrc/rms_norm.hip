@@ -30,30 +30,29 @@ struct norm_out_t {
 	float *rstd;
 };
 
-/* f * inverse as e4m3 */
-template <uint32_t V>
-__device__ __forceinline__ void store_q(uint8_t *__restrict__ p, uint32_t left, const float (&f)[V], float inverse)
+/* A chunk's own elements times `inverse` as e4m3 */
+template <uint32_t V> __device__ __forceinline__ void store_q(uint8_t *p, uint32_t skip, const float (&f)[V], float inverse)
 {
-	uint32_t w[V / 4];
-#pragma unroll
-	for (uint32_t i = 0; i < V / 4; i++) {
-		w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * inverse, f[4 * i + 1] * inverse, 0, false);
-		w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inverse, f[4 * i + 3] * inverse, (int)w[i], true);
-	}
-	if (left >= V) {
-		struct __attribute__((packed, aligned(1))) words_t {
-			uint32_t w[V / 4];
-		} all;
+	if constexpr (V == 1) {
+		if (skip == 0) {
+			p[0] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inverse, 0.0f, 0, false);
+		}
+	} else {
+		typedef uint32_t words_t __attribute__((ext_vector_type(V / 4), aligned(1)));
+		words_t w;
 #pragma unroll
 		for (uint32_t i = 0; i < V / 4; i++) {
-			all.w[i] = w[i];
+			const int low = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * inverse, f[4 * i + 1] * inverse, 0, false);
+			w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inverse, f[4 * i + 3] * inverse, low, true);
 		}
-		*reinterpret_cast<words_t *>(p) = all;
-	} else {
+		if (skip == 0) {
+			*reinterpret_cast<words_t *>(p) = w;
+		} else {
 #pragma unroll
-		for (uint32_t i = 0; i < V; i++) {
-			if (i < left) {
-				p[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+			for (uint32_t i = 0; i < V; i++) {
+				if (i >= skip) {
+					p[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+				}
 			}
 		}
 	}
@@ -78,16 +77,36 @@ __device__ __forceinline__ uint32_t max_bits_of_group(uint32_t m, uint32_t lanes
 	return m;
 }
 
-template <typename T>
-__device__ __forceinline__ void load_gain(const void *__restrict__ gain, bool gain_f32, uint32_t at, uint32_t left, float (&g)[kChunk<T>])
+template <typename T, uint32_t V>
+__device__ __forceinline__ void load_gain(const void *__restrict__ gain, bool gain_f32, uint32_t from, float (&g)[V])
 {
 	if (!gain_f32) {
-		load_chunk(static_cast<const T *>(gain) + at, left, g);
+		to_floats<T, V>(load_raw<false, T, V>(static_cast<const T *>(gain) + from), 0, g);
 		return;
 	}
 #pragma unroll
-	for (uint32_t i = 0; i < kChunk<T>; i++) {
-		g[i] = i < left ? static_cast<const float *>(gain)[at + i] : 0.0f;
+	for (uint32_t i = 0; i < V; i++) {
+		g[i] = static_cast<const float *>(gain)[from + i];
+	}
+}
+
+/* A chunk's own elements of a row of floats */
+template <uint32_t V> __device__ __forceinline__ void store_floats(float *p, uint32_t skip, const float (&f)[V])
+{
+	if constexpr (V == 8) {
+		if (skip == 0) {
+			store_piece<false, float, 4>(p, 0, reinterpret_cast<const float(&)[4]>(f[0]));
+			store_piece<false, float, 4>(p + 4, 0, reinterpret_cast<const float(&)[4]>(f[4]));
+		} else {
+#pragma unroll
+			for (uint32_t i = 0; i < V; i++) {
+				if (i >= skip) {
+					p[i] = f[i];
+				}
+			}
+		}
+	} else {
+		store_piece<false, float, V>(p, skip, f);
 	}
 }
 
@@ -98,35 +117,40 @@ __device__ __forceinline__ float scale_of(uint32_t amax_bits)
 	return s < 0x1p-126f ? 0x1p-126f : s;
 }
 
-/* sum may be x or residual: a lane reads what it writes, and first.  group_lanes: lanes that share a scale, 0: the whole row does */
-template <typename T, int WAVES, int R>
+/* sum may be x or residual: a lane has read what it writes before any lane of its row writes.  group_lanes: lanes that share a
+ * scale, 0: the whole row does */
+template <typename T, uint32_t V, int WAVES, int R, bool STREAM>
 __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const T *residual, const void *__restrict__ gain,
 							      uint64_t x_pitch, uint64_t residual_pitch, uint32_t first, uint32_t width,
 							      float eps, uint32_t group_lanes, bool gain_f32, norm_out_t o)
 {
-	constexpr uint32_t V = kChunk<T>, B = 64 * WAVES;
+	constexpr uint32_t B = 64 * WAVES;
 	__shared__ float part[2 * WAVES];
 	const uint64_t row = first + blockIdx.x;
-	const T *xr = row_at(x, x_pitch, row);
-	const T *rr = residual ? row_at(residual, residual_pitch, row) : nullptr;
+	raw_t<T, V> c[R], d[R];
+#pragma unroll
+	for (int k = 0; k < R; k++) {
+		c[k] = load_raw<STREAM, T, V>(row_at(x, x_pitch, row) + place_of<V>((k * B + threadIdx.x) * V, width).from);
+	}
+	if (residual) {
+#pragma unroll
+		for (int k = 0; k < R; k++) {
+			d[k] = load_raw<STREAM, T, V>(row_at(residual, residual_pitch, row) +
+						      place_of<V>((k * B + threadIdx.x) * V, width).from);
+		}
+	}
 	float v[R][V];
 	float squares = 0.0f;
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		const uint32_t at = (k * B + threadIdx.x) * V;
+		const uint32_t skip = place_of<V>((k * B + threadIdx.x) * V, width).skip;
+		to_floats<T, V>(c[k], skip, v[k]);
+		if (residual) {
+			float f[V];
+			to_floats<T, V>(d[k], skip, f);
 #pragma unroll
-		for (uint32_t i = 0; i < V; i++) {
-			v[k][i] = 0.0f;
-		}
-		if (at < width) {
-			load_chunk(xr + at, width - at, v[k]);
-			if (rr) {
-				float f[V];
-				load_chunk(rr + at, width - at, f);
-#pragma unroll
-				for (uint32_t i = 0; i < V; i++) {
-					v[k][i] += f[i];
-				}
+			for (uint32_t i = 0; i < V; i++) {
+				v[k][i] += f[i];
 			}
 		}
 #pragma unroll
@@ -142,24 +166,26 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 #pragma unroll
 	for (int k = 0; k < R; k++) {
 		const uint32_t at = (k * B + threadIdx.x) * V;
-		uint32_t m = 0;
-		if (at < width) {
-			if (o.sum) {
-				store_chunk(row_at(static_cast<T *>(o.sum), o.sum_pitch, row) + at, width - at, v[k]);
-			}
-			float g[V];
-			load_gain<T>(gain, gain_f32, at, width - at, g);
+		const place_t here = place_of<V>(at, width);
+		if (o.sum && at < width) {
+			store_piece<false, T, V>(row_at(static_cast<T *>(o.sum), o.sum_pitch, row) + here.from, here.skip, v[k]);
+		}
+		float g[V];
+		load_gain<T, V>(gain, gain_f32, here.from, g);
 #pragma unroll
-			for (uint32_t i = 0; i < V; i++) {
-				v[k][i] = v[k][i] * rstd * g[i];
-				m = max(m, i < width - at ? abs_bits(v[k][i]) : 0u); /* beyond: 0 rstd, a NaN where the row has none left */
-			}
-			if (o.out) {
-				store_chunk(row_at(static_cast<T *>(o.out), o.out_pitch, row) + at, width - at, v[k]);
-			}
+		for (uint32_t i = 0; i < V; i++) {
+			v[k][i] = v[k][i] * rstd * g[i];
+		}
+		if (o.out && at < width) {
+			store_piece<false, T, V>(row_at(static_cast<T *>(o.out), o.out_pitch, row) + here.from, here.skip, v[k]);
 		}
 		if (!o.q) {
 			continue;
+		}
+		uint32_t m = 0;
+#pragma unroll
+		for (uint32_t i = 0; i < V; i++) {
+			m = max(m, i < here.skip ? 0u : abs_bits(v[k][i])); /* a skipped 0 times a rstd or a gain that is no number is none */
 		}
 		if (group_lanes == 0) {
 			most = max(most, m);
@@ -167,8 +193,8 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 		}
 		const float scale = scale_of(max_bits_of_group(m, group_lanes));
 		if (at < width) {
+			store_q<V>(o.q + row * o.q_pitch + here.from, here.skip, v[k], 1.0f / scale);
 			const uint32_t chunk = k * B + threadIdx.x;
-			store_q(o.q + row * o.q_pitch + at, width - at, v[k], 1.0f / scale);
 			if ((chunk & (group_lanes - 1u)) == 0) {
 				row_at(o.scale, o.scale_pitch, row)[chunk / group_lanes] = scale;
 			}
@@ -179,8 +205,9 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 #pragma unroll
 		for (int k = 0; k < R; k++) {
 			const uint32_t at = (k * B + threadIdx.x) * V;
+			const place_t here = place_of<V>(at, width);
 			if (at < width) {
-				store_q(o.q + row * o.q_pitch + at, width - at, v[k], 1.0f / scale);
+				store_q<V>(o.q + row * o.q_pitch + here.from, here.skip, v[k], 1.0f / scale);
 			}
 		}
 		if (threadIdx.x == 0) {
@@ -190,56 +217,62 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 }
 
 /* dx = ds + rstd (g dn - h mean(g dn h)), h = s rstd; dg = sum over rows of dn h: each workgroup sums its own rows and the
- * partial sums are added up in the order of the workgroups, so that the result is the same every time */
-template <typename T, int WAVES, int R>
+ * partial sums are added up in the order of the workgroups, so that the result is the same every time.  dx may be dout or dsum:
+ * a lane has read what it writes. */
+template <typename T, uint32_t V, int WAVES, int R, bool STREAM>
 __global__ __launch_bounds__(64 * WAVES) void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s,
 								   const float *__restrict__ rstds, const void *__restrict__ gain,
-								   const T *dsum, uint64_t dout_pitch, uint64_t s_pitch,
-								   uint64_t dsum_pitch, uint32_t n_rows, uint32_t width, bool gain_f32,
-								   T *dx, uint64_t dx_pitch, float *__restrict__ partial)
+								   const T *dsum, uint64_t dout_pitch, uint64_t s_pitch, uint64_t dsum_pitch,
+								   uint32_t n_rows, uint32_t width, bool gain_f32, T *dx, uint64_t dx_pitch,
+								   float *__restrict__ partial)
 {
-	constexpr uint32_t V = kChunk<T>, B = 64 * WAVES;
+	constexpr uint32_t B = 64 * WAVES;
 	__shared__ float part[2][WAVES];
 	float g[R][V], dg[R][V];
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		const uint32_t at = (k * B + threadIdx.x) * V;
+		load_gain<T, V>(gain, gain_f32, place_of<V>((k * B + threadIdx.x) * V, width).from, g[k]);
 #pragma unroll
 		for (uint32_t i = 0; i < V; i++) {
-			dg[k][i] = g[k][i] = 0.0f;
-		}
-		if (at < width) {
-			load_gain<T>(gain, gain_f32, at, width - at, g[k]);
+			dg[k][i] = 0.0f;
 		}
 	}
 	uint32_t turn = 0;
 	for (uint64_t row = blockIdx.x; row < n_rows; row += gridDim.x, turn ^= 1u) {
-		const T *dr = row_at(dout, dout_pitch, row), *sr = row_at(s, s_pitch, row);
+		raw_t<T, V> dc[R], sc[R], pc[R];
+#pragma unroll
+		for (int k = 0; k < R; k++) {
+			const uint32_t from = place_of<V>((k * B + threadIdx.x) * V, width).from;
+			dc[k] = load_raw<STREAM, T, V>(row_at(dout, dout_pitch, row) + from);
+			sc[k] = load_raw<STREAM, T, V>(row_at(s, s_pitch, row) + from);
+		}
+		if (dsum) {
+#pragma unroll
+			for (int k = 0; k < R; k++) {
+				pc[k] = load_raw<STREAM, T, V>(row_at(dsum, dsum_pitch, row) +
+							       place_of<V>((k * B + threadIdx.x) * V, width).from);
+			}
+		}
 		const float rstd = rstds[row];
 		float d[R][V], h[R][V], along = 0.0f;
 #pragma unroll
 		for (int k = 0; k < R; k++) {
-			const uint32_t at = (k * B + threadIdx.x) * V;
-#pragma unroll
-			for (uint32_t i = 0; i < V; i++) {
-				d[k][i] = h[k][i] = 0.0f;
-			}
-			if (at < width) {
-				load_chunk(dr + at, width - at, d[k]);
-				load_chunk(sr + at, width - at, h[k]);
-			}
+			const uint32_t skip = place_of<V>((k * B + threadIdx.x) * V, width).skip;
+			to_floats<T, V>(dc[k], skip, d[k]);
+			to_floats<T, V>(sc[k], skip, h[k]);
 #pragma unroll
 			for (uint32_t i = 0; i < V; i++) {
 				h[k][i] *= rstd;
 				dg[k][i] = __builtin_fmaf(d[k][i], h[k][i], dg[k][i]);
 				d[k][i] *= g[k][i];
-				along = __builtin_fmaf(d[k][i], h[k][i], along);
+				along = i < skip ? along : __builtin_fmaf(d[k][i], h[k][i], along);
 			}
 		}
 		const float mean = block_sum<WAVES>(along, part[turn]) / (float)width;
 #pragma unroll
 		for (int k = 0; k < R; k++) {
 			const uint32_t at = (k * B + threadIdx.x) * V;
+			const place_t here = place_of<V>(at, width);
 			if (at < width) {
 				float r[V];
 #pragma unroll
@@ -247,13 +280,13 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_grad_kernel(const T *dout
 					r[i] = 0.0f;
 				}
 				if (dsum) {
-					load_chunk(row_at(dsum, dsum_pitch, row) + at, width - at, r);
+					to_floats<T, V>(pc[k], 0, r);
 				}
 #pragma unroll
 				for (uint32_t i = 0; i < V; i++) {
 					r[i] = __builtin_fmaf(rstd, __builtin_fmaf(-h[k][i], mean, d[k][i]), r[i]);
 				}
-				store_chunk(row_at(dx, dx_pitch, row) + at, width - at, r);
+				store_piece<false, T, V>(row_at(dx, dx_pitch, row) + here.from, here.skip, r);
 			}
 		}
 	}
@@ -263,13 +296,9 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_grad_kernel(const T *dout
 #pragma unroll
 	for (int k = 0; k < R; k++) {
 		const uint32_t at = (k * B + threadIdx.x) * V;
+		const place_t here = place_of<V>(at, width);
 		if (at < width) {
-			store_chunk(partial + (uint64_t)blockIdx.x * width + at, width - at >= 4 ? 4 : width - at,
-				    reinterpret_cast<float(&)[4]>(dg[k][0]));
-			if (V == 8 && at + 4 < width) {
-				store_chunk(partial + (uint64_t)blockIdx.x * width + at + 4, width - at - 4,
-					    reinterpret_cast<float(&)[4]>(dg[k][V - 4]));
-			}
+			store_floats<V>(partial + (uint64_t)blockIdx.x * width + here.from, here.skip, dg[k]);
 		}
 	}
 }
@@ -283,6 +312,7 @@ __global__ __launch_bounds__(64 * kGainWaves) void rms_norm_gain_kernel(const fl
 	const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, column = blockIdx.x * 64u + lane;
 	float total = 0.0f;
 	if (column < width) {
+#pragma unroll 8
 		for (uint32_t p = wave; p < parts; p += kGainWaves) {
 			total += partial[(uint64_t)p * width + column];
 		}
@@ -298,29 +328,37 @@ __global__ __launch_bounds__(64 * kGainWaves) void rms_norm_gain_kernel(const fl
 	}
 }
 
+constexpr uint32_t kGradBlocks = 512;
 /* Workgroups of the gradient: each reads and writes a row at a time */
 inline uint32_t grad_blocks(uint32_t n_rows)
 {
-	return n_rows < 1024u ? n_rows : 1024u;
+	return n_rows < kGradBlocks ? n_rows : kGradBlocks;
 }
 
 /* Calls f with the wavefronts of a workgroup and the chunks of a lane that hold a row of `chunks` */
-template <typename T, typename F> void with_row_shape(uint32_t chunks, F f)
+template <uint32_t V, typename F> void with_row_shape(uint32_t chunks, F f)
 {
-	if (chunks <= 64) {
-		f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-	} else if (chunks <= 256) {
-		f(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
-	} else if (chunks <= 512) {
-		f(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
-	} else if (chunks <= 1024) {
-		f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-	} else if (chunks <= 2048) {
-		f(std::integral_constant<int, 16>{}, std::integral_constant<int, 2>{});
-	} else if (kChunk<T> == 8 || chunks <= 4096) {
-		f(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+	auto with = [&](auto waves, auto r) { f(waves, r); };
+	if constexpr (V == 1) { /* narrower than a chunk */
+		with(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
 	} else {
-		f(std::integral_constant<int, 16>{}, std::integral_constant<int, 32 / (int)kChunk<T>>{});
+		if (chunks <= 64) {
+			with(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+		} else if (chunks <= 128) {
+			with(std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{});
+		} else if (chunks <= 256) {
+			with(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+		} else if (chunks <= 512) {
+			with(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+		} else if (chunks <= 1024) {
+			with(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+		} else if (chunks <= 2048) {
+			with(std::integral_constant<int, 16>{}, std::integral_constant<int, 2>{});
+		} else if (V == 8 || chunks <= 4096) {
+			with(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+		} else {
+			with(std::integral_constant<int, 16>{}, std::integral_constant<int, V == 4 ? 8 : 4>{});
+		}
 	}
 }
 
@@ -360,14 +398,18 @@ int ofi_amd_rms_norm(const void *d_x, uint64_t x_pitch, const void *d_residual, 
 		return -EINVAL;
 	}
 	const norm_out_t o = { d_sum, sum_pitch, d_out, out_pitch, static_cast<uint8_t *>(d_q), q_pitch, d_scale, scale_pitch, d_rstd };
-	with_row_type(type, [&](auto element) {
+	const bool stream_rows = on_chunks(d_x, x_pitch) && on_chunks(d_residual, residual_pitch);
+	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
-		with_row_shape<T>((width + kChunk<T> - 1) / kChunk<T>, [&](auto waves, auto r) {
+		constexpr uint32_t V = decltype(v)::value;
+		const uint32_t group_lanes = V == 1 ? 0 : group / V; /* narrower rows are one group, however long it is */
+		with_row_shape<V>((width + V - 1) / V, [&](auto waves, auto r) {
+			constexpr int W = decltype(waves)::value, R = decltype(r)::value;
 			for (uint32_t first = 0; first < n_rows; first += kRowsOfLaunch) {
-				launch_kernel(rms_norm_kernel<T, decltype(waves)::value, decltype(r)::value>,
-					      dim3(n_rows - first < kRowsOfLaunch ? n_rows - first : kRowsOfLaunch), dim3(64 * waves), 0,
+				launch_kernel(stream_rows ? rms_norm_kernel<T, V, W, R, true> : rms_norm_kernel<T, V, W, R, false>,
+					      dim3(n_rows - first < kRowsOfLaunch ? n_rows - first : kRowsOfLaunch), dim3(64 * W), 0,
 					      as_stream(stream), static_cast<const T *>(d_x), static_cast<const T *>(d_residual), d_gain, x_pitch,
-					      residual_pitch, first, width, eps, group / kChunk<T>, gain_type == OFI_AMD_FLOAT32, o);
+					      residual_pitch, first, width, eps, group_lanes, gain_type == OFI_AMD_FLOAT32, o);
 			}
 		});
 	});
@@ -408,11 +450,14 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
 	const uint32_t blocks = grad_blocks(n_rows);
 	float *partial = d_dgain ? static_cast<float *>(d_work) : nullptr;
 	if (n_rows != 0) {
-		with_row_type(type, [&](auto element) {
+		const bool stream_rows = on_chunks(d_dout, dout_pitch) && on_chunks(d_s, s_pitch) && on_chunks(d_dsum, dsum_pitch);
+		with_row_type(type, width, [&](auto element, auto v) {
 			using T = decltype(element);
-			with_row_shape<T>((width + kChunk<T> - 1) / kChunk<T>, [&](auto waves, auto r) {
-				launch_kernel(rms_norm_grad_kernel<T, decltype(waves)::value, decltype(r)::value>, dim3(blocks),
-					      dim3(64 * waves), 0, as_stream(stream), static_cast<const T *>(d_dout),
+			constexpr uint32_t V = decltype(v)::value;
+			with_row_shape<V>((width + V - 1) / V, [&](auto waves, auto r) {
+				constexpr int W = decltype(waves)::value, R = decltype(r)::value;
+				launch_kernel(stream_rows ? rms_norm_grad_kernel<T, V, W, R, true> : rms_norm_grad_kernel<T, V, W, R, false>,
+					      dim3(blocks), dim3(64 * W), 0, as_stream(stream), static_cast<const T *>(d_dout),
 					      static_cast<const T *>(d_s), d_rstd, d_gain, static_cast<const T *>(d_dsum), dout_pitch, s_pitch,
 					      dsum_pitch, n_rows, width, gain_type == OFI_AMD_FLOAT32, static_cast<T *>(d_dx), dx_pitch, partial);
 			});

@@ -1,9 +1,11 @@
 /*
- * What the kernels on rows of numbers share: 16-byte pieces of a row as floats, and sums and maxima over lanes.
+ * What the kernels on rows of numbers share: pieces of a row as floats, and sums and maxima over lanes.
  *
- * A row is cut into chunks of 16 bytes, one per lane.  Chunks are accessed as 16-byte words at whatever address the
- * row starts (the global memory path takes any alignment); only the last chunk of a row whose width is no whole number of
- * chunks goes element by element.
+ * A row is cut into chunks of V elements, one per lane: 16 bytes, at whatever address the row starts (the global memory path
+ * takes any alignment).  The last chunk of a row whose width is no whole number of chunks is read and computed as the 16 bytes
+ * that end with the row, so that no load is conditional: its first `skip` elements are its neighbour's, which stores them.
+ * Lanes beyond the row read those last 16 bytes too and skip all of them.  Rows narrower than a chunk are cut into single
+ * elements (V = 1).
  */
 #ifndef OFI_AMD_ROW_TYPES_HPP_
 #define OFI_AMD_ROW_TYPES_HPP_
@@ -24,48 +26,65 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 template <typename T> constexpr uint32_t kChunk = 16 / sizeof(T); /* elements of a chunk */
 
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) chunk_t {
-	T v __attribute__((ext_vector_type(16 / sizeof(T))));
+template <typename T, uint32_t V> struct piece_t {
+	typedef T raw __attribute__((ext_vector_type(V)));
+	typedef T anywhere __attribute__((ext_vector_type(V), aligned(sizeof(T)))); /* at an address of the element's alignment */
 };
-/* 16 bytes of anything at any address */
-struct __attribute__((packed, aligned(1))) any16_t {
-	u32x4_t v;
-};
+template <typename T, uint32_t V> using raw_t = typename piece_t<T, V>::raw;
+typedef uint32_t any16_t __attribute__((ext_vector_type(4), aligned(1))); /* 16 bytes of anything at any address */
 
-/* `left` elements of the row remain at p, at least one; those beyond read as 0 */
-template <typename T> __device__ __forceinline__ void load_chunk(const T *__restrict__ p, uint32_t left, float (&f)[kChunk<T>])
+/* Where the chunk at column `at` is read, and how many of its elements are not its own */
+struct place_t {
+	uint32_t from, skip;
+};
+template <uint32_t V> __device__ __forceinline__ place_t place_of(uint32_t at, uint32_t width)
 {
-	constexpr uint32_t V = kChunk<T>;
-	if (left >= V) {
-		const auto c = reinterpret_cast<const chunk_t<T> *>(p)->v;
+	const uint32_t from = min(at, width - V);
+	return { from, at - from };
+}
+
+/* STREAM: read once, not to be kept in the caches */
+template <bool STREAM, typename T, uint32_t V> __device__ __forceinline__ raw_t<T, V> load_raw(const T *p)
+{
+	const auto *q = reinterpret_cast<const typename piece_t<T, V>::anywhere *>(p);
+	return STREAM ? __builtin_nontemporal_load(q) : *q;
+}
+
+/* The chunk's own elements, 0 in place of the skipped ones */
+template <typename T, uint32_t V> __device__ __forceinline__ void to_floats(raw_t<T, V> c, uint32_t skip, float (&f)[V])
+{
+#pragma unroll
+	for (uint32_t i = 0; i < V; i++) {
+		f[i] = (float)c[i];
+	}
+	if (skip) {
 #pragma unroll
 		for (uint32_t i = 0; i < V; i++) {
-			f[i] = (float)c[i];
-		}
-	} else {
-#pragma unroll
-		for (uint32_t i = 0; i < V; i++) {
-			f[i] = i < left ? (float)p[i] : 0.0f;
+			f[i] = i < skip ? 0.0f : f[i];
 		}
 	}
 }
 
-/* Each element is rounded to the row's type once, to nearest even */
-template <typename T> __device__ __forceinline__ void store_chunk(T *__restrict__ p, uint32_t left, const float (&f)[kChunk<T>])
+/* The chunk's own elements go to the row's place `from`, each rounded to the row's type once, to nearest even */
+template <bool STREAM, typename T, uint32_t V> __device__ __forceinline__ void store_piece(T *p, uint32_t skip, const float (&f)[V])
 {
-	constexpr uint32_t V = kChunk<T>;
-	if (left >= V) {
-		chunk_t<T> c;
+	raw_t<T, V> c;
 #pragma unroll
-		for (uint32_t i = 0; i < V; i++) {
-			c.v[i] = (T)f[i];
+	for (uint32_t i = 0; i < V; i++) {
+		c[i] = (T)f[i];
+	}
+	if (skip == 0) {
+		auto *q = reinterpret_cast<typename piece_t<T, V>::anywhere *>(p);
+		if (STREAM) {
+			__builtin_nontemporal_store(c, q);
+		} else {
+			*q = c;
 		}
-		*reinterpret_cast<chunk_t<T> *>(p) = c;
 	} else {
 #pragma unroll
 		for (uint32_t i = 0; i < V; i++) {
-			if (i < left) {
-				p[i] = (T)f[i];
+			if (i >= skip) {
+				p[i] = c[i];
 			}
 		}
 	}
@@ -166,16 +185,31 @@ inline uint32_t row_type_size(int type)
 	return type == OFI_AMD_FLOAT32 ? 4u : type == OFI_AMD_BFLOAT16 || type == OFI_AMD_FLOAT16 ? 2u : 0u;
 }
 
-/* Calls f with a value of the row's type (checked before) */
-template <typename F> inline void with_row_type(int type, F f)
+/* Calls f with a value of the row's type (checked before) and the elements of its chunks */
+template <typename F> inline void with_row_type(int type, uint32_t width, F f)
 {
+	auto with = [&](auto element) {
+		constexpr uint32_t V = kChunk<decltype(element)>;
+		if (width >= V) {
+			f(element, std::integral_constant<uint32_t, V>{});
+		} else {
+			f(element, std::integral_constant<uint32_t, 1>{});
+		}
+	};
 	if (type == OFI_AMD_BFLOAT16) {
-		f(bf16_t{});
+		with(bf16_t{});
 	} else if (type == OFI_AMD_FLOAT16) {
-		f(f16_t{});
+		with(f16_t{});
 	} else {
-		f(float{});
+		with(float{});
 	}
+}
+
+/* Whether every chunk of the rows lies within a line: rows that are read past the caches (STREAM) have to.  A chunk across two
+ * lines would fetch both again for its neighbour. */
+inline bool on_chunks(const void *p, uint64_t pitch)
+{
+	return ((reinterpret_cast<uintptr_t>(p) | pitch) & 15u) == 0;
 }
 
 /* n rows of `bytes` at p, a pitch apart, each element on its own boundary */

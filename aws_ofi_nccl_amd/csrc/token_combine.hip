@@ -15,93 +15,138 @@ using namespace ofi_amd;
 
 constexpr uint32_t kMaxTopK = 64;
 constexpr uint32_t kMaxWidth = 1u << 20;
-constexpr int kWaves = 4;
+constexpr int kMostWaves = 8;
 constexpr uint32_t kAtOnce = 8; /* rows of a token that are read together */
 
-/* One chunk of the output per lane */
-template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void token_combine_kernel(const int32_t *__restrict__ row_of, const float *__restrict__ weight,
-								    const T *__restrict__ rows, const T *add, T *out, uint64_t rows_pitch,
-								    uint64_t add_pitch, uint64_t out_pitch, uint32_t max_rows, uint32_t top_k,
-								    uint32_t width)
+/* A workgroup of threadIdx.x lanes along a row and threadIdx.y tokens; each lane one chunk of the output at a time.  Up to kAtOnce
+ * rows are asked for before the first is used. */
+template <typename T, uint32_t V, bool STREAM>
+__global__ __launch_bounds__(64 * kMostWaves) void token_combine_kernel(const int32_t *__restrict__ row_of,
+									const float *__restrict__ weight, const T *__restrict__ rows,
+									const T *add, T *out, uint64_t rows_pitch, uint64_t add_pitch,
+									uint64_t out_pitch, uint32_t n_tokens, uint32_t max_rows,
+									uint32_t top_k, uint32_t width)
 {
-	constexpr uint32_t V = kChunk<T>;
-	const uint32_t token = blockIdx.x;
-	const uint32_t at = (blockIdx.y * 64u * kWaves + threadIdx.x) * V;
-	if (at >= width) {
+	const uint32_t token = blockIdx.x * blockDim.y + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.y);
+	if (token >= n_tokens) {
 		return;
 	}
-	float sum[V];
-#pragma unroll
-	for (uint32_t i = 0; i < V; i++) {
-		sum[i] = 0.0f;
-	}
-	if (add) {
-		load_chunk(row_at(add, add_pitch, token) + at, width - at, sum);
-	}
-	for (uint32_t k = 0; k < top_k; k++) {
-		const uint64_t p = (uint64_t)token * top_k + k;
-		const uint32_t row = (uint32_t)row_of[p];
-		if (row < max_rows) {
-			const float w = weight ? weight[p] : 1.0f;
-			float f[V];
-			load_chunk(row_at(rows, rows_pitch, row) + at, width - at, f);
-#pragma unroll
-			for (uint32_t i = 0; i < V; i++) {
-				sum[i] = __builtin_fmaf(w, f[i], sum[i]);
-			}
+	row_of += (uint64_t)token * top_k;
+	weight += weight ? (uint64_t)token * top_k : 0;
+	for (uint32_t at = threadIdx.x * V; at < width; at += blockDim.x * V) {
+		const place_t here = place_of<V>(at, width);
+		raw_t<T, V> first;
+		if (add) {
+			first = load_raw<STREAM, T, V>(row_at(add, add_pitch, token) + here.from);
 		}
-	}
-	store_chunk(row_at(out, out_pitch, token) + at, width - at, sum);
-}
-
-/* One workgroup per token, up to kAtOnce of its rows at a time */
-template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void token_combine_grad_kernel(const int32_t *__restrict__ row_of,
-									 const float *__restrict__ weight, const T *__restrict__ dout,
-									 const T *rows, T *drows, float *__restrict__ dweight,
-									 uint64_t dout_pitch, uint64_t rows_pitch, uint64_t drows_pitch,
-									 uint32_t max_rows, uint32_t top_k, uint32_t width)
-{
-	constexpr uint32_t V = kChunk<T>;
-	__shared__ float part[kWaves][kAtOnce];
-	const uint64_t token = blockIdx.x;
-	const T *dr = row_at(dout, dout_pitch, token);
-	for (uint32_t k0 = 0; k0 < top_k; k0 += kAtOnce) {
-		float dot[kAtOnce];
+		float sum[V];
 #pragma unroll
-		for (uint32_t k = 0; k < kAtOnce; k++) {
-			dot[k] = 0.0f;
+		for (uint32_t i = 0; i < V; i++) {
+			sum[i] = 0.0f;
 		}
-		for (uint32_t at = threadIdx.x * V; at < width; at += 64u * kWaves * V) {
-			float d[V];
-			load_chunk(dr + at, width - at, d);
+		for (uint32_t k0 = 0; k0 < top_k; k0 += kAtOnce) {
+			raw_t<T, V> c[kAtOnce];
+			uint32_t row[kAtOnce];
+			float w[kAtOnce];
 #pragma unroll
 			for (uint32_t k = 0; k < kAtOnce; k++) {
-				if (k0 + k >= top_k) {
-					break;
+				const uint32_t at_k = min(k0 + k, top_k - 1u);
+				row[k] = k0 + k < top_k ? (uint32_t)row_of[at_k] : ~0u;
+				w[k] = weight ? weight[at_k] : 1.0f;
+			}
+#pragma unroll
+			for (uint32_t k = 0; k < kAtOnce; k++) {
+				if (row[k] < max_rows) {
+					c[k] = load_raw<STREAM, T, V>(row_at(rows, rows_pitch, row[k]) + here.from);
 				}
-				const uint64_t p = token * top_k + k0 + k;
-				const uint32_t row = (uint32_t)row_of[p];
-				if (row >= max_rows) {
-					continue;
-				}
-				if (dweight) {
-					float f[V];
-					load_chunk(row_at(rows, rows_pitch, row) + at, width - at, f);
+			}
+			if (k0 == 0 && add) {
+				to_floats<T, V>(first, 0, sum);
+			}
+#pragma unroll
+			for (uint32_t k = 0; k < kAtOnce; k++) {
+				if (row[k] < max_rows) {
 #pragma unroll
 					for (uint32_t i = 0; i < V; i++) {
-						dot[k] = __builtin_fmaf(d[i], f[i], dot[k]);
+						sum[i] = __builtin_fmaf(w[k], (float)c[k][i], sum[i]);
 					}
 				}
-				if (drows) {
-					const float w = weight ? weight[p] : 1.0f;
-					float f[V];
+			}
+		}
+		store_piece<false, T, V>(row_at(out, out_pitch, token) + here.from, here.skip, sum);
+	}
+}
+
+/* One workgroup of `waves` wavefronts per token.  All rows that are read together are asked for before the first is written, so
+ * that drows may be rows. */
+template <typename T, uint32_t V, bool STREAM>
+__global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(const int32_t *__restrict__ row_of,
+									     const float *__restrict__ weight,
+									     const T *__restrict__ dout, const T *rows, T *drows,
+									     float *__restrict__ dweight, uint64_t dout_pitch,
+									     uint64_t rows_pitch, uint64_t drows_pitch, uint32_t max_rows,
+									     uint32_t top_k, uint32_t width)
+{
+	__shared__ float part[kMostWaves][kAtOnce];
+	const uint64_t token = blockIdx.x;
+	const uint32_t waves = blockDim.x >> 6;
+	const T *dr = row_at(dout, dout_pitch, token);
+	row_of += token * top_k;
+	weight += weight ? token * top_k : 0;
+	for (uint32_t k0 = 0; k0 < top_k; k0 += kAtOnce) {
+		float dot[kAtOnce], w[kAtOnce];
+		uint32_t row[kAtOnce];
+#pragma unroll
+		for (uint32_t k = 0; k < kAtOnce; k++) {
+			const uint32_t at_k = min(k0 + k, top_k - 1u);
+			row[k] = k0 + k < top_k ? (uint32_t)row_of[at_k] : ~0u;
+			w[k] = weight ? weight[at_k] : 1.0f;
+			dot[k] = 0.0f;
+		}
+		for (uint32_t at = threadIdx.x * V; at < width; at += blockDim.x * V) {
+			const place_t here = place_of<V>(at, width);
+			const raw_t<T, V> dc = load_raw<STREAM, T, V>(dr + here.from);
+			raw_t<T, V> c[kAtOnce];
+			if (dweight) {
+#pragma unroll
+				for (uint32_t k = 0; k < kAtOnce; k++) {
+					if (row[k] < max_rows) {
+						c[k] = load_raw<STREAM, T, V>(row_at(rows, rows_pitch, row[k]) + here.from);
+					}
+				}
+			}
+			float d[V];
+			to_floats<T, V>(dc, 0, d);
+			if (drows) {
+#pragma unroll
+				for (uint32_t k = 0; k < kAtOnce; k++) {
+					if (row[k] < max_rows) {
+						float f[V];
+#pragma unroll
+						for (uint32_t i = 0; i < V; i++) {
+							f[i] = w[k] * d[i];
+						}
+						store_piece<STREAM, T, V>(row_at(drows, drows_pitch, row[k]) + here.from, here.skip, f);
+					}
+				}
+			}
+			if (dweight) {
+				if (here.skip) {
 #pragma unroll
 					for (uint32_t i = 0; i < V; i++) {
-						f[i] = w * d[i];
+						d[i] = i < here.skip ? 0.0f : d[i];
 					}
-					store_chunk(row_at(drows, drows_pitch, row) + at, width - at, f);
+				}
+#pragma unroll
+				for (uint32_t k = 0; k < kAtOnce; k++) {
+					if (row[k] < max_rows) {
+						float f[V];
+						to_floats<T, V>(c[k], here.skip, f);
+#pragma unroll
+						for (uint32_t i = 0; i < V; i++) {
+							dot[k] = __builtin_fmaf(d[i], f[i], dot[k]);
+						}
+					}
 				}
 			}
 		}
@@ -118,9 +163,8 @@ __global__ __launch_bounds__(64 * kWaves) void token_combine_grad_kernel(const i
 		__syncthreads();
 		if (threadIdx.x < kAtOnce && k0 + threadIdx.x < top_k) {
 			float d = part[0][threadIdx.x];
-#pragma unroll
-			for (int w = 1; w < kWaves; w++) {
-				d += part[w][threadIdx.x];
+			for (uint32_t v = 1; v < waves; v++) {
+				d += part[v][threadIdx.x];
 			}
 			dweight[token * top_k + k0 + threadIdx.x] = d;
 		}
@@ -128,7 +172,13 @@ __global__ __launch_bounds__(64 * kWaves) void token_combine_grad_kernel(const i
 	}
 }
 
-constexpr uint32_t kTokensOfLaunch = 1u << 22; /* with 256 lanes each within the 32 bits of a launch's size */
+/* Wavefronts along a row of `chunks`: one workgroup has all of a row of up to 8 KiB in flight at once */
+inline uint32_t row_waves(uint32_t chunks)
+{
+	return chunks <= 64 ? 1 : chunks <= 128 ? 2 : chunks <= 256 ? 4 : kMostWaves;
+}
+
+constexpr uint32_t kTokensOfLaunch = 1u << 22; /* with 512 lanes each within the 32 bits of a launch's size */
 
 int check_call(uint32_t max_rows, const int32_t *d_row_of, const float *d_weight, uint32_t top_k, uint32_t width, uint32_t size,
 	       uint32_t n_tokens)
@@ -167,16 +217,18 @@ int ofi_amd_token_combine(const void *d_rows, uint64_t rows_pitch, uint32_t max_
 	    (d_add && !rows_ok(d_add, add_pitch, n_tokens, bytes, size)) || !rows_ok(d_out, out_pitch, n_tokens, bytes, size)) {
 		return -EINVAL;
 	}
-	with_row_type(type, [&](auto element) {
+	const bool stream_rows = on_chunks(d_rows, rows_pitch) && on_chunks(d_add, add_pitch);
+	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
-		constexpr uint32_t span = 64 * kWaves * kChunk<T>;
+		constexpr uint32_t V = decltype(v)::value;
+		const uint32_t waves = row_waves((width + V - 1) / V), tokens = waves < 4 ? 4 / waves : 1;
 		for (uint32_t at = 0; at < n_tokens; at += kTokensOfLaunch) {
-			launch_kernel(token_combine_kernel<T>,
-				      dim3(n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch, (width + span - 1) / span),
-				      dim3(64 * kWaves), 0, as_stream(stream), d_row_of + (uint64_t)at * top_k,
-				      d_weight ? d_weight + (uint64_t)at * top_k : nullptr, static_cast<const T *>(d_rows),
-				      d_add ? row_at(static_cast<const T *>(d_add), add_pitch, at) : nullptr,
-				      row_at(static_cast<T *>(d_out), out_pitch, at), rows_pitch, add_pitch, out_pitch, max_rows, top_k, width);
+			const uint32_t n = n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch;
+			launch_kernel(stream_rows ? token_combine_kernel<T, V, true> : token_combine_kernel<T, V, false>,
+				      dim3((n + tokens - 1) / tokens), dim3(64 * waves, tokens), 0, as_stream(stream),
+				      d_row_of + (uint64_t)at * top_k, d_weight ? d_weight + (uint64_t)at * top_k : nullptr,
+				      static_cast<const T *>(d_rows), d_add ? row_at(static_cast<const T *>(d_add), add_pitch, at) : nullptr,
+				      row_at(static_cast<T *>(d_out), out_pitch, at), rows_pitch, add_pitch, out_pitch, n, max_rows, top_k, width);
 		}
 	});
 	OFI_AMD_HIP_TRY(hipGetLastError());
@@ -203,11 +255,15 @@ int ofi_amd_token_combine_grad(const void *d_dout, uint64_t dout_pitch, const vo
 			       (d_drows && !rows_ok(d_drows, drows_pitch, max_rows, bytes, size))))) {
 		return -EINVAL;
 	}
-	with_row_type(type, [&](auto element) {
+	const bool stream_rows = on_chunks(d_rows, rows_pitch) && on_chunks(d_drows, drows_pitch) && on_chunks(d_dout, dout_pitch);
+	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
+		constexpr uint32_t V = decltype(v)::value;
+		const uint32_t waves = row_waves((width + V - 1) / V);
 		for (uint32_t at = 0; at < n_tokens; at += kTokensOfLaunch) {
-			launch_kernel(token_combine_grad_kernel<T>, dim3(n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch),
-				      dim3(64 * kWaves), 0, as_stream(stream), d_row_of + (uint64_t)at * top_k,
+			launch_kernel(stream_rows ? token_combine_grad_kernel<T, V, true> : token_combine_grad_kernel<T, V, false>,
+				      dim3(n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch), dim3(64 * waves), 0,
+				      as_stream(stream), d_row_of + (uint64_t)at * top_k,
 				      d_weight ? d_weight + (uint64_t)at * top_k : nullptr,
 				      row_at(static_cast<const T *>(d_dout), dout_pitch, at), static_cast<const T *>(d_rows),
 				      static_cast<T *>(d_drows), d_dweight ? d_dweight + (uint64_t)at * top_k : nullptr, dout_pitch, rows_pitch,

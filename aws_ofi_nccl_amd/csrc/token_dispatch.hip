@@ -18,9 +18,10 @@ constexpr uint32_t kMaxExperts = 1024;
 constexpr uint32_t kMaxTopK = 64;
 constexpr uint32_t kMaxRowBytes = 1u << 24;
 constexpr uint32_t kTokensOfLaunch = 1u << 22;
-constexpr int kSortWaves = 4;
-constexpr uint32_t kTile = 2048; /* pairs of a workgroup of the sort */
-constexpr uint32_t kTileOfWave = kTile / kSortWaves;
+constexpr int kSortWaves = 16;
+constexpr uint32_t kRounds = 8;                                  /* pairs of a lane */
+constexpr uint32_t kTileOfWave = 64 * kRounds;                   /* pairs of a wavefront, in order: lanes first, then rounds */
+constexpr uint32_t kTile = (uint32_t)kSortWaves * kTileOfWave;   /* of a workgroup of the sort */
 
 __device__ __forceinline__ uint32_t lanes_below(uint64_t mask)
 {
@@ -28,9 +29,8 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t mask)
 }
 
 /* The expert of pair p, or n_experts where it has none */
-template <typename I> __device__ __forceinline__ uint32_t expert_at(const I *__restrict__ expert, uint32_t p, uint32_t n_experts)
+template <typename I> __device__ __forceinline__ uint32_t known_expert(I e, uint32_t n_experts)
 {
-	const I e = expert[p];
 	return e >= 0 && e < (I)n_experts ? (uint32_t)e : n_experts;
 }
 
@@ -40,14 +40,23 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(const I *_
 								      uint32_t n_experts, uint32_t *__restrict__ counts)
 {
 	__shared__ uint32_t count[kMaxExperts + 1];
+	const uint64_t lo = (uint64_t)blockIdx.x * kTile;
+	I ids[kRounds];
+#pragma unroll
+	for (uint32_t i = 0; i < kRounds; i++) {
+		const uint64_t p = lo + i * 64 * kSortWaves + threadIdx.x;
+		ids[i] = p < n_pairs ? expert[p] : (I)-1;
+	}
 	for (uint32_t e = threadIdx.x; e <= n_experts; e += 64 * kSortWaves) {
 		count[e] = 0;
 	}
 	__syncthreads();
-	const uint32_t lo = blockIdx.x * kTile;
-	const uint32_t hi = min(n_pairs - lo, kTile);
-	for (uint32_t i = threadIdx.x; i < hi; i += 64 * kSortWaves) {
-		atomicAdd(&count[expert_at(expert, lo + i, n_experts)], 1u);
+#pragma unroll
+	for (uint32_t i = 0; i < kRounds; i++) {
+		const uint32_t e = known_expert(ids[i], n_experts);
+		if (e < n_experts) {
+			atomicAdd(&count[e], 1u);
+		}
 	}
 	__syncthreads();
 	for (uint32_t e = threadIdx.x; e < n_experts; e += 64 * kSortWaves) {
@@ -55,7 +64,9 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(const I *_
 	}
 }
 
-/* Rows of a tile's pairs.  Every workgroup adds up the tiles' counts by itself. */
+/* Rows of a tile's pairs: each wavefront ranks its own, the counts of the wavefronts and of the other tiles say where they begin.
+ * Every workgroup adds up the tiles' counts by itself; a tile that is alone needs none.  LDS: kSortWaves counters an expert, and of those
+ * without one. */
 template <typename I>
 __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *__restrict__ expert, uint32_t n_pairs,
 								      uint32_t n_experts, uint32_t n_tiles, uint32_t max_rows,
@@ -63,105 +74,113 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 								      int32_t *__restrict__ row_of, int32_t *__restrict__ pair_of,
 								      uint32_t *__restrict__ err)
 {
-	__shared__ uint32_t base[kMaxExperts + 1];              /* first row of the tile's pairs of an expert */
-	__shared__ uint32_t next[kSortWaves][kMaxExperts + 1];  /* next row of a wavefront's pairs of an expert */
+	extern __shared__ uint32_t next[]; /* [wavefront][expert]: first its pairs so far, then its first row */
 	__shared__ uint32_t carry[kSortWaves];
-	const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, tile = blockIdx.x;
-	uint32_t before = 0; /* rows of all experts in front of this round's */
-	for (uint32_t e0 = 0; e0 < n_experts; e0 += 64 * kSortWaves) {
-		const uint32_t e = e0 + threadIdx.x;
-		uint32_t total = 0, mine = 0;
-		if (e < n_experts) {
-			for (uint32_t t = 0; t < n_tiles; t++) {
-				const uint32_t c = counts[(uint64_t)t * n_experts + e];
-				mine = t == tile ? total : mine;
-				total += c;
-			}
-		}
-		uint32_t scan = total; /* inclusive over the wavefront */
+	const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, tile = blockIdx.x, stride = n_experts + 1;
+	const uint64_t lo = (uint64_t)tile * kTile + wave * kTileOfWave;
+	I ids[kRounds];
 #pragma unroll
-		for (uint32_t d = 1; d < 64; d <<= 1) {
-			const uint32_t up = __shfl_up(scan, d);
-			scan += lane >= d ? up : 0u;
-		}
-		if (lane == 63) {
-			carry[wave] = scan;
-		}
-		__syncthreads();
-		uint32_t front = before;
-#pragma unroll
-		for (int w = 0; w < kSortWaves; w++) {
-			front += (uint32_t)w < wave ? carry[w] : 0u;
-			before += carry[w];
-		}
-		if (e < n_experts) {
-			base[e] = front + scan - total + mine;
-			if (tile == 0) {
-				offset[e] = (int32_t)min(front + scan - total, max_rows);
-			}
-		}
-		__syncthreads();
+	for (uint32_t i = 0; i < kRounds; i++) {
+		const uint64_t p = lo + i * 64 + lane;
+		ids[i] = p < n_pairs ? expert[p] : (I)-1;
 	}
-	if (tile == 0 && threadIdx.x == 0) {
-		offset[n_experts] = (int32_t)min(before, max_rows);
-		if (before > max_rows) {
-			atomicOr(err, ASYNC_ERR_TOKEN_ROWS);
+	/* one expert a lane: there are at most as many as lanes */
+	static_assert(kMaxExperts <= 64 * kSortWaves, "one expert a lane");
+	uint32_t total = 0, mine = 0;
+	if (n_tiles > 1 && threadIdx.x < n_experts) {
+#pragma unroll 8
+		for (uint32_t t = 0; t < n_tiles; t++) {
+			const uint32_t c = counts[(uint64_t)t * n_experts + threadIdx.x];
+			mine += t < tile ? c : 0u;
+			total += c;
 		}
 	}
-	if (pair_of) { /* rows behind the last pair's */
-		for (uint64_t r = before + (uint64_t)tile * 64 * kSortWaves + threadIdx.x; r < max_rows; r += (uint64_t)gridDim.x * 64 * kSortWaves) {
-			pair_of[r] = -1;
-		}
-	}
-	/* what the wavefronts in front of this one place */
-	for (uint32_t e = threadIdx.x; e <= n_experts; e += 64 * kSortWaves) {
-#pragma unroll
-		for (int w = 0; w < kSortWaves; w++) {
-			next[w][e] = 0;
-		}
-	}
-	__syncthreads();
-	const uint32_t lo = tile * kTile + wave * kTileOfWave;
-	const uint32_t mine = lo < n_pairs ? min(n_pairs - lo, kTileOfWave) : 0u;
-	for (uint32_t i = lane; i < mine; i += 64) {
-		atomicAdd(&next[wave][expert_at(expert, lo + i, n_experts)], 1u);
-	}
-	__syncthreads();
-	for (uint32_t e = threadIdx.x; e < n_experts; e += 64 * kSortWaves) {
-		uint32_t at = base[e];
-#pragma unroll
-		for (int w = 0; w < kSortWaves; w++) {
-			const uint32_t c = next[w][e];
-			next[w][e] = at;
-			at += c;
-		}
+	for (uint32_t i = threadIdx.x; i < kSortWaves * stride; i += 64 * kSortWaves) {
+		next[i] = 0;
 	}
 	__syncthreads();
 	const uint32_t bits = 32u - (uint32_t)__builtin_clz(n_experts);
-	for (uint32_t i0 = 0; i0 < mine; i0 += 64) {
-		const uint32_t p = lo + i0 + lane;
-		const bool in = i0 + lane < mine;
-		const uint32_t e = in ? expert_at(expert, p, n_experts) : n_experts;
+	uint32_t *own = next + wave * stride;
+	uint32_t rank[kRounds];
+#pragma unroll
+	for (uint32_t i = 0; i < kRounds; i++) {
+		const uint32_t e = known_expert(ids[i], n_experts);
 		uint64_t same = ~0ull; /* lanes with this lane's expert */
 		for (uint32_t b = 0; b < bits; b++) {
 			const bool one = (e >> b) & 1u;
 			const uint64_t ones = __ballot(one);
 			same &= one ? ones : ~ones;
 		}
-		const uint32_t rank = lanes_below(same), of = (uint32_t)__popcll(same);
-		const uint32_t first = next[wave][e];
+		const uint32_t below = lanes_below(same), of = (uint32_t)__popcll(same), before = own[e];
+		rank[i] = before + below;
 		__builtin_amdgcn_wave_barrier(); /* every lane has read before the last of an expert's lanes writes */
-		if (e < n_experts && rank == of - 1u) {
-			next[wave][e] = first + of;
+		if (below == of - 1u) {
+			own[e] = before + of;
 		}
 		__builtin_amdgcn_wave_barrier();
-		if (in) {
-			const uint32_t row = first + rank;
-			const bool placed = e < n_experts && row < max_rows;
+	}
+	__syncthreads();
+	/* the expert's rows in front of each wavefront's; total: of all tiles */
+	uint32_t here = 0;
+	if (threadIdx.x < n_experts) {
+#pragma unroll
+		for (int w = 0; w < kSortWaves; w++) {
+			here += next[w * stride + threadIdx.x];
+		}
+		total = n_tiles > 1 ? total : here;
+	}
+	uint32_t scan = total; /* inclusive over the wavefront */
+#pragma unroll
+	for (uint32_t d = 1; d < 64; d <<= 1) {
+		const uint32_t up = __shfl_up(scan, d);
+		scan += lane >= d ? up : 0u;
+	}
+	if (lane == 63) {
+		carry[wave] = scan;
+	}
+	__syncthreads();
+	uint32_t front = 0, all = 0;
+#pragma unroll
+	for (int w = 0; w < kSortWaves; w++) {
+		front += (uint32_t)w < wave ? carry[w] : 0u;
+		all += carry[w];
+	}
+	front += scan - total;
+	if (threadIdx.x < n_experts) {
+		uint32_t at = front + mine;
+#pragma unroll
+		for (int w = 0; w < kSortWaves; w++) {
+			const uint32_t c = next[w * stride + threadIdx.x];
+			next[w * stride + threadIdx.x] = at;
+			at += c;
+		}
+		if (tile == 0) {
+			offset[threadIdx.x] = (int32_t)min(front, max_rows);
+		}
+	}
+	if (tile == 0 && threadIdx.x == 0) {
+		offset[n_experts] = (int32_t)min(all, max_rows);
+		if (all > max_rows) {
+			atomicOr(err, ASYNC_ERR_TOKEN_ROWS);
+		}
+	}
+	__syncthreads();
+#pragma unroll
+	for (uint32_t i = 0; i < kRounds; i++) {
+		const uint64_t p = lo + i * 64 + lane;
+		if (p < n_pairs) {
+			const uint32_t e = known_expert(ids[i], n_experts);
+			const uint32_t row = e < n_experts ? own[e] + rank[i] : ~0u;
+			const bool placed = row < max_rows;
 			row_of[p] = placed ? (int32_t)row : -1;
 			if (placed && pair_of) {
 				pair_of[row] = (int32_t)p;
 			}
+		}
+	}
+	if (pair_of) { /* rows behind the last pair's */
+		for (uint64_t r = all + (uint64_t)tile * 64 * kSortWaves + threadIdx.x; r < max_rows; r += (uint64_t)n_tiles * 64 * kSortWaves) {
+			pair_of[r] = -1;
 		}
 	}
 }
@@ -174,46 +193,52 @@ struct rows_t { /* rows of bytes and where they go */
 	uint32_t bytes;
 };
 
-/* One wavefront per 4 KiB of a token's row: it is read once and written to each of its places */
-constexpr uint32_t kSpan = 4096;
-__global__ __launch_bounds__(64) void token_rows_kernel(const int32_t *__restrict__ row_of, uint32_t first, uint32_t top_k, uint32_t spans,
-						        rows_t a, rows_t b)
+/* One workgroup per token: 4 KiB of its row are read at a time by a wavefront and written to each of its places; the first
+ * wavefronts have the row, those behind them the second row. */
+constexpr uint32_t kRows = 2; /* of 1 KiB */
+constexpr uint32_t kSpan = 1024 * kRows;
+constexpr uint32_t kMostWaves = 8;
+__global__ __launch_bounds__(64 * kMostWaves) void token_rows_kernel(const int32_t *__restrict__ row_of, uint32_t first, uint32_t top_k,
+								     uint32_t row_waves, rows_t a, rows_t b)
 {
-	const uint32_t lane = threadIdx.x;
+	const uint32_t lane = threadIdx.x & 63u;
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
 	const uint32_t token = first + blockIdx.x;
-	const bool second = blockIdx.y >= spans;
+	const bool second = wave >= row_waves;
 	const rows_t r = second ? b : a;
-	const uint32_t at = (blockIdx.y - (second ? spans : 0u)) * kSpan;
-	const uint32_t n = min(r.bytes - at, kSpan);
-	const uint8_t *from = r.from + token * r.from_pitch + at;
+	const uint32_t waves = second ? 1u : row_waves;
 	const int32_t *rows = row_of + (uint64_t)token * top_k;
-	u32x4_t v[4];
-	const uint32_t whole = n >> 4;
+	for (uint32_t at = (second ? 0u : wave) * kSpan; at < r.bytes; at += waves * kSpan) {
+		const uint32_t n = min(r.bytes - at, kSpan);
+		const uint8_t *from = r.from + token * r.from_pitch + at;
+		u32x4_t v[kRows];
+		const uint32_t whole = n >> 4;
 #pragma unroll
-	for (uint32_t i = 0; i < 4; i++) {
-		if (i * 64u + lane < whole) {
-			v[i] = reinterpret_cast<const any16_t *>(from + 16u * (i * 64u + lane))->v;
-		}
-	}
-	const uint32_t rest = n & 15u;
-	uint8_t tail = 0;
-	if (lane < rest) {
-		tail = from[16u * whole + lane];
-	}
-	for (uint32_t k = 0; k < top_k; k++) {
-		const int32_t row = rows[k];
-		if (row < 0) {
-			continue;
-		}
-		uint8_t *to = r.to + (uint64_t)row * r.to_pitch + at;
-#pragma unroll
-		for (uint32_t i = 0; i < 4; i++) {
+		for (uint32_t i = 0; i < kRows; i++) {
 			if (i * 64u + lane < whole) {
-				reinterpret_cast<any16_t *>(to + 16u * (i * 64u + lane))->v = v[i];
+				v[i] = *reinterpret_cast<const any16_t *>(from + 16u * (i * 64u + lane));
 			}
 		}
+		const uint32_t rest = n & 15u;
+		uint8_t tail = 0;
 		if (lane < rest) {
-			to[16u * whole + lane] = tail;
+			tail = from[16u * whole + lane];
+		}
+		for (uint32_t k = 0; k < top_k; k++) {
+			const int32_t row = rows[k];
+			if (row < 0) {
+				continue;
+			}
+			uint8_t *to = r.to + (uint64_t)row * r.to_pitch + at;
+#pragma unroll
+			for (uint32_t i = 0; i < kRows; i++) {
+				if (i * 64u + lane < whole) {
+					*reinterpret_cast<any16_t *>(to + 16u * (i * 64u + lane)) = v[i];
+				}
+			}
+			if (lane < rest) {
+				to[16u * whole + lane] = tail;
+			}
 		}
 	}
 }
@@ -229,7 +254,8 @@ extern "C" {
 
 uint64_t ofi_amd_token_dispatch_work_bytes(uint32_t n_tokens, uint32_t top_k, uint32_t n_experts)
 {
-	return (uint64_t)tiles_of((uint64_t)n_tokens * top_k) * n_experts * sizeof(uint32_t);
+	const uint64_t tiles = tiles_of((uint64_t)n_tokens * top_k);
+	return tiles == 1 ? 0 : tiles * n_experts * sizeof(uint32_t);
 }
 
 int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tokens, uint32_t top_k, uint32_t n_experts,
@@ -273,9 +299,12 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 	const uint32_t tiles = tiles_of(n_pairs);
 	auto sort = [&](const auto *expert) {
 		using I = typename std::remove_cv<typename std::remove_pointer<decltype(expert)>::type>::type;
-		launch_kernel(token_count_kernel<I>, dim3(tiles), dim3(64 * kSortWaves), 0, as_stream(stream), expert, (uint32_t)n_pairs,
-			      n_experts, static_cast<uint32_t *>(d_work));
-		launch_kernel(token_place_kernel<I>, dim3(tiles), dim3(64 * kSortWaves), 0, as_stream(stream), expert, (uint32_t)n_pairs,
+		if (tiles > 1) {
+			launch_kernel(token_count_kernel<I>, dim3(tiles), dim3(64 * kSortWaves), 0, as_stream(stream), expert, (uint32_t)n_pairs,
+				      n_experts, static_cast<uint32_t *>(d_work));
+		}
+		launch_kernel(token_place_kernel<I>, dim3(tiles), dim3(64 * kSortWaves), kSortWaves * (n_experts + 1) * sizeof(uint32_t),
+			      as_stream(stream), expert, (uint32_t)n_pairs,
 			      n_experts, tiles, max_rows, static_cast<const uint32_t *>(d_work), d_offset, d_row_of, d_pair_of, err);
 	};
 	if (expert_type == OFI_AMD_INT64) {
@@ -287,10 +316,11 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 		const rows_t a = { static_cast<const uint8_t *>(d_x), x_pitch, static_cast<uint8_t *>(d_rows), rows_pitch, row_bytes };
 		const rows_t b = { static_cast<const uint8_t *>(d_scale), scale_pitch, static_cast<uint8_t *>(d_scale_rows), scale_rows_pitch,
 				   scale_bytes };
-		const uint32_t spans = (row_bytes + kSpan - 1) / kSpan, more = d_scale ? (scale_bytes + kSpan - 1) / kSpan : 0;
+		const uint32_t spans = (row_bytes + kSpan - 1) / kSpan;
+		const uint32_t row_waves = spans < kMostWaves - 1 ? spans : kMostWaves - (d_scale ? 1 : 0);
 		for (uint32_t first = 0; first < n_tokens; first += kTokensOfLaunch) {
-			launch_kernel(token_rows_kernel, dim3(n_tokens - first < kTokensOfLaunch ? n_tokens - first : kTokensOfLaunch, spans + more),
-				      dim3(64), 0, as_stream(stream), d_row_of, first, top_k, spans, a, b);
+			launch_kernel(token_rows_kernel, dim3(n_tokens - first < kTokensOfLaunch ? n_tokens - first : kTokensOfLaunch),
+				      dim3(64 * (row_waves + (d_scale ? 1 : 0))), 0, as_stream(stream), d_row_of, first, top_k, row_waves, a, b);
 		}
 	}
 	OFI_AMD_HIP_TRY(hipGetLastError());
