@@ -19,9 +19,19 @@ constexpr uint32_t kMaxTopK = 64;
 constexpr uint32_t kMaxRowBytes = 1u << 24;
 constexpr uint32_t kTokensOfLaunch = 1u << 22;
 constexpr int kSortWaves = 16;
-constexpr uint32_t kRounds = 8;                                  /* pairs of a lane */
-constexpr uint32_t kTileOfWave = 64 * kRounds;                   /* pairs of a wavefront, in order: lanes first, then rounds */
-constexpr uint32_t kTile = (uint32_t)kSortWaves * kTileOfWave;   /* of a workgroup of the sort */
+constexpr uint32_t kMostRounds = 8; /* pairs of a lane of the sort */
+constexpr uint32_t kManyTiles = 32;
+
+/* A workgroup of the sort has 1024 pairs a round; tiles get more rounds before they get many.  Everybody adds up the counts of all
+ * tiles, 8 at a time, so that 32 tiles of 8 rounds cost less than 256 of one. */
+inline uint32_t rounds_of(uint64_t n_pairs)
+{
+	const uint64_t one = 64 * kSortWaves;
+	if (n_pairs <= one * kMostRounds) { /* a single tile */
+		return n_pairs <= one ? 1 : n_pairs <= 2 * one ? 2 : n_pairs <= 4 * one ? 4 : 8;
+	}
+	return n_pairs <= one * kManyTiles ? 1 : n_pairs <= 2 * one * kManyTiles ? 2 : n_pairs <= 4 * one * kManyTiles ? 4 : 8;
+}
 
 __device__ __forceinline__ uint32_t lanes_below(uint64_t mask)
 {
@@ -35,15 +45,15 @@ template <typename I> __device__ __forceinline__ uint32_t known_expert(I e, uint
 }
 
 /* counts[tile][e] */
-template <typename I>
+template <typename I, uint32_t ROUNDS>
 __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(const I *__restrict__ expert, uint32_t n_pairs,
 								      uint32_t n_experts, uint32_t *__restrict__ counts)
 {
 	__shared__ uint32_t count[kMaxExperts + 1];
-	const uint64_t lo = (uint64_t)blockIdx.x * kTile;
-	I ids[kRounds];
+	const uint64_t lo = (uint64_t)blockIdx.x * (64 * kSortWaves * ROUNDS);
+	I ids[ROUNDS];
 #pragma unroll
-	for (uint32_t i = 0; i < kRounds; i++) {
+	for (uint32_t i = 0; i < ROUNDS; i++) {
 		const uint64_t p = lo + i * 64 * kSortWaves + threadIdx.x;
 		ids[i] = p < n_pairs ? expert[p] : (I)-1;
 	}
@@ -52,7 +62,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(const I *_
 	}
 	__syncthreads();
 #pragma unroll
-	for (uint32_t i = 0; i < kRounds; i++) {
+	for (uint32_t i = 0; i < ROUNDS; i++) {
 		const uint32_t e = known_expert(ids[i], n_experts);
 		if (e < n_experts) {
 			atomicAdd(&count[e], 1u);
@@ -67,7 +77,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(const I *_
 /* Rows of a tile's pairs: each wavefront ranks its own, the counts of the wavefronts and of the other tiles say where they begin.
  * Every workgroup adds up the tiles' counts by itself; a tile that is alone needs none.  LDS: kSortWaves counters an expert, and of those
  * without one. */
-template <typename I>
+template <typename I, uint32_t ROUNDS>
 __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *__restrict__ expert, uint32_t n_pairs,
 								      uint32_t n_experts, uint32_t n_tiles, uint32_t max_rows,
 								      const uint32_t *__restrict__ counts, int32_t *__restrict__ offset,
@@ -77,10 +87,10 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 	extern __shared__ uint32_t next[]; /* [wavefront][expert]: first its pairs so far, then its first row */
 	__shared__ uint32_t carry[kSortWaves];
 	const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, tile = blockIdx.x, stride = n_experts + 1;
-	const uint64_t lo = (uint64_t)tile * kTile + wave * kTileOfWave;
-	I ids[kRounds];
+	const uint64_t lo = ((uint64_t)tile * kSortWaves + wave) * (64 * ROUNDS); /* its pairs in order: lanes first, then rounds */
+	I ids[ROUNDS];
 #pragma unroll
-	for (uint32_t i = 0; i < kRounds; i++) {
+	for (uint32_t i = 0; i < ROUNDS; i++) {
 		const uint64_t p = lo + i * 64 + lane;
 		ids[i] = p < n_pairs ? expert[p] : (I)-1;
 	}
@@ -101,15 +111,15 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 	__syncthreads();
 	const uint32_t bits = 32u - (uint32_t)__builtin_clz(n_experts);
 	uint32_t *own = next + wave * stride;
-	uint32_t rank[kRounds];
+	uint32_t rank[ROUNDS];
 #pragma unroll
-	for (uint32_t i = 0; i < kRounds; i++) {
+	for (uint32_t i = 0; i < ROUNDS; i++) {
 		const uint32_t e = known_expert(ids[i], n_experts);
 		uint64_t same = ~0ull; /* lanes with this lane's expert */
 		for (uint32_t b = 0; b < bits; b++) {
-			const bool one = (e >> b) & 1u;
+			const uint32_t one = 0u - ((e >> b) & 1u);
 			const uint64_t ones = __ballot(one);
-			same &= one ? ones : ~ones;
+			same &= ~(ones ^ ((uint64_t)one << 32 | one));
 		}
 		const uint32_t below = lanes_below(same), of = (uint32_t)__popcll(same), before = own[e];
 		rank[i] = before + below;
@@ -166,7 +176,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 	}
 	__syncthreads();
 #pragma unroll
-	for (uint32_t i = 0; i < kRounds; i++) {
+	for (uint32_t i = 0; i < ROUNDS; i++) {
 		const uint64_t p = lo + i * 64 + lane;
 		if (p < n_pairs) {
 			const uint32_t e = known_expert(ids[i], n_experts);
@@ -193,59 +203,200 @@ struct rows_t { /* rows of bytes and where they go */
 	uint32_t bytes;
 };
 
-/* One workgroup per token: 4 KiB of its row are read at a time by a wavefront and written to each of its places; the first
- * wavefronts have the row, those behind them the second row. */
 constexpr uint32_t kRows = 2; /* of 1 KiB */
 constexpr uint32_t kSpan = 1024 * kRows;
 constexpr uint32_t kMostWaves = 8;
-__global__ __launch_bounds__(64 * kMostWaves) void token_rows_kernel(const int32_t *__restrict__ row_of, uint32_t first, uint32_t top_k,
-								     uint32_t row_waves, rows_t a, rows_t b)
+constexpr uint32_t kAtOnce = 8;
+
+/* A token's rows: 2 KiB are read at a time by a wavefront and written to each of the places (a row number each, max_rows or more:
+ * none), the next ones when these are done.  The first row_waves wavefronts have row a, the one behind them row b. */
+template <typename P>
+__device__ __forceinline__ void copy_rows(uint32_t token, uint32_t wave, uint32_t row_waves, const rows_t &a, const rows_t &b,
+					  uint32_t top_k, uint32_t max_rows, P place)
 {
 	const uint32_t lane = threadIdx.x & 63u;
-	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-	const uint32_t token = first + blockIdx.x;
 	const bool second = wave >= row_waves;
 	const rows_t r = second ? b : a;
-	const uint32_t waves = second ? 1u : row_waves;
-	const int32_t *rows = row_of + (uint64_t)token * top_k;
-	for (uint32_t at = (second ? 0u : wave) * kSpan; at < r.bytes; at += waves * kSpan) {
-		const uint32_t n = min(r.bytes - at, kSpan);
-		const uint8_t *from = r.from + token * r.from_pitch + at;
-		u32x4_t v[kRows];
-		const uint32_t whole = n >> 4;
+	const uint32_t stride = second ? kSpan : row_waves * kSpan;
+	for (uint32_t k0 = 0; k0 < top_k; k0 += kAtOnce) {
+		uint32_t row[kAtOnce], least = ~0u;
 #pragma unroll
-		for (uint32_t i = 0; i < kRows; i++) {
-			if (i * 64u + lane < whole) {
-				v[i] = *reinterpret_cast<const any16_t *>(from + 16u * (i * 64u + lane));
-			}
+		for (uint32_t k = 0; k < kAtOnce; k++) {
+			row[k] = k0 + k < top_k ? place(k0 + k) : ~0u;
+			least = min(least, row[k]);
 		}
-		const uint32_t rest = n & 15u;
-		uint8_t tail = 0;
-		if (lane < rest) {
-			tail = from[16u * whole + lane];
+		if (least >= max_rows) {
+			continue; /* nobody asks for this token */
 		}
-		for (uint32_t k = 0; k < top_k; k++) {
-			const int32_t row = rows[k];
-			if (row < 0) {
-				continue;
-			}
-			uint8_t *to = r.to + (uint64_t)row * r.to_pitch + at;
+		for (uint32_t at = second ? 0u : wave * kSpan; at < r.bytes; at += stride) {
+			const uint32_t n = min(r.bytes - at, kSpan), whole = n >> 4, rest = n & 15u;
+			const uint8_t *from = r.from + token * r.from_pitch + at;
+			u32x4_t v[kRows];
 #pragma unroll
 			for (uint32_t i = 0; i < kRows; i++) {
 				if (i * 64u + lane < whole) {
-					*reinterpret_cast<any16_t *>(to + 16u * (i * 64u + lane)) = v[i];
+					v[i] = *reinterpret_cast<const any16_t *>(from + 16u * (i * 64u + lane));
 				}
 			}
+			uint8_t tail = 0;
 			if (lane < rest) {
-				to[16u * whole + lane] = tail;
+				tail = from[16u * whole + lane];
+			}
+#pragma unroll
+			for (uint32_t k = 0; k < kAtOnce; k++) {
+				if (row[k] < max_rows) {
+					uint8_t *to = r.to + row[k] * r.to_pitch + at;
+#pragma unroll
+					for (uint32_t i = 0; i < kRows; i++) {
+						if (i * 64u + lane < whole) {
+							*reinterpret_cast<any16_t *>(to + 16u * (i * 64u + lane)) = v[i];
+						}
+					}
+					if (lane < rest) {
+						to[16u * whole + lane] = tail;
+					}
+				}
 			}
 		}
 	}
 }
 
+/* One workgroup per token */
+__global__ __launch_bounds__(64 * kMostWaves) void token_rows_kernel(const int32_t *__restrict__ row_of, uint32_t first, uint32_t top_k,
+								     uint32_t row_waves, uint32_t max_rows, rows_t a, rows_t b)
+{
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+	const uint32_t token = first + blockIdx.x;
+	const int32_t *rows = row_of + (uint64_t)token * top_k;
+	copy_rows(token, wave, row_waves, a, b, top_k, max_rows, [&](uint32_t k) { return (uint32_t)rows[k]; });
+}
+
+/*
+ * Few pairs: table and rows in one launch.  The workgroup of a token counts the pairs in front of each of its own -- of a smaller
+ * expert, or of the same and a smaller number, which is one comparison of expert * kFew + pair -- and copies its rows there; the
+ * last workgroup makes the offsets.
+ */
+constexpr uint32_t kFew = 2048;
+static_assert((uint64_t)kMaxExperts * kFew < 0x7fffffffull, "keys within 32 bits");
+template <typename I>
+__global__ __launch_bounds__(64 * kMostWaves) void token_few_kernel(const I *__restrict__ expert, uint32_t n_tokens, uint32_t top_k,
+								    uint32_t n_experts, uint32_t row_waves, uint32_t max_rows, rows_t a,
+								    rows_t b, int32_t *__restrict__ offset, int32_t *__restrict__ row_of,
+								    int32_t *__restrict__ pair_of, uint32_t *__restrict__ err)
+{
+	__shared__ uint32_t counts[kMaxExperts > kMostWaves * kMaxTopK ? kMaxExperts : kMostWaves * kMaxTopK];
+	__shared__ uint32_t carry[kMostWaves];
+	const uint32_t lane = threadIdx.x & 63u, waves = blockDim.x >> 6, token = blockIdx.x, n_pairs = n_tokens * top_k;
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+	if (token == n_tokens) { /* the last workgroup */
+		const uint32_t per = (n_experts + blockDim.x - 1) / blockDim.x, lo = threadIdx.x * per; /* experts of a lane */
+		for (uint32_t e = threadIdx.x; e < n_experts; e += blockDim.x) {
+			counts[e] = 0;
+		}
+		__syncthreads();
+		for (uint32_t p = threadIdx.x; p < n_pairs; p += blockDim.x) {
+			const uint32_t e = known_expert(expert[p], n_experts);
+			if (e < n_experts) {
+				atomicAdd(&counts[e], 1u);
+			}
+		}
+		__syncthreads();
+		uint32_t own = 0;
+		for (uint32_t e = lo; e < min(lo + per, n_experts); e++) {
+			own += counts[e];
+		}
+		uint32_t scan = own;
+#pragma unroll
+		for (uint32_t d = 1; d < 64; d <<= 1) {
+			const uint32_t up = __shfl_up(scan, d);
+			scan += lane >= d ? up : 0u;
+		}
+		if (lane == 63) {
+			carry[wave] = scan;
+		}
+		__syncthreads();
+		uint32_t at = scan - own, all = 0;
+		for (uint32_t w = 0; w < waves; w++) {
+			at += w < wave ? carry[w] : 0u;
+			all += carry[w];
+		}
+		for (uint32_t e = lo; e < min(lo + per, n_experts); e++) {
+			offset[e] = (int32_t)min(at, max_rows);
+			at += counts[e];
+		}
+		if (threadIdx.x == 0) {
+			offset[n_experts] = (int32_t)min(all, max_rows);
+			if (all > max_rows) {
+				atomicOr(err, ASYNC_ERR_TOKEN_ROWS);
+			}
+		}
+		if (pair_of) {
+			for (uint64_t r = (uint64_t)all + threadIdx.x; r < max_rows; r += blockDim.x) {
+				pair_of[r] = -1;
+			}
+		}
+		return;
+	}
+	const uint32_t p0 = token * top_k;
+	for (uint32_t k0 = 0; k0 < top_k; k0 += kAtOnce) {
+		uint32_t key[kAtOnce], before[kAtOnce];
+#pragma unroll
+		for (uint32_t k = 0; k < kAtOnce; k++) {
+			const uint32_t p = p0 + min(k0 + k, top_k - 1u);
+			key[k] = known_expert(expert[p], n_experts) * kFew + p;
+			before[k] = 0;
+		}
+		for (uint32_t q = threadIdx.x; q - lane < n_pairs; q += blockDim.x) {
+			const uint32_t of = q < n_pairs ? known_expert(expert[q], n_experts) * kFew + q : ~0u;
+#pragma unroll
+			for (uint32_t k = 0; k < kAtOnce; k++) {
+				before[k] += (uint32_t)__popcll(__ballot(of < key[k]));
+			}
+		}
+		if (lane == 0) {
+#pragma unroll
+			for (uint32_t k = 0; k < kAtOnce; k++) {
+				if (k0 + k < top_k) {
+					counts[wave * top_k + k0 + k] = before[k];
+				}
+			}
+		}
+	}
+	__syncthreads();
+	for (uint32_t k = threadIdx.x; k < top_k; k += blockDim.x) {
+		uint32_t row = 0;
+		for (uint32_t w = 0; w < waves; w++) {
+			row += counts[w * top_k + k];
+		}
+		const bool placed = row < max_rows && known_expert(expert[p0 + k], n_experts) < n_experts;
+		row_of[p0 + k] = placed ? (int32_t)row : -1;
+		if (placed && pair_of) {
+			pair_of[row] = (int32_t)(p0 + k);
+		}
+		counts[k] = placed ? row : ~0u; /* the first wavefront's, which this lane has read */
+	}
+	__syncthreads();
+	copy_rows(token, wave, row_waves, a, b, top_k, max_rows,
+		  [&](uint32_t k) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)counts[k]); });
+}
+
 inline uint32_t tiles_of(uint64_t n_pairs)
 {
-	return n_pairs == 0 ? 1u : (uint32_t)((n_pairs + kTile - 1) / kTile);
+	const uint64_t tile = 64ull * kSortWaves * rounds_of(n_pairs);
+	return n_pairs == 0 ? 1u : (uint32_t)((n_pairs + tile - 1) / tile);
+}
+
+template <typename F> void with_rounds(uint32_t rounds, F f)
+{
+	if (rounds == 1) {
+		f(std::integral_constant<uint32_t, 1>{});
+	} else if (rounds == 2) {
+		f(std::integral_constant<uint32_t, 2>{});
+	} else if (rounds == 4) {
+		f(std::integral_constant<uint32_t, 4>{});
+	} else {
+		f(std::integral_constant<uint32_t, kMostRounds>{});
+	}
 }
 
 } // namespace
@@ -296,32 +447,38 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 	if (!err) {
 		return -ENOMEM;
 	}
-	const uint32_t tiles = tiles_of(n_pairs);
-	auto sort = [&](const auto *expert) {
+	const rows_t a = { static_cast<const uint8_t *>(d_x), x_pitch, static_cast<uint8_t *>(d_rows), rows_pitch, row_bytes };
+	const rows_t b = { static_cast<const uint8_t *>(d_scale), scale_pitch, static_cast<uint8_t *>(d_scale_rows), scale_rows_pitch,
+			   scale_bytes };
+	const uint32_t spans = d_x ? (row_bytes + kSpan - 1) / kSpan : 0, more = d_scale ? 1 : 0;
+	const uint32_t row_waves = spans < kMostWaves - more ? spans : kMostWaves - more;
+	auto run = [&](const auto *expert) {
 		using I = typename std::remove_cv<typename std::remove_pointer<decltype(expert)>::type>::type;
-		if (tiles > 1) {
-			launch_kernel(token_count_kernel<I>, dim3(tiles), dim3(64 * kSortWaves), 0, as_stream(stream), expert, (uint32_t)n_pairs,
-				      n_experts, static_cast<uint32_t *>(d_work));
+		if (d_x && n_pairs <= kFew) {
+			launch_kernel(token_few_kernel<I>, dim3(n_tokens + 1), dim3(64 * (row_waves + more)), 0, as_stream(stream), expert, n_tokens,
+				      top_k, n_experts, row_waves, max_rows, a, b, d_offset, d_row_of, d_pair_of, err);
+			return;
 		}
-		launch_kernel(token_place_kernel<I>, dim3(tiles), dim3(64 * kSortWaves), kSortWaves * (n_experts + 1) * sizeof(uint32_t),
-			      as_stream(stream), expert, (uint32_t)n_pairs,
-			      n_experts, tiles, max_rows, static_cast<const uint32_t *>(d_work), d_offset, d_row_of, d_pair_of, err);
+		const uint32_t tiles = tiles_of(n_pairs);
+		with_rounds(rounds_of(n_pairs), [&](auto rounds) {
+			constexpr uint32_t R = decltype(rounds)::value;
+			if (tiles > 1) {
+				launch_kernel(token_count_kernel<I, R>, dim3(tiles), dim3(64 * kSortWaves), 0, as_stream(stream), expert,
+					      (uint32_t)n_pairs, n_experts, static_cast<uint32_t *>(d_work));
+			}
+			launch_kernel(token_place_kernel<I, R>, dim3(tiles), dim3(64 * kSortWaves),
+				      kSortWaves * (n_experts + 1) * sizeof(uint32_t), as_stream(stream), expert, (uint32_t)n_pairs, n_experts, tiles,
+				      max_rows, static_cast<const uint32_t *>(d_work), d_offset, d_row_of, d_pair_of, err);
+		});
+		for (uint32_t first = 0; d_x && first < n_tokens; first += kTokensOfLaunch) {
+			launch_kernel(token_rows_kernel, dim3(n_tokens - first < kTokensOfLaunch ? n_tokens - first : kTokensOfLaunch),
+				      dim3(64 * (row_waves + more)), 0, as_stream(stream), d_row_of, first, top_k, row_waves, max_rows, a, b);
+		}
 	};
 	if (expert_type == OFI_AMD_INT64) {
-		sort(static_cast<const int64_t *>(d_expert));
+		run(static_cast<const int64_t *>(d_expert));
 	} else {
-		sort(static_cast<const int32_t *>(d_expert));
-	}
-	if (d_x && n_tokens != 0) {
-		const rows_t a = { static_cast<const uint8_t *>(d_x), x_pitch, static_cast<uint8_t *>(d_rows), rows_pitch, row_bytes };
-		const rows_t b = { static_cast<const uint8_t *>(d_scale), scale_pitch, static_cast<uint8_t *>(d_scale_rows), scale_rows_pitch,
-				   scale_bytes };
-		const uint32_t spans = (row_bytes + kSpan - 1) / kSpan;
-		const uint32_t row_waves = spans < kMostWaves - 1 ? spans : kMostWaves - (d_scale ? 1 : 0);
-		for (uint32_t first = 0; first < n_tokens; first += kTokensOfLaunch) {
-			launch_kernel(token_rows_kernel, dim3(n_tokens - first < kTokensOfLaunch ? n_tokens - first : kTokensOfLaunch),
-				      dim3(64 * (row_waves + (d_scale ? 1 : 0))), 0, as_stream(stream), d_row_of, first, top_k, row_waves, a, b);
-		}
+		run(static_cast<const int32_t *>(d_expert));
 	}
 	OFI_AMD_HIP_TRY(hipGetLastError());
 	return 0;
