@@ -10,12 +10,15 @@
 #include "common.hpp"
 #include "ofi_amd_hotpath.h"
 #include "row_types.hpp"
+#include <cstdlib>
 
 namespace {
 
 using namespace ofi_amd;
 
 constexpr uint32_t kMaxWidth = 32768;
+constexpr int kGradWaves = 8;
+constexpr uint32_t kGradBlocks = 512;
 constexpr uint32_t kRowsOfLaunch = 1u << 21; /* with 1024 lanes each within the 32 bits of a launch's size */
 
 struct norm_out_t {
@@ -31,7 +34,7 @@ struct norm_out_t {
 };
 
 /* A chunk's own elements times `inverse` as e4m3 */
-template <uint32_t V> __device__ __forceinline__ void store_q(uint8_t *p, uint32_t skip, const float (&f)[V], float inverse)
+template <bool STREAM, uint32_t V> __device__ __forceinline__ void store_q(uint8_t *p, uint32_t skip, const float (&f)[V], float inverse)
 {
 	if constexpr (V == 1) {
 		if (skip == 0) {
@@ -45,7 +48,9 @@ template <uint32_t V> __device__ __forceinline__ void store_q(uint8_t *p, uint32
 			const int low = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * inverse, f[4 * i + 1] * inverse, 0, false);
 			w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inverse, f[4 * i + 3] * inverse, low, true);
 		}
-		if (skip == 0) {
+		if (skip == 0 && STREAM) {
+			__builtin_nontemporal_store(w, reinterpret_cast<words_t *>(p));
+		} else if (skip == 0) {
 			*reinterpret_cast<words_t *>(p) = w;
 		} else {
 #pragma unroll
@@ -119,10 +124,11 @@ __device__ __forceinline__ float scale_of(uint32_t amax_bits)
 
 /* sum may be x or residual: a lane has read what it writes before any lane of its row writes.  group_lanes: lanes that share a
  * scale, 0: the whole row does */
-template <typename T, uint32_t V, int WAVES, int R, bool STREAM>
+template <typename T, uint32_t V, int WAVES, int R, flow_t FLOW>
 __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const T *residual, const void *__restrict__ gain,
 							      uint64_t x_pitch, uint64_t residual_pitch, uint32_t first, uint32_t width,
-							      float eps, uint32_t group_lanes, bool gain_f32, norm_out_t o)
+							      float eps, uint32_t group_lanes, bool gain_f32,
+							      norm_out_t o)
 {
 	constexpr uint32_t B = 64 * WAVES;
 	__shared__ float part[2 * WAVES];
@@ -130,12 +136,12 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 	raw_t<T, V> c[R], d[R];
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		c[k] = load_raw<STREAM, T, V>(row_at(x, x_pitch, row) + place_of<V>((k * B + threadIdx.x) * V, width).from);
+		c[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(x, x_pitch, row) + place_of<V>((k * B + threadIdx.x) * V, width).from);
 	}
 	if (residual) {
 #pragma unroll
 		for (int k = 0; k < R; k++) {
-			d[k] = load_raw<STREAM, T, V>(row_at(residual, residual_pitch, row) +
+			d[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(residual, residual_pitch, row) +
 						      place_of<V>((k * B + threadIdx.x) * V, width).from);
 		}
 	}
@@ -168,7 +174,7 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 		const uint32_t at = (k * B + threadIdx.x) * V;
 		const place_t here = place_of<V>(at, width);
 		if (o.sum && at < width) {
-			store_piece<false, T, V>(row_at(static_cast<T *>(o.sum), o.sum_pitch, row) + here.from, here.skip, v[k]);
+			store_piece<FLOW == STREAM_BOTH, T, V>(row_at(static_cast<T *>(o.sum), o.sum_pitch, row) + here.from, here.skip, v[k]);
 		}
 		float g[V];
 		load_gain<T, V>(gain, gain_f32, here.from, g);
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 			v[k][i] = v[k][i] * rstd * g[i];
 		}
 		if (o.out && at < width) {
-			store_piece<false, T, V>(row_at(static_cast<T *>(o.out), o.out_pitch, row) + here.from, here.skip, v[k]);
+			store_piece<FLOW == STREAM_BOTH, T, V>(row_at(static_cast<T *>(o.out), o.out_pitch, row) + here.from, here.skip, v[k]);
 		}
 		if (!o.q) {
 			continue;
@@ -193,7 +199,7 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 		}
 		const float scale = scale_of(max_bits_of_group(m, group_lanes));
 		if (at < width) {
-			store_q<V>(o.q + row * o.q_pitch + here.from, here.skip, v[k], 1.0f / scale);
+			store_q<FLOW == STREAM_BOTH, V>(o.q + row * o.q_pitch + here.from, here.skip, v[k], 1.0f / scale);
 			const uint32_t chunk = k * B + threadIdx.x;
 			if ((chunk & (group_lanes - 1u)) == 0) {
 				row_at(o.scale, o.scale_pitch, row)[chunk / group_lanes] = scale;
@@ -207,7 +213,7 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 			const uint32_t at = (k * B + threadIdx.x) * V;
 			const place_t here = place_of<V>(at, width);
 			if (at < width) {
-				store_q<V>(o.q + row * o.q_pitch + here.from, here.skip, v[k], 1.0f / scale);
+				store_q<FLOW == STREAM_BOTH, V>(o.q + row * o.q_pitch + here.from, here.skip, v[k], 1.0f / scale);
 			}
 		}
 		if (threadIdx.x == 0) {
@@ -216,22 +222,140 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 	}
 }
 
-/* dx = ds + rstd (g dn - h mean(g dn h)), h = s rstd; dg = sum over rows of dn h: each workgroup sums its own rows and the
- * partial sums are added up in the order of the workgroups, so that the result is the same every time.  dx may be dout or dsum:
- * a lane has read what it writes. */
-template <typename T, uint32_t V, int WAVES, int R, bool STREAM>
-__global__ __launch_bounds__(64 * WAVES) void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s,
-								   const float *__restrict__ rstds, const void *__restrict__ gain,
-								   const T *dsum, uint64_t dout_pitch, uint64_t s_pitch, uint64_t dsum_pitch,
-								   uint32_t n_rows, uint32_t width, bool gain_f32, T *dx, uint64_t dx_pitch,
-								   float *__restrict__ partial)
+/* Where the floats of a workgroup's rows are summed: each row's wavefronts, the same in all of them.  Every wavefront of the
+ * workgroup calls; s: two of these by turns. */
+template <int ROWS, int WAVES> __device__ __forceinline__ float rows_sum(float v, float (&s)[ROWS][WAVES], uint32_t y)
 {
-	constexpr uint32_t B = 64 * WAVES;
-	__shared__ float part[2][WAVES];
-	float g[R][V], dg[R][V];
+	v = sum_over<64>(v);
+	if (WAVES == 1) {
+		return v;
+	}
+	if ((threadIdx.x & 63u) == 0) {
+		s[y][threadIdx.x >> 6] = v;
+	}
+	__syncthreads();
+	v = s[y][0];
+#pragma unroll
+	for (int w = 1; w < WAVES; w++) {
+		v += s[y][w];
+	}
+	return v;
+}
+
+/*
+ * dx = ds + rstd (g dn - h mean(g dn h)), h = s rstd; dg = sum over rows of dn h: each workgroup sums its own rows and the
+ * partial sums are added up in the order of the workgroups, so that the result is the same every time.
+ *
+ * WAVES wavefronts hold a row, a chunk a lane; a workgroup has blockDim.y rows at once and asks for the next ones before it waits for
+ * the sum of these.  dx may be dout or dsum: a lane has read what it writes.
+ */
+template <typename T, uint32_t V, int WAVES, flow_t FLOW>
+__global__ __launch_bounds__(64 * (WAVES < kGradWaves ? kGradWaves : WAVES))
+void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s, const float *__restrict__ rstds, const void *__restrict__ gain,
+			  const T *dsum, uint64_t dout_pitch, uint64_t s_pitch, uint64_t dsum_pitch, uint32_t n_rows, uint32_t width,
+			  bool gain_f32, T *dx, uint64_t dx_pitch, float *__restrict__ partial)
+{
+	constexpr int ROWS = WAVES < kGradWaves ? kGradWaves / WAVES : 1;
+	__shared__ float part[2][ROWS][WAVES];
+	__shared__ float others[ROWS > 1 ? ROWS - 1 : 1][ROWS > 1 ? V : 1][64 * WAVES];
+	const uint32_t y = (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.y);
+	const place_t here = place_of<V>(threadIdx.x * V, width);
+	float g[V], dg[V];
+	load_gain<T, V>(gain, gain_f32, here.from, g);
+#pragma unroll
+	for (uint32_t i = 0; i < V; i++) {
+		dg[i] = 0.0f;
+	}
+	raw_t<T, V> dc, sc, pc;
+	float rstd = 0.0f;
+	auto ask = [&](uint64_t row) {
+		dc = load_raw<FLOW != STREAM_NONE, T, V>(row_at(dout, dout_pitch, row) + here.from);
+		sc = load_raw<FLOW != STREAM_NONE, T, V>(row_at(s, s_pitch, row) + here.from);
+		if (dsum) {
+			pc = load_raw<FLOW != STREAM_NONE, T, V>(row_at(dsum, dsum_pitch, row) + here.from);
+		}
+		rstd = rstds[row];
+	};
+	const uint64_t stride = (uint64_t)gridDim.x * blockDim.y;
+	uint64_t row = (uint64_t)blockIdx.x * blockDim.y + y;
+	if (row < n_rows) {
+		ask(row);
+	}
+	uint32_t turn = 0;
+	for (uint64_t first = (uint64_t)blockIdx.x * blockDim.y; first < n_rows; first += stride, row += stride, turn ^= 1u) {
+		const bool in = row < n_rows;
+		raw_t<T, V> p0 = pc;
+		const float r0 = rstd;
+		float d[V], h[V], along = 0.0f;
+		if (in) {
+			to_floats<T, V>(dc, here.skip, d);
+			to_floats<T, V>(sc, here.skip, h);
+#pragma unroll
+			for (uint32_t i = 0; i < V; i++) {
+				h[i] *= r0;
+				dg[i] = __builtin_fmaf(d[i], h[i], dg[i]);
+				d[i] *= g[i];
+				along = i < here.skip ? along : __builtin_fmaf(d[i], h[i], along);
+			}
+			if (row + stride < n_rows) {
+				ask(row + stride);
+			}
+		}
+		const float mean = rows_sum<ROWS, WAVES>(along, part[turn], y) / (float)width;
+		if (in && threadIdx.x * V < width) {
+			float r[V];
+#pragma unroll
+			for (uint32_t i = 0; i < V; i++) {
+				r[i] = 0.0f;
+			}
+			if (dsum) {
+				to_floats<T, V>(p0, 0, r);
+			}
+#pragma unroll
+			for (uint32_t i = 0; i < V; i++) {
+				r[i] = __builtin_fmaf(r0, __builtin_fmaf(-h[i], mean, d[i]), r[i]);
+			}
+			store_piece<FLOW == STREAM_BOTH, T, V>(row_at(dx, dx_pitch, row) + here.from, here.skip, r);
+		}
+	}
+	if (!partial) {
+		return;
+	}
+	if (ROWS > 1 && blockDim.y > 1) {
+		if (y > 0) {
+#pragma unroll
+			for (uint32_t i = 0; i < V; i++) {
+				others[y - 1][i][threadIdx.x] = dg[i];
+			}
+		}
+		__syncthreads();
+		if (y > 0) {
+			return;
+		}
+		for (uint32_t o = 0; o + 1 < blockDim.y; o++) {
+#pragma unroll
+			for (uint32_t i = 0; i < V; i++) {
+				dg[i] += others[o][i][threadIdx.x];
+			}
+		}
+	}
+	if (threadIdx.x * V < width) {
+		store_floats<V>(partial + (uint64_t)blockIdx.x * width + here.from, here.skip, dg);
+	}
+}
+
+/* The same for rows of more than 1024 chunks, which the registers do not hold beside the sums: read once for the mean, and once more,
+ * out of the caches, for the rest.  (s is not restricted: nothing of the first reading is to be kept.) */
+template <typename T, uint32_t V, int R>
+__global__ __launch_bounds__(1024) void rms_norm_grad_wide_kernel(const T *dout, const T *s, const float *__restrict__ rstds,
+								  const void *__restrict__ gain, const T *dsum, uint64_t dout_pitch,
+								  uint64_t s_pitch, uint64_t dsum_pitch, uint32_t n_rows, uint32_t width,
+								  bool gain_f32, T *dx, uint64_t dx_pitch, float *__restrict__ partial)
+{
+	__shared__ float part[2][1][16];
+	float dg[R][V];
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		load_gain<T, V>(gain, gain_f32, place_of<V>((k * B + threadIdx.x) * V, width).from, g[k]);
 #pragma unroll
 		for (uint32_t i = 0; i < V; i++) {
 			dg[k][i] = 0.0f;
@@ -239,65 +363,53 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_grad_kernel(const T *dout
 	}
 	uint32_t turn = 0;
 	for (uint64_t row = blockIdx.x; row < n_rows; row += gridDim.x, turn ^= 1u) {
-		raw_t<T, V> dc[R], sc[R], pc[R];
-#pragma unroll
-		for (int k = 0; k < R; k++) {
-			const uint32_t from = place_of<V>((k * B + threadIdx.x) * V, width).from;
-			dc[k] = load_raw<STREAM, T, V>(row_at(dout, dout_pitch, row) + from);
-			sc[k] = load_raw<STREAM, T, V>(row_at(s, s_pitch, row) + from);
-		}
-		if (dsum) {
-#pragma unroll
-			for (int k = 0; k < R; k++) {
-				pc[k] = load_raw<STREAM, T, V>(row_at(dsum, dsum_pitch, row) +
-							       place_of<V>((k * B + threadIdx.x) * V, width).from);
-			}
-		}
+		const T *dr = row_at(dout, dout_pitch, row), *sr = row_at(s, s_pitch, row);
 		const float rstd = rstds[row];
-		float d[R][V], h[R][V], along = 0.0f;
-#pragma unroll
+		float along = 0.0f;
+#pragma unroll 2
 		for (int k = 0; k < R; k++) {
-			const uint32_t skip = place_of<V>((k * B + threadIdx.x) * V, width).skip;
-			to_floats<T, V>(dc[k], skip, d[k]);
-			to_floats<T, V>(sc[k], skip, h[k]);
+			const place_t here = place_of<V>((k * 1024 + threadIdx.x) * V, width);
+			float g[V], d[V], h[V];
+			to_floats<T, V>(load_raw<false, T, V>(dr + here.from), here.skip, d);
+			to_floats<T, V>(load_raw<false, T, V>(sr + here.from), here.skip, h);
+			load_gain<T, V>(gain, gain_f32, here.from, g);
 #pragma unroll
 			for (uint32_t i = 0; i < V; i++) {
-				h[k][i] *= rstd;
-				dg[k][i] = __builtin_fmaf(d[k][i], h[k][i], dg[k][i]);
-				d[k][i] *= g[k][i];
-				along = i < skip ? along : __builtin_fmaf(d[k][i], h[k][i], along);
+				along = i < here.skip ? along : __builtin_fmaf(d[i] * g[i], h[i] * rstd, along);
 			}
 		}
-		const float mean = block_sum<WAVES>(along, part[turn]) / (float)width;
+		const float mean = rows_sum<1, 16>(along, part[turn], 0) / (float)width;
 #pragma unroll
 		for (int k = 0; k < R; k++) {
-			const uint32_t at = (k * B + threadIdx.x) * V;
-			const place_t here = place_of<V>(at, width);
+			const uint32_t at = (k * 1024 + threadIdx.x) * V;
 			if (at < width) {
-				float r[V];
+				const place_t here = place_of<V>(at, width);
+				float g[V], d[V], h[V], r[V];
+				to_floats<T, V>(load_raw<false, T, V>(dr + here.from), here.skip, d);
+				to_floats<T, V>(load_raw<false, T, V>(sr + here.from), here.skip, h);
+				load_gain<T, V>(gain, gain_f32, here.from, g);
 #pragma unroll
 				for (uint32_t i = 0; i < V; i++) {
 					r[i] = 0.0f;
 				}
 				if (dsum) {
-					to_floats<T, V>(pc[k], 0, r);
+					to_floats<T, V>(load_raw<false, T, V>(row_at(dsum, dsum_pitch, row) + here.from), 0, r);
 				}
 #pragma unroll
 				for (uint32_t i = 0; i < V; i++) {
-					r[i] = __builtin_fmaf(rstd, __builtin_fmaf(-h[k][i], mean, d[k][i]), r[i]);
+					h[i] *= rstd;
+					dg[k][i] = __builtin_fmaf(d[i], h[i], dg[k][i]);
+					r[i] = __builtin_fmaf(rstd, __builtin_fmaf(-h[i], mean, d[i] * g[i]), r[i]);
 				}
 				store_piece<false, T, V>(row_at(dx, dx_pitch, row) + here.from, here.skip, r);
 			}
 		}
 	}
-	if (!partial) {
-		return;
-	}
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		const uint32_t at = (k * B + threadIdx.x) * V;
-		const place_t here = place_of<V>(at, width);
-		if (at < width) {
+		const uint32_t at = (k * 1024 + threadIdx.x) * V;
+		if (partial && at < width) {
+			const place_t here = place_of<V>(at, width);
 			store_floats<V>(partial + (uint64_t)blockIdx.x * width + here.from, here.skip, dg[k]);
 		}
 	}
@@ -328,8 +440,7 @@ __global__ __launch_bounds__(64 * kGainWaves) void rms_norm_gain_kernel(const fl
 	}
 }
 
-constexpr uint32_t kGradBlocks = 512;
-/* Workgroups of the gradient: each reads and writes a row at a time */
+/* Workgroups of the gradient */
 inline uint32_t grad_blocks(uint32_t n_rows)
 {
 	return n_rows < kGradBlocks ? n_rows : kGradBlocks;
@@ -398,7 +509,9 @@ int ofi_amd_rms_norm(const void *d_x, uint64_t x_pitch, const void *d_residual, 
 		return -EINVAL;
 	}
 	const norm_out_t o = { d_sum, sum_pitch, d_out, out_pitch, static_cast<uint8_t *>(d_q), q_pitch, d_scale, scale_pitch, d_rstd };
-	const bool stream_rows = on_chunks(d_x, x_pitch) && on_chunks(d_residual, residual_pitch);
+	const flow_t flow = flow_of(n_rows * (bytes * (1u + !!d_residual + !!d_sum + !!d_out) + (d_q ? width : 0)),
+				    on_chunks(d_x, x_pitch) && on_chunks(d_residual, residual_pitch) && on_chunks(d_sum, sum_pitch) &&
+					    on_chunks(d_out, out_pitch) && on_chunks(d_q, q_pitch));
 	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
 		constexpr uint32_t V = decltype(v)::value;
@@ -406,7 +519,7 @@ int ofi_amd_rms_norm(const void *d_x, uint64_t x_pitch, const void *d_residual, 
 		with_row_shape<V>((width + V - 1) / V, [&](auto waves, auto r) {
 			constexpr int W = decltype(waves)::value, R = decltype(r)::value;
 			for (uint32_t first = 0; first < n_rows; first += kRowsOfLaunch) {
-				launch_kernel(stream_rows ? rms_norm_kernel<T, V, W, R, true> : rms_norm_kernel<T, V, W, R, false>,
+				launch_kernel(by_flow(flow, rms_norm_kernel<T, V, W, R, STREAM_NONE>, rms_norm_kernel<T, V, W, R, STREAM_LOADS>, rms_norm_kernel<T, V, W, R, STREAM_BOTH>),
 					      dim3(n_rows - first < kRowsOfLaunch ? n_rows - first : kRowsOfLaunch), dim3(64 * W), 0,
 					      as_stream(stream), static_cast<const T *>(d_x), static_cast<const T *>(d_residual), d_gain, x_pitch,
 					      residual_pitch, first, width, eps, group_lanes, gain_type == OFI_AMD_FLOAT32, o);
@@ -450,17 +563,43 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
 	const uint32_t blocks = grad_blocks(n_rows);
 	float *partial = d_dgain ? static_cast<float *>(d_work) : nullptr;
 	if (n_rows != 0) {
-		const bool stream_rows = on_chunks(d_dout, dout_pitch) && on_chunks(d_s, s_pitch) && on_chunks(d_dsum, dsum_pitch);
+		const flow_t flow = flow_of(n_rows * bytes * (3u + !!d_dsum), on_chunks(d_dout, dout_pitch) && on_chunks(d_s, s_pitch) &&
+											      on_chunks(d_dsum, dsum_pitch) && on_chunks(d_dx, dx_pitch));
 		with_row_type(type, width, [&](auto element, auto v) {
 			using T = decltype(element);
 			constexpr uint32_t V = decltype(v)::value;
-			with_row_shape<V>((width + V - 1) / V, [&](auto waves, auto r) {
-				constexpr int W = decltype(waves)::value, R = decltype(r)::value;
-				launch_kernel(stream_rows ? rms_norm_grad_kernel<T, V, W, R, true> : rms_norm_grad_kernel<T, V, W, R, false>,
-					      dim3(blocks), dim3(64 * W), 0, as_stream(stream), static_cast<const T *>(d_dout),
+			auto launch = [&](auto kernel, dim3 block) {
+				launch_kernel(kernel, dim3(blocks), block, 0, as_stream(stream), static_cast<const T *>(d_dout),
 					      static_cast<const T *>(d_s), d_rstd, d_gain, static_cast<const T *>(d_dsum), dout_pitch, s_pitch,
 					      dsum_pitch, n_rows, width, gain_type == OFI_AMD_FLOAT32, static_cast<T *>(d_dx), dx_pitch, partial);
-			});
+			};
+			auto rows = [&](auto waves) {
+				/* rows of a workgroup at once, but one where more would leave workgroups without any */
+				constexpr uint32_t W = decltype(waves)::value, most = W < (uint32_t)kGradWaves ? kGradWaves / W : 1;
+				const uint32_t each = (n_rows + kGradBlocks - 1) / kGradBlocks;
+				launch(by_flow(flow, rms_norm_grad_kernel<T, V, W, STREAM_NONE>, rms_norm_grad_kernel<T, V, W, STREAM_LOADS>, rms_norm_grad_kernel<T, V, W, STREAM_BOTH>),
+				       dim3(64 * W, each < most ? each : most));
+			};
+			const uint32_t chunks = (width + V - 1) / V;
+			if constexpr (V == 1) {
+				rows(std::integral_constant<uint32_t, 1>{});
+			} else if (chunks <= 64) {
+				rows(std::integral_constant<uint32_t, 1>{});
+			} else if (chunks <= 128) {
+				rows(std::integral_constant<uint32_t, 2>{});
+			} else if (chunks <= 256) {
+				rows(std::integral_constant<uint32_t, 4>{});
+			} else if (chunks <= 512) {
+				rows(std::integral_constant<uint32_t, 8>{});
+			} else if (chunks <= 1024) {
+				rows(std::integral_constant<uint32_t, 16>{});
+			} else if (chunks <= 2048) {
+				launch(rms_norm_grad_wide_kernel<T, V, 2>, dim3(1024));
+			} else if (V == 8 || chunks <= 4096) {
+				launch(rms_norm_grad_wide_kernel<T, V, 4>, dim3(1024));
+			} else {
+				launch(rms_norm_grad_wide_kernel<T, V, V == 4 ? 8 : 4>, dim3(1024));
+			}
 		});
 	}
 	if (d_dgain) { /* of no rows: zeros */

@@ -8,6 +8,7 @@
 #include "common.hpp"
 #include "ofi_amd_hotpath.h"
 #include "row_types.hpp"
+#include <cstdlib>
 
 namespace {
 
@@ -20,7 +21,7 @@ constexpr uint32_t kAtOnce = 8; /* rows of a token that are read together */
 
 /* A workgroup of threadIdx.x lanes along a row and threadIdx.y tokens; each lane one chunk of the output at a time.  Up to kAtOnce
  * rows are asked for before the first is used. */
-template <typename T, uint32_t V, bool STREAM>
+template <typename T, uint32_t V, flow_t FLOW>
 __global__ __launch_bounds__(64 * kMostWaves) void token_combine_kernel(const int32_t *__restrict__ row_of,
 									const float *__restrict__ weight, const T *__restrict__ rows,
 									const T *add, T *out, uint64_t rows_pitch, uint64_t add_pitch,
@@ -37,7 +38,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_kernel(const in
 		const place_t here = place_of<V>(at, width);
 		raw_t<T, V> first;
 		if (add) {
-			first = load_raw<STREAM, T, V>(row_at(add, add_pitch, token) + here.from);
+			first = load_raw<FLOW != STREAM_NONE, T, V>(row_at(add, add_pitch, token) + here.from);
 		}
 		float sum[V];
 #pragma unroll
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_kernel(const in
 #pragma unroll
 			for (uint32_t k = 0; k < kAtOnce; k++) {
 				if (row[k] < max_rows) {
-					c[k] = load_raw<STREAM, T, V>(row_at(rows, rows_pitch, row[k]) + here.from);
+					c[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(rows, rows_pitch, row[k]) + here.from);
 				}
 			}
 			if (k0 == 0 && add) {
@@ -73,13 +74,13 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_kernel(const in
 				}
 			}
 		}
-		store_piece<false, T, V>(row_at(out, out_pitch, token) + here.from, here.skip, sum);
+		store_piece<FLOW == STREAM_BOTH, T, V>(row_at(out, out_pitch, token) + here.from, here.skip, sum);
 	}
 }
 
 /* One workgroup of `waves` wavefronts per token.  All rows that are read together are asked for before the first is written, so
  * that drows may be rows. */
-template <typename T, uint32_t V, bool STREAM>
+template <typename T, uint32_t V, flow_t FLOW>
 __global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(const int32_t *__restrict__ row_of,
 									     const float *__restrict__ weight,
 									     const T *__restrict__ dout, const T *rows, T *drows,
@@ -105,13 +106,13 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(con
 		}
 		for (uint32_t at = threadIdx.x * V; at < width; at += blockDim.x * V) {
 			const place_t here = place_of<V>(at, width);
-			const raw_t<T, V> dc = load_raw<STREAM, T, V>(dr + here.from);
+			const raw_t<T, V> dc = load_raw<FLOW != STREAM_NONE, T, V>(dr + here.from);
 			raw_t<T, V> c[kAtOnce];
 			if (dweight) {
 #pragma unroll
 				for (uint32_t k = 0; k < kAtOnce; k++) {
 					if (row[k] < max_rows) {
-						c[k] = load_raw<STREAM, T, V>(row_at(rows, rows_pitch, row[k]) + here.from);
+						c[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(rows, rows_pitch, row[k]) + here.from);
 					}
 				}
 			}
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(con
 						for (uint32_t i = 0; i < V; i++) {
 							f[i] = w[k] * d[i];
 						}
-						store_piece<STREAM, T, V>(row_at(drows, drows_pitch, row[k]) + here.from, here.skip, f);
+						store_piece<FLOW == STREAM_BOTH, T, V>(row_at(drows, drows_pitch, row[k]) + here.from, here.skip, f);
 					}
 				}
 			}
@@ -217,14 +218,16 @@ int ofi_amd_token_combine(const void *d_rows, uint64_t rows_pitch, uint32_t max_
 	    (d_add && !rows_ok(d_add, add_pitch, n_tokens, bytes, size)) || !rows_ok(d_out, out_pitch, n_tokens, bytes, size)) {
 		return -EINVAL;
 	}
-	const bool stream_rows = on_chunks(d_rows, rows_pitch) && on_chunks(d_add, add_pitch);
+	const uint64_t pairs = (uint64_t)n_tokens * top_k, named = pairs < max_rows ? pairs : max_rows;
+	const flow_t flow = flow_of((named + n_tokens * (1ull + !!d_add)) * bytes,
+				    on_chunks(d_rows, rows_pitch) && on_chunks(d_add, add_pitch) && on_chunks(d_out, out_pitch));
 	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
 		constexpr uint32_t V = decltype(v)::value;
 		const uint32_t waves = row_waves((width + V - 1) / V), tokens = waves < 4 ? 4 / waves : 1;
 		for (uint32_t at = 0; at < n_tokens; at += kTokensOfLaunch) {
 			const uint32_t n = n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch;
-			launch_kernel(stream_rows ? token_combine_kernel<T, V, true> : token_combine_kernel<T, V, false>,
+			launch_kernel(by_flow(flow, token_combine_kernel<T, V, STREAM_NONE>, token_combine_kernel<T, V, STREAM_LOADS>, token_combine_kernel<T, V, STREAM_BOTH>),
 				      dim3((n + tokens - 1) / tokens), dim3(64 * waves, tokens), 0, as_stream(stream),
 				      d_row_of + (uint64_t)at * top_k, d_weight ? d_weight + (uint64_t)at * top_k : nullptr,
 				      static_cast<const T *>(d_rows), d_add ? row_at(static_cast<const T *>(d_add), add_pitch, at) : nullptr,
@@ -255,13 +258,15 @@ int ofi_amd_token_combine_grad(const void *d_dout, uint64_t dout_pitch, const vo
 			       (d_drows && !rows_ok(d_drows, drows_pitch, max_rows, bytes, size))))) {
 		return -EINVAL;
 	}
-	const bool stream_rows = on_chunks(d_rows, rows_pitch) && on_chunks(d_drows, drows_pitch) && on_chunks(d_dout, dout_pitch);
+	const uint64_t pairs = (uint64_t)n_tokens * top_k, named = pairs < max_rows ? pairs : max_rows;
+	const flow_t flow = flow_of((named * (!!d_dweight + !!d_drows) + n_tokens) * bytes,
+				    on_chunks(d_rows, rows_pitch) && on_chunks(d_drows, drows_pitch) && on_chunks(d_dout, dout_pitch));
 	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
 		constexpr uint32_t V = decltype(v)::value;
 		const uint32_t waves = row_waves((width + V - 1) / V);
 		for (uint32_t at = 0; at < n_tokens; at += kTokensOfLaunch) {
-			launch_kernel(stream_rows ? token_combine_grad_kernel<T, V, true> : token_combine_grad_kernel<T, V, false>,
+			launch_kernel(by_flow(flow, token_combine_grad_kernel<T, V, STREAM_NONE>, token_combine_grad_kernel<T, V, STREAM_LOADS>, token_combine_grad_kernel<T, V, STREAM_BOTH>),
 				      dim3(n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch), dim3(64 * waves), 0,
 				      as_stream(stream), d_row_of + (uint64_t)at * top_k,
 				      d_weight ? d_weight + (uint64_t)at * top_k : nullptr,

@@ -23,7 +23,7 @@ constexpr uint32_t kMostRounds = 8; /* pairs of a lane of the sort */
 constexpr uint32_t kManyTiles = 32;
 
 /* A workgroup of the sort has 1024 pairs a round; tiles get more rounds before they get many.  Everybody adds up the counts of all
- * tiles, 8 at a time, so that 32 tiles of 8 rounds cost less than 256 of one. */
+ * tiles, 32 at a time, so that 32 tiles of 8 rounds cost less than 256 of one. */
 inline uint32_t rounds_of(uint64_t n_pairs)
 {
 	const uint64_t one = 64 * kSortWaves;
@@ -98,11 +98,17 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 	static_assert(kMaxExperts <= 64 * kSortWaves, "one expert a lane");
 	uint32_t total = 0, mine = 0;
 	if (n_tiles > 1 && threadIdx.x < n_experts) {
-#pragma unroll 8
-		for (uint32_t t = 0; t < n_tiles; t++) {
-			const uint32_t c = counts[(uint64_t)t * n_experts + threadIdx.x];
-			mine += t < tile ? c : 0u;
-			total += c;
+		for (uint32_t t0 = 0; t0 < n_tiles; t0 += kManyTiles) {
+			uint32_t c[kManyTiles];
+#pragma unroll
+			for (uint32_t t = 0; t < kManyTiles; t++) {
+				c[t] = counts[(uint64_t)min(t0 + t, n_tiles - 1) * n_experts + threadIdx.x];
+			}
+#pragma unroll
+			for (uint32_t t = 0; t < kManyTiles; t++) {
+				mine += t0 + t < tile ? c[t] : 0u;
+				total += t0 + t < n_tiles ? c[t] : 0u;
+			}
 		}
 	}
 	for (uint32_t i = threadIdx.x; i < kSortWaves * stride; i += 64 * kSortWaves) {
@@ -111,17 +117,24 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 	__syncthreads();
 	const uint32_t bits = 32u - (uint32_t)__builtin_clz(n_experts);
 	uint32_t *own = next + wave * stride;
+	uint64_t same[ROUNDS]; /* lanes with this lane's expert; the rounds beside each other, as each bit waits for its ballot */
+#pragma unroll
+	for (uint32_t i = 0; i < ROUNDS; i++) {
+		same[i] = ~0ull;
+	}
+	for (uint32_t b = 0; b < bits; b++) {
+#pragma unroll
+		for (uint32_t i = 0; i < ROUNDS; i++) {
+			const uint32_t one = 0u - ((known_expert(ids[i], n_experts) >> b) & 1u);
+			const uint64_t ones = __ballot(one);
+			same[i] &= ~(ones ^ ((uint64_t)one << 32 | one));
+		}
+	}
 	uint32_t rank[ROUNDS];
 #pragma unroll
 	for (uint32_t i = 0; i < ROUNDS; i++) {
-		const uint32_t e = known_expert(ids[i], n_experts);
-		uint64_t same = ~0ull; /* lanes with this lane's expert */
-		for (uint32_t b = 0; b < bits; b++) {
-			const uint32_t one = 0u - ((e >> b) & 1u);
-			const uint64_t ones = __ballot(one);
-			same &= ~(ones ^ ((uint64_t)one << 32 | one));
-		}
-		const uint32_t below = lanes_below(same), of = (uint32_t)__popcll(same), before = own[e];
+		const uint32_t e = known_expert(ids[i], n_experts), before = own[e];
+		const uint32_t below = lanes_below(same[i]), of = (uint32_t)__popcll(same[i]);
 		rank[i] = before + below;
 		__builtin_amdgcn_wave_barrier(); /* every lane has read before the last of an expert's lanes writes */
 		if (below == of - 1u) {
