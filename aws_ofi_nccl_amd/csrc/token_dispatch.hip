@@ -20,7 +20,8 @@ constexpr uint32_t kMaxRowBytes = 1u << 24;
 constexpr uint32_t kTokensOfLaunch = 1u << 22;
 constexpr int kSortWaves = 16;
 constexpr uint32_t kMostRounds = 8; /* pairs of a lane of the sort */
-constexpr uint32_t kManyTiles = 32;
+constexpr uint32_t kManyTiles = 64;
+constexpr uint32_t kTilesAtOnce = 32;
 
 /* A workgroup of the sort has 1024 pairs a round; tiles get more rounds before they get many.  Everybody adds up the counts of all
  * tiles, 32 at a time, so that 32 tiles of 8 rounds cost less than 256 of one. */
@@ -98,14 +99,14 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 	static_assert(kMaxExperts <= 64 * kSortWaves, "one expert a lane");
 	uint32_t total = 0, mine = 0;
 	if (n_tiles > 1 && threadIdx.x < n_experts) {
-		for (uint32_t t0 = 0; t0 < n_tiles; t0 += kManyTiles) {
-			uint32_t c[kManyTiles];
+		for (uint32_t t0 = 0; t0 < n_tiles; t0 += kTilesAtOnce) {
+			uint32_t c[kTilesAtOnce];
 #pragma unroll
-			for (uint32_t t = 0; t < kManyTiles; t++) {
+			for (uint32_t t = 0; t < kTilesAtOnce; t++) {
 				c[t] = counts[(uint64_t)min(t0 + t, n_tiles - 1) * n_experts + threadIdx.x];
 			}
 #pragma unroll
-			for (uint32_t t = 0; t < kManyTiles; t++) {
+			for (uint32_t t = 0; t < kTilesAtOnce; t++) {
 				mine += t0 + t < tile ? c[t] : 0u;
 				total += t0 + t < n_tiles ? c[t] : 0u;
 			}
