@@ -17,6 +17,7 @@ namespace {
 using namespace ofi_amd;
 
 constexpr uint32_t kMaxWidth = 32768;
+constexpr int kMostWaves = 16;
 constexpr int kGradWaves = 8;
 constexpr uint32_t kGradBlocks = 512;
 constexpr uint32_t kRowsOfLaunch = 1u << 21; /* with 1024 lanes each within the 32 bits of a launch's size */
@@ -122,34 +123,40 @@ __device__ __forceinline__ float scale_of(uint32_t amax_bits)
 	return s < 0x1p-126f ? 0x1p-126f : s;
 }
 
-/* sum may be x or residual: a lane has read what it writes before any lane of its row writes.  group_lanes: lanes that share a
- * scale, 0: the whole row does */
-template <typename T, uint32_t V, int WAVES, int R, flow_t FLOW>
-__global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const T *residual, const void *__restrict__ gain,
-							      uint64_t x_pitch, uint64_t residual_pitch, uint32_t first, uint32_t width,
-							      float eps, uint32_t group_lanes, bool gain_f32,
-							      norm_out_t o)
+/*
+ * A row is held by the LANES lanes of a part of a wavefront, or (LANES 64) by the wavefronts along x, R chunks a lane.  sum may be x or
+ * residual: a lane has read what it writes before any lane of its row writes.  group_lanes: lanes that share a scale, 0: the
+ * whole row does.
+ */
+template <typename T, uint32_t V, int R, int LANES, flow_t FLOW>
+__global__ __launch_bounds__(64 * kMostWaves) void rms_norm_kernel(const T *x, const T *residual, const void *__restrict__ gain,
+								   uint64_t x_pitch, uint64_t residual_pitch, uint32_t first,
+								   uint32_t n_rows, uint32_t width, float eps, uint32_t group_lanes,
+								   bool gain_f32, norm_out_t o)
 {
-	constexpr uint32_t B = 64 * WAVES;
-	__shared__ float part[2 * WAVES];
-	const uint64_t row = first + blockIdx.x;
+	const uint32_t B = LANES < 64 ? LANES : blockDim.x, waves = LANES < 64 ? 1 : blockDim.x >> 6;
+	const uint32_t lane = LANES < 64 ? threadIdx.x & (LANES - 1) : threadIdx.x;
+	__shared__ uint32_t part[2][LANES < 64 ? 1 : kMostWaves];
+	const uint32_t wanted = LANES < 64 ? first + (blockIdx.x * blockDim.x + threadIdx.x) / LANES : first + blockIdx.x;
+	const bool in = LANES == 64 || wanted < n_rows;
+	const uint64_t row = in ? wanted : n_rows - 1;
 	raw_t<T, V> c[R], d[R];
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		c[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(x, x_pitch, row) + place_of<V>((k * B + threadIdx.x) * V, width).from);
+		c[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(x, x_pitch, row) + place_of<V>((k * B + lane) * V, width).from);
 	}
 	if (residual) {
 #pragma unroll
 		for (int k = 0; k < R; k++) {
 			d[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(residual, residual_pitch, row) +
-						      place_of<V>((k * B + threadIdx.x) * V, width).from);
+								   place_of<V>((k * B + lane) * V, width).from);
 		}
 	}
 	float v[R][V];
 	float squares = 0.0f;
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		const uint32_t skip = place_of<V>((k * B + threadIdx.x) * V, width).skip;
+		const uint32_t skip = place_of<V>((k * B + lane) * V, width).skip;
 		to_floats<T, V>(c[k], skip, v[k]);
 		if (residual) {
 			float f[V];
@@ -164,16 +171,18 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 			squares = __builtin_fmaf(v[k][i], v[k][i], squares);
 		}
 	}
-	const float rstd = 1.0f / __builtin_sqrtf(block_sum<WAVES>(squares, part) / (float)width + eps);
-	if (o.rstd && threadIdx.x == 0) {
+	squares = LANES < 64 ? sum_over<LANES>(squares) : block_sum(squares, part[0], waves);
+	const float rstd = 1.0f / __builtin_sqrtf(squares / (float)width + eps);
+	if (o.rstd && in && lane == 0) {
 		o.rstd[row] = rstd;
 	}
 	uint32_t most = 0;
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		const uint32_t at = (k * B + threadIdx.x) * V;
+		const uint32_t at = (k * B + lane) * V;
 		const place_t here = place_of<V>(at, width);
-		if (o.sum && at < width) {
+		const bool mine = in && at < width;
+		if (o.sum && mine) {
 			store_piece<FLOW == STREAM_BOTH, T, V>(row_at(static_cast<T *>(o.sum), o.sum_pitch, row) + here.from, here.skip, v[k]);
 		}
 		float g[V];
@@ -182,7 +191,7 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 		for (uint32_t i = 0; i < V; i++) {
 			v[k][i] = v[k][i] * rstd * g[i];
 		}
-		if (o.out && at < width) {
+		if (o.out && mine) {
 			store_piece<FLOW == STREAM_BOTH, T, V>(row_at(static_cast<T *>(o.out), o.out_pitch, row) + here.from, here.skip, v[k]);
 		}
 		if (!o.q) {
@@ -198,67 +207,46 @@ __global__ __launch_bounds__(64 * WAVES) void rms_norm_kernel(const T *x, const 
 			continue;
 		}
 		const float scale = scale_of(max_bits_of_group(m, group_lanes));
-		if (at < width) {
+		if (mine) {
 			store_q<FLOW == STREAM_BOTH, V>(o.q + row * o.q_pitch + here.from, here.skip, v[k], 1.0f / scale);
-			const uint32_t chunk = k * B + threadIdx.x;
+			const uint32_t chunk = k * B + lane;
 			if ((chunk & (group_lanes - 1u)) == 0) {
 				row_at(o.scale, o.scale_pitch, row)[chunk / group_lanes] = scale;
 			}
 		}
 	}
 	if (o.q && group_lanes == 0) {
-		const float scale = scale_of(block_max_bits<WAVES>(most, reinterpret_cast<uint32_t *>(part) + WAVES));
+		const float scale = scale_of(LANES < 64 ? max_bits_over<LANES>(most) : block_max_bits(most, part[1], waves));
 #pragma unroll
 		for (int k = 0; k < R; k++) {
-			const uint32_t at = (k * B + threadIdx.x) * V;
+			const uint32_t at = (k * B + lane) * V;
 			const place_t here = place_of<V>(at, width);
-			if (at < width) {
+			if (in && at < width) {
 				store_q<FLOW == STREAM_BOTH, V>(o.q + row * o.q_pitch + here.from, here.skip, v[k], 1.0f / scale);
 			}
 		}
-		if (threadIdx.x == 0) {
+		if (in && lane == 0) {
 			row_at(o.scale, o.scale_pitch, row)[0] = scale;
 		}
 	}
-}
-
-/* Where the floats of a workgroup's rows are summed: each row's wavefronts, the same in all of them.  Every wavefront of the
- * workgroup calls; s: two of these by turns. */
-template <int ROWS, int WAVES> __device__ __forceinline__ float rows_sum(float v, float (&s)[ROWS][WAVES], uint32_t y)
-{
-	v = sum_over<64>(v);
-	if (WAVES == 1) {
-		return v;
-	}
-	if ((threadIdx.x & 63u) == 0) {
-		s[y][threadIdx.x >> 6] = v;
-	}
-	__syncthreads();
-	v = s[y][0];
-#pragma unroll
-	for (int w = 1; w < WAVES; w++) {
-		v += s[y][w];
-	}
-	return v;
 }
 
 /*
  * dx = ds + rstd (g dn - h mean(g dn h)), h = s rstd; dg = sum over rows of dn h: each workgroup sums its own rows and the
  * partial sums are added up in the order of the workgroups, so that the result is the same every time.
  *
- * WAVES wavefronts hold a row, a chunk a lane; a workgroup has blockDim.y rows at once and asks for the next ones before it waits for
+ * The wavefronts along x hold a row, a chunk a lane; a workgroup has blockDim.y rows at once and asks for the next ones before it waits for
  * the sum of these.  dx may be dout or dsum: a lane has read what it writes.
  */
-template <typename T, uint32_t V, int WAVES, flow_t FLOW>
-__global__ __launch_bounds__(64 * (WAVES < kGradWaves ? kGradWaves : WAVES))
+template <typename T, uint32_t V, int MOST, flow_t FLOW>
+__global__ __launch_bounds__(64 * MOST)
 void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s, const float *__restrict__ rstds, const void *__restrict__ gain,
 			  const T *dsum, uint64_t dout_pitch, uint64_t s_pitch, uint64_t dsum_pitch, uint32_t n_rows, uint32_t width,
 			  bool gain_f32, T *dx, uint64_t dx_pitch, float *__restrict__ partial)
 {
-	constexpr int ROWS = WAVES < kGradWaves ? kGradWaves / WAVES : 1;
-	__shared__ float part[2][ROWS][WAVES];
-	__shared__ float others[ROWS > 1 ? ROWS - 1 : 1][ROWS > 1 ? V : 1][64 * WAVES];
-	const uint32_t y = (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.y);
+	__shared__ uint32_t part[2][kGradWaves][kMostWaves];
+	__shared__ float others[MOST == kGradWaves ? (MOST - 1) * 64 * V : 1]; /* [row but the first][element][lane] */
+	const uint32_t waves = blockDim.x >> 6, y = (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.y);
 	const place_t here = place_of<V>(threadIdx.x * V, width);
 	float g[V], dg[V];
 	load_gain<T, V>(gain, gain_f32, here.from, g);
@@ -301,7 +289,7 @@ void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s, const float *_
 				ask(row + stride);
 			}
 		}
-		const float mean = rows_sum<ROWS, WAVES>(along, part[turn], y) / (float)width;
+		const float mean = block_sum(along, part[turn][y], waves) / (float)width;
 		if (in && threadIdx.x * V < width) {
 			float r[V];
 #pragma unroll
@@ -321,21 +309,22 @@ void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s, const float *_
 	if (!partial) {
 		return;
 	}
-	if (ROWS > 1 && blockDim.y > 1) {
+	if (MOST == kGradWaves && blockDim.y > 1) {
+		float *o = others + threadIdx.x;
 		if (y > 0) {
 #pragma unroll
 			for (uint32_t i = 0; i < V; i++) {
-				others[y - 1][i][threadIdx.x] = dg[i];
+				o[((y - 1) * V + i) * blockDim.x] = dg[i];
 			}
 		}
 		__syncthreads();
 		if (y > 0) {
 			return;
 		}
-		for (uint32_t o = 0; o + 1 < blockDim.y; o++) {
+		for (uint32_t k = 0; k + 1 < blockDim.y; k++) {
 #pragma unroll
 			for (uint32_t i = 0; i < V; i++) {
-				dg[i] += others[o][i][threadIdx.x];
+				dg[i] += o[(k * V + i) * blockDim.x];
 			}
 		}
 	}
@@ -347,12 +336,12 @@ void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s, const float *_
 /* The same for rows of more than 1024 chunks, which the registers do not hold beside the sums: read once for the mean, and once more,
  * out of the caches, for the rest.  (s is not restricted: nothing of the first reading is to be kept.) */
 template <typename T, uint32_t V, int R>
-__global__ __launch_bounds__(1024) void rms_norm_grad_wide_kernel(const T *dout, const T *s, const float *__restrict__ rstds,
+__global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(const T *dout, const T *s, const float *__restrict__ rstds,
 								  const void *__restrict__ gain, const T *dsum, uint64_t dout_pitch,
 								  uint64_t s_pitch, uint64_t dsum_pitch, uint32_t n_rows, uint32_t width,
 								  bool gain_f32, T *dx, uint64_t dx_pitch, float *__restrict__ partial)
 {
-	__shared__ float part[2][1][16];
+	__shared__ uint32_t part[2][kMostWaves];
 	float dg[R][V];
 #pragma unroll
 	for (int k = 0; k < R; k++) {
@@ -368,7 +357,7 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_wide_kernel(const T *dout,
 		float along = 0.0f;
 #pragma unroll 2
 		for (int k = 0; k < R; k++) {
-			const place_t here = place_of<V>((k * 1024 + threadIdx.x) * V, width);
+			const place_t here = place_of<V>((k * blockDim.x + threadIdx.x) * V, width);
 			float g[V], d[V], h[V];
 			to_floats<T, V>(load_raw<false, T, V>(dr + here.from), here.skip, d);
 			to_floats<T, V>(load_raw<false, T, V>(sr + here.from), here.skip, h);
@@ -378,10 +367,10 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_wide_kernel(const T *dout,
 				along = i < here.skip ? along : __builtin_fmaf(d[i] * g[i], h[i] * rstd, along);
 			}
 		}
-		const float mean = rows_sum<1, 16>(along, part[turn], 0) / (float)width;
+		const float mean = block_sum(along, part[turn], blockDim.x >> 6) / (float)width;
 #pragma unroll
 		for (int k = 0; k < R; k++) {
-			const uint32_t at = (k * 1024 + threadIdx.x) * V;
+			const uint32_t at = (k * blockDim.x + threadIdx.x) * V;
 			if (at < width) {
 				const place_t here = place_of<V>(at, width);
 				float g[V], d[V], h[V], r[V];
@@ -407,7 +396,7 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_wide_kernel(const T *dout,
 	}
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		const uint32_t at = (k * 1024 + threadIdx.x) * V;
+		const uint32_t at = (k * blockDim.x + threadIdx.x) * V;
 		if (partial && at < width) {
 			const place_t here = place_of<V>(at, width);
 			store_floats<V>(partial + (uint64_t)blockIdx.x * width + here.from, here.skip, dg[k]);
@@ -446,31 +435,32 @@ inline uint32_t grad_blocks(uint32_t n_rows)
 	return n_rows < kGradBlocks ? n_rows : kGradBlocks;
 }
 
-/* Calls f with the wavefronts of a workgroup and the chunks of a lane that hold a row of `chunks` */
-template <uint32_t V, typename F> void with_row_shape(uint32_t chunks, F f)
+/* Calls f with the chunks of a lane, at least `least`, for which a row of `chunks` has a lane of a workgroup of the most wavefronts */
+template <uint32_t V, typename F> void with_chunks_of_lane(uint32_t chunks, uint32_t least, F f)
 {
-	auto with = [&](auto waves, auto r) { f(waves, r); };
-	if constexpr (V == 1) { /* narrower than a chunk */
-		with(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+	constexpr uint32_t lanes = 64 * kMostWaves;
+	if constexpr (V == 1) {
+		f(std::integral_constant<int, 1>{});
+	} else if (chunks <= lanes && least <= 1) {
+		f(std::integral_constant<int, 1>{});
+	} else if (chunks <= 2 * lanes) {
+		f(std::integral_constant<int, 2>{});
+	} else if (V == 8 || chunks <= 4 * lanes) {
+		f(std::integral_constant<int, 4>{});
 	} else {
-		if (chunks <= 64) {
-			with(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-		} else if (chunks <= 128) {
-			with(std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{});
-		} else if (chunks <= 256) {
-			with(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
-		} else if (chunks <= 512) {
-			with(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
-		} else if (chunks <= 1024) {
-			with(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
-		} else if (chunks <= 2048) {
-			with(std::integral_constant<int, 16>{}, std::integral_constant<int, 2>{});
-		} else if (V == 8 || chunks <= 4096) {
-			with(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
-		} else {
-			with(std::integral_constant<int, 16>{}, std::integral_constant<int, V == 4 ? 8 : 4>{});
-		}
+		f(std::integral_constant<int, V == 8 ? 4 : 8>{});
 	}
+}
+
+/*
+ * Chunks of a lane of the norm.  One where the rows have no more chunks than the chip has lanes (256 units of 2048): the most
+ * wavefronts, the shortest wait.  Beyond, two: half the wavefronts for each sum.  Rows of 4096 and 8192 bfloat16 to e4m3 by us with
+ * one / two: 1 row 2.6 / 3.6 and 3.1 / 3.8; 256 rows 4.1 / 5.0 and 5.4 / 6.0; 1024 rows 8.6 / 9.3 and 14.0 / 13.5; 8192 rows
+ * 44.7 / 44.0 and 91.3 / 80.6; 16,384 rows 82.3 / 79.1 and 176 / 158 (three to four: 82.8 and 162).
+ */
+inline uint32_t least_chunks(uint32_t n_rows, uint32_t chunks)
+{
+	return chunks > 64 && (uint64_t)n_rows * chunks > (1u << 19) ? 2 : 1;
 }
 
 } // namespace
@@ -515,16 +505,29 @@ int ofi_amd_rms_norm(const void *d_x, uint64_t x_pitch, const void *d_residual, 
 	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
 		constexpr uint32_t V = decltype(v)::value;
-		const uint32_t group_lanes = V == 1 ? 0 : group / V; /* narrower rows are one group, however long it is */
-		with_row_shape<V>((width + V - 1) / V, [&](auto waves, auto r) {
-			constexpr int W = decltype(waves)::value, R = decltype(r)::value;
+		const uint32_t chunks = (width + V - 1) / V;
+		const uint32_t group_lanes = group >= width ? 0 : group / V; /* a row within one group is one */
+		auto launch = [&](auto kernel, uint32_t rows, uint32_t lanes) { /* workgroups of so many rows and lanes */
 			for (uint32_t first = 0; first < n_rows; first += kRowsOfLaunch) {
-				launch_kernel(by_flow(flow, rms_norm_kernel<T, V, W, R, STREAM_NONE>, rms_norm_kernel<T, V, W, R, STREAM_LOADS>, rms_norm_kernel<T, V, W, R, STREAM_BOTH>),
-					      dim3(n_rows - first < kRowsOfLaunch ? n_rows - first : kRowsOfLaunch), dim3(64 * W), 0,
-					      as_stream(stream), static_cast<const T *>(d_x), static_cast<const T *>(d_residual), d_gain, x_pitch,
-					      residual_pitch, first, width, eps, group_lanes, gain_type == OFI_AMD_FLOAT32, o);
+				const uint32_t n = n_rows - first < kRowsOfLaunch ? n_rows - first : kRowsOfLaunch;
+				launch_kernel(kernel, dim3((n + rows - 1) / rows), dim3(lanes), 0, as_stream(stream), static_cast<const T *>(d_x),
+					      static_cast<const T *>(d_residual), d_gain, x_pitch, residual_pitch, first, n_rows, width, eps,
+					      group_lanes, gain_type == OFI_AMD_FLOAT32, o);
 			}
-		});
+		};
+		if (chunks <= 16) {
+			launch(by_flow(flow, rms_norm_kernel<T, V, 1, 16, STREAM_NONE>, rms_norm_kernel<T, V, 1, 16, STREAM_LOADS>,
+				       rms_norm_kernel<T, V, 1, 16, STREAM_BOTH>), 16, 256);
+		} else if (chunks <= 32) {
+			launch(by_flow(flow, rms_norm_kernel<T, V, 1, 32, STREAM_NONE>, rms_norm_kernel<T, V, 1, 32, STREAM_LOADS>,
+				       rms_norm_kernel<T, V, 1, 32, STREAM_BOTH>), 8, 256);
+		} else {
+			with_chunks_of_lane<V>(chunks, least_chunks(n_rows, chunks), [&](auto r) {
+				constexpr int R = decltype(r)::value;
+				launch(by_flow(flow, rms_norm_kernel<T, V, R, 64, STREAM_NONE>, rms_norm_kernel<T, V, R, 64, STREAM_LOADS>,
+					       rms_norm_kernel<T, V, R, 64, STREAM_BOTH>), 1, (chunks + 64 * R - 1) / (64 * R) * 64);
+			});
+		}
 	});
 	OFI_AMD_HIP_TRY(hipGetLastError());
 	return 0;
@@ -573,33 +576,25 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
 					      static_cast<const T *>(d_s), d_rstd, d_gain, static_cast<const T *>(d_dsum), dout_pitch, s_pitch,
 					      dsum_pitch, n_rows, width, gain_type == OFI_AMD_FLOAT32, static_cast<T *>(d_dx), dx_pitch, partial);
 			};
-			auto rows = [&](auto waves) {
-				/* rows of a workgroup at once, but one where more would leave workgroups without any */
-				constexpr uint32_t W = decltype(waves)::value, most = W < (uint32_t)kGradWaves ? kGradWaves / W : 1;
-				const uint32_t each = (n_rows + kGradBlocks - 1) / kGradBlocks;
-				launch(by_flow(flow, rms_norm_grad_kernel<T, V, W, STREAM_NONE>, rms_norm_grad_kernel<T, V, W, STREAM_LOADS>, rms_norm_grad_kernel<T, V, W, STREAM_BOTH>),
-				       dim3(64 * W, each < most ? each : most));
-			};
-			const uint32_t chunks = (width + V - 1) / V;
-			if constexpr (V == 1) {
-				rows(std::integral_constant<uint32_t, 1>{});
-			} else if (chunks <= 64) {
-				rows(std::integral_constant<uint32_t, 1>{});
-			} else if (chunks <= 128) {
-				rows(std::integral_constant<uint32_t, 2>{});
-			} else if (chunks <= 256) {
-				rows(std::integral_constant<uint32_t, 4>{});
-			} else if (chunks <= 512) {
-				rows(std::integral_constant<uint32_t, 8>{});
-			} else if (chunks <= 1024) {
-				rows(std::integral_constant<uint32_t, 16>{});
-			} else if (chunks <= 2048) {
-				launch(rms_norm_grad_wide_kernel<T, V, 2>, dim3(1024));
-			} else if (V == 8 || chunks <= 4096) {
-				launch(rms_norm_grad_wide_kernel<T, V, 4>, dim3(1024));
-			} else {
-				launch(rms_norm_grad_wide_kernel<T, V, V == 4 ? 8 : 4>, dim3(1024));
-			}
+			const uint32_t chunks = (width + V - 1) / V, waves = (chunks + 63) / 64;
+			with_chunks_of_lane<V>(chunks, 1, [&](auto r) {
+				constexpr int R = decltype(r)::value;
+				if constexpr (R > 1) {
+					launch(rms_norm_grad_wide_kernel<T, V, R>, dim3(64 * ((waves + R - 1) / R)));
+				} else if (waves > (uint32_t)kGradWaves) {
+					launch(by_flow(flow, rms_norm_grad_kernel<T, V, kMostWaves, STREAM_NONE>,
+						       rms_norm_grad_kernel<T, V, kMostWaves, STREAM_LOADS>,
+						       rms_norm_grad_kernel<T, V, kMostWaves, STREAM_BOTH>),
+					       dim3(64 * waves));
+				} else {
+					/* rows of a workgroup at once, but one where more would leave workgroups without any */
+					const uint32_t most = kGradWaves / waves, each = (n_rows + kGradBlocks - 1) / kGradBlocks;
+					launch(by_flow(flow, rms_norm_grad_kernel<T, V, kGradWaves, STREAM_NONE>,
+						       rms_norm_grad_kernel<T, V, kGradWaves, STREAM_LOADS>,
+						       rms_norm_grad_kernel<T, V, kGradWaves, STREAM_BOTH>),
+					       dim3(64 * waves, each < most ? each : most));
+				}
+			});
 		});
 	}
 	if (d_dgain) { /* of no rows: zeros */

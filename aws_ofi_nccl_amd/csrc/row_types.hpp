@@ -145,41 +145,38 @@ template <int LANES> __device__ __forceinline__ uint32_t max_bits_over(uint32_t 
 
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-/* The same in every wavefront of a workgroup of WAVES of them; s: WAVES words of LDS that nothing else uses meanwhile */
-template <int WAVES> __device__ __forceinline__ float block_sum(float v, float *s)
+/* The value of every wavefront of a row's put together by op, in all of their lanes.  s: a word for each of up to 16 wavefronts, which
+ * nothing else uses meanwhile.  All wavefronts of the workgroup call. */
+template <typename Op> __device__ __forceinline__ uint32_t over_waves(uint32_t v, uint32_t *s, uint32_t waves, uint32_t none, Op op)
 {
-	v = sum_over<64>(v);
-	if (WAVES == 1) {
+	if (waves == 1) {
 		return v;
 	}
-	if ((threadIdx.x & 63u) == 0) {
+	const uint32_t lane = threadIdx.x & 63u;
+	if (lane == 0) {
 		s[threadIdx.x >> 6] = v;
 	}
 	__syncthreads();
-	float total = s[0];
-#pragma unroll
-	for (int w = 1; w < WAVES; w++) {
-		total += s[w];
-	}
-	return total;
+	return over_lanes<16>((lane & 15u) < waves ? s[lane & 15u] : none, op);
 }
 
-template <int WAVES> __device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t *s)
+__device__ __forceinline__ float block_sum(float v, uint32_t *s, uint32_t waves)
 {
-	v = max_bits_over<64>(v);
-	if (WAVES == 1) {
-		return v;
-	}
-	if ((threadIdx.x & 63u) == 0) {
-		s[threadIdx.x >> 6] = v;
-	}
-	__syncthreads();
-	uint32_t most = s[0];
-#pragma unroll
-	for (int w = 1; w < WAVES; w++) {
-		most = s[w] > most ? s[w] : most;
-	}
-	return most;
+	return __uint_as_float(over_waves(__float_as_uint(sum_over<64>(v)), s, waves, 0u, [](uint32_t a, uint32_t b) {
+		return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+	}));
+}
+
+__device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t *s, uint32_t waves)
+{
+	return over_waves(max_bits_over<64>(v), s, waves, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+
+/* Wavefronts that take a row of `chunks` in the fewest rounds of at most `most`, as even as they can be */
+inline uint32_t even_waves(uint32_t chunks, uint32_t most)
+{
+	const uint32_t all = (chunks + 63) / 64, rounds = (all + most - 1) / most;
+	return (all + rounds - 1) / rounds;
 }
 
 /* Bytes of an element of a row's type, 0 for a type that rows do not have */

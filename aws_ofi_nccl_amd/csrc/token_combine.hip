@@ -16,7 +16,7 @@ using namespace ofi_amd;
 
 constexpr uint32_t kMaxTopK = 64;
 constexpr uint32_t kMaxWidth = 1u << 20;
-constexpr int kMostWaves = 8;
+constexpr uint32_t kMostWaves = 8; /* a workgroup has all of a row of up to 8 KiB in flight at once */
 constexpr uint32_t kAtOnce = 8; /* rows of a token that are read together */
 
 /* A workgroup of threadIdx.x lanes along a row and threadIdx.y tokens; each lane one chunk of the output at a time.  Up to kAtOnce
@@ -173,12 +173,6 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(con
 	}
 }
 
-/* Wavefronts along a row of `chunks`: one workgroup has all of a row of up to 8 KiB in flight at once */
-inline uint32_t row_waves(uint32_t chunks)
-{
-	return chunks <= 64 ? 1 : chunks <= 128 ? 2 : chunks <= 256 ? 4 : kMostWaves;
-}
-
 constexpr uint32_t kTokensOfLaunch = 1u << 22; /* with 512 lanes each within the 32 bits of a launch's size */
 
 int check_call(uint32_t max_rows, const int32_t *d_row_of, const float *d_weight, uint32_t top_k, uint32_t width, uint32_t size,
@@ -224,10 +218,12 @@ int ofi_amd_token_combine(const void *d_rows, uint64_t rows_pitch, uint32_t max_
 	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
 		constexpr uint32_t V = decltype(v)::value;
-		const uint32_t waves = row_waves((width + V - 1) / V), tokens = waves < 4 ? 4 / waves : 1;
+		const uint32_t waves = even_waves((width + V - 1) / V, kMostWaves), tokens = waves < 4 ? 4 / waves : 1;
+		auto kernel = by_flow(flow, token_combine_kernel<T, V, STREAM_NONE>, token_combine_kernel<T, V, STREAM_LOADS>,
+				      token_combine_kernel<T, V, STREAM_BOTH>);
 		for (uint32_t at = 0; at < n_tokens; at += kTokensOfLaunch) {
 			const uint32_t n = n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch;
-			launch_kernel(by_flow(flow, token_combine_kernel<T, V, STREAM_NONE>, token_combine_kernel<T, V, STREAM_LOADS>, token_combine_kernel<T, V, STREAM_BOTH>),
+			launch_kernel(kernel,
 				      dim3((n + tokens - 1) / tokens), dim3(64 * waves, tokens), 0, as_stream(stream),
 				      d_row_of + (uint64_t)at * top_k, d_weight ? d_weight + (uint64_t)at * top_k : nullptr,
 				      static_cast<const T *>(d_rows), d_add ? row_at(static_cast<const T *>(d_add), add_pitch, at) : nullptr,
@@ -264,9 +260,11 @@ int ofi_amd_token_combine_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
 		constexpr uint32_t V = decltype(v)::value;
-		const uint32_t waves = row_waves((width + V - 1) / V);
+		const uint32_t waves = even_waves((width + V - 1) / V, kMostWaves);
+		auto kernel = by_flow(flow, token_combine_grad_kernel<T, V, STREAM_NONE>, token_combine_grad_kernel<T, V, STREAM_LOADS>,
+				      token_combine_grad_kernel<T, V, STREAM_BOTH>);
 		for (uint32_t at = 0; at < n_tokens; at += kTokensOfLaunch) {
-			launch_kernel(by_flow(flow, token_combine_grad_kernel<T, V, STREAM_NONE>, token_combine_grad_kernel<T, V, STREAM_LOADS>, token_combine_grad_kernel<T, V, STREAM_BOTH>),
+			launch_kernel(kernel,
 				      dim3(n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch), dim3(64 * waves), 0,
 				      as_stream(stream), d_row_of + (uint64_t)at * top_k,
 				      d_weight ? d_weight + (uint64_t)at * top_k : nullptr,

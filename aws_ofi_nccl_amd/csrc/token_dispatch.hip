@@ -465,7 +465,7 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 	const rows_t b = { static_cast<const uint8_t *>(d_scale), scale_pitch, static_cast<uint8_t *>(d_scale_rows), scale_rows_pitch,
 			   scale_bytes };
 	const uint32_t spans = d_x ? (row_bytes + kSpan - 1) / kSpan : 0, more = d_scale ? 1 : 0;
-	const uint32_t row_waves = spans < kMostWaves - more ? spans : kMostWaves - more;
+	const uint32_t row_waves = d_x ? even_waves(64 * spans, kMostWaves - more) : 0;
 	auto run = [&](const auto *expert) {
 		using I = typename std::remove_cv<typename std::remove_pointer<decltype(expert)>::type>::type;
 		if (d_x && n_pairs <= kFew) {
