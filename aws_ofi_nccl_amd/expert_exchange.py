@@ -1,0 +1,260 @@
+"""One expert-parallel layer over the put path: norm into 8-bit rows, rows sorted by expert, one put per rank, experts,
+the results fetched back, weighted sums -- and the gradients of all of it.
+
+    python -m aws_ofi_nccl_amd.expert_exchange [--tokens 512] [--width 1024] [--experts 16] [--top-k 4] [--ranks 4]
+
+The operators are the library's (`ofi_amd_rms_norm`, `ofi_amd_token_dispatch`, `ofi_amd_token_combine` and their
+gradients).  The exchange goes through `ofi_amd_rma_iput` / `_iputSignal` / `_iget` over the device fabric: the ranks are
+windows of this process on one GPU, and what a rank gets is the run of sorted rows of its experts, whose place and length are
+two of the offsets.  The experts themselves, and a check of everything against the formulas, are plain torch.
+"""
+import argparse
+import ctypes
+import sys
+import time
+
+import numpy as np
+import torch
+
+import aws_ofi_nccl_amd as _m
+
+GROUP = 128          # columns that share a scale
+EPS = 1e-6
+SIGNAL_BASE = 0x7F5500000000
+SIGNAL_INC = 1
+
+
+def _ptr(t):
+    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+
+
+def _stream():
+    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _rows(t):
+    return t.data_ptr(), t.stride(0) * t.element_size()
+
+
+class Window:
+    """What one rank registers: room for `rows` sorted rows of 8 bits, their scales, and rows of results in bfloat16."""
+
+    def __init__(self, rows, width):
+        groups = -(-width // GROUP)
+        self.scale_at = -(-rows * width // 256) * 256
+        self.result_at = self.scale_at + -(-rows * groups * 4 // 256) * 256
+        self.bytes = torch.zeros(self.result_at + rows * width * 2, dtype=torch.uint8, device="cuda")
+        self.q = self.bytes[:rows * width].view(torch.float8_e4m3fn).view(rows, width)
+        self.scale = self.bytes[self.scale_at:self.scale_at + rows * groups * 4].view(torch.float32).view(rows, groups)
+        self.result = self.bytes[self.result_at:].view(torch.bfloat16).view(rows, width)
+
+
+class Link:
+    """An initiator context over the device fabric, and `ranks` windows that its puts and gets reach."""
+
+    def __init__(self, lib, ranks, rows, width):
+        self.lib, self.ranks = lib, ranks
+        self.own = Window(rows, width)
+        self.windows = [Window(rows, width) for _ in range(ranks)]
+        self.counters = torch.zeros(ranks, dtype=torch.int64, device="cuda")
+        torch.cuda.synchronize()
+        regions = (_m.GinSignalRegion * ranks)(*[_m.GinSignalRegion(SIGNAL_BASE + (r << 24), 8, self.counters[r:].data_ptr())
+                                                 for r in range(ranks)])
+        self.fabric, self.context = ctypes.c_void_p(), ctypes.c_void_p()
+        _m.check(lib.ofi_amd_devfab_create(4, 256, ranks, (ctypes.c_uint32 * ranks)(*range(ranks)), regions, ranks, _stream(),
+                                           ctypes.byref(self.fabric)), "devfab_create")
+        ops = _m.GinFabricOps()
+        _m.check(lib.ofi_amd_devfab_ops(self.fabric, ctypes.byref(ops)), "devfab_ops")
+        _m.check(lib.ofi_amd_rma_ctx_create(ranks, 4, 131072, 64, ctypes.byref(ops), 4096, 5000, ctypes.byref(self.context)),
+                 "rma_ctx_create")
+        self.on_ack = _m.DEVFAB_ACK_FN(ctypes.cast(lib.ofi_amd_rma_ack_received, ctypes.c_void_p).value)
+        _m.check(lib.ofi_amd_devfab_on_ack(self.fabric, self.on_ack, self.context), "devfab_on_ack")
+        own = self.own.bytes.data_ptr()
+        self.mr_own = self._register(own, [own] * ranks)
+        self.mr_ranks = self._register(own, [w.bytes.data_ptr() for w in self.windows])
+        self.mr_signal = self._register(SIGNAL_BASE, [SIGNAL_BASE + (r << 24) for r in range(ranks)])
+        self.requests = []
+
+    def _register(self, local, remote):
+        handle, addresses = ctypes.c_void_p(), np.array(remote, dtype=np.uint64)
+        keys = np.arange(self.ranks * 4, dtype=np.uint64) + 0x100
+        _m.check(self.lib.ofi_amd_rma_mr_create(self.context, local, addresses.ctypes.data, addresses.ctypes.data, keys.ctypes.data,
+                                                ctypes.byref(handle)), "rma_mr_create")
+        return handle
+
+    def _started(self, rc, request, what):
+        _m.check(-rc, what)
+        self.requests.append(request)
+
+    def put(self, rank, at, size):
+        request = ctypes.c_void_p()
+        self._started(self.lib.ofi_amd_rma_iput(self.context, 0, at, self.mr_own, size, at, self.mr_ranks, rank, 0,
+                                                ctypes.byref(request)), request, "rma_iput")
+
+    def put_signal(self, rank, at, size):
+        request = ctypes.c_void_p()
+        self._started(self.lib.ofi_amd_rma_iputSignal(self.context, 0, at, self.mr_own, size, at, self.mr_ranks, rank, 0,
+                                                      self.mr_signal, 1, SIGNAL_INC, True, 0, ctypes.byref(request)), request,
+                      "rma_iputSignal")
+
+    def get(self, rank, at, size):
+        request = ctypes.c_void_p()
+        self._started(self.lib.ofi_amd_rma_iget(self.context, 0, at, self.mr_ranks, size, at, self.mr_own, rank, 0,
+                                                ctypes.byref(request)), request, "rma_iget")
+
+    def finish(self):
+        """Until every operation is done and its bytes are there."""
+        done = ctypes.c_int()
+        end = time.monotonic() + 20.0
+        while self.requests:
+            _m.check(-self.lib.ofi_amd_rma_test(self.context, self.requests[0], ctypes.byref(done)), "rma_test")
+            if done.value:
+                self.requests.pop(0)
+            elif time.monotonic() > end:
+                raise RuntimeError("%d operations did not complete" % len(self.requests))
+            else:
+                _m.check(-self.lib.ofi_amd_rma_rmaProgress(self.context), "rmaProgress")
+        _m.check(self.lib.ofi_amd_devfab_quiesce(self.fabric, 0), "devfab_quiesce")
+
+    def close(self):
+        for handle in (self.mr_own, self.mr_ranks, self.mr_signal):
+            self.lib.ofi_amd_rma_mr_destroy(handle)
+        self.lib.ofi_amd_rma_ctx_destroy(self.context)
+        self.lib.ofi_amd_devfab_destroy(self.fabric)
+
+
+def dequantised(q, scale, width):
+    return (q.float() * scale.repeat_interleave(GROUP, dim=1)[:, :width])
+
+
+def experts_of(rows, up, down):
+    """A token's expert: two products with a nonlinearity between them."""
+    return torch.nn.functional.silu(rows @ up) @ down
+
+
+def layer(lib, link, x, residual, gain, ids, weight, up, down, dout=None):
+    """The layer's output (and with dout the gradients), through the library and the link."""
+    tokens, width = x.shape
+    top_k, experts, ranks = ids.shape[1], up.shape[0], link.ranks
+    pairs, groups, own = tokens * top_k, -(-width // GROUP), link.own
+    total, rstd = torch.empty_like(x), torch.empty(tokens, device="cuda")
+    q = torch.empty(tokens, width, dtype=torch.float8_e4m3fn, device="cuda")
+    scale = torch.empty(tokens, groups, device="cuda")
+    _m.check(lib.ofi_amd_rms_norm(*_rows(x), *_rows(residual), _ptr(gain), _m.BFLOAT16, tokens, width, _m.BFLOAT16, EPS, *_rows(total),
+                                  None, 0, *_rows(q), *_rows(scale), GROUP, _ptr(rstd), _stream()), "rms_norm")
+    offset = torch.empty(experts + 1, dtype=torch.int32, device="cuda")
+    row_of = torch.empty(tokens, top_k, dtype=torch.int32, device="cuda")
+    work = torch.empty(max(16, lib.ofi_amd_token_dispatch_work_bytes(tokens, top_k, experts)), dtype=torch.uint8, device="cuda")
+    _m.check(lib.ofi_amd_token_dispatch(_ptr(ids), _m.INT64, tokens, top_k, experts, pairs, _ptr(offset), _ptr(row_of), None, *_rows(q),
+                                        *_rows(own.q), width, *_rows(scale), *_rows(own.scale), groups * 4, _ptr(work), work.numel(),
+                                        _stream()), "token_dispatch")
+    first = offset.cpu().tolist()                     # where each expert's rows begin: the host plans the puts
+    bound = [r * experts // ranks for r in range(ranks + 1)]
+    runs = [(first[bound[r]], first[bound[r + 1]]) for r in range(ranks)]
+    for r, (lo, hi) in enumerate(runs):
+        if hi > lo:
+            link.put(r, own.scale_at + lo * groups * 4, (hi - lo) * groups * 4)
+            link.put_signal(r, lo * width, (hi - lo) * width)
+    link.finish()
+    inputs, outputs = [], []
+    for e, r in ((e, r) for r in range(ranks) for e in range(bound[r], bound[r + 1])):
+        w, lo, hi = link.windows[r], first[e], first[e + 1]    # each rank's own work, on what has arrived in its window
+        rows = dequantised(w.q[lo:hi], w.scale[lo:hi], width)
+        rows.requires_grad_(dout is not None)
+        y = experts_of(rows, up[e], down[e])
+        w.result[lo:hi] = y.detach().to(torch.bfloat16)
+        inputs.append(rows)
+        outputs.append(y)
+    torch.cuda.synchronize()
+    for r, (lo, hi) in enumerate(runs):
+        if hi > lo:
+            link.get(r, own.result_at + lo * width * 2, (hi - lo) * width * 2)
+    link.finish()
+    out = torch.empty_like(x)
+    _m.check(lib.ofi_amd_token_combine(*_rows(own.result), pairs, _ptr(row_of), _ptr(weight), tokens, top_k, width, _m.BFLOAT16,
+                                       *_rows(total), *_rows(out), _stream()), "token_combine")
+    got = dict(out=out, total=total, rstd=rstd, q=q, scale=scale, first=first, row_of=row_of, runs=runs)
+    if dout is None:
+        return got
+    drows, dweight = torch.zeros(pairs, width, dtype=torch.bfloat16, device="cuda"), torch.empty_like(weight)
+    _m.check(lib.ofi_amd_token_combine_grad(*_rows(dout), *_rows(own.result), pairs, _ptr(row_of), _ptr(weight), tokens, top_k, width,
+                                            _m.BFLOAT16, *_rows(drows), _ptr(dweight), _stream()), "token_combine_grad")
+    dsorted = torch.zeros_like(drows)
+    for e in range(experts):                          # the experts' own gradient
+        lo, hi = first[e], first[e + 1]
+        if hi > lo:
+            dsorted[lo:hi] = torch.autograd.grad(outputs[e], inputs[e], drows[lo:hi].float())[0].to(torch.bfloat16)
+    dnormed = torch.empty_like(x)
+    _m.check(lib.ofi_amd_token_combine(*_rows(dsorted), pairs, _ptr(row_of), None, tokens, top_k, width, _m.BFLOAT16, None, 0,
+                                       *_rows(dnormed), _stream()), "token_combine")
+    dx, dgain = torch.empty_like(x), torch.empty(width, device="cuda")
+    work = torch.empty(lib.ofi_amd_rms_norm_grad_work_bytes(tokens, width), dtype=torch.uint8, device="cuda")
+    _m.check(lib.ofi_amd_rms_norm_grad(*_rows(dnormed), *_rows(total), _ptr(rstd), _ptr(gain), _m.BFLOAT16, tokens, width, _m.BFLOAT16,
+                                       *_rows(dout), *_rows(dx), _ptr(dgain), _ptr(work), work.numel(), _stream()), "rms_norm_grad")
+    got.update(dx=dx, dgain=dgain, dweight=dweight)
+    return got
+
+
+def plain(got, x, residual, gain, ids, weight, up, down, dout):
+    """The same by torch alone in 64 bits, from the 8-bit rows that the layer sent: their rounding is passed through by gradients."""
+    width = x.shape[1]
+    s = (x.double() + residual.double()).requires_grad_(True)
+    g, w = gain.double().requires_grad_(True), weight.double().requires_grad_(True)
+    n = s / torch.sqrt((s * s).mean(dim=1, keepdim=True) + EPS) * g
+    sent = dequantised(got["q"], got["scale"], width).double()
+    n = n + (sent - n).detach()
+    out = s
+    for k in range(ids.shape[1]):
+        y = torch.zeros_like(s)
+        for e in range(up.shape[0]):
+            here = torch.nonzero(ids[:, k] == e)[:, 0]
+            y = y.index_add(0, here, experts_of(n[here], up[e].double(), down[e].double()))
+        out = out + w[:, k, None] * y
+    ds, dg, dw = torch.autograd.grad(out, (s, g, w), dout.double())
+    normed = (s / torch.sqrt((s * s).mean(dim=1, keepdim=True) + EPS) * g).detach()
+    return dict(out=out.detach(), dx=ds, dgain=dg, dweight=dw, sent_off=((sent - normed).norm() / normed.norm()).item())
+
+
+def main(argv=None):
+    ap = argparse.ArgumentParser(prog="expert_exchange", description=__doc__.splitlines()[0])
+    for name, value in (("tokens", 512), ("width", 1024), ("experts", 16), ("top-k", 4), ("ranks", 4), ("inner", 256), ("seed", 1)):
+        ap.add_argument("--" + name, type=int, default=value)
+    args = ap.parse_args(argv)
+    if not (args.tokens > 0 and args.width > 0 and 0 < args.ranks <= args.experts and 0 < args.top_k <= args.experts and args.inner > 0):
+        ap.error("sizes are positive, ranks and top-k at most as many as experts")
+    lib = _m.load()
+    _m.check(lib.ofi_amd_gpu_init(), "ofi_amd_gpu_init")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(args.seed)
+    normal = lambda *shape: torch.randn(*shape, generator=g, device="cuda")
+    x, residual, dout = (normal(args.tokens, args.width).to(torch.bfloat16) for _ in range(3))
+    gain = (1 + 0.1 * normal(args.width)).to(torch.bfloat16)
+    top, ids = torch.topk(normal(args.tokens, args.experts), args.top_k, dim=1)
+    weight = torch.softmax(top, dim=1).contiguous()
+    up = normal(args.experts, args.width, args.inner) / args.width ** 0.5
+    down = normal(args.experts, args.inner, args.width) / args.inner ** 0.5
+    link = Link(lib, args.ranks, args.tokens * args.top_k, args.width)
+    try:
+        for _ in range(2):
+            began = time.perf_counter()
+            got = layer(lib, link, x, residual, gain, ids, weight, up, down, dout)
+            torch.cuda.synchronize()
+            took = time.perf_counter() - began
+        arrived = link.counters.cpu().tolist()
+    finally:
+        link.close()
+    want = plain(got, x, residual, gain, ids, weight, up, down, dout)
+    off = {k: ((got[k].double() - want[k]).norm() / want[k].norm()).item() for k in ("out", "dx", "dgain", "dweight")}
+    print("%d tokens x %d choices -> %d rows to %d ranks, signals %s, forward and backward %.2f ms" % (
+        args.tokens, args.top_k, got["first"][-1], args.ranks, arrived, took * 1e3))
+    print("off from the formulas in 64 bits: " + ", ".join("%s %.2g" % kv for kv in off.items()) +
+          "; 8-bit rows off from the norm: %.2g" % want["sent_off"])
+    # bfloat16 results: a rounding (2^-8 of a value at most) of each of the few tensors on the way; e4m3: half a step of 2^-4
+    ok = all(v < 0.015 for v in off.values()) and want["sent_off"] < 0.04 and all(
+        n == (2 if hi > lo else 0) for n, (lo, hi) in zip(arrived, got["runs"]))
+    print("ok" if ok else "DIFFERS")
+    return 0 if ok else 1
+
+
+if __name__ == "__main__":
+    sys.exit(main())
