@@ -404,26 +404,32 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(con
 	}
 }
 
-/* 64 columns of a workgroup, its wavefronts at the parts by turns */
-constexpr int kGainWaves = 16;
-__global__ __launch_bounds__(64 * kGainWaves) void rms_norm_gain_kernel(const float *__restrict__ partial, float *__restrict__ dgain,
-									uint32_t parts, uint32_t width)
+/* kGainColumns columns of a workgroup, its lanes at the parts by turns, with all of their loads on the way at once */
+constexpr uint32_t kGainColumns = 32, kGainTurns = 1024 / kGainColumns, kPartsOfLane = kGradBlocks / kGainTurns;
+static_assert(kGradBlocks % kGainTurns == 0, "all parts are added");
+__global__ __launch_bounds__(1024) void rms_norm_gain_kernel(const float *__restrict__ partial, float *__restrict__ dgain, uint32_t parts,
+							     uint32_t width)
 {
-	__shared__ float sums[kGainWaves][64];
-	const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, column = blockIdx.x * 64u + lane;
+	__shared__ float sums[kGainTurns][kGainColumns];
+	const uint32_t x = threadIdx.x % kGainColumns, turn = threadIdx.x / kGainColumns, column = blockIdx.x * kGainColumns + x;
 	float total = 0.0f;
-	if (column < width) {
-#pragma unroll 8
-		for (uint32_t p = wave; p < parts; p += kGainWaves) {
-			total += partial[(uint64_t)p * width + column];
+	if (column < width && turn < parts) {
+		float f[kPartsOfLane];
+#pragma unroll
+		for (uint32_t p = 0; p < kPartsOfLane; p++) {
+			f[p] = partial[(uint64_t)min(turn + p * kGainTurns, parts - 1) * width + column];
+		}
+#pragma unroll
+		for (uint32_t p = 0; p < kPartsOfLane; p++) {
+			total += turn + p * kGainTurns < parts ? f[p] : 0.0f;
 		}
 	}
-	sums[wave][lane] = total;
+	sums[turn][x] = total;
 	__syncthreads();
-	if (wave == 0 && column < width) {
+	if (turn == 0 && column < width) {
 #pragma unroll
-		for (int w = 1; w < kGainWaves; w++) {
-			total += sums[w][lane];
+		for (uint32_t t = 1; t < kGainTurns; t++) {
+			total += sums[t][x];
 		}
 		dgain[column] = total;
 	}
@@ -598,8 +604,8 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
 		});
 	}
 	if (d_dgain) { /* of no rows: zeros */
-		launch_kernel(rms_norm_gain_kernel, dim3((width + 63u) / 64u), dim3(64 * kGainWaves), 0, as_stream(stream), partial, d_dgain,
-			      blocks, width);
+		launch_kernel(rms_norm_gain_kernel, dim3((width + kGainColumns - 1) / kGainColumns), dim3(1024), 0, as_stream(stream), partial,
+			      d_dgain, blocks, width);
 	}
 	OFI_AMD_HIP_TRY(hipGetLastError());
 	return 0;

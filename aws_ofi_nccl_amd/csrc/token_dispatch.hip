@@ -243,9 +243,26 @@ __device__ __forceinline__ void copy_rows(uint32_t token, uint32_t wave, uint32_
 			continue; /* nobody asks for this token */
 		}
 		for (uint32_t at = second ? 0u : wave * kSpan; at < r.bytes; at += stride) {
-			const uint32_t n = min(r.bytes - at, kSpan), whole = n >> 4, rest = n & 15u;
 			const uint8_t *from = r.from + token * r.from_pitch + at;
 			u32x4_t v[kRows];
+			if (r.bytes - at >= kSpan) {
+#pragma unroll
+				for (uint32_t i = 0; i < kRows; i++) {
+					v[i] = *reinterpret_cast<const any16_t *>(from + 16u * (i * 64u + lane));
+				}
+#pragma unroll
+				for (uint32_t k = 0; k < kAtOnce; k++) {
+					if (row[k] < max_rows) {
+						uint8_t *to = r.to + row[k] * r.to_pitch + at;
+#pragma unroll
+						for (uint32_t i = 0; i < kRows; i++) {
+							*reinterpret_cast<any16_t *>(to + 16u * (i * 64u + lane)) = v[i];
+						}
+					}
+				}
+				continue;
+			}
+			const uint32_t n = r.bytes - at, whole = n >> 4, rest = n & 15u;
 #pragma unroll
 			for (uint32_t i = 0; i < kRows; i++) {
 				if (i * 64u + lane < whole) {
