@@ -75,10 +75,14 @@ __device__ __forceinline__ uint32_t max_bits_of_group(uint32_t m, uint32_t lanes
 		m = max(m, dpp<0x140>(m));
 	}
 	if (lanes >= 32) {
-		m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+		uint32_t o = m;
+		swap_rows16(m, o);
+		m = max(m, o);
 	}
 	if (lanes >= 64) {
-		m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+		uint32_t o = m;
+		swap_halves(m, o);
+		m = max(m, o);
 	}
 	return m;
 }

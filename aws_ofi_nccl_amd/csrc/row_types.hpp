@@ -105,6 +105,22 @@ template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v)
 	return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 
+/* Rows of 16 lanes exchanged: {a0, b0, a2, b2} and {a1, b1, a3, b3} */
+__device__ __forceinline__ void swap_rows16(uint32_t &a, uint32_t &b)
+{
+	const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+	a = r[0];
+	b = r[1];
+}
+
+/* Halves exchanged: {a low, b low} and {a high, b high} */
+__device__ __forceinline__ void swap_halves(uint32_t &a, uint32_t &b)
+{
+	const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+	a = r[0];
+	b = r[1];
+}
+
 /* op over each group of LANES neighbouring lanes (a power of two), the result in all of them.  The order of the operations
  * depends on the lane number alone. */
 template <int LANES, typename Op> __device__ __forceinline__ uint32_t over_lanes(uint32_t v, Op op)
@@ -122,10 +138,14 @@ template <int LANES, typename Op> __device__ __forceinline__ uint32_t over_lanes
 		v = op(v, dpp<0x140>(v)); /* row_mirror */
 	}
 	if (LANES >= 32) {
-		v = op(v, (uint32_t)__shfl_xor((int)v, 16));
+		uint32_t w = v;
+		swap_rows16(v, w);
+		v = op(v, w);
 	}
 	if (LANES >= 64) {
-		v = op(v, (uint32_t)__shfl_xor((int)v, 32));
+		uint32_t w = v;
+		swap_halves(v, w);
+		v = op(v, w);
 	}
 	return v;
 }
@@ -135,6 +155,38 @@ template <int LANES> __device__ __forceinline__ float sum_over(float v)
 	return __uint_as_float(over_lanes<LANES>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
 		return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
 	}));
+}
+
+__device__ __forceinline__ float sum_of_halves(float a, float b)
+{
+	uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+	swap_halves(x, y);
+	return __uint_as_float(x) + __uint_as_float(y);
+}
+
+__device__ __forceinline__ float sum_of_rows16(float a, float b)
+{
+	uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+	swap_rows16(x, y);
+	return __uint_as_float(x) + __uint_as_float(y);
+}
+
+/* Eight sums over the wavefront at once: the one of v[lane / 8], in all eight of those lanes.  Half of what is added is another value
+ * at each of the first three steps, so that there are ten additions instead of 48. */
+__device__ __forceinline__ float eight_sums(const float (&v)[8], uint32_t lane)
+{
+	float four[4], two[2];
+#pragma unroll
+	for (int i = 0; i < 4; i++) {
+		four[i] = sum_of_halves(v[i], v[i + 4]);
+	}
+#pragma unroll
+	for (int i = 0; i < 2; i++) {
+		two[i] = sum_of_rows16(four[i], four[i + 2]);
+	}
+	const bool odd = lane & 8u;
+	const float keep = odd ? two[1] : two[0], give = odd ? two[0] : two[1];
+	return sum_over<8>(keep + __uint_as_float(dpp<0x140>(__float_as_uint(give)))); /* row_mirror */
 }
 
 /* Maximum of absolute values given as their bits: a NaN's are above an infinity's, so that a NaN comes out */

@@ -154,12 +154,10 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(con
 		if (!dweight) {
 			continue;
 		}
-#pragma unroll
-		for (uint32_t k = 0; k < kAtOnce; k++) {
-			const float d = sum_over<64>(dot[k]);
-			if ((threadIdx.x & 63u) == 0) {
-				part[threadIdx.x >> 6][k] = d;
-			}
+		const uint32_t lane = threadIdx.x & 63u;
+		const float sum = eight_sums(dot, lane);
+		if ((lane & 7u) == 0) {
+			part[threadIdx.x >> 6][lane >> 3] = sum;
 		}
 		__syncthreads();
 		if (threadIdx.x < kAtOnce && k0 + threadIdx.x < top_k) {
