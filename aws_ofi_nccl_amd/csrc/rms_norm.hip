@@ -3,7 +3,9 @@
  *
  *   s = x + r,  rstd = 1 / sqrt(mean(s^2) + eps),  n = s rstd g,  q = e4m3(n / scale),  scale = max(amax|n| / 448, 2^-126)
  *
- * per group of columns or per row.  One workgroup holds a row in registers, so that x and r are read once.
+ * per group of columns or per row.  A row is held in registers from its reading to its writing, so that every byte crosses the memory
+ * interface once, and memory is what bounds it: 16,384 rows of 8192 bfloat16 with residual to e4m3, 944 MB, 154.6 us = 6.1 TB/s
+ * (counters: 537 MB read, 406 MB written, which is every input and output once).
  */
 #include <type_traits>
 
@@ -239,8 +241,12 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_kernel(const T *x, c
  * dx = ds + rstd (g dn - h mean(g dn h)), h = s rstd; dg = sum over rows of dn h: each workgroup sums its own rows and the
  * partial sums are added up in the order of the workgroups, so that the result is the same every time.
  *
- * The wavefronts along x hold a row, a chunk a lane; a workgroup has blockDim.y rows at once and asks for the next ones before it waits for
- * the sum of these.  dx may be dout or dsum: a lane has read what it writes.
+ * The wavefronts along x hold a row, a chunk a lane; a workgroup has blockDim.y rows at once and asks for the next
+ * ones before it waits for the sum of these.  dx may be dout or dsum: a lane has read what it writes.
+ *
+ * Memory bounds it: 16,384 rows of 4096 bfloat16 with dsum, 537 MB, 88 us and 5 for the parts = 5.8 TB/s.  512 workgroups: with 384,
+ * 768, 1024 of them 105, 105, 109 us in all for 97.  Two rows ahead were no faster (103), nor rows next to each other in a workgroup
+ * (110).
  */
 template <typename T, uint32_t V, int MOST, flow_t FLOW>
 __global__ __launch_bounds__(64 * MOST)
@@ -337,9 +343,14 @@ void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s, const float *_
 	}
 }
 
-/* The same for rows of more than 1024 chunks, which the registers do not hold beside the sums: read once for the mean, and once more,
- * out of the caches, for the rest.  (s is not restricted: nothing of the first reading is to be kept.) */
-template <typename T, uint32_t V, int R>
+/*
+ * The same for rows of more than 1024 chunks, R a lane, without the next row's beside them: 8192 rows of 16,384 bfloat16 217 us (5.0 TB/s).
+ * KEPT: a row is held over its sum as it lies in memory (as floats it would not fit).  The longest rows, 32 values a lane, do not fit
+ * beside their sums either way -- 2000 rows of 32,768 bfloat16 took 284 us so, and 639 with floats -- and are read again, out of
+ * the caches: 159.
+ */
+template <int R, uint32_t V> constexpr bool kKept = R * V <= 16;
+template <typename T, uint32_t V, int R, flow_t FLOW>
 __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(const T *dout, const T *s, const float *__restrict__ rstds,
 								  const void *__restrict__ gain, const T *dsum, uint64_t dout_pitch,
 								  uint64_t s_pitch, uint64_t dsum_pitch, uint32_t n_rows, uint32_t width,
@@ -356,19 +367,41 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(con
 	}
 	uint32_t turn = 0;
 	for (uint64_t row = blockIdx.x; row < n_rows; row += gridDim.x, turn ^= 1u) {
-		const T *dr = row_at(dout, dout_pitch, row), *sr = row_at(s, s_pitch, row);
+		constexpr int H = kKept<R, V> ? R : 1; /* chunks held */
+		raw_t<T, V> dc[H], sc[H];
+		auto ask = [&](int k, int slot) {
+			const uint32_t from = place_of<V>((k * blockDim.x + threadIdx.x) * V, width).from;
+			dc[slot] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(dout, dout_pitch, row) + from);
+			sc[slot] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(s, s_pitch, row) + from);
+		};
 		const float rstd = rstds[row];
 		float along = 0.0f;
-#pragma unroll 2
-		for (int k = 0; k < R; k++) {
+		auto sum = [&](int k, int slot) {
 			const place_t here = place_of<V>((k * blockDim.x + threadIdx.x) * V, width);
 			float g[V], d[V], h[V];
-			to_floats<T, V>(load_raw<false, T, V>(dr + here.from), here.skip, d);
-			to_floats<T, V>(load_raw<false, T, V>(sr + here.from), here.skip, h);
+			to_floats<T, V>(dc[slot], here.skip, d);
+			to_floats<T, V>(sc[slot], here.skip, h);
 			load_gain<T, V>(gain, gain_f32, here.from, g);
 #pragma unroll
 			for (uint32_t i = 0; i < V; i++) {
 				along = i < here.skip ? along : __builtin_fmaf(d[i] * g[i], h[i] * rstd, along);
+			}
+		};
+		if constexpr (kKept<R, V>) {
+#pragma unroll
+			for (int k = 0; k < R; k++) {
+				ask(k, k);
+			}
+#pragma unroll
+			for (int k = 0; k < R; k++) {
+				sum(k, k);
+				asm volatile("" : "+v"(dc[k]), "+v"(sc[k])); /* nothing made of them is kept */
+			}
+		} else {
+#pragma unroll 1
+			for (int k = 0; k < R; k++) {
+				ask(k, 0);
+				sum(k, 0);
 			}
 		}
 		const float mean = block_sum(along, part[turn], blockDim.x >> 6) / (float)width;
@@ -378,15 +411,19 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(con
 			if (at < width) {
 				const place_t here = place_of<V>(at, width);
 				float g[V], d[V], h[V], r[V];
-				to_floats<T, V>(load_raw<false, T, V>(dr + here.from), here.skip, d);
-				to_floats<T, V>(load_raw<false, T, V>(sr + here.from), here.skip, h);
+				const int slot = kKept<R, V> ? k : 0;
+				if (!kKept<R, V>) {
+					ask(k, slot);
+				}
+				to_floats<T, V>(dc[slot], here.skip, d);
+				to_floats<T, V>(sc[slot], here.skip, h);
 				load_gain<T, V>(gain, gain_f32, here.from, g);
 #pragma unroll
 				for (uint32_t i = 0; i < V; i++) {
 					r[i] = 0.0f;
 				}
 				if (dsum) {
-					to_floats<T, V>(load_raw<false, T, V>(row_at(dsum, dsum_pitch, row) + here.from), 0, r);
+					to_floats<T, V>(load_raw<FLOW != STREAM_NONE, T, V>(row_at(dsum, dsum_pitch, row) + here.from), 0, r);
 				}
 #pragma unroll
 				for (uint32_t i = 0; i < V; i++) {
@@ -394,7 +431,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(con
 					dg[k][i] = __builtin_fmaf(d[i], h[i], dg[k][i]);
 					r[i] = __builtin_fmaf(rstd, __builtin_fmaf(-h[i], mean, d[i] * g[i]), r[i]);
 				}
-				store_piece<false, T, V>(row_at(dx, dx_pitch, row) + here.from, here.skip, r);
+				store_piece<FLOW == STREAM_BOTH, T, V>(row_at(dx, dx_pitch, row) + here.from, here.skip, r);
 			}
 		}
 	}
@@ -408,7 +445,8 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(con
 	}
 }
 
-/* kGainColumns columns of a workgroup, its lanes at the parts by turns, with all of their loads on the way at once */
+/* kGainColumns columns of a workgroup, its lanes at the parts by turns, with all of their loads on the way at once: 5 us for 512 parts of
+ * 4096 (64 columns 5.5), most of it the way of fresh lines from the other dies */
 constexpr uint32_t kGainColumns = 32, kGainTurns = 1024 / kGainColumns, kPartsOfLane = kGradBlocks / kGainTurns;
 static_assert(kGradBlocks % kGainTurns == 0, "all parts are added");
 __global__ __launch_bounds__(1024) void rms_norm_gain_kernel(const float *__restrict__ partial, float *__restrict__ dgain, uint32_t parts,
@@ -590,7 +628,15 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
 			with_chunks_of_lane<V>(chunks, 1, [&](auto r) {
 				constexpr int R = decltype(r)::value;
 				if constexpr (R > 1) {
-					launch(rms_norm_grad_wide_kernel<T, V, R>, dim3(64 * ((waves + R - 1) / R)));
+					const dim3 lanes(64 * ((waves + R - 1) / R));
+					if constexpr (kKept<R, V>) {
+						launch(by_flow(flow, rms_norm_grad_wide_kernel<T, V, R, STREAM_NONE>,
+							       rms_norm_grad_wide_kernel<T, V, R, STREAM_LOADS>,
+							       rms_norm_grad_wide_kernel<T, V, R, STREAM_BOTH>),
+						       lanes);
+					} else {
+						launch(rms_norm_grad_wide_kernel<T, V, R, STREAM_NONE>, lanes);
+					}
 				} else if (waves > (uint32_t)kGradWaves) {
 					launch(by_flow(flow, rms_norm_grad_kernel<T, V, kMostWaves, STREAM_NONE>,
 						       rms_norm_grad_kernel<T, V, kMostWaves, STREAM_LOADS>,

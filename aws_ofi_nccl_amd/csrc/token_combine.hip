@@ -4,6 +4,9 @@
  *   out_t = add_t + sum_k w_tk y[row_tk]        dy[row_tk] = w_tk dout_t        dw_tk = <dout_t, y[row_tk]>
  *
  * A pair without a row (an index outside the rows) is passed over, whatever its weight is.
+ *
+ * Memory bounds both: 16,384 tokens of 8 rows of 8 KiB, sums and an addend 1.34 GB in 235 us = 5.7 TB/s, gradients 2.28 GB in 439 us =
+ * 5.2 TB/s (nine streams read and eight written; the same reads and writes without the arithmetic 445).  Counters: every byte once.
  */
 #include "common.hpp"
 #include "ofi_amd_hotpath.h"
@@ -20,7 +23,8 @@ constexpr uint32_t kMostWaves = 8; /* a workgroup has all of a row of up to 8 Ki
 constexpr uint32_t kAtOnce = 8; /* rows of a token that are read together */
 
 /* A workgroup of threadIdx.x lanes along a row and threadIdx.y tokens; each lane one chunk of the output at a time.  Up to kAtOnce
- * rows are asked for before the first is used. */
+ * rows are asked for before the first is used.  Eight wavefronts a row are faster than four with two chunks a lane or one with all of
+ * them (237, 239, 245 us of reads and writes alone), a token's rows are not brought closer by giving each die a run of tokens (246). */
 template <typename T, uint32_t V, flow_t FLOW>
 __global__ __launch_bounds__(64 * kMostWaves) void token_combine_kernel(const int32_t *__restrict__ row_of,
 									const float *__restrict__ weight, const T *__restrict__ rows,

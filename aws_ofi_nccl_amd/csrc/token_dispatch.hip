@@ -4,7 +4,11 @@
  *   row(p) = #{q : e_q < e_p} + #{q < p : e_q = e_p}     over pairs whose expert lies in [0, n_experts)
  *
  * so that the rows of an expert -- and of a rank that holds a run of experts -- are one piece of memory, which one put carries.
- * No order of atomics shows in the result.
+ * No order of atomics shows in the result: they only count.
+ *
+ * Up to 2048 pairs are one launch, up to 8192 two (table, rows), more three (counts of the tiles first).  32,768 tokens of 8 KiB to
+ * 8 of 128 experts: counts 4.9 us, table 8.8, rows 476 for 2.42 GB read and written (5.1 TB/s; the same kernel with the rows written one
+ * after the other 441, which is what reading once and writing eight times comes to on this part).
  */
 #include "common.hpp"
 #include "ofi_amd_hotpath.h"
@@ -23,8 +27,8 @@ constexpr uint32_t kMostRounds = 8; /* pairs of a lane of the sort */
 constexpr uint32_t kManyTiles = 64;
 constexpr uint32_t kTilesAtOnce = 32;
 
-/* A workgroup of the sort has 1024 pairs a round; tiles get more rounds before they get many.  Everybody adds up the counts of all
- * tiles, 32 at a time, so that 32 tiles of 8 rounds cost less than 256 of one. */
+/* A workgroup of the sort has 1024 pairs a round.  Everybody adds up the counts of all tiles, 32 at a time, and each unit's scattered
+ * stores of pair_of take their turns: 262,144 pairs as 32 tiles of 8 rounds 11.6 us, 64 of 4 8.8, 128 of 2 9.2, 256 of one 11.9. */
 inline uint32_t rounds_of(uint64_t n_pairs)
 {
 	const uint64_t one = 64 * kSortWaves;
@@ -75,9 +79,11 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(const I *_
 	}
 }
 
-/* Rows of a tile's pairs: each wavefront ranks its own, the counts of the wavefronts and of the other tiles say where they begin.
- * Every workgroup adds up the tiles' counts by itself; a tile that is alone needs none.  LDS: kSortWaves counters an expert, and of those
- * without one. */
+/*
+ * Rows of a tile's pairs: each wavefront ranks its own -- lanes with the same expert find each other by a ballot for each bit of its
+ * number, the rounds beside each other --, the counts of the wavefronts and of the other tiles say where they begin.  A tile that is
+ * alone needs no counts.  LDS: kSortWaves counters an expert, and for the pairs without one.
+ */
 template <typename I, uint32_t ROUNDS>
 __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *__restrict__ expert, uint32_t n_pairs,
 								      uint32_t n_experts, uint32_t n_tiles, uint32_t max_rows,
@@ -222,8 +228,12 @@ constexpr uint32_t kSpan = 1024 * kRows;
 constexpr uint32_t kMostWaves = 8;
 constexpr uint32_t kAtOnce = 8;
 
-/* A token's rows: 2 KiB are read at a time by a wavefront and written to each of the places (a row number each, max_rows or more:
- * none), the next ones when these are done.  The first row_waves wavefronts have row a, the one behind them row b. */
+/*
+ * A token's rows: 2 KiB are read at a time by a wavefront and written to each of the places (a row number each, max_rows or more:
+ * none).  The first row_waves wavefronts have row a, the one behind them row b.  Reading a row once and writing it everywhere beats
+ * reading it for each place (560 us and more for 455); ordinary stores beat streaming ones here (455 and 464), as do 2 KiB a wavefront
+ * 4 and 8 (466, 475) -- times of this copy alone, 32,768 rows of 8 KiB to 8 places each.
+ */
 template <typename P>
 __device__ __forceinline__ void copy_rows(uint32_t token, uint32_t wave, uint32_t row_waves, const rows_t &a, const rows_t &b,
 					  uint32_t top_k, uint32_t max_rows, P place)
@@ -305,9 +315,12 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_rows_kernel(const int32
 /*
  * Few pairs: table and rows in one launch.  The workgroup of a token counts the pairs in front of each of its own -- of a smaller
  * expert, or of the same and a smaller number, which is one comparison of expert * kFew + pair -- and copies its rows there; the
- * last workgroup makes the offsets.
+ * last workgroup makes the offsets.  8 pairs 4.0 us on the GPU (table and rows apart: 7.2 and 2.2).  Every workgroup looks at all pairs:
+ * 2048 of 256 tokens 10.9 us a call, 2056 in two launches 13.4; 2000 of as many tokens 14.0 in one and 13.3 in two, 4096 of 512 15.8
+ * and 14.7.
  */
-constexpr uint32_t kFew = 2048;
+constexpr uint32_t kFew = 2048, kFewTokens = 1024;
+constexpr uint32_t kFewWaves = 4; /* at least, to count, however short the rows are */
 static_assert((uint64_t)kMaxExperts * kFew < 0x7fffffffull, "keys within 32 bits");
 template <typename I>
 __global__ __launch_bounds__(64 * kMostWaves) void token_few_kernel(const I *__restrict__ expert, uint32_t n_tokens, uint32_t top_k,
@@ -407,8 +420,10 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_few_kernel(const I *__r
 		counts[k] = placed ? row : ~0u; /* the first wavefront's, which this lane has read */
 	}
 	__syncthreads();
-	copy_rows(token, wave, row_waves, a, b, top_k, max_rows,
-		  [&](uint32_t k) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)counts[k]); });
+	if (wave < row_waves + (b.to ? 1u : 0u)) {
+		copy_rows(token, wave, row_waves, a, b, top_k, max_rows,
+			  [&](uint32_t k) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)counts[k]); });
+	}
 }
 
 inline uint32_t tiles_of(uint64_t n_pairs)
@@ -485,9 +500,10 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 	const uint32_t row_waves = d_x ? even_waves(64 * spans, kMostWaves - more) : 0;
 	auto run = [&](const auto *expert) {
 		using I = typename std::remove_cv<typename std::remove_pointer<decltype(expert)>::type>::type;
-		if (d_x && n_pairs <= kFew) {
-			launch_kernel(token_few_kernel<I>, dim3(n_tokens + 1), dim3(64 * (row_waves + more)), 0, as_stream(stream), expert, n_tokens,
-				      top_k, n_experts, row_waves, max_rows, a, b, d_offset, d_row_of, d_pair_of, err);
+		if (d_x && n_pairs <= kFew && n_tokens <= kFewTokens) {
+			const uint32_t waves = row_waves + more < kFewWaves ? kFewWaves : row_waves + more;
+			launch_kernel(token_few_kernel<I>, dim3(n_tokens + 1), dim3(64 * waves), 0, as_stream(stream), expert, n_tokens, top_k,
+				      n_experts, row_waves, max_rows, a, b, d_offset, d_row_of, d_pair_of, err);
 			return;
 		}
 		const uint32_t tiles = tiles_of(n_pairs);

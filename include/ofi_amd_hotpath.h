@@ -952,9 +952,10 @@ int ofi_amd_tuner_ctx_stats(const void *context, ofi_amd_tuner_ctx_stats_t *out)
  *    less than 2^40), and need no alignment beyond their element's.  Rows, pitches and tables that
  *    lie on 16 bytes are faster.  Sums, statistics and products are held in 32 bits; each output is
  *    rounded once, to nearest even.  Results do not depend on the order in which the GPU runs things:
- *    the same call gives the same bits.  Nothing is allocated; calls may be captured into a graph
- *    (after ofi_amd_gpu_init()).  -EINVAL: a missing or misaligned argument, a type or group not
- *    named here, a pitch below a row; -E2BIG: beyond the stated limits.
+ *    the same call gives the same bits.  Buffers of one call do not overlap but where it says so.
+ *    Nothing is allocated; calls may be captured into a graph (after ofi_amd_gpu_init()).  -EINVAL: a
+ *    missing or misaligned argument, a type or group not named here, a pitch below a row; -E2BIG:
+ *    beyond the stated limits.
  * ====================================================================== */
 
 /* Types, by their numbers in ncclDataType_t */
@@ -986,7 +987,7 @@ int ofi_amd_rms_norm(const void *d_x, uint64_t x_pitch, const void *d_residual, 
  * what reaches s past the norm.  With h = s * rstd:
  *   dx = dsum + rstd * (gain * dout - h * mean(gain * dout * h))   in `type`: of x and of residual
  *   dgain[i] = sum over rows of dout * h                           in float32
- * d_dgain may be NULL; otherwise d_work holds ofi_amd_rms_norm_grad_work_bytes bytes on a 16-byte
+ * d_dgain may be NULL; otherwise d_work holds ofi_amd_rms_norm_grad_work_bytes bytes on a 4-byte
  * boundary, free again when the call's work has ended.  No rows: dgain is zeros.  d_dx may be d_dout
  * or d_dsum, with the same pitch.  The 8-bit rounding is passed through as if it were not there.
  */
@@ -1009,7 +1010,7 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
  * more have none: d_row_of is -1, d_offset ends at max_rows, and bit 4 of ofi_amd_async_error_fetch is set.
  * Rows of e4m3 with scales go as they are: the copy is of bytes, at any alignment.
  * n_experts <= 1024, top_k <= 64, row_bytes and scale_bytes <= 2^24, pairs and max_rows < 2^31.
- * d_work: ofi_amd_token_dispatch_work_bytes bytes on a 16-byte boundary (NULL where that is 0), free
+ * d_work: ofi_amd_token_dispatch_work_bytes bytes on a 4-byte boundary (NULL where that is 0), free
  * again when the call's work has ended.
  * The gradient of d_x is ofi_amd_token_combine of the gradient of d_rows without weights.
  */

@@ -78,7 +78,9 @@ def test_norms(lib, gpu, n, width, pitch, kind, group):
 
 @pytest.mark.parametrize("n,width,pitch,kind,in_place", [(5000, 4096, 4096, "bf16", None), (12000, 4092, 4096, "bf16", "dsum"),
                                                          (9000, 8192, 8192, "bf16", "dout"), (70000, 512, 512, "f32", None),
-                                                         (200000, 250, 256, "f16", None)])
+                                                         (200000, 250, 256, "f16", None), (3000, 16380, 16384, "bf16", "dout"),
+                                                         (2000, 12288, 12288, "f32", "dsum"), (600, 32768, 32768, "f32", None),
+                                                         (1500, 32000, 32000, "bf16", "dsum")])
 def test_gradients_of_norms(lib, gpu, n, width, pitch, kind, in_place):
     dtype, code, u = TYPES[kind]
     g = gen(n)
