@@ -29,6 +29,11 @@ nothing else of interest, which keeps counter runs short.  The shapes:
             align<N>     the same as configured with every destination a multiple of N bytes
                          (N = 16, 64 or 128); "slots+align<N>" combines the two
             host         2048 rx buffers in pinned host memory
+  norm      <tokens>     rows of 8192 bfloat16 with residual to e4m3, a scale for 128 (default 16,384 rows)
+  norm_grad <tokens>     the norm's gradient, rows of 4096 bfloat16 (default 16,384)
+  dispatch  <tokens>     rows of 8 KiB to 8 of 128 experts each (default 32,768)
+  combine   <tokens>     8 rows of 8 KiB bfloat16 and an addend to a token, weighted (default 16,384)
+  combine_grad <tokens>  the sum's gradients (default 16,384)
 """
 import argparse
 import ctypes
@@ -39,9 +44,54 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SEED = 1234
 
 
+TOKEN_ROWS = {"norm": 16384, "norm_grad": 16384, "dispatch": 32768, "combine": 16384, "combine_grad": 16384}
+
+
+def token_step(m, lib, torch, kernel, tokens, stream):
+    """One call of a norm or token exchange on `tokens` tokens, as a function; everything it works on is kept by it."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(SEED)
+    normal = lambda n, width: torch.randn(n, width, generator=g, device="cuda", dtype=torch.float32).to(torch.bfloat16)
+    width, top_k, experts, bf16 = 8192 if kernel == "norm" else 4096, 8, 128, m.BFLOAT16
+    at = lambda t: (t.data_ptr(), t.stride(0) * t.element_size())
+    x = normal(tokens, width)
+    if kernel == "norm":
+        residual, total, gain = normal(tokens, width), torch.empty_like(x), torch.ones(width, dtype=x.dtype, device="cuda")
+        q, scale = torch.empty(tokens, width, dtype=torch.uint8, device="cuda"), torch.empty(tokens, width // 128, device="cuda")
+        return lambda: m.check(lib.ofi_amd_rms_norm(*at(x), *at(residual), gain.data_ptr(), bf16, tokens, width, bf16, 1e-6, *at(total),
+                                                    None, 0, *at(q), *at(scale), 128, None, stream), "rms_norm")
+    if kernel == "norm_grad":
+        dout, dsum, dx = normal(tokens, width), normal(tokens, width), torch.empty_like(x)
+        rstd, gain = torch.ones(tokens, device="cuda"), torch.ones(width, dtype=x.dtype, device="cuda")
+        dgain = torch.empty(width, device="cuda")
+        work = torch.empty(lib.ofi_amd_rms_norm_grad_work_bytes(tokens, width), dtype=torch.uint8, device="cuda")
+        return lambda: m.check(lib.ofi_amd_rms_norm_grad(*at(dout), *at(x), rstd.data_ptr(), gain.data_ptr(), bf16, tokens, width, bf16,
+                                                         *at(dsum), *at(dx), dgain.data_ptr(), work.data_ptr(), work.numel(), stream),
+                               "rms_norm_grad")
+    pairs = tokens * top_k
+    ids = torch.topk(torch.randn(tokens, experts, generator=g, device="cuda"), top_k, dim=1).indices.contiguous()
+    offset, row_of = (torch.empty(n, dtype=torch.int32, device="cuda") for n in (experts + 1, pairs))
+    work = torch.empty(max(16, lib.ofi_amd_token_dispatch_work_bytes(tokens, top_k, experts)), dtype=torch.uint8, device="cuda")
+    rows = torch.zeros(pairs, width, dtype=x.dtype, device="cuda")
+    dispatch = lambda: m.check(lib.ofi_amd_token_dispatch(ids.data_ptr(), m.INT64, tokens, top_k, experts, pairs, offset.data_ptr(),
+                                                          row_of.data_ptr(), None, *at(x), *at(rows), 2 * width, None, 0, None, 0, 0,
+                                                          work.data_ptr(), work.numel(), stream), "token_dispatch")
+    if kernel == "dispatch":
+        return dispatch
+    dispatch()
+    weight = torch.rand(tokens, top_k, generator=g, device="cuda")
+    if kernel == "combine":
+        out = torch.empty_like(x)
+        return lambda: m.check(lib.ofi_amd_token_combine(*at(rows), pairs, row_of.data_ptr(), weight.data_ptr(), tokens, top_k, width, bf16,
+                                                         *at(x), *at(out), stream), "token_combine")
+    drows, dweight = torch.empty_like(rows), torch.empty_like(weight)
+    return lambda: m.check(lib.ofi_amd_token_combine_grad(*at(x), *at(rows), pairs, row_of.data_ptr(), weight.data_ptr(), tokens, top_k,
+                                                          width, bf16, *at(drows), dweight.data_ptr(), stream), "token_combine_grad")
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--kernel", required=True, choices=["bounce", "copy", "fill", "table", "striping", "model", "region", "eager"])
+    ap.add_argument("--kernel", required=True, choices=["bounce", "copy", "fill", "table", "striping", "model", "region", "eager"] + sorted(TOKEN_ROWS))
     ap.add_argument("--shape", default=None)
     ap.add_argument("--launches", type=int, default=30)
     ap.add_argument("--buffers", type=int, default=None,
@@ -112,6 +162,8 @@ def main():
                 d_src.data_ptr(), d_src.numel(), d_arena.data_ptr(), w["arena_bytes"], d_so.data_ptr(),
                 d_do.data_ptr(), d_len.data_ptr(), n, flush, stream), "bounce_scatter")
         print("payload bytes per launch: %d, buffers: %d" % (w["src_bytes"], n))
+    elif args.kernel in TOKEN_ROWS:
+        step = token_step(m, lib, torch, args.kernel, int(args.shape or TOKEN_ROWS[args.kernel]), stream)
     elif args.kernel == "fill":
         d_fill = torch.empty(int(args.shape or "100") << 20, dtype=torch.uint8, device="cuda")
         step = lambda: d_fill.fill_(7)
