@@ -563,6 +563,7 @@ int ofi_amd_rms_norm(const void *d_x, uint64_t x_pitch, const void *d_residual, 
 					      group_lanes, gain_type == OFI_AMD_FLOAT32, o);
 			}
 		};
+		/* narrow rows share a wavefront: 30,000 rows of 256 bfloat16 to e4m3 15.9 us with one to each, 12.8 with two */
 		if (chunks <= 16) {
 			launch(by_flow(flow, rms_norm_kernel<T, V, 1, 16, STREAM_NONE>, rms_norm_kernel<T, V, 1, 16, STREAM_LOADS>,
 				       rms_norm_kernel<T, V, 1, 16, STREAM_BOTH>), 16, 256);
@@ -643,7 +644,8 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
 						       rms_norm_grad_kernel<T, V, kMostWaves, STREAM_BOTH>),
 					       dim3(64 * waves));
 				} else {
-					/* rows of a workgroup at once, but one where more would leave workgroups without any */
+					/* rows of a workgroup at once, so that it has eight wavefronts (30,000 rows of 1024 bfloat16 60.2 us with
+					 * one row, 43.8 with four), but fewer where that would leave workgroups without any */
 					const uint32_t most = kGradWaves / waves, each = (n_rows + kGradBlocks - 1) / kGradBlocks;
 					launch(by_flow(flow, rms_norm_grad_kernel<T, V, kGradWaves, STREAM_NONE>,
 						       rms_norm_grad_kernel<T, V, kGradWaves, STREAM_LOADS>,

@@ -320,7 +320,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_rows_kernel(const int32
  * and 14.7.
  */
 constexpr uint32_t kFew = 2048, kFewTokens = 1024;
-constexpr uint32_t kFewWaves = 4; /* at least, to count, however short the rows are */
+constexpr uint32_t kFewWaves = 4; /* at least, to count, however short the rows are (4096 pairs by one wavefront: 21.8 us for 15.8) */
 static_assert((uint64_t)kMaxExperts * kFew < 0x7fffffffull, "keys within 32 bits");
 template <typename I>
 __global__ __launch_bounds__(64 * kMostWaves) void token_few_kernel(const I *__restrict__ expert, uint32_t n_tokens, uint32_t top_k,
