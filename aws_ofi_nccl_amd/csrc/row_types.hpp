@@ -71,11 +71,12 @@ template <typename T, uint32_t V> __device__ __forceinline__ void to_floats(raw_
 /* The chunk's own elements go to the row's place `from`, each rounded to the row's type once, to nearest even */
 template <bool STREAM, typename T, uint32_t V> __device__ __forceinline__ void store_piece(T *p, uint32_t skip, const float (&f)[V])
 {
-	raw_t<T, V> c;
+	float all __attribute__((ext_vector_type(V)));
 #pragma unroll
 	for (uint32_t i = 0; i < V; i++) {
-		c[i] = (T)f[i];
+		all[i] = f[i];
 	}
+	const raw_t<T, V> c = __builtin_convertvector(all, raw_t<T, V>);
 	if (skip == 0) {
 		auto *q = reinterpret_cast<typename piece_t<T, V>::anywhere *>(p);
 		if (STREAM) {

@@ -320,7 +320,8 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_rows_kernel(const int32
  * and 14.7.
  */
 constexpr uint32_t kFew = 2048, kFewTokens = 1024;
-constexpr uint32_t kFewWaves = 4; /* at least, to count, however short the rows are (4096 pairs by one wavefront: 21.8 us for 15.8) */
+constexpr uint32_t kFewWaves = 4; /* at least, to count more than 512, however short the rows are: 4096 by one wavefront 21.8 us for 15.8,
+				   * 8 by four 4.4 for 4.0 */
 static_assert((uint64_t)kMaxExperts * kFew < 0x7fffffffull, "keys within 32 bits");
 template <typename I>
 __global__ __launch_bounds__(64 * kMostWaves) void token_few_kernel(const I *__restrict__ expert, uint32_t n_tokens, uint32_t top_k,
@@ -501,7 +502,7 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 	auto run = [&](const auto *expert) {
 		using I = typename std::remove_cv<typename std::remove_pointer<decltype(expert)>::type>::type;
 		if (d_x && n_pairs <= kFew && n_tokens <= kFewTokens) {
-			const uint32_t waves = row_waves + more < kFewWaves ? kFewWaves : row_waves + more;
+			const uint32_t least = n_pairs > 512 ? kFewWaves : 1, waves = row_waves + more < least ? least : row_waves + more;
 			launch_kernel(token_few_kernel<I>, dim3(n_tokens + 1), dim3(64 * waves), 0, as_stream(stream), expert, n_tokens, top_k,
 				      n_experts, row_waves, max_rows, a, b, d_offset, d_row_of, d_pair_of, err);
 			return;
