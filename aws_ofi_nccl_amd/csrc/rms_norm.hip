@@ -547,9 +547,7 @@ int ofi_amd_rms_norm(const void *d_x, uint64_t x_pitch, const void *d_residual, 
 		return -EINVAL;
 	}
 	const norm_out_t o = { d_sum, sum_pitch, d_out, out_pitch, static_cast<uint8_t *>(d_q), q_pitch, d_scale, scale_pitch, d_rstd };
-	const flow_t flow = flow_of(n_rows * (bytes * (1u + !!d_residual + !!d_sum + !!d_out) + (d_q ? width : 0)),
-				    on_chunks(d_x, x_pitch) && on_chunks(d_residual, residual_pitch) && on_chunks(d_sum, sum_pitch) &&
-					    on_chunks(d_out, out_pitch) && on_chunks(d_q, q_pitch));
+	const flow_t flow = flow_of(n_rows * (bytes * (1u + !!d_residual + !!d_sum + !!d_out) + (d_q ? width : 0)));
 	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
 		constexpr uint32_t V = decltype(v)::value;
@@ -615,8 +613,7 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
 	const uint32_t blocks = grad_blocks(n_rows);
 	float *partial = d_dgain ? static_cast<float *>(d_work) : nullptr;
 	if (n_rows != 0) {
-		const flow_t flow = flow_of(n_rows * bytes * (3u + !!d_dsum), on_chunks(d_dout, dout_pitch) && on_chunks(d_s, s_pitch) &&
-											      on_chunks(d_dsum, dsum_pitch) && on_chunks(d_dx, dx_pitch));
+		const flow_t flow = flow_of(n_rows * bytes * (3u + !!d_dsum));
 		with_row_type(type, width, [&](auto element, auto v) {
 			using T = decltype(element);
 			constexpr uint32_t V = decltype(v)::value;

@@ -258,13 +258,6 @@ template <typename F> inline void with_row_type(int type, uint32_t width, F f)
 	}
 }
 
-/* Whether each chunk of the rows lies within a line.  What goes past the caches has to: a chunk across two lines would fetch both
- * again for its neighbour (sums of rows of 4092 bytes: 15.9 us for 8.3). */
-inline bool on_chunks(const void *p, uint64_t pitch)
-{
-	return ((reinterpret_cast<uintptr_t>(p) | pitch) & 15u) == 0;
-}
-
 /*
  * By what a call reads and writes.  Inputs that fill much of the memory-side cache of 256 MB have not stayed there since they were
  * made, and read past the caches they come faster; outputs of a call that overflows it will not be found there either.  Measured on
@@ -273,10 +266,12 @@ inline bool on_chunks(const void *p, uint64_t pitch)
  *   their gradient                 71 MB 14.8 17.3 16.4   143 MB 32.9 27.2 29.9    571 MB 118.1 118.3 113.4   2283 MB 454 460 444
  *   norms of 8192 values to e4m3   59 MB 13.7 14.1 14.1   236 MB 46.1 43.8 42.6    472 MB 84.4 82.8 80.3      944 MB 164.9 164.3 157.5
  *   gradients of norms of 4096     67 MB 17.4 19.1 -      134 MB 32.2 29.1 29.9    268 MB 54.9 48.4 50.9      537 MB 102.4 96.8 94.4
+ * Rows that do not start on chunks go the same way (sums of rows of 8190 bytes, 1343 MB, 262 268 247; their norms' gradient, 537 MB, 131 132
+ * 122), although what lies across two lines is fetched twice where the caches would have had it (43 MB of rows of 4092 bytes 8.3 15.9 -).
  */
-inline flow_t flow_of(uint64_t moved, bool aligned)
+inline flow_t flow_of(uint64_t moved)
 {
-	return !aligned || moved <= (100u << 20) ? STREAM_NONE : moved <= (256u << 20) ? STREAM_LOADS : STREAM_BOTH;
+	return moved <= (100u << 20) ? STREAM_NONE : moved <= (256u << 20) ? STREAM_LOADS : STREAM_BOTH;
 }
 
 /* The kernel of a flow */
