@@ -256,10 +256,11 @@ int ofi_amd_token_combine_grad(const void *d_dout, uint64_t dout_pitch, const vo
 		return -EINVAL;
 	}
 	const uint64_t pairs = (uint64_t)n_tokens * top_k, named = pairs < max_rows ? pairs : max_rows;
-	/* As many rows are written as read.  Where those do not start on 16 bytes and do not stay in the caches, streaming costs more than it
-	 * gives: rows of 8190 bytes, 2283 MB, us with neither 485, streaming loads 522, both 525 (285 MB 66.8 67.7 -, 143 MB 36.6 31.5 -) */
+	/* As many rows are written as read, and their ends share lines with other rows.  Where the rows do not start on 64 bytes and do not
+	 * stay in the caches, streaming costs more than it gives: 2280 MB, us with neither, streaming loads, both: rows of 8190 bytes
+	 * 485 522 525, of 8176 465 491 484, of 8128 457 472 452 (285 MB of 8190 66.8 67.7 -, 143 MB 36.6 31.5 -) */
 	const uint64_t moved = (named * (!!d_dweight + !!d_drows) + n_tokens) * bytes;
-	const bool aligned = ((reinterpret_cast<uintptr_t>(d_drows) | drows_pitch) & 15u) == 0;
+	const bool aligned = ((reinterpret_cast<uintptr_t>(d_drows) | drows_pitch) & 63u) == 0;
 	const flow_t flow = flow_of(moved) == STREAM_BOTH && !aligned ? STREAM_NONE : flow_of(moved);
 	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
