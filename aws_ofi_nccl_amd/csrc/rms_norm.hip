@@ -146,16 +146,30 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_kernel(const T *x, c
 	const uint32_t wanted = LANES < 64 ? first + (blockIdx.x * blockDim.x + threadIdx.x) / LANES : first + blockIdx.x;
 	const bool in = LANES == 64 || wanted < n_rows;
 	const uint64_t row = in ? wanted : n_rows - 1;
+	const T *xr = row_at(x, x_pitch, row), *rr = residual ? row_at(residual, residual_pitch, row) : nullptr;
+	const uint32_t x_lag = lag_of<V>(xr), r_lag = lag_of<V>(rr);
 	raw_t<T, V> c[R], d[R];
+	uint32_t c_rest[R], d_rest[R];
 #pragma unroll
 	for (int k = 0; k < R; k++) {
-		c[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(x, x_pitch, row) + place_of<V>((k * B + lane) * V, width).from);
+		c[k] = load_raw<FLOW != STREAM_NONE, T, V>(xr + place_of<V>((k * B + lane) * V, width).from - x_lag);
 	}
-	if (residual) {
+	if (rr) {
 #pragma unroll
 		for (int k = 0; k < R; k++) {
-			d[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(residual, residual_pitch, row) +
-								   place_of<V>((k * B + lane) * V, width).from);
+			d[k] = load_raw<FLOW != STREAM_NONE, T, V>(rr + place_of<V>((k * B + lane) * V, width).from - r_lag);
+		}
+	}
+	if (x_lag) {
+#pragma unroll
+		for (int k = 0; k < R; k++) {
+			c_rest[k] = load_rest<T, V, LANES>(xr + place_of<V>((k * B + lane) * V, width).from, x_lag, (k * B + lane) * V, width);
+		}
+	}
+	if (r_lag) {
+#pragma unroll
+		for (int k = 0; k < R; k++) {
+			d_rest[k] = load_rest<T, V, LANES>(rr + place_of<V>((k * B + lane) * V, width).from, r_lag, (k * B + lane) * V, width);
 		}
 	}
 	float v[R][V];
@@ -163,9 +177,11 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_kernel(const T *x, c
 #pragma unroll
 	for (int k = 0; k < R; k++) {
 		const uint32_t skip = place_of<V>((k * B + lane) * V, width).skip;
+		catch_up<T, V, LANES>(c[k], c_rest[k], x_lag, (k * B + lane) * V, width);
 		to_floats<T, V>(c[k], skip, v[k]);
-		if (residual) {
+		if (rr) {
 			float f[V];
+			catch_up<T, V, LANES>(d[k], d_rest[k], r_lag, (k * B + lane) * V, width);
 			to_floats<T, V>(d[k], skip, f);
 #pragma unroll
 			for (uint32_t i = 0; i < V; i++) {
@@ -264,13 +280,31 @@ void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s, const float *_
 	for (uint32_t i = 0; i < V; i++) {
 		dg[i] = 0.0f;
 	}
-	raw_t<T, V> dc, sc, pc;
+	const uint32_t at = threadIdx.x * V;
+	struct asked_t { /* a chunk on its way */
+		raw_t<T, V> c;
+		uint32_t rest, lag;
+	} dc, sc, pc;
 	float rstd = 0.0f;
+	auto ask_one = [&](asked_t &a, const T *r) {
+		a.lag = lag_of<V>(r);
+		a.c = load_raw<FLOW != STREAM_NONE, T, V>(r + here.from - a.lag);
+	};
+	auto ask_rest = [&](asked_t &a, const T *r) { a.rest = load_rest<T, V, 64>(r + here.from, a.lag, at, width); };
 	auto ask = [&](uint64_t row) {
-		dc = load_raw<FLOW != STREAM_NONE, T, V>(row_at(dout, dout_pitch, row) + here.from);
-		sc = load_raw<FLOW != STREAM_NONE, T, V>(row_at(s, s_pitch, row) + here.from);
-		if (dsum) {
-			pc = load_raw<FLOW != STREAM_NONE, T, V>(row_at(dsum, dsum_pitch, row) + here.from);
+		const T *dr = row_at(dout, dout_pitch, row), *sr = row_at(s, s_pitch, row);
+		const T *pr = dsum ? row_at(dsum, dsum_pitch, row) : nullptr;
+		ask_one(dc, dr);
+		ask_one(sc, sr);
+		if (pr) {
+			ask_one(pc, pr);
+		} else {
+			pc.lag = 0;
+		}
+		if (dc.lag | sc.lag | pc.lag) {
+			ask_rest(dc, dr);
+			ask_rest(sc, sr);
+			ask_rest(pc, pr);
 		}
 		rstd = rstds[row];
 	};
@@ -282,12 +316,15 @@ void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s, const float *_
 	uint32_t turn = 0;
 	for (uint64_t first = (uint64_t)blockIdx.x * blockDim.y; first < n_rows; first += stride, row += stride, turn ^= 1u) {
 		const bool in = row < n_rows;
-		raw_t<T, V> p0 = pc;
+		raw_t<T, V> p0 = pc.c;
 		const float r0 = rstd;
 		float d[V], h[V], along = 0.0f;
 		if (in) {
-			to_floats<T, V>(dc, here.skip, d);
-			to_floats<T, V>(sc, here.skip, h);
+			catch_up<T, V, 64>(dc.c, dc.rest, dc.lag, at, width);
+			catch_up<T, V, 64>(sc.c, sc.rest, sc.lag, at, width);
+			catch_up<T, V, 64>(p0, pc.rest, pc.lag, at, width);
+			to_floats<T, V>(dc.c, here.skip, d);
+			to_floats<T, V>(sc.c, here.skip, h);
 #pragma unroll
 			for (uint32_t i = 0; i < V; i++) {
 				h[i] *= r0;

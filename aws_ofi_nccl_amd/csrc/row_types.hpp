@@ -106,6 +106,42 @@ template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v)
 	return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 
+/*
+ * Rows of two-byte elements that start between two words.  Loads there run at little over half the rate, so that a chunk is read from
+ * the word in front of it (load_raw of lag elements earlier).  Its last element is then the next lane's first; where the next lane is
+ * another wavefront's or another row's, or ends with the row, a load of its own brings the word (load_rest, for few lanes).  Nothing
+ * beyond the words that hold the chunk's ends is read.
+ */
+template <uint32_t V, typename T> __device__ __forceinline__ uint32_t lag_of(const T *row)
+{
+	return sizeof(T) == 2 && V > 1 ? (uint32_t)(reinterpret_cast<uintptr_t>(row) >> 1) & 1u : 0u;
+}
+
+/* LANES of a row in a wavefront; chunk: where the lane's chunk lies, at: its column */
+template <typename T, uint32_t V, uint32_t LANES>
+__device__ __forceinline__ uint32_t load_rest(const T *chunk, uint32_t lag, uint32_t at, uint32_t width)
+{
+	const bool alone = (threadIdx.x & (LANES - 1)) == LANES - 1 || at + 2 * V > width;
+	return V > 1 && lag && alone ? *reinterpret_cast<const uint32_t *>(chunk + V - 1) : 0u;
+}
+
+/* All lanes of the wavefront call */
+template <typename T, uint32_t V, uint32_t LANES>
+__device__ __forceinline__ void catch_up(raw_t<T, V> &c, uint32_t rest, uint32_t lag, uint32_t at, uint32_t width)
+{
+	if constexpr (sizeof(T) == 2 && V > 1) {
+		u32x4_t w = __builtin_bit_cast(u32x4_t, c);
+		const bool alone = (threadIdx.x & (LANES - 1)) == LANES - 1 || at + 2 * V > width;
+		const uint32_t next = dpp<0x130>(w.x); /* wave_shl:1 */
+		const uint32_t end = alone ? rest : next;
+		if (lag) {
+			w = u32x4_t{ __builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16),
+				     __builtin_amdgcn_alignbit(w.w, w.z, 16), __builtin_amdgcn_alignbit(end, w.w, 16) };
+			c = __builtin_bit_cast(raw_t<T, V>, w);
+		}
+	}
+}
+
 /* Rows of 16 lanes exchanged: {a0, b0, a2, b2} and {a1, b1, a3, b3} */
 __device__ __forceinline__ void swap_rows16(uint32_t &a, uint32_t &b)
 {

@@ -43,7 +43,9 @@ def parts(n, width):
 
 @pytest.mark.parametrize("n,width,pitch,kind,group", [(4000, 8190, 8192, "bf16", 128), (9000, 8192, 8192, "bf16", 128),
                                                       (3000, 16384, 16384, "bf16", 0), (20000, 2044, 2048, "f32", 64),
-                                                      (60000, 1024, 1024, "f16", 256), ((1 << 21) + 5, 16, 16, "f16", 0)])
+                                                      (60000, 1024, 1024, "f16", 256), ((1 << 21) + 5, 16, 16, "f16", 0),
+                                                      (9000, 4001, 4003, "bf16", 0), (50000, 250, 251, "f16", 64),
+                                                      (100000, 97, 101, "bf16", 32), (7000, 8191, 8191, "f16", 128)])
 def test_norms(lib, gpu, n, width, pitch, kind, group):
     dtype, code, u = TYPES[kind]
     g = gen(n)
@@ -80,7 +82,8 @@ def test_norms(lib, gpu, n, width, pitch, kind, group):
                                                          (9000, 8192, 8192, "bf16", "dout"), (70000, 512, 512, "f32", None),
                                                          (200000, 250, 256, "f16", None), (3000, 16380, 16384, "bf16", "dout"),
                                                          (2000, 12288, 12288, "f32", "dsum"), (600, 32768, 32768, "f32", None),
-                                                         (1500, 32000, 32000, "bf16", "dsum")])
+                                                         (1500, 32000, 32000, "bf16", "dsum"), (9000, 4001, 4003, "bf16", "dsum"),
+                                                         (50000, 1021, 1023, "f16", None)])
 def test_gradients_of_norms(lib, gpu, n, width, pitch, kind, in_place):
     dtype, code, u = TYPES[kind]
     g = gen(n)
