@@ -13,13 +13,15 @@ GUARD = 0xA5
 
 class Rows:
     """n rows of `width` elements, `pad` elements apart beyond the width, `shift` elements into an allocation filled with
-    guard bytes.  .t is the tensor of the rows; untouched() tells whether every byte outside them is as it was."""
+    guard bytes (Rows.guard).  .t is the tensor of the rows; untouched() tells whether every byte outside them is as it was."""
+
+    guard = GUARD
 
     def __init__(self, n, width, dtype, pad=0, shift=0, values=None):
         size = torch.empty((), dtype=dtype).element_size()
         self.n, self.width, self.pad, self.pitch = n, width, pad, (width + pad) * size
         count = shift + n * (width + pad) + 64
-        self.bytes = torch.full((count * size,), GUARD, dtype=torch.uint8, device="cuda")
+        self.bytes = torch.full((count * size,), self.guard, dtype=torch.uint8, device="cuda")
         self.shift = shift
         whole = self.bytes.view(dtype) if size > 1 else self.bytes.view(torch.uint8).view(dtype)
         self.t = whole[shift:shift + n * (width + pad)].view(n, width + pad)[:, :width] if n else whole[:0].view(0, max(1, width))
@@ -34,8 +36,8 @@ class Rows:
         rest = self.bytes.clone()
         if self.n:
             lo = self.shift * self.size
-            rest[lo:lo + self.n * self.pitch].view(self.n, self.pitch)[:, :self.width * self.size] = GUARD
-        return bool((rest == GUARD).all())
+            rest[lo:lo + self.n * self.pitch].view(self.n, self.pitch)[:, :self.width * self.size] = self.guard
+        return bool((rest == self.guard).all())
 
 
 def ptr(t):

@@ -239,6 +239,16 @@ def test_gradient_against_differences(lib, gpu):
     assert abs(by_g - (got["dgain"] * dg).sum().item()) <= 1e-5 * (got["dgain"] * dg).abs().sum().item()
 
 
+@pytest.mark.parametrize("width", [5, 8, 100, 129, 255, 520, 1001, 2047, 4099, 9001])
+@pytest.mark.parametrize("pad,shift", [(3, 1), (2, 1), (9, 0)])
+def test_what_lies_beside_the_rows_does_not_reach_them(lib, gpu, monkeypatch, width, pad, shift):
+    """Bytes of 0xff are NaN in every type."""
+    monkeypatch.setattr(Rows, "guard", 0xFF)
+    for kind in ("bf16", "f16", "f32"):
+        check_norm(lib, 7, width, kind, 32, pad=pad, shift=shift, seed=width)
+        check_grad(lib, 7, width, kind, pad=pad, shift=shift, seed=width)
+
+
 def test_no_rows(lib, gpu):
     x, gain, dgain = Rows(0, 8, torch.float32), torch.ones(8, device="cuda"), torch.full((8,), 5.0, device="cuda")
     assert norm(lib, x, gain, 8, "f32", total=x) == 0

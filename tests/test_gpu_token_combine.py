@@ -96,6 +96,17 @@ def test_pitches_and_alignments(lib, gpu, pad, shift):
         check_combine(lib, 60, 6, 1160, kind, pad=pad, shift=shift)
 
 
+@pytest.mark.parametrize("width", [5, 8, 100, 513, 1001, 2047, 4099])
+@pytest.mark.parametrize("pad,shift", [(3, 1), (9, 0)])
+def test_what_lies_beside_the_rows_does_not_reach_them(lib, gpu, monkeypatch, width, pad, shift):
+    """Bytes of 0xff are NaN in every type."""
+    monkeypatch.setattr(Rows, "guard", 0xFF)
+    for kind in TYPES:
+        check_combine(lib, 9, 5, width, kind, pad=pad, shift=shift, seed=width)
+        check_grad(lib, 9, 5, width, kind, pad=pad, shift=shift, seed=width)
+        check_grad(lib, 9, 5, width, kind, pad=pad, shift=shift, seed=width, in_place=True, missing=0.0)
+
+
 def test_the_output_may_replace_the_addend(lib, gpu):
     check_combine(lib, 33, 8, 1025, "bf16", in_place=True)
 
