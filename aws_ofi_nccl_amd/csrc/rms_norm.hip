@@ -22,6 +22,7 @@ constexpr uint32_t kMaxWidth = 32768;
 constexpr int kMostWaves = 16;
 constexpr int kGradWaves = 8;
 constexpr uint32_t kGradBlocks = 512;
+constexpr uint32_t kFewRows = 256, kFewWaves = 16;
 constexpr uint32_t kRowsOfLaunch = 1u << 21; /* with 1024 lanes each within the 32 bits of a launch's size */
 
 struct norm_out_t {
@@ -482,6 +483,73 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(con
 	}
 }
 
+/*
+ * Few rows, in one launch: rstd is an input, so that dg needs nothing of dx.  The first n_rows workgroups make a row of dx each, those
+ * behind them 64 columns of dg, their wavefronts at the rows by turns.  They read dout too, so that dx may not be dout.  Rows of 4096
+ * bfloat16, us a call in one launch and in two: 1 to 128 rows 10.0 and 13.9, 256 10.4 and 13.8, 384 12.0 and 13.8, 512 17 and 13.7.
+ */
+template <typename T, uint32_t V>
+__global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_few_kernel(const T *__restrict__ dout, const T *__restrict__ s,
+									    const float *__restrict__ rstds, const void *__restrict__ gain,
+									    const T *dsum, uint64_t dout_pitch, uint64_t s_pitch,
+									    uint64_t dsum_pitch, uint32_t n_rows, uint32_t width,
+									    bool gain_f32, T *dx, uint64_t dx_pitch,
+									    float *__restrict__ dgain)
+{
+	__shared__ float sums[kMostWaves][64];
+	__shared__ uint32_t part[kMostWaves];
+	const uint32_t waves = blockDim.x >> 6;
+	if (blockIdx.x < n_rows) {
+		const uint64_t row = blockIdx.x;
+		const uint32_t at = threadIdx.x * V;
+		const place_t here = place_of<V>(at, width);
+		const raw_t<T, V> dc = load_raw<false, T, V>(row_at(dout, dout_pitch, row) + here.from);
+		const raw_t<T, V> sc = load_raw<false, T, V>(row_at(s, s_pitch, row) + here.from);
+		raw_t<T, V> pc = dc;
+		if (dsum) {
+			pc = load_raw<false, T, V>(row_at(dsum, dsum_pitch, row) + here.from);
+		}
+		const float rstd = rstds[row];
+		float g[V], d[V], h[V], along = 0.0f;
+		load_gain<T, V>(gain, gain_f32, here.from, g);
+		to_floats<T, V>(dc, here.skip, d);
+		to_floats<T, V>(sc, here.skip, h);
+#pragma unroll
+		for (uint32_t i = 0; i < V; i++) {
+			h[i] *= rstd;
+			d[i] *= g[i];
+			along = i < here.skip ? along : __builtin_fmaf(d[i], h[i], along);
+		}
+		const float mean = block_sum(along, part, waves) / (float)width;
+		if (at < width) {
+			float r[V];
+			to_floats<T, V>(pc, 0, r);
+#pragma unroll
+			for (uint32_t i = 0; i < V; i++) {
+				r[i] = __builtin_fmaf(rstd, __builtin_fmaf(-h[i], mean, d[i]), dsum ? r[i] : 0.0f);
+			}
+			store_piece<false, T, V>(row_at(dx, dx_pitch, row) + here.from, here.skip, r);
+		}
+		return;
+	}
+	const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, column = (blockIdx.x - n_rows) * 64u + lane;
+	float total = 0.0f;
+	if (column < width) {
+#pragma unroll 8
+		for (uint32_t row = wave; row < n_rows; row += waves) {
+			total = __builtin_fmaf((float)row_at(dout, dout_pitch, row)[column], (float)row_at(s, s_pitch, row)[column] * rstds[row], total);
+		}
+	}
+	sums[wave][lane] = total;
+	__syncthreads();
+	if (wave == 0 && column < width) {
+		for (uint32_t w = 1; w < waves; w++) {
+			total += sums[w][lane];
+		}
+		dgain[column] = total;
+	}
+}
+
 /* kGainColumns columns of a workgroup, its lanes at the parts by turns, with all of their loads on the way at once: 5 us for 512 parts of
  * 4096 (64 columns 5.5), most of it the way of fresh lines from the other dies */
 constexpr uint32_t kGainColumns = 32, kGainTurns = 1024 / kGainColumns, kPartsOfLane = kGradBlocks / kGainTurns;
@@ -646,6 +714,19 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
 			    !rows_ok(d_rstd, 0, 1, 0, 4) || !rows_ok(d_gain, 0, 1, 0, gain_type == OFI_AMD_FLOAT32 ? 4 : size) ||
 			    (d_dsum && !rows_ok(d_dsum, dsum_pitch, n_rows, bytes, size)) || !rows_ok(d_dx, dx_pitch, n_rows, bytes, size))) {
 		return -EINVAL;
+	}
+	const uint32_t size_chunk = width >= 16 / size ? 16 / size : 1, all_chunks = (width + size_chunk - 1) / size_chunk;
+	if (d_dgain && n_rows != 0 && n_rows <= kFewRows && all_chunks <= 64 * kMostWaves && d_dx != d_dout) {
+		with_row_type(type, width, [&](auto element, auto v) {
+			using T = decltype(element);
+			const uint32_t waves = (all_chunks + 63) / 64;
+			launch_kernel(rms_norm_grad_few_kernel<T, decltype(v)::value>, dim3(n_rows + (width + 63) / 64),
+				      dim3(64 * (waves < kFewWaves ? kFewWaves : waves)), 0, as_stream(stream), static_cast<const T *>(d_dout),
+				      static_cast<const T *>(d_s), d_rstd, d_gain, static_cast<const T *>(d_dsum), dout_pitch, s_pitch, dsum_pitch,
+				      n_rows, width, gain_type == OFI_AMD_FLOAT32, static_cast<T *>(d_dx), dx_pitch, d_dgain);
+		});
+		OFI_AMD_HIP_TRY(hipGetLastError());
+		return 0;
 	}
 	const uint32_t blocks = grad_blocks(n_rows);
 	float *partial = d_dgain ? static_cast<float *>(d_work) : nullptr;

@@ -213,8 +213,15 @@ def test_gradient_pitches(lib, gpu, rows, width, pad, shift):
 
 
 @pytest.mark.parametrize("in_place", ["dout", "dsum"])
-def test_the_gradient_may_replace_an_input(lib, gpu, in_place):
-    check_grad(lib, 1100, 1030, "bf16", in_place=in_place)
+@pytest.mark.parametrize("rows,width", [(1100, 1030), (40, 1030), (256, 4099), (3, 10000), (2, 30000)])
+def test_the_gradient_may_replace_an_input(lib, gpu, in_place, rows, width):
+    check_grad(lib, rows, width, "bf16", in_place=in_place)
+
+
+@pytest.mark.parametrize("rows", [1, 17, 255, 256, 257])
+@pytest.mark.parametrize("width", [1, 7, 64, 65, 1999, 8192, 8193])
+def test_gradient_of_few_rows(lib, gpu, rows, width):
+    check_grad(lib, rows, width, "f16", pad=rows % 3, seed=rows + width)
 
 
 def test_gradient_without_the_gains_and_with_a_gain_in_32_bits(lib, gpu):
