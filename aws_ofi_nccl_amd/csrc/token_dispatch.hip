@@ -21,7 +21,7 @@ using namespace ofi_amd;
 constexpr uint32_t kMaxExperts = 1024;
 constexpr uint32_t kMaxTopK = 64;
 constexpr uint32_t kMaxRowBytes = 1u << 24;
-constexpr uint32_t kTokensOfLaunch = 1u << 22;
+constexpr uint32_t kTokensOfLaunch = 1u << 21;
 constexpr int kSortWaves = 16;
 constexpr uint32_t kMostRounds = 8; /* pairs of a lane of the sort */
 constexpr uint32_t kManyTiles = 64;
@@ -302,12 +302,65 @@ __device__ __forceinline__ void copy_rows(uint32_t token, uint32_t wave, uint32_
 	}
 }
 
-/* One workgroup per token */
-__global__ __launch_bounds__(64 * kMostWaves) void token_rows_kernel(const int32_t *__restrict__ row_of, uint32_t first, uint32_t top_k,
-								     uint32_t row_waves, uint32_t max_rows, rows_t a, rows_t b)
+/*
+ * Short rows (scales) by their place: a wavefront has rows in order, so that their lines are written whole by one die, where every
+ * token's own copy would leave pieces of lines to eight.  The rows read for them lie in the caches.  A row has a power of two of
+ * lanes, a wavefront two rounds of kShortAtOnce rows for each of them.  us a call with the tokens' own copies and so: 16,384 x 8 rows of
+ * 7168 bytes and 224 247 and 229, of 5120 and 160 (4096 tokens) 48.9 and 46.7, 32,768 x 8 of 256 and 8 42 and 31, 16,384 x 8 of 8192
+ * and 256, whose lines are whole anyway, 256 and 260.
+ */
+constexpr uint32_t kShortBytes = 255, kShortAtOnce = 8;
+__host__ __device__ inline uint32_t lanes_of_short(uint32_t bytes)
 {
+	uint32_t lanes = 1;
+	while (lanes * 4 < bytes) {
+		lanes *= 2;
+	}
+	return lanes;
+}
+__device__ __forceinline__ void gather_rows(uint64_t wave, const int32_t *__restrict__ pair_of, uint32_t top_k, uint32_t max_rows, const rows_t &b)
+{
+	const uint32_t lane = threadIdx.x & 63u, words = b.bytes >> 2, lanes = lanes_of_short(b.bytes);
+	const uint32_t rows = 64u / lanes, word = lane & (lanes - 1u), mine = lane / lanes;
+	for (uint32_t round = 0; round < 2; round++) {
+		const uint64_t r0 = (wave * 2 + round) * kShortAtOnce * rows + mine;
+		uint32_t v[kShortAtOnce];
+		int32_t pair[kShortAtOnce];
+#pragma unroll
+		for (uint32_t i = 0; i < kShortAtOnce; i++) {
+			pair[i] = r0 + i * rows < max_rows && word < words ? pair_of[r0 + i * rows] : -1;
+		}
+#pragma unroll
+		for (uint32_t i = 0; i < kShortAtOnce; i++) {
+			if (pair[i] >= 0) {
+				v[i] = reinterpret_cast<const uint32_t *>(b.from + (uint32_t)pair[i] / top_k * b.from_pitch)[word];
+			}
+		}
+#pragma unroll
+		for (uint32_t i = 0; i < kShortAtOnce; i++) {
+			if (pair[i] >= 0) {
+				reinterpret_cast<uint32_t *>(b.to + (r0 + i * rows) * b.to_pitch)[word] = v[i];
+			}
+		}
+	}
+}
+
+/* The first workgroups have the short rows, those behind them blockDim.y tokens each */
+__global__ __launch_bounds__(64 * kMostWaves) void token_rows_kernel(const int32_t *__restrict__ row_of,
+								     const int32_t *__restrict__ pair_of, uint32_t first, uint32_t n_tokens,
+								     uint32_t top_k, uint32_t row_waves, uint32_t max_rows,
+								     uint32_t short_blocks, uint32_t short_first, rows_t a, rows_t b)
+{
+	if (blockIdx.x < short_blocks) {
+		const uint32_t waves = (blockDim.x >> 6) * blockDim.y, wave = threadIdx.y * (blockDim.x >> 6) + (threadIdx.x >> 6);
+		gather_rows((uint64_t)(short_first + blockIdx.x) * waves + wave, pair_of, top_k, max_rows, b);
+		return;
+	}
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-	const uint32_t token = first + blockIdx.x;
+	const uint32_t token = first + (blockIdx.x - short_blocks) * blockDim.y + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.y);
+	if (token >= n_tokens) {
+		return;
+	}
 	const int32_t *rows = row_of + (uint64_t)token * top_k;
 	copy_rows(token, wave, row_waves, a, b, top_k, max_rows, [&](uint32_t k) { return (uint32_t)rows[k]; });
 }
@@ -518,9 +571,26 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 				      kSortWaves * (n_experts + 1) * sizeof(uint32_t), as_stream(stream), expert, (uint32_t)n_pairs, n_experts, tiles,
 				      max_rows, static_cast<const uint32_t *>(d_work), d_offset, d_row_of, d_pair_of, err);
 		});
-		for (uint32_t first = 0; d_x && first < n_tokens; first += kTokensOfLaunch) {
-			launch_kernel(token_rows_kernel, dim3(n_tokens - first < kTokensOfLaunch ? n_tokens - first : kTokensOfLaunch),
-				      dim3(64 * (row_waves + more)), 0, as_stream(stream), d_row_of, first, top_k, row_waves, max_rows, a, b);
+		if (!d_x) {
+			return; /* the table alone */
+		}
+		/* the scales by their place where the table says which pair is there */
+		const bool apart = more && d_pair_of && scale_bytes <= kShortBytes &&
+				   ((reinterpret_cast<uintptr_t>(d_scale) | reinterpret_cast<uintptr_t>(d_scale_rows) | scale_pitch | scale_rows_pitch |
+				     scale_bytes) & 3u) == 0;
+		const uint32_t waves = row_waves + (apart ? 0 : more), tokens = waves <= 2 ? 4 / waves : 1;
+		/* workgroups of the short rows, as many with each launch as it has of the tokens */
+		const uint32_t each = waves * tokens * 2 * kShortAtOnce * (apart ? 64 / lanes_of_short(scale_bytes) : 1);
+		const uint32_t most = n_pairs < max_rows ? (uint32_t)n_pairs : max_rows, all_short = apart ? (most + each - 1) / each : 0;
+		const uint32_t launches = (n_tokens + kTokensOfLaunch - 1) / kTokensOfLaunch;
+		uint32_t short_first = 0;
+		for (uint32_t first = 0; first < n_tokens; first += kTokensOfLaunch) {
+			const uint32_t n = n_tokens - first < kTokensOfLaunch ? n_tokens - first : kTokensOfLaunch;
+			const uint32_t part = (all_short + launches - 1) / launches, left = all_short - short_first;
+			const uint32_t short_blocks = left < part ? left : part;
+			launch_kernel(token_rows_kernel, dim3(short_blocks + (n + tokens - 1) / tokens), dim3(64 * waves, tokens), 0, as_stream(stream),
+				      d_row_of, d_pair_of, first, first + n, top_k, row_waves, max_rows, short_blocks, short_first, a, b);
+			short_first += short_blocks;
 		}
 	};
 	if (expert_type == OFI_AMD_INT64) {

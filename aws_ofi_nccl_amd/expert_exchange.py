@@ -144,8 +144,9 @@ def layer(lib, link, x, residual, gain, ids, weight, up, down, dout=None):
                                   None, 0, *_rows(q), *_rows(scale), GROUP, _ptr(rstd), _stream()), "rms_norm")
     offset = torch.empty(experts + 1, dtype=torch.int32, device="cuda")
     row_of = torch.empty(tokens, top_k, dtype=torch.int32, device="cuda")
+    pair_of = torch.empty(pairs, dtype=torch.int32, device="cuda")
     work = torch.empty(max(16, lib.ofi_amd_token_dispatch_work_bytes(tokens, top_k, experts)), dtype=torch.uint8, device="cuda")
-    _m.check(lib.ofi_amd_token_dispatch(_ptr(ids), _m.INT64, tokens, top_k, experts, pairs, _ptr(offset), _ptr(row_of), None, *_rows(q),
+    _m.check(lib.ofi_amd_token_dispatch(_ptr(ids), _m.INT64, tokens, top_k, experts, pairs, _ptr(offset), _ptr(row_of), _ptr(pair_of), *_rows(q),
                                         *_rows(own.q), width, *_rows(scale), *_rows(own.scale), groups * 4, _ptr(work), work.numel(),
                                         _stream()), "token_dispatch")
     first = offset.cpu().tolist()                     # where each expert's rows begin: the host plans the puts

@@ -1003,7 +1003,8 @@ int ofi_amd_rms_norm_grad(const void *d_dout, uint64_t dout_pitch, const void *d
  * [0, n_experts) is a pair without a row: a choice that is not taken, or an expert that is elsewhere.
  *   d_offset[0..n_experts]   the first row of each expert and the rows in all
  *   d_row_of[pair]           the pair's row or -1
- *   d_pair_of[0..max_rows)   (optional) the row's pair, or -1 behind the last
+ *   d_pair_of[0..max_rows)   (optional) the row's pair, or -1 behind the last; short rows of scales
+ *                            in whole words are copied faster where it is there
  * and copies row_bytes of token t's row of d_x to the row of each of its pairs in d_rows, and
  * scale_bytes of its row of d_scale to d_scale_rows; either copy may be left out (NULL; no scales
  * without rows).  Rows behind the last pair's are not written.  Pairs whose row would be max_rows or

@@ -116,7 +116,11 @@ int tokens()
 			}
 			const uint32_t pairs = n * top_k, experts = 1 + n % 1024;
 			for (const uint32_t bytes : { 1u, 100u, 4096u, 14336u, 16384u, 1u << 20 }) {
-				uint64_t placed = 0, copied = 0, counted = 0;
+				/* scales by their place, by token, too long for the former */
+				const uint32_t scale = bytes == 100 ? 252 : bytes == 16384 ? 256 : 4;
+				const bool apart = bytes != 1 && scale < 256;
+				const uint64_t per = scale == 252 ? 16 : 1024; /* short rows of a wavefront */
+				uint64_t placed = 0, copied = 0, counted = 0, short_rows = 0;
 				bool few = false;
 				on_launch = [&](const launch_t &l) {
 					sane(l);
@@ -131,20 +135,29 @@ int tokens()
 						CHECK(l.shared == 64u * (experts + 1) && l.arg<uint32_t>(3) == l.grid.x);
 						CHECK(counted == (l.grid.x > 1 ? placed : 0));
 					} else {
-						CHECK(is(l, "token_rows_kernel") && placed >= pairs && l.arg<uint32_t>(1) == copied);
-						CHECK(l.block.x <= 512 && l.block.x >= 64 * (l.arg<uint32_t>(3) + 1)); /* and the scales' */
-						copied += l.grid.x;
+						const uint32_t waves = l.arg<uint32_t>(5), shorts = l.arg<uint32_t>(7), end = l.arg<uint32_t>(3);
+						CHECK(is(l, "token_rows_kernel") && placed >= pairs && l.arg<uint32_t>(2) == copied && end <= n);
+						CHECK(l.block.x * l.block.y <= 512 && l.arg<uint32_t>(8) == short_rows / (l.block.x / 64 * l.block.y * per));
+						CHECK(l.block.x == 64 * (waves + (apart ? 0 : 1)) && (apart || shorts == 0));
+						CHECK((uint64_t)(l.grid.x - shorts) * l.block.y >= end - copied);
+						copied = end;
+						short_rows += (uint64_t)shorts * (l.block.x / 64) * l.block.y * per;
 					}
 				};
 				const uint64_t need = ofi_amd_token_dispatch_work_bytes(n, top_k, experts);
 				CHECK(ofi_amd_token_dispatch(p, OFI_AMD_INT64, n, top_k, experts, pairs, reinterpret_cast<int32_t *>(p),
-							     reinterpret_cast<int32_t *>(p), nullptr, p, pitch, p, pitch, bytes, p, pitch, p, pitch, 4, p,
-							     need, nullptr) == 0);
-				CHECK(copied == n && placed >= pairs);
+							     reinterpret_cast<int32_t *>(p), bytes == 1 ? nullptr : reinterpret_cast<int32_t *>(p), p,
+							     pitch, p, pitch, bytes, p, pitch, p, pitch, scale, p, need, nullptr) == 0);
+				CHECK(copied == n && placed >= pairs && (few || !apart || short_rows >= pairs));
 				CHECK(few || need == (placed > 8192 ? placed / 1024 / (pairs <= 65536 ? 1 : pairs <= 131072 ? 2 : pairs <= 262144 ? 4 : 8) *
 									      experts * 4
 								    : 0));
 			}
+			int rows_copied = 0; /* the table alone */
+			on_launch = [&](const launch_t &l) { rows_copied += !is(l, "token_count_kernel") && !is(l, "token_place_kernel"); };
+			CHECK(ofi_amd_token_dispatch(p, OFI_AMD_INT32, n, top_k, experts, 7, reinterpret_cast<int32_t *>(p), reinterpret_cast<int32_t *>(p),
+						     nullptr, nullptr, 0, nullptr, 0, 0, nullptr, 0, nullptr, 0, 0, p, ~0ull, nullptr) == 0);
+			CHECK(rows_copied == 0);
 			for (const auto &t : kTypes) {
 				for (const uint32_t width : { 1u, 8u, 60u, 257u, 4096u, 5000u, 1u << 18 }) {
 					uint64_t at = 0;
@@ -208,6 +221,13 @@ int refusals()
 	for (const uint32_t group : { 1u, 16u, 48u, 100u, 512u }) {
 		CHECK(norm(p, 256, p, bf, 4, 64, bf, 0, p, p, f, group) == -EINVAL);
 	}
+	/* nothing to do, or next to nothing */
+	CHECK(ofi_amd_token_dispatch(nullptr, OFI_AMD_INT32, 0, 2, 8, 0, i, nullptr, nullptr, nullptr, 0, nullptr, 0, 0, nullptr, 0, nullptr, 0, 0,
+				     nullptr, 0, nullptr) == 0);
+	CHECK(ofi_amd_token_dispatch(nullptr, OFI_AMD_INT32, 0, 2, 8, 0, i, nullptr, nullptr, p, 64, p, 64, 64, nullptr, 0, nullptr, 0, 0, nullptr, 0,
+				     nullptr) == 0);
+	CHECK(launches == 2);
+	launches = 0;
 	CHECK(norm(nullptr, 0, nullptr, bf, 0, 64, bf, 0, p, nullptr, nullptr, 0) == 0 && launches == 0); /* no rows */
 	auto grad = [&](void *dout, float *rstd, uint32_t n, uint32_t width, void *dx, float *dgain, void *work, uint64_t bytes) {
 		return ofi_amd_rms_norm_grad(dout, 256, p, 256, rstd, p, f32, n, width, bf, nullptr, 0, dx, 256, dgain, work, bytes, nullptr);

@@ -123,6 +123,15 @@ def test_row_lengths_pitches_and_alignments(lib, gpu, row_bytes, pad, shift):
     check(lib, 1100, 2, 16, seed=row_bytes, row_bytes=row_bytes, pad=pad, shift=shift)
 
 
+@pytest.mark.parametrize("scale_bytes", [1, 4, 6, 8, 12, 20, 32, 60, 64, 100, 128, 132, 224, 252, 255, 256, 260, 1000])
+@pytest.mark.parametrize("pad,shift,pairs", [(0, 0, True), (4, 4, True), (1, 0, True), (0, 0, False)])
+def test_scales_beside_rows(lib, gpu, scale_bytes, pad, shift, pairs):
+    """Short rows in whole words are copied by their place where the table of pairs is asked for; others by token."""
+    check(lib, 700, 8, 24, seed=scale_bytes, row_bytes=300, scale_bytes=scale_bytes, pad=pad, shift=shift, pairs=pairs, invalid=0.4)
+    check(lib, 1500, 3, 24, seed=scale_bytes, row_bytes=5000, scale_bytes=scale_bytes, pad=pad, shift=shift, pairs=pairs, max_rows=2001)
+    check(lib, 40, 3, 24, seed=scale_bytes, row_bytes=48, scale_bytes=scale_bytes, pad=pad, shift=shift, pairs=pairs, max_rows=200)
+
+
 @pytest.mark.parametrize("tokens", [5, 300, 5000])
 def test_nothing_but_one_expert_and_nothing_at_all(lib, gpu, tokens):
     check(lib, tokens, 8, 256, skew=False, invalid=0.0)
