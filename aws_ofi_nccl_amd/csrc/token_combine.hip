@@ -20,65 +20,87 @@ using namespace ofi_amd;
 constexpr uint32_t kMaxTopK = 64;
 constexpr uint32_t kMaxWidth = 1u << 20;
 constexpr uint32_t kMostWaves = 8; /* a workgroup has all of a row of up to 8 KiB in flight at once */
-constexpr uint32_t kAtOnce = 8; /* rows of a token that are read together */
+constexpr int kAtOnce = 8; /* rows of a token that are read together */
 
-/* A workgroup of threadIdx.x lanes along a row and threadIdx.y tokens; each lane one chunk of the output at a time.  Up to kAtOnce
- * rows are asked for before the first is used.  Eight wavefronts a row are faster than four with two chunks a lane or one with all of
- * them (237, 239, 245 us of reads and writes alone), a token's rows are not brought closer by giving each die a run of tokens (246). */
-template <typename T, uint32_t V, flow_t FLOW>
+/* A workgroup of threadIdx.x lanes along a row and threadIdx.y tokens.  A lane asks for ROWS rows' chunks before it uses the first, of
+ * one chunk of the output at a time, or of four where a token has at most two rows, so that enough is in flight there too.
+ * Eight wavefronts a row are faster than four with two chunks a lane or one with all of them for eight rows (237, 239, 245 us of reads
+ * and writes alone), a token's rows are not brought closer by giving each die a run of tokens (246).  Four chunks against one, 10,636
+ * tokens of 4,224 floats on no more than 4 bytes: one row 61 for 93 us, two rows 91 for 104; of 4,096 bf16 and an addend, 16,384
+ * tokens: 66 for 69 and 88 for 89, but 3,000 tokens of two rows 18.9 for 18.4. */
+template <typename T, uint32_t V, int ROWS, flow_t FLOW>
 __global__ __launch_bounds__(64 * kMostWaves) void token_combine_kernel(const int32_t *__restrict__ row_of,
 									const float *__restrict__ weight, const T *__restrict__ rows,
 									const T *add, T *out, uint64_t rows_pitch, uint64_t add_pitch,
 									uint64_t out_pitch, uint32_t n_tokens, uint32_t max_rows,
 									uint32_t top_k, uint32_t width)
 {
+	constexpr int U = ROWS <= 2 ? 4 : 1; /* chunks of a lane */
 	const uint32_t token = blockIdx.x * blockDim.y + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.y);
 	if (token >= n_tokens) {
 		return;
 	}
 	row_of += (uint64_t)token * top_k;
 	weight += weight ? (uint64_t)token * top_k : 0;
-	for (uint32_t at = threadIdx.x * V; at < width; at += blockDim.x * V) {
-		const place_t here = place_of<V>(at, width);
-		raw_t<T, V> first;
-		if (add) {
-			first = load_raw<FLOW != STREAM_NONE, T, V>(row_at(add, add_pitch, token) + here.from);
-		}
-		float sum[V];
+	const uint32_t step = blockDim.x * V;
+	for (uint32_t at = threadIdx.x * V; at < width; at += U * step) {
+		place_t here[U];
+		raw_t<T, V> first[U];
 #pragma unroll
-		for (uint32_t i = 0; i < V; i++) {
-			sum[i] = 0.0f;
+		for (int u = 0; u < U; u++) {
+			here[u] = place_of<V>(at + u * step, width);
+			if (add) {
+				first[u] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(add, add_pitch, token) + here[u].from);
+			}
 		}
-		for (uint32_t k0 = 0; k0 < top_k; k0 += kAtOnce) {
-			raw_t<T, V> c[kAtOnce];
-			uint32_t row[kAtOnce];
-			float w[kAtOnce];
+		float sum[U][V];
+		for (uint32_t k0 = 0; k0 < top_k; k0 += ROWS) {
+			raw_t<T, V> c[ROWS][U];
+			uint32_t row[ROWS];
+			float w[ROWS];
 #pragma unroll
-			for (uint32_t k = 0; k < kAtOnce; k++) {
+			for (uint32_t k = 0; k < ROWS; k++) {
 				const uint32_t at_k = min(k0 + k, top_k - 1u);
 				row[k] = k0 + k < top_k ? (uint32_t)row_of[at_k] : ~0u;
 				w[k] = weight ? weight[at_k] : 1.0f;
 			}
 #pragma unroll
-			for (uint32_t k = 0; k < kAtOnce; k++) {
+			for (uint32_t k = 0; k < ROWS; k++) {
 				if (row[k] < max_rows) {
-					c[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(rows, rows_pitch, row[k]) + here.from);
+#pragma unroll
+					for (int u = 0; u < U; u++) {
+						c[k][u] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(rows, rows_pitch, row[k]) + here[u].from);
+					}
 				}
 			}
-			if (k0 == 0 && add) {
-				to_floats<T, V>(first, 0, sum);
-			}
+			if (k0 == 0) {
 #pragma unroll
-			for (uint32_t k = 0; k < kAtOnce; k++) {
-				if (row[k] < max_rows) {
+				for (int u = 0; u < U; u++) {
 #pragma unroll
 					for (uint32_t i = 0; i < V; i++) {
-						sum[i] = __builtin_fmaf(w[k], (float)c[k][i], sum[i]);
+						sum[u][i] = add ? (float)first[u][i] : 0.0f;
+					}
+				}
+			}
+#pragma unroll
+			for (uint32_t k = 0; k < ROWS; k++) {
+				if (row[k] < max_rows) {
+#pragma unroll
+					for (int u = 0; u < U; u++) {
+#pragma unroll
+						for (uint32_t i = 0; i < V; i++) {
+							sum[u][i] = __builtin_fmaf(w[k], (float)c[k][u][i], sum[u][i]);
+						}
 					}
 				}
 			}
 		}
-		store_piece<FLOW == STREAM_BOTH, T, V>(row_at(out, out_pitch, token) + here.from, here.skip, sum);
+#pragma unroll
+		for (int u = 0; u < U; u++) {
+			if (at + u * step < width) {
+				store_piece<FLOW == STREAM_BOTH, T, V>(row_at(out, out_pitch, token) + here[u].from, here[u].skip, sum[u]);
+			}
+		}
 	}
 }
 
@@ -219,9 +241,20 @@ int ofi_amd_token_combine(const void *d_rows, uint64_t rows_pitch, uint32_t max_
 	with_row_type(type, width, [&](auto element, auto v) {
 		using T = decltype(element);
 		constexpr uint32_t V = decltype(v)::value;
-		const uint32_t waves = even_waves((width + V - 1) / V, kMostWaves), tokens = waves < 4 ? 4 / waves : 1;
-		auto kernel = by_flow(flow, token_combine_kernel<T, V, STREAM_NONE>, token_combine_kernel<T, V, STREAM_LOADS>,
-				      token_combine_kernel<T, V, STREAM_BOTH>);
+		const bool few = V > 1 && top_k <= 2; /* four chunks of a lane, token_combine_kernel */
+		const uint32_t chunks = (width + V - 1) / V, waves = even_waves(few ? (chunks + 3) / 4 : chunks, kMostWaves);
+		const uint32_t tokens = waves < 4 ? 4 / waves : 1;
+		auto kernel = by_flow(flow, token_combine_kernel<T, V, kAtOnce, STREAM_NONE>, token_combine_kernel<T, V, kAtOnce, STREAM_LOADS>,
+				      token_combine_kernel<T, V, kAtOnce, STREAM_BOTH>);
+		if constexpr (V > 1) {
+			if (top_k == 1) {
+				kernel = by_flow(flow, token_combine_kernel<T, V, 1, STREAM_NONE>, token_combine_kernel<T, V, 1, STREAM_LOADS>,
+						 token_combine_kernel<T, V, 1, STREAM_BOTH>);
+			} else if (few) {
+				kernel = by_flow(flow, token_combine_kernel<T, V, 2, STREAM_NONE>, token_combine_kernel<T, V, 2, STREAM_LOADS>,
+						 token_combine_kernel<T, V, 2, STREAM_BOTH>);
+			}
+		}
 		for (uint32_t at = 0; at < n_tokens; at += kTokensOfLaunch) {
 			const uint32_t n = n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch;
 			launch_kernel(kernel,

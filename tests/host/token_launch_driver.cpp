@@ -168,7 +168,8 @@ int tokens()
 						const uint32_t here = l.arg<uint32_t>(8);
 						CHECK((uint64_t)l.grid.x * l.block.y >= here && (uint64_t)(l.grid.x - 1) * l.block.y < here);
 						CHECK(l.arg<const int32_t *>(0) == reinterpret_cast<int32_t *>(p) + at * top_k);
-						CHECK((uint64_t)l.block.x * chunk >= width || l.block.x > 256);
+						const uint32_t each = chunk > 1 && top_k <= 2 ? 4 : 1; /* chunks of a lane */
+						CHECK((uint64_t)l.block.x * each * chunk >= width || l.block.x > 256);
 						at += here;
 					};
 					CHECK(ofi_amd_token_combine(p, pitch, pairs, reinterpret_cast<int32_t *>(p), nullptr, n, top_k, width, t.type, nullptr, 0, p,

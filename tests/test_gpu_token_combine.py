@@ -107,6 +107,16 @@ def test_what_lies_beside_the_rows_does_not_reach_them(lib, gpu, monkeypatch, wi
         check_grad(lib, 9, 5, width, kind, pad=pad, shift=shift, seed=width, in_place=True, missing=0.0)
 
 
+@pytest.mark.parametrize("top_k", [1, 2])
+@pytest.mark.parametrize("width", [1, 7, 8, 9, 255, 257, 1024, 2049, 4224, 8191, 16385, 20000, 40000])
+def test_one_and_two_rows_of_a_token(lib, gpu, monkeypatch, width, top_k):
+    monkeypatch.setattr(Rows, "guard", 0xFF)
+    for kind in TYPES:
+        check_combine(lib, 13, top_k, width, kind, seed=width)
+        check_combine(lib, 6, top_k, width, kind, seed=width, pad=3, shift=1, weighted=False, added=False)
+        check_combine(lib, 6, top_k, width, kind, seed=width, pad=3, shift=1, in_place=True, missing=0.5)
+
+
 def test_the_output_may_replace_the_addend(lib, gpu):
     check_combine(lib, 33, 8, 1025, "bf16", in_place=True)
 
