@@ -105,9 +105,12 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_kernel(const in
 }
 
 /* One workgroup of `waves` wavefronts per token.  All rows that are read together are asked for before the first is written, so
- * that drows may be rows. */
-template <typename T, uint32_t V, flow_t FLOW>
-__global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(const int32_t *__restrict__ row_of,
+ * that drows may be rows.  Registers for six wavefronts a SIMD: left to itself the compiler takes 98 for floats, which leaves room for
+ * two workgroups of six wavefronts where four fit (8,000 x 8 rows of 4,224 floats 587 us, with six 462; of 8,107 492 and 479; rows of
+ * 2,048, eight wavefronts once, 445 and 450).  Tokens of one row have a kernel for one row: 16,384 of 4,096 bf16 72 us for 85, 10,636
+ * of 4,224 floats 100 for 108; two and four rows at once gain nothing (126 for 123, 232 for 232). */
+template <typename T, uint32_t V, int ROWS, flow_t FLOW>
+__global__ __launch_bounds__(64 * kMostWaves, 6) void token_combine_grad_kernel(const int32_t *__restrict__ row_of,
 									     const float *__restrict__ weight,
 									     const T *__restrict__ dout, const T *rows, T *drows,
 									     float *__restrict__ dweight, uint64_t dout_pitch,
@@ -120,23 +123,22 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(con
 	const T *dr = row_at(dout, dout_pitch, token);
 	row_of += token * top_k;
 	weight += weight ? token * top_k : 0;
-	for (uint32_t k0 = 0; k0 < top_k; k0 += kAtOnce) {
-		float dot[kAtOnce], w[kAtOnce];
-		uint32_t row[kAtOnce];
+	for (uint32_t k0 = 0; k0 < top_k; k0 += ROWS) {
+		float dot[kAtOnce] = {}, w[ROWS];
+		uint32_t row[ROWS];
 #pragma unroll
-		for (uint32_t k = 0; k < kAtOnce; k++) {
+		for (uint32_t k = 0; k < ROWS; k++) {
 			const uint32_t at_k = min(k0 + k, top_k - 1u);
 			row[k] = k0 + k < top_k ? (uint32_t)row_of[at_k] : ~0u;
 			w[k] = weight ? weight[at_k] : 1.0f;
-			dot[k] = 0.0f;
 		}
 		for (uint32_t at = threadIdx.x * V; at < width; at += blockDim.x * V) {
 			const place_t here = place_of<V>(at, width);
 			const raw_t<T, V> dc = load_raw<FLOW != STREAM_NONE, T, V>(dr + here.from);
-			raw_t<T, V> c[kAtOnce];
+			raw_t<T, V> c[ROWS];
 			if (dweight) {
 #pragma unroll
-				for (uint32_t k = 0; k < kAtOnce; k++) {
+				for (uint32_t k = 0; k < ROWS; k++) {
 					if (row[k] < max_rows) {
 						c[k] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(rows, rows_pitch, row[k]) + here.from);
 					}
@@ -146,7 +148,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(con
 			to_floats<T, V>(dc, 0, d);
 			if (drows) {
 #pragma unroll
-				for (uint32_t k = 0; k < kAtOnce; k++) {
+				for (uint32_t k = 0; k < ROWS; k++) {
 					if (row[k] < max_rows) {
 						float f[V];
 #pragma unroll
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(con
 					}
 				}
 #pragma unroll
-				for (uint32_t k = 0; k < kAtOnce; k++) {
+				for (uint32_t k = 0; k < ROWS; k++) {
 					if (row[k] < max_rows) {
 						float f[V];
 						to_floats<T, V>(c[k], here.skip, f);
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_combine_grad_kernel(con
 			part[threadIdx.x >> 6][lane >> 3] = sum;
 		}
 		__syncthreads();
-		if (threadIdx.x < kAtOnce && k0 + threadIdx.x < top_k) {
+		if (threadIdx.x < ROWS && k0 + threadIdx.x < top_k) {
 			float d = part[0][threadIdx.x];
 			for (uint32_t v = 1; v < waves; v++) {
 				d += part[v][threadIdx.x];
@@ -299,8 +301,15 @@ int ofi_amd_token_combine_grad(const void *d_dout, uint64_t dout_pitch, const vo
 		using T = decltype(element);
 		constexpr uint32_t V = decltype(v)::value;
 		const uint32_t waves = even_waves((width + V - 1) / V, kMostWaves);
-		auto kernel = by_flow(flow, token_combine_grad_kernel<T, V, STREAM_NONE>, token_combine_grad_kernel<T, V, STREAM_LOADS>,
-				      token_combine_grad_kernel<T, V, STREAM_BOTH>);
+		auto kernel = by_flow(flow, token_combine_grad_kernel<T, V, kAtOnce, STREAM_NONE>,
+				      token_combine_grad_kernel<T, V, kAtOnce, STREAM_LOADS>,
+				      token_combine_grad_kernel<T, V, kAtOnce, STREAM_BOTH>);
+		if constexpr (V > 1) {
+			if (top_k == 1) {
+				kernel = by_flow(flow, token_combine_grad_kernel<T, V, 1, STREAM_NONE>, token_combine_grad_kernel<T, V, 1, STREAM_LOADS>,
+						 token_combine_grad_kernel<T, V, 1, STREAM_BOTH>);
+			}
+		}
 		for (uint32_t at = 0; at < n_tokens; at += kTokensOfLaunch) {
 			launch_kernel(kernel,
 				      dim3(n_tokens - at < kTokensOfLaunch ? n_tokens - at : kTokensOfLaunch), dim3(64 * waves), 0,

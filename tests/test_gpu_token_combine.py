@@ -199,6 +199,15 @@ def test_gradient_widths(lib, gpu, kind, width):
     check_grad(lib, 3, 5, width, kind, seed=width, pad=1, shift=1, weighted=False)
 
 
+@pytest.mark.parametrize("width", [1, 7, 8, 9, 257, 1024, 2049, 4224, 8191, 16385, 40000])
+def test_gradient_of_one_row_of_a_token(lib, gpu, monkeypatch, width):
+    monkeypatch.setattr(Rows, "guard", 0xFF)
+    for kind in TYPES:
+        check_grad(lib, 13, 1, width, kind, seed=width)
+        check_grad(lib, 6, 1, width, kind, seed=width, pad=3, shift=1, weighted=False)
+        check_grad(lib, 6, 1, width, kind, seed=width, pad=3, shift=1, in_place=True, missing=0.0)
+
+
 @pytest.mark.parametrize("top_k", [1, 2, 3, 4, 5, 6, 7, 8, 9, 16, 17, 31, 64])
 @pytest.mark.parametrize("tokens", [1, 19, 2600])
 def test_gradient_choices(lib, gpu, top_k, tokens):
