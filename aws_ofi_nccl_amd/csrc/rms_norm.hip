@@ -385,7 +385,8 @@ void rms_norm_grad_kernel(const T *dout, const T *__restrict__ s, const float *_
  * The same for rows of more than 1024 chunks, R a lane, without the next row's beside them: 8192 rows of 16,384 bfloat16 217 us (5.0 TB/s).
  * KEPT: a row is held over its sum as it lies in memory (as floats it would not fit).  The longest rows, 32 values a lane, do not fit
  * beside their sums either way -- 2000 rows of 32,768 bfloat16 took 284 us so, and 639 with floats -- and are read again, out of
- * the caches: 159.
+ * the caches: 159, and 4000 of 20,000, whose workgroups fit a CU twice if no lane holds gains, 170 for 216 (3000 of 24,000 floats
+ * 292 for 287).
  */
 template <int R, uint32_t V> constexpr bool kKept = R * V <= 16;
 template <typename T, uint32_t V, int R, flow_t FLOW>
@@ -413,13 +414,17 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(con
 			sc[slot] = load_raw<FLOW != STREAM_NONE, T, V>(row_at(s, s_pitch, row) + from);
 		};
 		const float rstd = rstds[row];
+		const void *gains = gain;
+		if constexpr (!kKept<R, V>) {
+			asm volatile("" : "+s"(gains)); /* read with every row: held over them they cost the second workgroup of a CU */
+		}
 		float along = 0.0f;
 		auto sum = [&](int k, int slot) {
 			const place_t here = place_of<V>((k * blockDim.x + threadIdx.x) * V, width);
 			float g[V], d[V], h[V];
 			to_floats<T, V>(dc[slot], here.skip, d);
 			to_floats<T, V>(sc[slot], here.skip, h);
-			load_gain<T, V>(gain, gain_f32, here.from, g);
+			load_gain<T, V>(gains, gain_f32, here.from, g);
 #pragma unroll
 			for (uint32_t i = 0; i < V; i++) {
 				along = i < here.skip ? along : __builtin_fmaf(d[i] * g[i], h[i] * rstd, along);
@@ -455,7 +460,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void rms_norm_grad_wide_kernel(con
 				}
 				to_floats<T, V>(dc[slot], here.skip, d);
 				to_floats<T, V>(sc[slot], here.skip, h);
-				load_gain<T, V>(gain, gain_f32, here.from, g);
+				load_gain<T, V>(gains, gain_f32, here.from, g);
 #pragma unroll
 				for (uint32_t i = 0; i < V; i++) {
 					r[i] = 0.0f;
