@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 
 #include "ofi_amd_hotpath.h"
+#include "row_places.hpp"
 
 namespace ofi_amd {
 
@@ -32,16 +33,6 @@ template <typename T, uint32_t V> struct piece_t {
 };
 template <typename T, uint32_t V> using raw_t = typename piece_t<T, V>::raw;
 typedef uint32_t any16_t __attribute__((ext_vector_type(4), aligned(1))); /* 16 bytes of anything at any address */
-
-/* Where the chunk at column `at` is read, and how many of its elements are not its own */
-struct place_t {
-	uint32_t from, skip;
-};
-template <uint32_t V> __device__ __forceinline__ place_t place_of(uint32_t at, uint32_t width)
-{
-	const uint32_t from = min(at, width - V);
-	return { from, at - from };
-}
 
 /* What a kernel reads and writes past the caches */
 enum flow_t { STREAM_NONE, STREAM_LOADS, STREAM_BOTH };
@@ -106,23 +97,17 @@ template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v)
 	return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 
-/*
- * Rows of two-byte elements that start between two words.  Loads there run at little over half the rate, so that a chunk is read from
- * the word in front of it (load_raw of lag elements earlier).  Its last element is then the next lane's first; where the next lane is
- * another wavefront's or another row's, or ends with the row, a load of its own brings the word (load_rest, for few lanes).  Nothing
- * beyond the words that hold the chunk's ends is read.
- */
 template <uint32_t V, typename T> __device__ __forceinline__ uint32_t lag_of(const T *row)
 {
-	return sizeof(T) == 2 && V > 1 ? (uint32_t)(reinterpret_cast<uintptr_t>(row) >> 1) & 1u : 0u;
+	return lag_at<V>(reinterpret_cast<uintptr_t>(row), sizeof(T));
 }
 
 /* LANES of a row in a wavefront; chunk: where the lane's chunk lies, at: its column */
 template <typename T, uint32_t V, uint32_t LANES>
 __device__ __forceinline__ uint32_t load_rest(const T *chunk, uint32_t lag, uint32_t at, uint32_t width)
 {
-	const bool alone = (threadIdx.x & (LANES - 1)) == LANES - 1 || at + 2 * V > width;
-	return V > 1 && lag && alone ? *reinterpret_cast<const uint32_t *>(chunk + V - 1) : 0u;
+	const bool lone = is_lone<V, LANES>(threadIdx.x, at, width);
+	return V > 1 && lag && lone ? *reinterpret_cast<const rest_t *>(chunk + kRestAt<V>) : 0u;
 }
 
 /* All lanes of the wavefront call */
@@ -131,9 +116,8 @@ __device__ __forceinline__ void catch_up(raw_t<T, V> &c, uint32_t rest, uint32_t
 {
 	if constexpr (sizeof(T) == 2 && V > 1) {
 		u32x4_t w = __builtin_bit_cast(u32x4_t, c);
-		const bool alone = (threadIdx.x & (LANES - 1)) == LANES - 1 || at + 2 * V > width;
 		const uint32_t next = dpp<0x130>(w.x); /* wave_shl:1 */
-		const uint32_t end = alone ? rest : next;
+		const uint32_t end = is_lone<V, LANES>(threadIdx.x, at, width) ? rest : next; /* its lower half */
 		if (lag) {
 			w = u32x4_t{ __builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16),
 				     __builtin_amdgcn_alignbit(w.w, w.z, 16), __builtin_amdgcn_alignbit(end, w.w, 16) };
