@@ -80,6 +80,27 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(const I *_
 }
 
 /*
+ * Rows that no pair can have, from n_pairs to max_rows, which a caller's buffers may have many more of than a call has pairs: their -1 in
+ * pair_of come from workgroups of their own behind the others, kFillsOfLane of them a lane (beyond kMostFills workgroups more).  8 pairs
+ * into 1,048,576 rows 5.4 us a call, 415 with one workgroup for all of them.
+ */
+constexpr uint32_t kFillsOfLane = 16, kMostFills = 2048;
+inline uint32_t fill_blocks(const int32_t *pair_of, uint64_t n_pairs, uint32_t max_rows, uint32_t lanes)
+{
+	if (!pair_of || max_rows <= n_pairs) {
+		return 0;
+	}
+	const uint64_t blocks = (max_rows - n_pairs + lanes * kFillsOfLane - 1) / (lanes * kFillsOfLane);
+	return blocks < kMostFills ? (uint32_t)blocks : kMostFills;
+}
+__device__ __forceinline__ void fill_rows(int32_t *__restrict__ pair_of, uint32_t n_pairs, uint32_t max_rows, uint32_t block, uint32_t blocks)
+{
+	for (uint64_t r = (uint64_t)n_pairs + block * blockDim.x + threadIdx.x; r < max_rows; r += (uint64_t)blocks * blockDim.x) {
+		pair_of[r] = -1;
+	}
+}
+
+/*
  * Rows of a tile's pairs: each wavefront ranks its own -- lanes with the same expert find each other by a ballot for each bit of its
  * number, the rounds beside each other --, the counts of the wavefronts and of the other tiles say where they begin.  A tile that is
  * alone needs no counts.  LDS: kSortWaves counters an expert, and for the pairs without one.
@@ -94,6 +115,10 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 	extern __shared__ uint32_t next[]; /* [wavefront][expert]: first its pairs so far, then its first row */
 	__shared__ uint32_t carry[kSortWaves];
 	const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, tile = blockIdx.x, stride = n_experts + 1;
+	if (tile >= n_tiles) {
+		fill_rows(pair_of, n_pairs, max_rows, tile - n_tiles, gridDim.x - n_tiles);
+		return;
+	}
 	const uint64_t lo = ((uint64_t)tile * kSortWaves + wave) * (64 * ROUNDS); /* its pairs in order: lanes first, then rounds */
 	I ids[ROUNDS];
 #pragma unroll
@@ -208,8 +233,9 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 			}
 		}
 	}
-	if (pair_of) { /* rows behind the last pair's */
-		for (uint64_t r = all + (uint64_t)tile * 64 * kSortWaves + threadIdx.x; r < max_rows; r += (uint64_t)n_tiles * 64 * kSortWaves) {
+	if (pair_of) { /* rows behind the last pair's, as far as there are pairs */
+		const uint32_t end = min(n_pairs, max_rows);
+		for (uint64_t r = all + (uint64_t)tile * 64 * kSortWaves + threadIdx.x; r < end; r += (uint64_t)n_tiles * 64 * kSortWaves) {
 			pair_of[r] = -1;
 		}
 	}
@@ -368,7 +394,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_rows_kernel(const int32
 /*
  * Few pairs: table and rows in one launch.  The workgroup of a token counts the pairs in front of each of its own -- of a smaller
  * expert, or of the same and a smaller number, which is one comparison of expert * kFew + pair -- and copies its rows there; the
- * last workgroup makes the offsets.  8 pairs 4.0 us on the GPU (table and rows apart: 7.2 and 2.2).  Every workgroup looks at all pairs:
+ * workgroup behind them makes the offsets.  8 pairs 4.0 us on the GPU (table and rows apart: 7.2 and 2.2).  Every workgroup looks at all pairs:
  * 2048 of 256 tokens 10.9 us a call, 2056 in two launches 13.4; 2000 of as many tokens 14.0 in one and 13.3 in two, 4096 of 512 15.8
  * and 14.7.
  */
@@ -386,7 +412,11 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_few_kernel(const I *__r
 	__shared__ uint32_t carry[kMostWaves];
 	const uint32_t lane = threadIdx.x & 63u, waves = blockDim.x >> 6, token = blockIdx.x, n_pairs = n_tokens * top_k;
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-	if (token == n_tokens) { /* the last workgroup */
+	if (token > n_tokens) {
+		fill_rows(pair_of, n_pairs, max_rows, token - n_tokens - 1, gridDim.x - n_tokens - 1);
+		return;
+	}
+	if (token == n_tokens) { /* behind those of the tokens */
 		const uint32_t per = (n_experts + blockDim.x - 1) / blockDim.x, lo = threadIdx.x * per; /* experts of a lane */
 		for (uint32_t e = threadIdx.x; e < n_experts; e += blockDim.x) {
 			counts[e] = 0;
@@ -429,7 +459,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void token_few_kernel(const I *__r
 			}
 		}
 		if (pair_of) {
-			for (uint64_t r = (uint64_t)all + threadIdx.x; r < max_rows; r += blockDim.x) {
+			for (uint32_t r = all + threadIdx.x; r < min(n_pairs, max_rows); r += blockDim.x) {
 				pair_of[r] = -1;
 			}
 		}
@@ -556,18 +586,19 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 		using I = typename std::remove_cv<typename std::remove_pointer<decltype(expert)>::type>::type;
 		if (d_x && n_pairs <= kFew && n_tokens <= kFewTokens) {
 			const uint32_t least = n_pairs > 512 ? kFewWaves : 1, waves = row_waves + more < least ? least : row_waves + more;
-			launch_kernel(token_few_kernel<I>, dim3(n_tokens + 1), dim3(64 * waves), 0, as_stream(stream), expert, n_tokens, top_k,
+			const uint32_t fills = fill_blocks(d_pair_of, n_pairs, max_rows, 64 * waves);
+			launch_kernel(token_few_kernel<I>, dim3(n_tokens + 1 + fills), dim3(64 * waves), 0, as_stream(stream), expert, n_tokens, top_k,
 				      n_experts, row_waves, max_rows, a, b, d_offset, d_row_of, d_pair_of, err);
 			return;
 		}
-		const uint32_t tiles = tiles_of(n_pairs);
+		const uint32_t tiles = tiles_of(n_pairs), fills = fill_blocks(d_pair_of, n_pairs, max_rows, 64 * kSortWaves);
 		with_rounds(rounds_of(n_pairs), [&](auto rounds) {
 			constexpr uint32_t R = decltype(rounds)::value;
 			if (tiles > 1) {
 				launch_kernel(token_count_kernel<I, R>, dim3(tiles), dim3(64 * kSortWaves), 0, as_stream(stream), expert,
 					      (uint32_t)n_pairs, n_experts, static_cast<uint32_t *>(d_work));
 			}
-			launch_kernel(token_place_kernel<I, R>, dim3(tiles), dim3(64 * kSortWaves),
+			launch_kernel(token_place_kernel<I, R>, dim3(tiles + fills), dim3(64 * kSortWaves),
 				      kSortWaves * (n_experts + 1) * sizeof(uint32_t), as_stream(stream), expert, (uint32_t)n_pairs, n_experts, tiles,
 				      max_rows, static_cast<const uint32_t *>(d_work), d_offset, d_row_of, d_pair_of, err);
 		});
