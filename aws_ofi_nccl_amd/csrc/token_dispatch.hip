@@ -6,9 +6,9 @@
  * so that the rows of an expert -- and of a rank that holds a run of experts -- are one piece of memory, which one put carries.
  * No order of atomics shows in the result: they only count.
  *
- * Up to 2048 pairs are one launch, up to 8192 two (table, rows), more three (counts of the tiles first).  32,768 tokens of 8 KiB to
- * 8 of 128 experts: counts 4.9 us, table 8.8, rows 476 for 2.42 GB read and written (5.1 TB/s; the same kernel with the rows written one
- * after the other 441, which is what reading once and writing eight times comes to on this part).
+ * Up to 2048 pairs are one launch, up to 8192 two (table, rows), more three (counts of the tiles first), beyond 1,048,576 four (sums of
+ * the counts).  32,768 tokens of 8 KiB to 8 of 128 experts: counts 4.9 us, table 8.8, rows 476 for 2.42 GB read and written (5.1 TB/s; the
+ * same kernel with the rows written one after the other 441, which is what reading once and writing eight times comes to on this part).
  */
 #include "common.hpp"
 #include "ofi_amd_hotpath.h"
@@ -27,8 +27,14 @@ constexpr uint32_t kMostRounds = 8; /* pairs of a lane of the sort */
 constexpr uint32_t kManyTiles = 64;
 constexpr uint32_t kTilesAtOnce = 32;
 
-/* A workgroup of the sort has 1024 pairs a round.  Everybody adds up the counts of all tiles, 32 at a time, and each unit's scattered
- * stores of pair_of take their turns: 262,144 pairs as 32 tiles of 8 rounds 11.6 us, 64 of 4 8.8, 128 of 2 9.2, 256 of one 11.9. */
+/* Beyond so many tiles their counts are summed up first, by one more launch: every tile of the table adding up all of them would be a
+ * time by the square of the pairs.  The table alone, us with everybody's own sums and with one: 1,048,576 pairs (128 tiles) of 64 / 256 /
+ * 1024 experts 17.9 19.5, 20.7 22.0, 28.6 24.7; twice as many 24.9 23.2, 28.1 26.0, 47.0 35.5; 8,388,608 161 66, 175 78, 355 105;
+ * 67,108,864 of 256 and 1024 7,200 568, 17,150 742. */
+constexpr uint32_t kTilesSummed = 128;
+
+/* A workgroup of the sort has 1024 pairs a round.  Everybody adds up the counts of all (up to kTilesSummed) tiles, 32 at a time, and
+ * each unit's scattered stores of pair_of take their turns: 262,144 pairs as 32 tiles of 8 rounds 11.6 us, 64 of 4 8.8, 128 of 2 9.2, 256 of one 11.9. */
 inline uint32_t rounds_of(uint64_t n_pairs)
 {
 	const uint64_t one = 64 * kSortWaves;
@@ -49,12 +55,55 @@ template <typename I> __device__ __forceinline__ uint32_t known_expert(I e, uint
 	return e >= 0 && e < (I)n_experts ? (uint32_t)e : n_experts;
 }
 
-/* counts[tile][e] */
+/* Each count becomes the sum of those of its expert up to its own tile: a workgroup has kSumExperts experts, and shares the tiles of
+ * each among kSumParts lanes */
+constexpr uint32_t kSumExperts = 16, kSumParts = 64 * kSortWaves / kSumExperts, kSumAtOnce = 16;
+static_assert(kMaxExperts <= kSumExperts * kTilesSummed, "as many workgroups as tiles are enough");
+__device__ __forceinline__ void sum_counts(uint32_t n_experts, uint32_t n_tiles, uint32_t *counts, uint32_t *s)
+{
+	const uint32_t x = threadIdx.x % kSumExperts, part = threadIdx.x / kSumExperts, e = blockIdx.x * kSumExperts + x;
+	const uint32_t each = (n_tiles + kSumParts - 1) / kSumParts, lo = min(part * each, n_tiles), hi = min(lo + each, n_tiles);
+	auto over = [&](auto f) { /* f(tile, its count) */
+		for (uint32_t t0 = lo; t0 < hi && e < n_experts; t0 += kSumAtOnce) {
+			uint32_t c[kSumAtOnce];
+#pragma unroll
+			for (uint32_t t = 0; t < kSumAtOnce; t++) {
+				c[t] = counts[(uint64_t)min(t0 + t, hi - 1) * n_experts + e];
+			}
+#pragma unroll
+			for (uint32_t t = 0; t < kSumAtOnce; t++) {
+				if (t0 + t < hi) {
+					f(t0 + t, c[t]);
+				}
+			}
+		}
+	};
+	uint32_t sum = 0;
+	over([&](uint32_t, uint32_t c) { sum += c; });
+	s[threadIdx.x] = sum;
+	__syncthreads();
+	sum = 0;
+	for (uint32_t p = 0; p < part; p++) {
+		sum += s[p * kSumExperts + x];
+	}
+	over([&](uint32_t t, uint32_t c) {
+		sum += c;
+		counts[(uint64_t)t * n_experts + e] = sum;
+	});
+}
+
+/* counts[tile][e]; a second launch, with n_tiles, has as many workgroups, of which the first sum them up */
 template <typename I, uint32_t ROUNDS>
 __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(const I *__restrict__ expert, uint32_t n_pairs,
-								      uint32_t n_experts, uint32_t *__restrict__ counts)
+								      uint32_t n_experts, uint32_t *__restrict__ counts, uint32_t n_tiles)
 {
 	__shared__ uint32_t count[kMaxExperts + 1];
+	if (n_tiles) {
+		if (blockIdx.x * kSumExperts < n_experts) {
+			sum_counts(n_experts, n_tiles, counts, count);
+		}
+		return;
+	}
 	const uint64_t lo = (uint64_t)blockIdx.x * (64 * kSortWaves * ROUNDS);
 	I ids[ROUNDS];
 #pragma unroll
@@ -129,7 +178,10 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *_
 	/* one expert a lane: there are at most as many as lanes */
 	static_assert(kMaxExperts <= 64 * kSortWaves, "one expert a lane");
 	uint32_t total = 0, mine = 0;
-	if (n_tiles > 1 && threadIdx.x < n_experts) {
+	if (n_tiles > kTilesSummed && threadIdx.x < n_experts) {
+		mine = tile ? counts[(uint64_t)(tile - 1) * n_experts + threadIdx.x] : 0u;
+		total = counts[(uint64_t)(n_tiles - 1) * n_experts + threadIdx.x];
+	} else if (n_tiles > 1 && threadIdx.x < n_experts) {
 		for (uint32_t t0 = 0; t0 < n_tiles; t0 += kTilesAtOnce) {
 			uint32_t c[kTilesAtOnce];
 #pragma unroll
@@ -596,7 +648,11 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 			constexpr uint32_t R = decltype(rounds)::value;
 			if (tiles > 1) {
 				launch_kernel(token_count_kernel<I, R>, dim3(tiles), dim3(64 * kSortWaves), 0, as_stream(stream), expert,
-					      (uint32_t)n_pairs, n_experts, static_cast<uint32_t *>(d_work));
+					      (uint32_t)n_pairs, n_experts, static_cast<uint32_t *>(d_work), 0u);
+			}
+			if (tiles > kTilesSummed) {
+				launch_kernel(token_count_kernel<I, R>, dim3(tiles), dim3(64 * kSortWaves), 0, as_stream(stream), expert,
+					      (uint32_t)n_pairs, n_experts, static_cast<uint32_t *>(d_work), tiles);
 			}
 			launch_kernel(token_place_kernel<I, R>, dim3(tiles + fills), dim3(64 * kSortWaves),
 				      kSortWaves * (n_experts + 1) * sizeof(uint32_t), as_stream(stream), expert, (uint32_t)n_pairs, n_experts, tiles,
