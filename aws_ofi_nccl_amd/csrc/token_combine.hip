@@ -284,11 +284,14 @@ int ofi_amd_token_combine_grad(const void *d_dout, uint64_t dout_pitch, const vo
 		return rc;
 	}
 	const uint64_t bytes = (uint64_t)width * size;
-	if (!rows_ok(d_dout, dout_pitch, n_tokens, bytes, size) || (!d_drows && !d_dweight) ||
+	if (!rows_ok(d_dout, dout_pitch, n_tokens, bytes, size) || (max_rows != 0 && !d_drows && !d_dweight) ||
 	    (reinterpret_cast<uintptr_t>(d_dweight) & 3u) ||
 	    (max_rows != 0 && ((d_dweight && !rows_ok(d_rows, rows_pitch, max_rows, bytes, size)) ||
 			       (d_drows && !rows_ok(d_drows, drows_pitch, max_rows, bytes, size))))) {
 		return -EINVAL;
+	}
+	if (!d_drows && !d_dweight) { /* gradients of no rows, whose buffer may be NULL */
+		return 0;
 	}
 	const uint64_t pairs = (uint64_t)n_tokens * top_k, named = pairs < max_rows ? pairs : max_rows;
 	/* As many rows are written as read, and their ends share lines with other rows.  Where the rows do not start on 64 bytes and do not

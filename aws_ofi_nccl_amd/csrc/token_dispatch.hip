@@ -601,6 +601,10 @@ int ofi_amd_token_dispatch(const void *d_expert, int expert_type, uint32_t n_tok
 	if (rc != 0) {
 		return rc;
 	}
+	if (n_tokens == 0 || max_rows == 0) { /* nothing to copy, and empty buffers may be NULL */
+		d_x = d_scale = nullptr;
+		d_rows = d_scale_rows = nullptr;
+	}
 	if ((expert_type != OFI_AMD_INT32 && expert_type != OFI_AMD_INT64) || top_k == 0 || n_experts == 0 || !d_offset ||
 	    (reinterpret_cast<uintptr_t>(d_offset) & 3u) || (reinterpret_cast<uintptr_t>(d_pair_of) & 3u) || (!d_x != !d_rows) ||
 	    (!d_scale != !d_scale_rows) || (d_scale && !d_x)) {

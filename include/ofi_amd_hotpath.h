@@ -952,10 +952,10 @@ int ofi_amd_tuner_ctx_stats(const void *context, ofi_amd_tuner_ctx_stats_t *out)
  *    less than 2^40), and need no alignment beyond their element's.  Rows, pitches and tables that
  *    lie on 16 bytes are faster.  Sums, statistics and products are held in 32 bits; each output is
  *    rounded once, to nearest even.  Results do not depend on the order in which the GPU runs things:
- *    the same call gives the same bits.  Buffers of one call do not overlap but where it says so.
- *    Nothing is allocated; calls may be captured into a graph (after ofi_amd_gpu_init()).  -EINVAL: a
- *    missing or misaligned argument, a type or group not named here, a pitch below a row; -E2BIG:
- *    beyond the stated limits.
+ *    the same call gives the same bits.  Buffers of one call do not overlap but where it says so;
+ *    those of no rows or no tokens may be NULL.  Nothing is allocated; calls may be captured into a
+ *    graph (after ofi_amd_gpu_init()).  -EINVAL: a missing or misaligned argument, a type or group not
+ *    named here, a pitch below a row; -E2BIG: beyond the stated limits.
  * ====================================================================== */
 
 /* Types, by their numbers in ncclDataType_t */
