@@ -11,7 +11,6 @@
 #include "common.hpp"
 #include "ofi_amd_hotpath.h"
 #include "row_types.hpp"
-#include <cstdlib>
 
 namespace {
 

@@ -975,7 +975,8 @@ int ofi_amd_tuner_ctx_stats(const void *context, ofi_amd_tuner_ctx_stats_t *out)
  * d_scale[row][j] = max(largest |n| of columns [j*group, (j+1)*group) / 448, 2^-126).  group is 32,
  * 64, 128 or 256, or 0 for one scale per row; d_scale rows are scale_pitch bytes apart.  n is made
  * from the unrounded s.  A row that holds a NaN or an infinity has NaN where the formulas have, and
- * the scale of a group with a NaN in it is NaN.  d_sum may be d_x or d_residual, with the same pitch.
+ * the scale of a group with a NaN in it is NaN; a row whose squares add up beyond float32's range has
+ * an rstd of 0.  d_sum may be d_x or d_residual, with the same pitch.
  */
 int ofi_amd_rms_norm(const void *d_x, uint64_t x_pitch, const void *d_residual, uint64_t residual_pitch, const void *d_gain,
 		     int gain_type, uint32_t n_rows, uint32_t width, int type, float eps, void *d_sum, uint64_t sum_pitch,
