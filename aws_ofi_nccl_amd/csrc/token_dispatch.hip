@@ -152,7 +152,7 @@ __device__ __forceinline__ void fill_rows(int32_t *__restrict__ pair_of, uint32_
 /*
  * Rows of a tile's pairs: each wavefront ranks its own -- lanes with the same expert find each other by a ballot for each bit of its
  * number, the rounds beside each other --, the counts of the wavefronts and of the other tiles say where they begin.  A tile that is
- * alone needs no counts.  LDS: kSortWaves counters an expert, and for the pairs without one.
+ * alone needs no counts, one of more than kTilesSummed finds their sums.  LDS: kSortWaves counters an expert, and for the pairs without one.
  */
 template <typename I, uint32_t ROUNDS>
 __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(const I *__restrict__ expert, uint32_t n_pairs,
