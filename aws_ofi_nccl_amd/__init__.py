@@ -573,6 +573,17 @@ PROTOTYPES = {
                                              c_vp, c_u64, c_vp]),
     "ofi_amd_token_combine_grad": (ctypes.c_int, [c_vp, c_u64, c_vp, c_u64, c_u32, c_vp, c_vp, c_u32, c_u32, c_u32,
                                                   c_i32, c_vp, c_u64, c_vp, c_vp]),
+    "ofi_amd_expert_gated": (ctypes.c_int, [c_vp, c_u64, c_vp, c_u64, c_i32, c_vp, c_u32, c_u32, c_vp, c_u64, c_u64, c_vp, c_u32,
+                                            c_u32, c_i32, c_vp, c_u64, c_i32, c_vp, c_u64, c_vp, c_u64, c_i32, c_vp, c_u64, c_vp]),
+    "ofi_amd_expert_product": (ctypes.c_int, [c_vp, c_u64, c_vp, c_u64, c_i32, c_vp, c_u32, c_u32, c_vp, c_u64, c_u64, c_vp, c_u32,
+                                              c_u32, c_vp, c_i32, c_i32, c_vp, c_u64, c_vp, c_u64, c_i32, c_vp, c_u64, c_vp, c_u64,
+                                              c_i32, c_vp, c_u64, c_vp]),
+    "ofi_amd_expert_hidden_grad": (ctypes.c_int, [c_vp, c_u64, c_i32, c_vp, c_u32, c_u32, c_vp, c_u64, c_u64, c_u32, c_u32, c_i32,
+                                                  c_i32, c_vp, c_u64, c_i32, c_vp, c_u64, c_vp, c_u64, c_vp, c_u64, c_vp]),
+    "ofi_amd_expert_rows_grad": (ctypes.c_int, [c_vp, c_u64, c_i32, c_vp, c_u32, c_u32, c_vp, c_u64, c_u64, c_u32, c_u32, c_vp,
+                                                c_u64, c_vp, c_u64, c_vp]),
+    "ofi_amd_expert_weight_grad": (ctypes.c_int, [c_vp, c_u64, c_vp, c_u64, c_i32, c_vp, c_u32, c_u32, c_u32, c_u32, c_vp, c_vp,
+                                                  c_u64, c_u64, c_i32, c_vp, c_vp, c_vp]),
 }
 
 
@@ -595,8 +606,10 @@ def load(path=None):
     return lib
 
 
-# ncclDataType_t numbers of the types that ofi_amd_rms_norm and ofi_amd_token_* take
-INT32, INT64, FLOAT16, FLOAT32, BFLOAT16 = 2, 4, 6, 7, 9
+# ncclDataType_t numbers of the types that ofi_amd_rms_norm, ofi_amd_token_* and ofi_amd_expert_* take
+INT32, INT64, FLOAT16, FLOAT32, BFLOAT16, E4M3 = 2, 4, 6, 7, 9, 10
+# the activations of ofi_amd_expert_*
+NO_ACTIVATION, RELU, SILU, GELU = 0, 1, 2, 3
 
 
 def check(rc, what="call"):

@@ -1,0 +1,304 @@
+/*
+ * Products of rows sorted by expert with their expert's weights:
+ *   gated      h = act(x G^T) (x U^T), both projections in one kernel, and what the activation was taken of kept for the way back
+ *   product    y = act(x W^T + b) + r
+ * x and the weights run along the summed axis.  Rows of e4m3 and their weights have a scale for every 128 of it, which are what one
+ * step sums: a step's sums are multiplied by both scales in 32 bits and added.
+ */
+#include "expert_tiles.hpp"
+
+namespace ofi_amd {
+namespace {
+
+struct forward_t {
+	const float *scale, *weight_scale;
+	uint64_t scale_pitch;
+	matrix_t bias, residual, out, saved;
+	int activation;
+	bool gated;
+};
+
+template <typename T, uint32_t WM, uint32_t WN>
+__global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int32_t *offset, const uint8_t *x, const uint8_t *w, uint32_t n_experts,
+								      uint32_t max_rows, uint32_t width, uint32_t n, uint32_t n_tiles,
+								      uint32_t first_tile, uint64_t x_pitch, uint64_t w_pitch,
+								      uint64_t expert_pitch, forward_t o)
+{
+	constexpr uint32_t BM = 64 * WM, THREADS = 64 * WM * WN, G = 8 / WN;
+	constexpr bool SCALED = sizeof(T) == 1;
+	using rows_tile = along_t<T, BM, THREADS>;
+	using part_tile = along_t<T, kBlock, THREADS>;
+	constexpr uint32_t kTile = rows_tile::kBytes + 2 * part_tile::kBytes;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kTile];
+
+	const tile_t tile = tile_of<BM>(offset, n_experts, max_rows, n_tiles, first_tile + blockIdx.x);
+	if (!tile.any) {
+		return;
+	}
+	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+	/* column 0 of both parts, in the matrix of n columns; a gated block's parts are n rows of weights apart */
+	const uint32_t c0 = tile.nt * (o.gated ? kBlock : 2 * kBlock), c1 = o.gated ? c0 : c0 + kBlock;
+	const uint32_t there0 = n - c0 < kBlock ? n - c0 : kBlock, there1 = c1 >= n ? 0 : n - c1 < kBlock ? n - c1 : kBlock;
+	const uint8_t *const weights = w + tile.expert * expert_pitch;
+	const int64_t bytes = (int64_t)width * sizeof(T);
+	rows_tile rows = { x + tile.from * x_pitch, x_pitch, tile.rows, bytes };
+	part_tile part0 = { weights + c0 * w_pitch, w_pitch, there0, bytes };
+	part_tile part1 = { weights + (there1 ? (o.gated ? (uint64_t)n : 0) + c1 : 0) * w_pitch, w_pitch, there1, bytes };
+
+	f32x4_t sums[4][2][G];
+#pragma unroll
+	for (int m = 0; m < 4; m++) {
+#pragma unroll
+		for (int j = 0; j < (int)(2 * G); j++) {
+			sums[m][j / G][j % G] = f32x4_t{ 0, 0, 0, 0 };
+		}
+	}
+	const along_frag_t row_frag(wm * 64, lane), column_frag(wn * 16 * G, lane);
+	const uint32_t steps = (width + kStepOf<T> - 1) / kStepOf<T>;
+	/* 8-bit rows: a lane's row of each of its four groups */
+	const float *row_scale[4], *weight_scale[2];
+	if constexpr (SCALED) {
+		const uint32_t k_blocks = blocks_of(width), n_blocks = blocks_of(n);
+		const float *of_expert = o.weight_scale + (uint64_t)tile.expert * (o.gated ? 2 : 1) * n_blocks * k_blocks;
+		weight_scale[0] = of_expert + (uint64_t)(c0 / kBlock) * k_blocks;
+		weight_scale[1] = there1 ? of_expert + (uint64_t)((o.gated ? n_blocks : 0) + c1 / kBlock) * k_blocks : weight_scale[0];
+#pragma unroll
+		for (int m = 0; m < 4; m++) {
+			const uint32_t r = wm * 64 + m * 16 + (lane & 15u);
+			row_scale[m] = row_at(o.scale, o.scale_pitch, tile.from + (r < tile.rows ? r : tile.rows - 1));
+		}
+	}
+	rows.load(0);
+	part0.load(0);
+	part1.load(0);
+	for (uint32_t step = 0; step < steps; step++) {
+		uint8_t *const now = lds + (step & 1u) * kTile, *const columns0 = now + rows_tile::kBytes;
+		uint8_t *const columns1 = columns0 + part_tile::kBytes;
+		rows.store(now);
+		part0.store(columns0);
+		part1.store(columns1);
+		__syncthreads(); /* the other tile's readers are past it, too */
+		if (step + 1 < steps) {
+			rows.load(step + 1);
+			part0.load(step + 1);
+			part1.load(step + 1);
+		}
+		if constexpr (SCALED) {
+			float by[4][2];
+#pragma unroll
+			for (int m = 0; m < 4; m++) {
+				const float s = row_scale[m][step];
+				by[m][0] = s * weight_scale[0][step];
+				by[m][1] = s * weight_scale[1][step];
+			}
+			u32x4_t r[4][2];
+#pragma unroll
+			for (int m = 0; m < 4; m++) {
+				r[m][0] = row_frag.get(now, m, 0);
+				r[m][1] = row_frag.get(now, m, 1);
+			}
+#pragma unroll
+			for (int j = 0; j < (int)(2 * G); j++) {
+				const uint8_t *const columns = j < (int)G ? columns0 : columns1;
+				const u32x4_t a = column_frag.get(columns, j % G, 0), b = column_frag.get(columns, j % G, 1);
+#pragma unroll
+				for (int m = 0; m < 4; m++) {
+					const f32x4_t s = multiply8(a, b, r[m][0], r[m][1]);
+					f32x4_t &to = sums[m][j / G][j % G];
+#pragma unroll
+					for (int i = 0; i < 4; i++) {
+						to[i] = __builtin_fmaf(s[i], by[m][j / G], to[i]);
+					}
+				}
+			}
+		} else {
+#pragma unroll
+			for (uint32_t half = 0; half < 2; half++) {
+				u32x4_t r[4];
+#pragma unroll
+				for (int m = 0; m < 4; m++) {
+					r[m] = row_frag.get(now, m, half);
+				}
+#pragma unroll
+				for (int j = 0; j < (int)(2 * G); j++) {
+					const u32x4_t c = column_frag.get(j < (int)G ? columns0 : columns1, j % G, half);
+#pragma unroll
+					for (int m = 0; m < 4; m++) {
+						sums[m][j / G][j % G] = multiply<T>(c, r[m], sums[m][j / G][j % G]);
+					}
+				}
+			}
+		}
+	}
+
+	const uint32_t c = (lane & 31u) * 4, blocks = blocks_of(n), block0 = c0 / kBlock, block1 = c1 / kBlock;
+	const uint32_t left0 = c < there0 ? there0 - c : 0, left1 = c < there1 ? there1 - c : 0;
+	f32x4_t bias0 = { 0, 0, 0, 0 }, bias1 = { 0, 0, 0, 0 };
+	if (o.bias.p) {
+		bias0 = read_values(o.bias, 0, (uint64_t)tile.expert * n + c0 + c, left0, 0);
+		bias1 = read_values(o.bias, 0, (uint64_t)tile.expert * n + c1 + c, left1, 0);
+	}
+	struct in_t {
+		f32x4_t add0, add1;
+	};
+	for_rows<WM, WN>(
+		sums, lds,
+		[&](uint32_t r) {
+			in_t in = {};
+			if (o.residual.p && r < tile.rows) {
+				in.add0 = read_values(o.residual, tile.from + r, c0 + c, left0, 0);
+				in.add1 = read_values(o.residual, tile.from + r, c1 + c, left1, 0);
+			}
+			return in;
+		},
+		[&](uint32_t r, f32x4_t a, f32x4_t b, const in_t &in) {
+			const uint64_t row = tile.from + r;
+			const bool write = r < tile.rows;
+			a += bias0;
+			b += bias1;
+			if (o.saved.p) {
+				write_any(o.saved, row, c0 + c, left0, block0, a, write);
+				write_any(o.saved, row, (o.gated ? (uint64_t)n : 0) + c1 + c, left1, (o.gated ? blocks : 0) + block1, b, write);
+			}
+			with_activation(o.activation, [&](auto activation) {
+#pragma unroll
+				for (int i = 0; i < 4; i++) {
+					a[i] = activated<decltype(activation)::value>(a[i]);
+					b[i] = o.gated ? b[i] : activated<decltype(activation)::value>(b[i]);
+				}
+			});
+			if (o.gated) {
+				a *= b;
+			} else {
+				write_any(o.out, row, c1 + c, left1, block1, b + in.add1, write);
+			}
+			write_any(o.out, row, c0 + c, left0, block0, a + in.add0, write);
+		});
+}
+
+int forward(const void *d_rows, uint64_t rows_pitch, int type, const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows,
+	    const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t width, uint32_t n, const forward_t &o, void *stream)
+{
+	const uint32_t bm = row_tile_for(max_rows, n_experts), n_tiles = (n + (o.gated ? kBlock : 2 * kBlock) - 1) / (o.gated ? kBlock : 2 * kBlock);
+	const uint64_t tiles = most_row_tiles(max_rows, n_experts, bm) * n_tiles;
+	if (tiles > 0x7fffffffull) {
+		return -E2BIG;
+	}
+	auto with = [&](auto element) {
+		using T = decltype(element);
+		auto kernel = bm == 256 ? expert_forward_kernel<T, 4, 2> : bm == 128 ? expert_forward_kernel<T, 2, 4> : expert_forward_kernel<T, 1, 4>;
+		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
+			launch_kernel(kernel, dim3(count), dim3(bm == 64 ? 256 : 512), 0, as_stream(stream), d_offset,
+				      static_cast<const uint8_t *>(d_rows), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, width, n,
+				      n_tiles, first, rows_pitch, weight_pitch, expert_pitch, o);
+		});
+	};
+	if (type == OFI_AMD_BFLOAT16) {
+		with(bf16_t{});
+	} else if (type == OFI_AMD_FLOAT16) {
+		with(f16_t{});
+	} else {
+		with(e4m3_t{});
+	}
+	OFI_AMD_HIP_TRY(hipGetLastError());
+	return 0;
+}
+
+/* Rows that are written: `columns` values in parts of n */
+bool output_ok(const matrix_t &m, uint64_t rows, uint32_t n, uint32_t parts)
+{
+	const uint32_t size = product_type_size(m.type);
+	return size && rows_ok(m.p, m.pitch, rows, (uint64_t)parts * n * size, size) &&
+	       (m.type != OFI_AMD_E4M3 || scales_ok(m.scale, m.scale_pitch, rows, parts * blocks_of(n)));
+}
+
+matrix_t matrix(void *p, uint64_t pitch, int type, float *scale, uint64_t scale_pitch)
+{
+	return { static_cast<uint8_t *>(p), pitch, type, scale, scale_pitch };
+}
+
+/* 16-bit rows have 16-bit outputs of their own type or 8-bit ones; 8-bit rows have any */
+bool types_fit(int type, int other) { return product_type_size(other) && (type == OFI_AMD_E4M3 || other == OFI_AMD_E4M3 || other == type); }
+
+} // namespace
+} // namespace ofi_amd
+
+using namespace ofi_amd;
+
+extern "C" {
+
+int ofi_amd_expert_gated(const void *d_rows, uint64_t rows_pitch, const float *d_scale, uint64_t scale_pitch, int type, const int32_t *d_offset,
+			 uint32_t n_experts, uint32_t max_rows, const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch,
+			 const float *d_weight_scale, uint32_t width, uint32_t inner, int activation, void *d_out, uint64_t out_pitch,
+			 int out_type, float *d_out_scale, uint64_t out_scale_pitch, void *d_saved, uint64_t saved_pitch, int saved_type,
+			 float *d_saved_scale, uint64_t saved_scale_pitch, void *stream)
+{
+	int rc = require_device();
+	if (rc != 0) {
+		return rc;
+	}
+	const uint32_t size = product_type_size(type);
+	if (!size || !activation_ok(activation) || !types_fit(type, out_type) || (d_saved && !types_fit(type, saved_type))) {
+		return -EINVAL;
+	}
+	rc = check_experts(d_offset, n_experts, max_rows, width, inner);
+	if (rc != 0 || max_rows == 0) {
+		return rc;
+	}
+	forward_t o = {};
+	o.scale = d_scale;
+	o.scale_pitch = scale_pitch;
+	o.weight_scale = d_weight_scale;
+	o.activation = activation;
+	o.gated = true;
+	o.out = matrix(d_out, out_pitch, out_type, d_out_scale, out_scale_pitch);
+	o.saved = matrix(d_saved, saved_pitch, saved_type, d_saved_scale, saved_scale_pitch);
+	if (!rows_ok(d_rows, rows_pitch, max_rows, (uint64_t)width * size, size) ||
+	    !stack_ok(d_weight, weight_pitch, expert_pitch, n_experts, 2ull * inner, (uint64_t)width * size, size) ||
+	    !output_ok(o.out, max_rows, inner, 1) || (d_saved && !output_ok(o.saved, max_rows, inner, 2)) ||
+	    (type == OFI_AMD_E4M3 && (!scales_ok(d_scale, scale_pitch, max_rows, blocks_of(width)) || !scales_ok(d_weight_scale, 4, 1, 1)))) {
+		return -EINVAL;
+	}
+	return forward(d_rows, rows_pitch, type, d_offset, n_experts, max_rows, d_weight, weight_pitch, expert_pitch, width, inner, o, stream);
+}
+
+int ofi_amd_expert_product(const void *d_rows, uint64_t rows_pitch, const float *d_scale, uint64_t scale_pitch, int type,
+			   const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows, const void *d_weight, uint64_t weight_pitch,
+			   uint64_t expert_pitch, const float *d_weight_scale, uint32_t width, uint32_t out_width, const void *d_bias,
+			   int bias_type, int activation, const void *d_residual, uint64_t residual_pitch, void *d_out, uint64_t out_pitch,
+			   int out_type, float *d_out_scale, uint64_t out_scale_pitch, void *d_saved, uint64_t saved_pitch, int saved_type,
+			   float *d_saved_scale, uint64_t saved_scale_pitch, void *stream)
+{
+	int rc = require_device();
+	if (rc != 0) {
+		return rc;
+	}
+	const uint32_t size = product_type_size(type), bias_size = d_bias ? row_type_size(bias_type) : 1;
+	if (!size || !bias_size || !activation_ok(activation) || !types_fit(type, out_type) || (d_saved && !types_fit(type, saved_type)) ||
+	    (reinterpret_cast<uintptr_t>(d_bias) % bias_size) || (d_residual && out_type == OFI_AMD_E4M3)) {
+		return -EINVAL;
+	}
+	rc = check_experts(d_offset, n_experts, max_rows, width, out_width);
+	if (rc != 0 || max_rows == 0) {
+		return rc;
+	}
+	forward_t o = {};
+	o.scale = d_scale;
+	o.scale_pitch = scale_pitch;
+	o.weight_scale = d_weight_scale;
+	o.bias = matrix(const_cast<void *>(d_bias), 0, bias_type, nullptr, 0);
+	o.activation = activation;
+	o.out = matrix(d_out, out_pitch, out_type, d_out_scale, out_scale_pitch);
+	o.saved = matrix(d_saved, saved_pitch, saved_type, d_saved_scale, saved_scale_pitch);
+	o.residual = matrix(const_cast<void *>(d_residual), residual_pitch, out_type, nullptr, 0);
+	if (!rows_ok(d_rows, rows_pitch, max_rows, (uint64_t)width * size, size) ||
+	    !stack_ok(d_weight, weight_pitch, expert_pitch, n_experts, out_width, (uint64_t)width * size, size) ||
+	    !output_ok(o.out, max_rows, out_width, 1) || (d_saved && !output_ok(o.saved, max_rows, out_width, 1)) ||
+	    (d_residual && !output_ok(o.residual, max_rows, out_width, 1)) ||
+	    (type == OFI_AMD_E4M3 && (!scales_ok(d_scale, scale_pitch, max_rows, blocks_of(width)) || !scales_ok(d_weight_scale, 4, 1, 1)))) {
+		return -EINVAL;
+	}
+	return forward(d_rows, rows_pitch, type, d_offset, n_experts, max_rows, d_weight, weight_pitch, expert_pitch, width, out_width, o, stream);
+}
+
+} /* extern "C" */

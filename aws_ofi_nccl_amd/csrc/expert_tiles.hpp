@@ -1,0 +1,594 @@
+/*
+ * What the experts' products share: which rows of which expert a workgroup takes, how tiles of both operands come into LDS and
+ * from there to the matrix cores, and how sums leave in rows.
+ *
+ * A workgroup of WM x WN wavefronts computes BM = 64 WM rows (of the result) by two parts of 128 columns: a part is the gate's or the
+ * other projection's share of a gated block, or half of 256 neighbouring columns.  A wavefront has 64 rows and 128 / WN columns of both
+ * parts, so that a gate's sums and those they are multiplied with lie in the same lane, and each part is one block of 128 columns that
+ * shares an 8-bit scale.
+ *
+ * The summed axis is taken in steps: 128 bytes of a row where the operand's rows run along it ("along"), 64 rows where they run
+ * across it ("across").  Two tiles of LDS take turns: while one is computed on, the other is filled.
+ *   along    16-byte chunk c of row r lies at slot c ^ (r & 7) of the row: eight rows' same chunk, which eight lanes read at once,
+ *            are in eight different groups of banks
+ *   across   row k's chunk c lies at slot c ^ 2 (k & 3 | (k >> 3 & 1) << 2): four rows' same 32 bytes, which sixteen lanes read and
+ *            exchange (ds_read_b64_tr_b16: lane l of sixteen gets column l of four rows), are in different groups too
+ * The matrix instruction's first operand is the column tile, so that a lane's four sums are neighbouring columns of one row (columns
+ * 4 (lane / 16) + i of a group of 16, row lane % 16).
+ */
+#ifndef OFI_AMD_EXPERT_TILES_HPP_
+#define OFI_AMD_EXPERT_TILES_HPP_
+
+#include "common.hpp"
+#include "row_types.hpp"
+
+namespace ofi_amd {
+
+struct e4m3_t {
+	uint8_t bits;
+};
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+
+constexpr uint32_t kBlock = 128;       /* columns that share a scale, and columns of a part */
+constexpr uint32_t kStepBytes = 128;   /* of a row along the summed axis, in a step */
+constexpr uint32_t kStepRows = 64;     /* rows across it */
+constexpr uint32_t kMostExperts = 1024, kMostExpertWidth = 1u << 20;
+
+template <typename T> constexpr uint32_t kStepOf = kStepBytes / sizeof(T); /* elements of the summed axis in a step */
+
+__host__ __device__ inline uint32_t blocks_of(uint32_t width) { return (width + kBlock - 1) / kBlock; }
+
+/* ---- rows of experts ---------------------------------------------------------------------------------------- */
+
+/* first: the expert's first row; from: the tile's, rows: those it has; nt: which of the column tiles */
+struct tile_t {
+	uint32_t expert, from, rows, nt;
+	bool any;
+};
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+/* Rows [lo, hi) of expert e, whatever the offsets are: within the rows there are */
+__device__ __forceinline__ void run_of(const int32_t *offset, uint32_t e, uint32_t max_rows, uint32_t &lo, uint32_t &hi)
+{
+	const int32_t a = offset ? offset[e] : 0, b = offset ? offset[e + 1] : (int32_t)max_rows;
+	lo = a < 0 ? 0u : (uint32_t)a < max_rows ? (uint32_t)a : max_rows;
+	hi = b < 0 ? 0u : (uint32_t)b < max_rows ? (uint32_t)b : max_rows;
+	hi = hi < lo ? lo : hi;
+}
+
+/* Sum over the lanes up to this one */
+__device__ __forceinline__ uint32_t running_sum(uint32_t v, uint32_t lane)
+{
+#pragma unroll
+	for (uint32_t d = 1; d < 64; d *= 2) {
+		const uint32_t up = (uint32_t)__shfl_up((int)v, d, 64);
+		v += lane >= d ? up : 0u;
+	}
+	return v;
+}
+
+/*
+ * The tile that workgroup `id` of the launch takes.  Tiles are numbered expert by expert, an expert's in bands of eight row tiles, a
+ * band's column by column: what an XCD's 32 compute units work on at once is about eight row tiles by four column tiles, which its L2
+ * holds a step of.  Workgroups go to the eight XCDs in turn, so each XCD gets an eighth of the numbers in one piece.
+ */
+template <uint32_t BM>
+__device__ __forceinline__ tile_t tile_of(const int32_t *offset, uint32_t n_experts, uint32_t max_rows, uint32_t n_tiles, uint32_t id)
+{
+	const uint32_t lane = threadIdx.x & 63u;
+	uint32_t total = 0, at = 0, e0 = 0, lo = 0, hi = 0, before = 0, mine = 0;
+	for (e0 = 0; e0 < n_experts; e0 += 64) {
+		lo = hi = 0;
+		if (e0 + lane < n_experts) {
+			run_of(offset, e0 + lane, max_rows, lo, hi);
+		}
+		mine = (hi - lo + BM - 1) / BM;
+		const uint32_t sum = running_sum(mine, lane);
+		before = total + sum - mine;
+		total += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+	}
+	tile_t t = {};
+	const uint32_t tiles = total * n_tiles, share = (tiles + 7) / 8;
+	at = (id & 7u) * share + (id >> 3);
+	if ((id >> 3) >= share || at >= tiles) {
+		return t;
+	}
+	if (n_experts > 64) { /* the lanes know the last experts: again, up to the one that has the tile */
+		uint32_t sums = 0;
+		for (e0 = 0; e0 < n_experts; e0 += 64) {
+			lo = hi = 0;
+			if (e0 + lane < n_experts) {
+				run_of(offset, e0 + lane, max_rows, lo, hi);
+			}
+			mine = (hi - lo + BM - 1) / BM;
+			const uint32_t sum = running_sum(mine, lane);
+			before = sums + sum - mine;
+			sums += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+			if (at < sums * n_tiles) {
+				break;
+			}
+		}
+	} else {
+		e0 = 0;
+	}
+	const uint64_t has = __ballot(mine != 0 && at >= before * n_tiles && at < (before + mine) * n_tiles);
+	if (!has) {
+		return t;
+	}
+	const int who = (int)__builtin_ctzll(has);
+	const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)lo, who), end = (uint32_t)__builtin_amdgcn_readlane((int)hi, who);
+	const uint32_t row_tiles = (uint32_t)__builtin_amdgcn_readlane((int)mine, who);
+	at = uniform(at) - (uint32_t)__builtin_amdgcn_readlane((int)before, who) * n_tiles;
+	const uint32_t band = at / (8 * n_tiles), in_band = at - band * 8 * n_tiles;
+	const uint32_t height = row_tiles - band * 8 < 8 ? row_tiles - band * 8 : 8;
+	t.expert = e0 + (uint32_t)who;
+	t.nt = in_band / height;
+	t.from = first + (band * 8 + in_band % height) * BM;
+	t.rows = end - t.from < BM ? end - t.from : BM;
+	t.any = true;
+	return t;
+}
+
+/* ---- operands ----------------------------------------------------------------------------------------------- */
+
+/* Up to 16 bytes of a row's `left` bytes from p on, zeros behind them; any alignment */
+template <typename T> __device__ __forceinline__ u32x4_t chunk_at(const uint8_t *p, int64_t left)
+{
+	if (left >= 16) {
+		return *reinterpret_cast<const any16_t *>(p);
+	}
+	u32x4_t v = { 0, 0, 0, 0 };
+	if (left > 0) {
+#pragma unroll
+		for (uint32_t i = 0; i < 16 / sizeof(T); i++) {
+			if ((int64_t)(i * sizeof(T)) < left) {
+				if constexpr (sizeof(T) == 2) {
+					v[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << (16 * (i & 1));
+				} else {
+					v[i / 4] |= (uint32_t)p[i] << (8 * (i & 3));
+				}
+			}
+		}
+	}
+	return v;
+}
+
+/*
+ * ROWS rows of an operand whose rows run along the summed axis.  base: the first row's start; rows of them are there, each of `bytes`;
+ * what is not there is zeros.
+ */
+template <typename T, uint32_t ROWS, uint32_t THREADS> struct along_t {
+	static constexpr uint32_t kChunks = ROWS * 8 / THREADS, kRowsOfRound = THREADS / 8, kBytes = ROWS * kStepBytes;
+	const uint8_t *base;
+	uint64_t pitch;
+	uint32_t rows;
+	int64_t bytes;
+	u32x4_t held[kChunks];
+
+	__device__ __forceinline__ void load(uint32_t step)
+	{
+		const uint32_t row = threadIdx.x / 8, chunk = (threadIdx.x & 7u) ^ (row & 7u);
+		const int64_t at = (int64_t)step * kStepBytes + chunk * 16;
+#pragma unroll
+		for (uint32_t t = 0; t < kChunks; t++) {
+			const uint32_t r = t * kRowsOfRound + row;
+			held[t] = chunk_at<T>(base + (uint64_t)(r < rows ? r : 0) * pitch + at, r < rows ? bytes - at : 0);
+		}
+	}
+	__device__ __forceinline__ void store(uint8_t *lds) const
+	{
+#pragma unroll
+		for (uint32_t t = 0; t < kChunks; t++) {
+			*reinterpret_cast<u32x4_t *>(lds + (t * THREADS + threadIdx.x) * 16) = held[t];
+		}
+	}
+};
+
+/* The rows of `along` that a lane feeds to a matrix instruction: 32 bytes of each, in two halves of 16 */
+struct along_frag_t {
+	uint32_t at;
+	__device__ __forceinline__ along_frag_t(uint32_t first_row, uint32_t lane)
+		: at((first_row + (lane & 15u)) * kStepBytes + (((lane >> 4) ^ (lane & 7u)) << 4))
+	{
+	}
+	/* group: of 16 rows; half: of the step */
+	__device__ __forceinline__ u32x4_t get(const uint8_t *lds, uint32_t group, uint32_t half) const
+	{
+		return *reinterpret_cast<const u32x4_t *>(lds + ((at + group * 16 * kStepBytes) ^ (half << 6)));
+	}
+};
+
+template <uint32_t W> __device__ __forceinline__ uint32_t across_slot(uint32_t k)
+{
+	return (((k & 3u) | ((k >> 3) & 1u) << 2) << 1) & (W / 8 - 1);
+}
+
+/* W columns of an operand whose rows run across the summed axis; two-byte elements.  base: column 0 of the first row */
+template <typename T, uint32_t W, uint32_t THREADS> struct across_t {
+	static constexpr uint32_t kOfRow = W / 8, kChunks = kStepRows * kOfRow / THREADS, kBytes = kStepRows * W * 2;
+	const uint8_t *base;
+	uint64_t pitch;
+	uint32_t rows;  /* of the summed axis */
+	int64_t bytes;  /* of the columns there are, at most W's */
+	u32x4_t held[kChunks];
+
+	__device__ __forceinline__ void load(uint32_t step)
+	{
+#pragma unroll
+		for (uint32_t t = 0; t < kChunks; t++) {
+			const uint32_t slot = t * THREADS + threadIdx.x, k = slot / kOfRow, r = step * kStepRows + k;
+			const uint32_t chunk = (slot % kOfRow) ^ across_slot<W>(k);
+			held[t] = chunk_at<T>(base + (uint64_t)(r < rows ? r : 0) * pitch + chunk * 16, r < rows ? bytes - (int64_t)chunk * 16 : 0);
+		}
+	}
+	__device__ __forceinline__ void store(uint8_t *lds) const
+	{
+#pragma unroll
+		for (uint32_t t = 0; t < kChunks; t++) {
+			*reinterpret_cast<u32x4_t *>(lds + (t * THREADS + threadIdx.x) * 16) = held[t];
+		}
+	}
+};
+
+/* The columns of `across` that a lane feeds to a matrix instruction: eight of the summed axis in four bytes-of-two each twice */
+template <uint32_t W> struct across_frag_t {
+	uint32_t row, swizzle, low;
+	__device__ __forceinline__ across_frag_t(uint32_t lane)
+	{
+		const uint32_t k = (lane >> 4) * 8 + ((lane & 15u) >> 2);
+		row = k * W * 2 + (lane & 1u) * 8;
+		swizzle = across_slot<W>(k);
+		low = (lane & 3u) >> 1;
+	}
+	/* column: the first of 16 */
+	__device__ __forceinline__ u32x4_t get(uint8_t *lds, uint32_t column, uint32_t half) const
+	{
+		const uint32_t at = row + (((column / 8 ^ swizzle) + low) << 4) + half * 32 * W * 2;
+		const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(lds + at));
+		const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(lds + at + 4 * W * 2));
+		const u32x2_t lo = __builtin_bit_cast(u32x2_t, a), hi = __builtin_bit_cast(u32x2_t, b);
+		return u32x4_t{ lo.x, lo.y, hi.x, hi.y };
+	}
+};
+
+/* sums[i] += column tile x row tile, 32 of the summed axis */
+template <typename T> __device__ __forceinline__ f32x4_t multiply(u32x4_t columns, u32x4_t rows, f32x4_t sums)
+{
+	if constexpr (std::is_same<T, bf16_t>::value) {
+		return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, columns), __builtin_bit_cast(bf16x8_t, rows), sums, 0,
+							       0, 0);
+	} else {
+		return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, columns), __builtin_bit_cast(f16x8_t, rows), sums, 0,
+							      0, 0);
+	}
+}
+
+/* The same for 128 values of e4m3: both operands take the summed axis in the same order, whichever that is */
+__device__ __forceinline__ f32x4_t multiply8(u32x4_t columns0, u32x4_t columns1, u32x4_t rows0, u32x4_t rows1)
+{
+	struct pair_t {
+		u32x4_t a, b;
+	};
+	const i32x8_t c = __builtin_bit_cast(i32x8_t, pair_t{ columns0, columns1 }), r = __builtin_bit_cast(i32x8_t, pair_t{ rows0, rows1 });
+	return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(c, r, f32x4_t{ 0, 0, 0, 0 }, 0, 0, 0, 127, 0, 127); /* both scales 2^0 */
+}
+
+/* ---- sums ----------------------------------------------------------------------------------------------------- */
+
+/*
+ * A tile's sums by rows: finish(row of the tile, columns of part 0, of part 1, what load(row) gave), four neighbouring columns of both
+ * parts in a lane, from column 4 (lane % 32) of the part on; half a wavefront has a row, so that what is read and written of it is one
+ * piece.  The sums go through LDS, a quarter of the rows at a time: 2 to 3 hundredths of the tile's time at 4096 summed, for
+ * epilogues of a twentieth of the registers that whole columns in a lane would take.
+ */
+template <uint32_t WM, uint32_t WN, typename Load, typename Finish>
+__device__ __forceinline__ void for_rows(const f32x4_t (&sums)[4][2][8 / WN], uint8_t *lds, Load load, Finish finish)
+{
+	constexpr uint32_t G = 8 / WN, kRows = WM * 16, kTurns = kRows / (WM * WN) / 2;
+	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+	__syncthreads(); /* the tiles have been read */
+	auto quarter = [&](auto which) __attribute__((always_inline)) {
+		constexpr uint32_t m = decltype(which)::value;
+		uint8_t *const buffer = lds + (m & 1u) * kRows * 1024;
+		decltype(load(0u)) in[kTurns];
+		uint32_t at[kTurns], row[kTurns];
+#pragma unroll
+		for (uint32_t i = 0; i < kTurns; i++) {
+			at[i] = (wave * kTurns + i) * 2 + (lane >> 5);
+			row[i] = at[i] / 16 * 64 + m * 16 + at[i] % 16;
+			in[i] = load(row[i]);
+		}
+#pragma unroll
+		for (uint32_t p = 0; p < 2; p++) {
+#pragma unroll
+			for (uint32_t j = 0; j < G; j++) {
+				const uint32_t r = wm * 16 + (lane & 15u), chunk = p * 32 + (wn * G + j) * 4 + (lane >> 4);
+				*reinterpret_cast<f32x4_t *>(buffer + r * 1024 + ((chunk ^ (r & 15u)) << 4)) = sums[m][p][j];
+			}
+		}
+		__syncthreads(); /* and the other buffer's readers are past it */
+#pragma unroll
+		for (uint32_t i = 0; i < kTurns; i++) {
+			const uint8_t *const from = buffer + at[i] * 1024;
+			const uint32_t chunk = (lane & 31u) ^ (at[i] & 15u);
+			const f32x4_t a = *reinterpret_cast<const f32x4_t *>(from + (chunk << 4));
+			const f32x4_t b = *reinterpret_cast<const f32x4_t *>(from + ((chunk + 32) << 4));
+			finish(row[i], a, b, in[i]);
+		}
+	};
+	quarter(std::integral_constant<uint32_t, 0>{});
+	quarter(std::integral_constant<uint32_t, 1>{});
+	quarter(std::integral_constant<uint32_t, 2>{});
+	quarter(std::integral_constant<uint32_t, 3>{});
+}
+
+/* Where the columns of a matrix of 16-bit, float32 or e4m3 values are read and written; none: p NULL */
+struct matrix_t {
+	uint8_t *p;
+	uint64_t pitch;
+	int type;
+	float *scale; /* of e4m3: one to each block of columns */
+	uint64_t scale_pitch;
+};
+
+/* Four values of a row from p on, of which `left` are there; zeros for the others */
+template <typename T> __device__ __forceinline__ f32x4_t read_as(const uint8_t *p, uint32_t left)
+{
+	f32x4_t v = { 0, 0, 0, 0 };
+	if (left >= 4) {
+		v = __builtin_convertvector(*reinterpret_cast<const typename piece_t<T, 4>::anywhere *>(p), f32x4_t);
+	} else {
+#pragma unroll
+		for (uint32_t i = 0; i < 3; i++) {
+			if (i < left) {
+				v[i] = (float)reinterpret_cast<const T *>(p)[i];
+			}
+		}
+	}
+	return v;
+}
+
+__device__ __forceinline__ f32x4_t read_e4m3(const uint8_t *p, uint32_t left, float scale)
+{
+	typedef uint32_t any4_t __attribute__((aligned(1)));
+	uint32_t w = 0;
+	if (left >= 4) {
+		w = *reinterpret_cast<const any4_t *>(p);
+	} else {
+#pragma unroll
+		for (uint32_t i = 0; i < 3; i++) {
+			if (i < left) {
+				w |= (uint32_t)p[i] << (8 * i);
+			}
+		}
+	}
+	const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+	return f32x4_t{ a[0], a[1], b[0], b[1] } * scale;
+}
+
+/* block: of the columns, for their scale */
+__device__ __forceinline__ f32x4_t read_values(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block)
+{
+	const uint8_t *p = m.p + row * m.pitch;
+	switch (m.type) {
+	case OFI_AMD_BFLOAT16: return read_as<bf16_t>(p + column * 2, left);
+	case OFI_AMD_FLOAT16: return read_as<f16_t>(p + column * 2, left);
+	case OFI_AMD_FLOAT32: return read_as<float>(p + column * 4, left);
+	default: return read_e4m3(p + column, left, row_at(m.scale, m.scale_pitch, row)[block]);
+	}
+}
+
+/* Each value is rounded to the matrix's type once, to nearest even */
+template <typename T> __device__ __forceinline__ void write_as(uint8_t *p, uint32_t left, f32x4_t v)
+{
+	const auto r = __builtin_convertvector(v, raw_t<T, 4>);
+	if (left >= 4) {
+		*reinterpret_cast<typename piece_t<T, 4>::anywhere *>(p) = r;
+	} else {
+#pragma unroll
+		for (uint32_t i = 0; i < 3; i++) {
+			if (i < left) {
+				reinterpret_cast<T *>(p)[i] = r[i];
+			}
+		}
+	}
+}
+
+__device__ __forceinline__ void write_values(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, f32x4_t v)
+{
+	uint8_t *p = m.p + row * m.pitch;
+	switch (m.type) {
+	case OFI_AMD_BFLOAT16: write_as<bf16_t>(p + column * 2, left, v); break;
+	case OFI_AMD_FLOAT16: write_as<f16_t>(p + column * 2, left, v); break;
+	default: write_as<float>(p + column * 4, left, v);
+	}
+}
+
+/* A block of 128 columns of a row, which the 32 lanes of half a wavefront hold: values divided by their scale as the norms divide
+ * them (with a division's rounding, then rounded to e4m3), and the scale.  All 32 lanes call; `write`: whether the row is there. */
+__device__ __forceinline__ void write_block(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block, f32x4_t v, bool write)
+{
+	uint32_t most = 0;
+#pragma unroll
+	for (uint32_t i = 0; i < 4; i++) {
+		const uint32_t bits = i < left ? abs_bits(v[i]) : 0u;
+		most = bits > most ? bits : most;
+	}
+	const float scale = scale_of(max_bits_over<32>(most));
+	const divisor_t by = divisor_of(scale);
+	const int low = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[0], by), quotient(v[1], by), 0, false);
+	const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[2], by), quotient(v[3], by), low, true);
+	if (!write || left == 0) {
+		return;
+	}
+	if ((threadIdx.x & 31u) == 0) {
+		row_at(m.scale, m.scale_pitch, row)[block] = scale;
+	}
+	typedef uint32_t any4_t __attribute__((aligned(1)));
+	uint8_t *p = m.p + row * m.pitch + column;
+	if (left >= 4) {
+		*reinterpret_cast<any4_t *>(p) = w;
+	} else {
+#pragma unroll
+		for (uint32_t i = 0; i < 3; i++) {
+			if (i < left) {
+				p[i] = (uint8_t)(w >> (8 * i));
+			}
+		}
+	}
+}
+
+/* The same to 16-bit types without blocks */
+__device__ __forceinline__ void write_any(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block, f32x4_t v, bool write)
+{
+	if (m.type == OFI_AMD_E4M3) {
+		write_block(m, row, column, left, block, v, write);
+	} else if (write && left) {
+		write_values(m, row, column, left, v);
+	}
+}
+
+/* ---- activations ------------------------------------------------------------------------------------------------ */
+
+/* 1 / (1 + e^-v): e^-v beyond float32's range leaves 0.  The reciprocal is the instruction's, off by one unit of 2^-24 or so */
+__device__ __forceinline__ float logistic(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+
+/*
+ * The normal distribution's share below v, and e^(-v^2/2).  Below 0 it is e^(-v^2/2) t P(t) with t = 1 / (1 + 0.45 |v| / sqrt 2): t P(t)
+ * is half of e^(z^2) erfc(z), fitted over all z >= 0 (least squares in Chebyshev polynomials, weights drawn to the largest relative
+ * errors), 3e-8 off at most; in 32 bits 5e-7 of the share, also where it is tiny.  About 20 operations.
+ */
+__device__ __forceinline__ float normal_share(float v, float &bell)
+{
+	constexpr float kP[] = { 1.269426605e-01f, 1.269415725e-01f, 1.141360073e-01f, 8.762432375e-02f, 5.998388820e-02f,
+				-1.120403144e-02f, 7.124375690e-02f, -1.503351952e-01f, 9.536814225e-02f, -2.070111786e-02f };
+	const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fabsf(v), 0.45f * 0.70710678118654752f, 1.0f));
+	float p = kP[9];
+#pragma unroll
+	for (int i = 8; i >= 0; i--) {
+		p = __builtin_fmaf(p, t, kP[i]);
+	}
+	bell = __expf(-0.5f * v * v);
+	const float below = p * t * bell;
+	return v < 0.0f ? below : 1.0f - below;
+}
+
+template <int ACTIVATION> __device__ __forceinline__ float activated(float v)
+{
+	if constexpr (ACTIVATION == OFI_AMD_RELU) {
+		return v < 0.0f ? 0.0f : v;
+	} else if constexpr (ACTIVATION == OFI_AMD_SILU) {
+		return v * logistic(v);
+	} else if constexpr (ACTIVATION == OFI_AMD_GELU) {
+		float bell;
+		return v * normal_share(v, bell);
+	} else {
+		return v;
+	}
+}
+
+/* The activation's value and its derivative.  0 has RELU's derivative 0. */
+template <int ACTIVATION> __device__ __forceinline__ void activated_with_slope(float v, float &value, float &slope)
+{
+	if constexpr (ACTIVATION == OFI_AMD_RELU) {
+		value = v < 0.0f ? 0.0f : v;
+		slope = v > 0.0f ? 1.0f : v <= 0.0f ? 0.0f : v;
+	} else if constexpr (ACTIVATION == OFI_AMD_SILU) {
+		const float s = logistic(v);
+		value = v * s;
+		slope = __builtin_fmaf(value, 1.0f - s, s);
+	} else if constexpr (ACTIVATION == OFI_AMD_GELU) {
+		float bell;
+		const float share = normal_share(v, bell);
+		value = v * share;
+		slope = __builtin_fmaf(v * 0.39894228040143268f, bell, share);
+	} else {
+		value = v;
+		slope = 1.0f;
+	}
+}
+
+/* f with the activation as a constant */
+template <typename F> __device__ __forceinline__ void with_activation(int activation, F f)
+{
+	switch (activation) {
+	case OFI_AMD_RELU: f(std::integral_constant<int, OFI_AMD_RELU>{}); break;
+	case OFI_AMD_SILU: f(std::integral_constant<int, OFI_AMD_SILU>{}); break;
+	case OFI_AMD_GELU: f(std::integral_constant<int, OFI_AMD_GELU>{}); break;
+	default: f(std::integral_constant<int, OFI_AMD_NO_ACTIVATION>{});
+	}
+}
+
+/* ---- on the host -------------------------------------------------------------------------------------------------- */
+
+/* Bytes of an element of rows and weights, 0 for a type they do not have */
+inline uint32_t product_type_size(int type)
+{
+	return type == OFI_AMD_BFLOAT16 || type == OFI_AMD_FLOAT16 ? 2u : type == OFI_AMD_E4M3 ? 1u : 0u;
+}
+
+inline int check_experts(const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows, uint32_t a, uint32_t b)
+{
+	if (n_experts == 0 || a == 0 || b == 0 || (reinterpret_cast<uintptr_t>(d_offset) & 3u) || (!d_offset && n_experts != 1)) {
+		return -EINVAL;
+	}
+	if (n_experts > kMostExperts || max_rows > 0x7fffffffu || a > kMostExpertWidth || b > kMostExpertWidth) {
+		return -E2BIG;
+	}
+	return 0;
+}
+
+/* n_experts matrices of n rows */
+inline bool stack_ok(const void *p, uint64_t pitch, uint64_t expert_pitch, uint32_t n_experts, uint64_t n, uint64_t bytes, uint32_t element)
+{
+	return rows_ok(p, pitch, n, bytes, element) && expert_pitch % element == 0 && expert_pitch < (1ull << 50) &&
+	       (n_experts == 1 || expert_pitch >= (n - 1) * pitch + bytes);
+}
+
+inline bool scales_ok(const void *p, uint64_t pitch, uint64_t n, uint32_t blocks) { return rows_ok(p, pitch, n, 4ull * blocks, 4); }
+
+/* Rows of `bytes` that whole chunks of 16 bytes make up, and that start on them, a tile of 256 rows within 31 bits */
+inline bool in_chunks(const void *p, uint64_t pitch, uint64_t bytes)
+{
+	return ((reinterpret_cast<uintptr_t>(p) | pitch | bytes) & 15u) == 0 && pitch <= (1u << 22);
+}
+
+constexpr uint32_t kTilesOfLaunch = 1u << 22; /* with 512 lanes each within the 32 bits of a launch's size */
+
+/* Calls launch(first tile, tiles) until all are launched; the tiles' number is a multiple of 8 */
+template <typename F> inline void launch_tiles(uint64_t tiles, F launch)
+{
+	tiles = (tiles + 7) / 8 * 8;
+	for (uint64_t at = 0; at < tiles; at += kTilesOfLaunch) {
+		launch((uint32_t)at, (uint32_t)(tiles - at < kTilesOfLaunch ? tiles - at : kTilesOfLaunch));
+	}
+}
+
+/* Row tiles of BM that `max_rows` rows of experts can make */
+inline uint64_t most_row_tiles(uint32_t max_rows, uint32_t n_experts, uint32_t bm)
+{
+	const uint64_t parts = n_experts < max_rows ? n_experts : max_rows; /* experts whose last tile may be part of one */
+	return (max_rows - parts) / bm + parts;
+}
+
+/* Row tiles of 256, 128 or 64: as many as there are rows for */
+inline uint32_t row_tile_for(uint32_t max_rows, uint32_t n_experts)
+{
+	const uint32_t of_expert = (max_rows + n_experts - 1) / n_experts;
+	return of_expert > 128 ? 256 : of_expert > 64 ? 128 : 64;
+}
+
+inline bool activation_ok(int a) { return a == OFI_AMD_NO_ACTIVATION || a == OFI_AMD_RELU || a == OFI_AMD_SILU || a == OFI_AMD_GELU; }
+
+} // namespace ofi_amd
+
+#endif

@@ -1,0 +1,205 @@
+/*
+ * Gradients of the experts' weights and biases: dW_e = add + sum over the expert's rows of dy[r]^T x[r], db_e = add + sum of dy[r].
+ * Both operands run across the summed axis, which is as long as the expert has rows; a workgroup sums all of it for one tile of
+ * one expert's matrix, so that every sum runs in the rows' order.  The bias is the product with a column of ones.
+ */
+#include "expert_tiles.hpp"
+
+namespace ofi_amd {
+namespace {
+
+struct weight_grad_t {
+	matrix_t add, out;
+	uint64_t expert_pitch; /* of both */
+	const float *bias_add;
+	float *dbias;
+};
+
+template <typename T> constexpr uint32_t kTwoOnes = 0x3f803f80u; /* bfloat16 */
+template <> constexpr uint32_t kTwoOnes<f16_t> = 0x3c003c00u;
+
+/* rows of the result: m (dout's columns); columns: n (x's) */
+template <typename T, uint32_t WM, uint32_t WN>
+__global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const int32_t *offset, const uint8_t *dout, const uint8_t *x,
+									  uint32_t max_rows, uint32_t m_width, uint32_t n_width,
+									  uint32_t m_tiles, uint32_t n_tiles, uint32_t tiles, uint32_t first_tile,
+									  uint64_t dout_pitch, uint64_t x_pitch, weight_grad_t o)
+{
+	constexpr uint32_t BM = 64 * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
+	using rows_tile = across_t<T, BM, THREADS>;
+	using columns_tile = across_t<T, BN, THREADS>;
+	constexpr uint32_t kTile = rows_tile::kBytes + columns_tile::kBytes;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kTile];
+
+	/* an eighth of the tiles in one piece for each XCD; in an expert, bands of eight row tiles */
+	const uint32_t id = first_tile + blockIdx.x, share = (tiles + 7) / 8, at = (id & 7u) * share + (id >> 3);
+	if ((id >> 3) >= share || at >= tiles) {
+		return;
+	}
+	const uint32_t expert = at / (m_tiles * n_tiles), in_expert = at % (m_tiles * n_tiles);
+	const uint32_t band = in_expert / (8 * n_tiles), in_band = in_expert - band * 8 * n_tiles;
+	const uint32_t height = m_tiles - band * 8 < 8 ? m_tiles - band * 8 : 8;
+	const uint32_t m0 = (band * 8 + in_band % height) * BM, n0 = in_band / height * BN;
+	uint32_t lo, hi;
+	run_of(offset, expert, max_rows, lo, hi);
+	lo = uniform(lo);
+	hi = uniform(hi);
+
+	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+	const uint32_t m_there = m_width - m0 < BM ? m_width - m0 : BM, n_there = n_width - n0 < BN ? n_width - n0 : BN;
+	rows_tile rows = { dout + lo * dout_pitch + m0 * 2, dout_pitch, hi - lo, (int64_t)m_there * 2 };
+	columns_tile columns = { x + lo * x_pitch + n0 * 2, x_pitch, hi - lo, (int64_t)n_there * 2 };
+	const bool with_bias = o.dbias && n0 == 0 && wn == 0;
+
+	f32x4_t sums[4][2][G], bias[4];
+#pragma unroll
+	for (int m = 0; m < 4; m++) {
+		bias[m] = f32x4_t{ 0, 0, 0, 0 };
+#pragma unroll
+		for (int j = 0; j < (int)(2 * G); j++) {
+			sums[m][j / G][j % G] = f32x4_t{ 0, 0, 0, 0 };
+		}
+	}
+	const across_frag_t<BM> row_frag(lane);
+	const across_frag_t<BN> column_frag(lane);
+	const uint32_t steps = (hi - lo + kStepRows - 1) / kStepRows;
+	if (steps) {
+		rows.load(0);
+		columns.load(0);
+	}
+	for (uint32_t step = 0; step < steps; step++) {
+		uint8_t *const now = lds + (step & 1u) * kTile, *const now_columns = now + rows_tile::kBytes;
+		rows.store(now);
+		columns.store(now_columns);
+		__syncthreads(); /* the other tile's readers are past it, too */
+		if (step + 1 < steps) {
+			rows.load(step + 1);
+			columns.load(step + 1);
+		}
+#pragma unroll
+		for (uint32_t half = 0; half < 2; half++) {
+			u32x4_t r[4];
+#pragma unroll
+			for (int m = 0; m < 4; m++) {
+				r[m] = row_frag.get(now, wm * 64 + m * 16, half);
+			}
+			if (with_bias) {
+				const u32x4_t ones = { kTwoOnes<T>, kTwoOnes<T>, kTwoOnes<T>, kTwoOnes<T> };
+#pragma unroll
+				for (int m = 0; m < 4; m++) {
+					bias[m] = multiply<T>(ones, r[m], bias[m]);
+				}
+			}
+#pragma unroll
+			for (int j = 0; j < (int)(2 * G); j++) {
+				const u32x4_t c = column_frag.get(now_columns, j / G * kBlock + wn * 16 * G + j % G * 16, half);
+#pragma unroll
+				for (int m = 0; m < 4; m++) {
+					sums[m][j / G][j % G] = multiply<T>(c, r[m], sums[m][j / G][j % G]);
+				}
+			}
+		}
+	}
+
+	if (with_bias && lane < 16) {
+#pragma unroll
+		for (int m = 0; m < 4; m++) {
+			const uint32_t r = wm * 64 + m * 16 + lane;
+			if (r < m_there) {
+				const uint64_t i = (uint64_t)expert * m_width + m0 + r;
+				o.dbias[i] = bias[m][0] + (o.bias_add ? o.bias_add[i] : 0.0f);
+			}
+		}
+	}
+	const matrix_t out = { o.out.p + expert * o.expert_pitch, o.out.pitch, o.out.type, nullptr, 0 };
+	const matrix_t add = { o.add.p ? o.add.p + expert * o.expert_pitch : nullptr, o.add.pitch, o.add.type, nullptr, 0 };
+	const uint32_t c = (lane & 31u) * 4;
+	const uint32_t left[2] = { c < n_there ? n_there - c : 0, c + kBlock < n_there ? n_there - c - kBlock : 0 };
+	struct in_t {
+		f32x4_t was[2];
+	};
+	for_rows<WM, WN>(
+		sums, lds,
+		[&](uint32_t r) {
+			in_t in = {};
+#pragma unroll
+			for (int p = 0; p < 2; p++) {
+				if (add.p && r < m_there && left[p]) {
+					in.was[p] = read_values(add, m0 + r, n0 + p * kBlock + c, left[p], 0);
+				}
+			}
+			return in;
+		},
+		[&](uint32_t r, f32x4_t a, f32x4_t b, const in_t &in) {
+#pragma unroll
+			for (int p = 0; p < 2; p++) {
+				if (r < m_there && left[p]) {
+					write_values(out, m0 + r, n0 + p * kBlock + c, left[p], (p ? b : a) + in.was[p]);
+				}
+			}
+		});
+}
+
+} // namespace
+} // namespace ofi_amd
+
+using namespace ofi_amd;
+
+extern "C" {
+
+int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const void *d_rows, uint64_t rows_pitch, int type,
+			       const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows, uint32_t width, uint32_t out_width,
+			       const void *d_add, void *d_dweight, uint64_t dweight_pitch, uint64_t expert_pitch, int dweight_type,
+			       const float *d_bias_add, float *d_dbias, void *stream)
+{
+	int rc = require_device();
+	if (rc != 0) {
+		return rc;
+	}
+	if ((type != OFI_AMD_BFLOAT16 && type != OFI_AMD_FLOAT16) || (dweight_type != type && dweight_type != OFI_AMD_FLOAT32)) {
+		return -EINVAL;
+	}
+	rc = check_experts(d_offset, n_experts, max_rows, width, out_width);
+	if (rc != 0) {
+		return rc;
+	}
+	const uint32_t size = row_type_size(dweight_type);
+	if ((max_rows != 0 && (!rows_ok(d_dout, dout_pitch, max_rows, 2ull * out_width, 2) ||
+			       !rows_ok(d_rows, rows_pitch, max_rows, 2ull * width, 2))) ||
+	    !stack_ok(d_dweight, dweight_pitch, expert_pitch, n_experts, out_width, (uint64_t)width * size, size) ||
+	    (reinterpret_cast<uintptr_t>(d_add) % size) || ((reinterpret_cast<uintptr_t>(d_dbias) | reinterpret_cast<uintptr_t>(d_bias_add)) & 3u)) {
+		return -EINVAL;
+	}
+	/* tiles of 256 x 256 where they are enough for the GPU, else of 128 x 256 */
+	const uint32_t n_tiles = (width + 255) / 256;
+	const bool wide = (uint64_t)n_experts * ((out_width + 255) / 256) * n_tiles >= 256;
+	const uint32_t bm = wide ? 256 : 128, m_tiles = (out_width + bm - 1) / bm;
+	const uint64_t tiles = (uint64_t)n_experts * m_tiles * n_tiles;
+	if (tiles > 0x7fffffffull) {
+		return -E2BIG;
+	}
+	weight_grad_t o = {};
+	o.out = { static_cast<uint8_t *>(d_dweight), dweight_pitch, dweight_type, nullptr, 0 };
+	o.add = { static_cast<uint8_t *>(const_cast<void *>(d_add)), dweight_pitch, dweight_type, nullptr, 0 };
+	o.expert_pitch = expert_pitch;
+	o.bias_add = d_bias_add;
+	o.dbias = d_dbias;
+	auto with = [&](auto element) {
+		using T = decltype(element);
+		auto kernel = wide ? expert_weight_grad_kernel<T, 4, 2> : expert_weight_grad_kernel<T, 2, 4>;
+		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
+			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset, static_cast<const uint8_t *>(d_dout),
+				      static_cast<const uint8_t *>(d_rows), max_rows, out_width, width, m_tiles, n_tiles, (uint32_t)tiles, first,
+				      dout_pitch, rows_pitch, o);
+		});
+	};
+	if (type == OFI_AMD_BFLOAT16) {
+		with(bf16_t{});
+	} else {
+		with(f16_t{});
+	}
+	OFI_AMD_HIP_TRY(hipGetLastError());
+	return 0;
+}
+
+} /* extern "C" */

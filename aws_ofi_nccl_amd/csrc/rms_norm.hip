@@ -36,25 +36,6 @@ struct norm_out_t {
 	float *rstd;
 };
 
-/*
- * Quotients by a scale, rounded as a division rounds them: the product with its inverse, and what that product leaves over times the
- * inverse once more, three operations where a division takes ten (16,384 rows of 8192 bfloat16 155.6 us, with the product alone 155.3;
- * thirty in a row on the same tensors, which the clocks give way to, 164 and 161).
- * An infinite scale leaves nothing over: the finite values beside it are 0.
- */
-struct divisor_t {
-	float inverse, finite;
-};
-__device__ __forceinline__ divisor_t divisor_of(float scale)
-{
-	return { 1.0f / scale, scale < __builtin_inff() ? scale : 0.0f };
-}
-__device__ __forceinline__ float quotient(float f, divisor_t by)
-{
-	const float q = f * by.inverse;
-	return __builtin_fmaf(-__builtin_fmaf(q, by.finite, -f), by.inverse, q); /* so that -0 stays -0 */
-}
-
 /* A chunk's own elements, divided, as e4m3 */
 template <bool STREAM, uint32_t V> __device__ __forceinline__ void store_q(uint8_t *p, uint32_t skip, const float (&f)[V], divisor_t by)
 {
@@ -139,13 +120,6 @@ template <uint32_t V> __device__ __forceinline__ void store_floats(float *p, uin
 	} else {
 		store_piece<false, float, V>(p, skip, f);
 	}
-}
-
-__device__ __forceinline__ float scale_of(uint32_t amax_bits)
-{
-	/* __builtin_fmaxf would drop a NaN, which every value of its group is then to show */
-	const float s = __uint_as_float(amax_bits) / 448.0f;
-	return s < 0x1p-126f ? 0x1p-126f : s;
 }
 
 /*

@@ -218,6 +218,33 @@ template <int LANES> __device__ __forceinline__ uint32_t max_bits_over(uint32_t 
 
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
+/*
+ * Quotients by a scale, rounded as a division rounds them: the product with its inverse, and what that product leaves over times the
+ * inverse once more, three operations where a division takes ten (16,384 rows of 8192 bfloat16 155.6 us, with the product alone 155.3;
+ * thirty in a row on the same tensors, which the clocks give way to, 164 and 161).
+ * An infinite scale leaves nothing over: the finite values beside it are 0.
+ */
+struct divisor_t {
+	float inverse, finite;
+};
+__device__ __forceinline__ divisor_t divisor_of(float scale)
+{
+	return { 1.0f / scale, scale < __builtin_inff() ? scale : 0.0f };
+}
+__device__ __forceinline__ float quotient(float f, divisor_t by)
+{
+	const float q = f * by.inverse;
+	return __builtin_fmaf(-__builtin_fmaf(q, by.finite, -f), by.inverse, q); /* so that -0 stays -0 */
+}
+
+/* The scale of a group's values from the largest one's bits */
+__device__ __forceinline__ float scale_of(uint32_t amax_bits)
+{
+	/* __builtin_fmaxf would drop a NaN, which every value of its group is then to show */
+	const float s = __uint_as_float(amax_bits) / 448.0f;
+	return s < 0x1p-126f ? 0x1p-126f : s;
+}
+
 /* The value of every wavefront of a row's put together by op, in all of their lanes.  s: a word for each of up to 16 wavefronts, which
  * nothing else uses meanwhile.  All wavefronts of the workgroup call. */
 template <typename Op> __device__ __forceinline__ uint32_t over_waves(uint32_t v, uint32_t *s, uint32_t waves, uint32_t none, Op op)

@@ -964,6 +964,7 @@ int ofi_amd_tuner_ctx_stats(const void *context, ofi_amd_tuner_ctx_stats_t *out)
 #define OFI_AMD_FLOAT16 6
 #define OFI_AMD_FLOAT32 7
 #define OFI_AMD_BFLOAT16 9
+#define OFI_AMD_E4M3 10 /* OCP e4m3, in section 7 */
 
 /*
  * For each of n_rows rows of `width` values (1..32768) of `type` (float16, bfloat16, float32):
@@ -1043,6 +1044,95 @@ int ofi_amd_token_combine(const void *d_rows, uint64_t rows_pitch, uint32_t max_
 int ofi_amd_token_combine_grad(const void *d_dout, uint64_t dout_pitch, const void *d_rows, uint64_t rows_pitch,
 			       uint32_t max_rows, const int32_t *d_row_of, const float *d_weight, uint32_t n_tokens, uint32_t top_k,
 			       uint32_t width, int type, void *d_drows, uint64_t drows_pitch, float *d_dweight, void *stream);
+
+/* ======================================================================
+ * 7. Experts: what stands between token_dispatch and token_combine.
+ *    Rows sorted by expert go through their expert's gated block and the product behind it;
+ *    training keeps what the activation was taken of, in 16 bits or in 8, and goes back from there.
+ *    The conventions are those of section 6.  In addition:
+ *
+ *    Experts.  The rows of expert e are [d_offset[e], d_offset[e + 1]), as ofi_amd_token_dispatch leaves
+ *    them; no other row is read or written.  d_offset NULL: one expert, which has all max_rows rows (an
+ *    ordinary layer's product).  Offsets are taken within [0, max_rows] and have to grow; they stay on
+ *    the GPU.  n_experts 1..1024, widths 1..2^20, max_rows < 2^31; -E2BIG beyond, or where a call has
+ *    2^31 tiles of 64 rows and 128 columns or more.
+ *    Weights are matrices of one row for each output, weight_pitch bytes from row to row and expert_pitch
+ *    from expert to expert.
+ *    Types are float16 or bfloat16 for rows and weights alike.  The forward products also take OCP e4m3
+ *    for both: rows with a scale (float32) for each 128 columns, as ofi_amd_rms_norm leaves them with
+ *    group 128, weights with a scale for each block of 128 x 128, [expert][block of outputs][block of
+ *    columns], dense; the blocks of a gated block's second half begin with it.  Values are sums of
+ *    q * q * scale * scale in 32 bits.
+ *    Outputs of e4m3 have a scale for each 128 columns, max(largest / 448, 2^-126), as
+ *    ofi_amd_rms_norm's; it and the values are made from the unrounded 32-bit ones.  An output of 16-bit
+ *    rows is of their type or e4m3, one of e4m3 rows of any of the three.
+ * ====================================================================== */
+
+/* relu(0) has the derivative 0; gelu is v times the normal distribution's share below v (no tanh) */
+#define OFI_AMD_NO_ACTIVATION 0
+#define OFI_AMD_RELU 1
+#define OFI_AMD_SILU 2
+#define OFI_AMD_GELU 3
+
+/*
+ * out[r] = act(x[r] G_e^T) * (x[r] U_e^T), `inner` columns; an expert's weights are 2 * inner rows of
+ * `width`, those of G first.
+ * d_saved (or NULL): x[r] G_e^T, then x[r] U_e^T, 2 * inner columns, for ofi_amd_expert_hidden_grad: the
+ * checkpoint of the block, in 16 bits or e4m3 (scales: 2 * ceil(inner / 128) a row).
+ * d_scale and d_weight_scale are looked at for e4m3 rows, d_out_scale and d_saved_scale for e4m3 outputs.
+ */
+int ofi_amd_expert_gated(const void *d_rows, uint64_t rows_pitch, const float *d_scale, uint64_t scale_pitch, int type,
+			 const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows, const void *d_weight, uint64_t weight_pitch,
+			 uint64_t expert_pitch, const float *d_weight_scale, uint32_t width, uint32_t inner, int activation, void *d_out,
+			 uint64_t out_pitch, int out_type, float *d_out_scale, uint64_t out_scale_pitch, void *d_saved,
+			 uint64_t saved_pitch, int saved_type, float *d_saved_scale, uint64_t saved_scale_pitch, void *stream);
+
+/*
+ * out[r] = act(x[r] W_e^T + bias_e) + residual[r], `out_width` columns.  d_bias (or NULL): [expert][out_width],
+ * dense, float32, float16 or bfloat16.  d_residual (or NULL; not with an e4m3 output) is of out's type;
+ * d_out may be d_residual, with the same pitch.  d_saved (or NULL): x[r] W_e^T + bias_e, `out_width` columns.
+ */
+int ofi_amd_expert_product(const void *d_rows, uint64_t rows_pitch, const float *d_scale, uint64_t scale_pitch, int type,
+			   const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows, const void *d_weight, uint64_t weight_pitch,
+			   uint64_t expert_pitch, const float *d_weight_scale, uint32_t width, uint32_t out_width, const void *d_bias,
+			   int bias_type, int activation, const void *d_residual, uint64_t residual_pitch, void *d_out,
+			   uint64_t out_pitch, int out_type, float *d_out_scale, uint64_t out_scale_pitch, void *d_saved,
+			   uint64_t saved_pitch, int saved_type, float *d_saved_scale, uint64_t saved_scale_pitch, void *stream);
+
+/*
+ * Back through the product behind a block and the block's activation.  dh = dout[r] W_e, where W_e is the
+ * product's weight, `width` rows (its outputs, the columns of dout) of `inner`; saved is what
+ * ofi_amd_expert_gated (gated 1: g and u) or ofi_amd_expert_product (gated 0: g) left.
+ *   gated   dsaved = (dh * u * act'(g), dh * act(g)), 2 * inner columns;   hidden = act(g) * u
+ *   else    dsaved = dh * act'(g), inner columns;                          hidden = act(g)
+ * dsaved and hidden (or NULL: the block's output again, for the weights' gradient of the product, so that
+ * it need not be kept) are of dout's type.  d_saved and d_dsaved do not overlap.
+ */
+int ofi_amd_expert_hidden_grad(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d_offset, uint32_t n_experts,
+			       uint32_t max_rows, const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t width,
+			       uint32_t inner, int gated, int activation, const void *d_saved, uint64_t saved_pitch, int saved_type,
+			       const float *d_saved_scale, uint64_t saved_scale_pitch, void *d_dsaved, uint64_t dsaved_pitch,
+			       void *d_hidden, uint64_t hidden_pitch, void *stream);
+
+/*
+ * drows[r] = add[r] + dout[r] W_e, `width` columns: the gradient of a product's rows.  W_e has `out_width`
+ * rows of `width` (2 * inner for a gated block, whose dout is dsaved).  d_add (or NULL) is of the same type;
+ * d_drows may be d_add, with the same pitch.
+ */
+int ofi_amd_expert_rows_grad(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d_offset, uint32_t n_experts,
+			     uint32_t max_rows, const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t width,
+			     uint32_t out_width, const void *d_add, uint64_t add_pitch, void *d_drows, uint64_t drows_pitch, void *stream);
+
+/*
+ * dweight_e = add_e + sum over the expert's rows of dout[r]^T x[r], out_width rows of `width`, float32 or the
+ * rows' type; dbias_e = bias_add_e + sum of dout[r] (or NULL), [expert][out_width] in float32.  d_add and
+ * d_bias_add (or NULL: 0) lie like the outputs, and may be them.  An expert without rows gets what is added,
+ * or zeros.
+ */
+int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const void *d_rows, uint64_t rows_pitch, int type,
+			       const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows, uint32_t width, uint32_t out_width,
+			       const void *d_add, void *d_dweight, uint64_t dweight_pitch, uint64_t expert_pitch, int dweight_type,
+			       const float *d_bias_add, float *d_dbias, void *stream);
 
 #ifdef __cplusplus
 }
