@@ -18,7 +18,7 @@ struct backward_t {
 };
 
 /* k: the product's outputs, n: its columns */
-template <typename T, uint32_t WM, uint32_t WN, bool HIDDEN>
+template <typename T, uint32_t WM, uint32_t WN, bool HIDDEN, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int32_t *offset, const uint8_t *dout, const uint8_t *w,
 								       uint32_t n_experts, uint32_t max_rows, uint32_t k, uint32_t n,
 								       uint32_t n_tiles, uint32_t first_tile, uint64_t dout_pitch,
@@ -50,16 +50,29 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int
 	const along_frag_t row_frag(wm * 64, lane);
 	const across_frag_t<BN> column_frag(lane);
 	const uint32_t steps = (k + kStepRows - 1) / kStepRows;
-	rows.load(0);
-	columns.load(0);
+	if (DIRECT) {
+		rows.fill(0, lds);
+		columns.fill(0, lds + rows_tile::kBytes);
+	} else {
+		rows.load(0);
+		columns.load(0);
+	}
 	for (uint32_t step = 0; step < steps; step++) {
 		uint8_t *const now = lds + (step & 1u) * kTile, *const now_columns = now + rows_tile::kBytes;
-		rows.store(now);
-		columns.store(now_columns);
-		__syncthreads(); /* the other tile's readers are past it, too */
+		if (!DIRECT) {
+			rows.store(now);
+			columns.store(now_columns);
+		}
+		__syncthreads(); /* this tile is there, and the other one's readers are past it */
 		if (step + 1 < steps) {
-			rows.load(step + 1);
-			columns.load(step + 1);
+			uint8_t *const next = lds + ((step + 1) & 1u) * kTile;
+			if (DIRECT) {
+				rows.fill(step + 1, next);
+				columns.fill(step + 1, next + rows_tile::kBytes);
+			} else {
+				rows.load(step + 1);
+				columns.load(step + 1);
+			}
 		}
 #pragma unroll
 		for (uint32_t half = 0; half < 2; half++) {
@@ -148,10 +161,14 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
+	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * k) && in_chunks(d_weight, weight_pitch, 2ull * n) && expert_pitch % 16 == 0;
 	auto with = [&](auto element) {
 		using T = decltype(element);
-		auto kernel = bm == 256 ? expert_backward_kernel<T, 4, 2, HIDDEN>
-					: bm == 128 ? expert_backward_kernel<T, 2, 4, HIDDEN> : expert_backward_kernel<T, 1, 4, HIDDEN>;
+		auto kernel =
+			direct ? (bm == 256 ? expert_backward_kernel<T, 4, 2, HIDDEN, true>
+					    : bm == 128 ? expert_backward_kernel<T, 2, 4, HIDDEN, true> : expert_backward_kernel<T, 1, 4, HIDDEN, true>)
+			       : (bm == 256 ? expert_backward_kernel<T, 4, 2, HIDDEN, false>
+					    : bm == 128 ? expert_backward_kernel<T, 2, 4, HIDDEN, false> : expert_backward_kernel<T, 1, 4, HIDDEN, false>);
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			launch_kernel(kernel, dim3(count), dim3(bm == 64 ? 256 : 512), 0, as_stream(stream), d_offset,
 				      static_cast<const uint8_t *>(d_dout), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, k, n,

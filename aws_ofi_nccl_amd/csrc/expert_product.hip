@@ -18,7 +18,7 @@ struct forward_t {
 	bool gated;
 };
 
-template <typename T, uint32_t WM, uint32_t WN>
+template <typename T, uint32_t WM, uint32_t WN, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int32_t *offset, const uint8_t *x, const uint8_t *w, uint32_t n_experts,
 								      uint32_t max_rows, uint32_t width, uint32_t n, uint32_t n_tiles,
 								      uint32_t first_tile, uint64_t x_pitch, uint64_t w_pitch,
@@ -68,20 +68,37 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 			row_scale[m] = row_at(o.scale, o.scale_pitch, tile.from + (r < tile.rows ? r : tile.rows - 1));
 		}
 	}
-	rows.load(0);
-	part0.load(0);
-	part1.load(0);
+	auto fill = [&](uint32_t step) {
+		uint8_t *const to = lds + (step & 1u) * kTile;
+		rows.fill(step, to);
+		part0.fill(step, to + rows_tile::kBytes);
+		part1.fill(step, to + rows_tile::kBytes + part_tile::kBytes);
+	};
+	auto load = [&](uint32_t step) {
+		rows.load(step);
+		part0.load(step);
+		part1.load(step);
+	};
+	if (DIRECT) {
+		fill(0);
+	} else {
+		load(0);
+	}
 	for (uint32_t step = 0; step < steps; step++) {
 		uint8_t *const now = lds + (step & 1u) * kTile, *const columns0 = now + rows_tile::kBytes;
 		uint8_t *const columns1 = columns0 + part_tile::kBytes;
-		rows.store(now);
-		part0.store(columns0);
-		part1.store(columns1);
-		__syncthreads(); /* the other tile's readers are past it, too */
+		if (!DIRECT) {
+			rows.store(now);
+			part0.store(columns0);
+			part1.store(columns1);
+		}
+		__syncthreads(); /* this tile is there, and the other one's readers are past it */
 		if (step + 1 < steps) {
-			rows.load(step + 1);
-			part0.load(step + 1);
-			part1.load(step + 1);
+			if (DIRECT) {
+				fill(step + 1);
+			} else {
+				load(step + 1);
+			}
 		}
 		if constexpr (SCALED) {
 			float by[4][2];
@@ -91,23 +108,35 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 				by[m][0] = s * weight_scale[0][step];
 				by[m][1] = s * weight_scale[1][step];
 			}
-			u32x4_t r[4][2];
+			u32x4_t r[4][4];
 #pragma unroll
 			for (int m = 0; m < 4; m++) {
-				r[m][0] = row_frag.get(now, m, 0);
-				r[m][1] = row_frag.get(now, m, 1);
+#pragma unroll
+				for (uint32_t half = 0; half < 2; half++) {
+					const u32x4_t q = row_frag.get(now, m, half);
+					r[m][2 * half] = widened(q.x, q.y);
+					r[m][2 * half + 1] = widened(q.z, q.w);
+				}
 			}
 #pragma unroll
 			for (int j = 0; j < (int)(2 * G); j++) {
 				const uint8_t *const columns = j < (int)G ? columns0 : columns1;
-				const u32x4_t a = column_frag.get(columns, j % G, 0), b = column_frag.get(columns, j % G, 1);
+				const u32x4_t q0 = column_frag.get(columns, j % G, 0), q1 = column_frag.get(columns, j % G, 1);
+				const u32x4_t c[4] = { widened(q0.x, q0.y), widened(q0.z, q0.w), widened(q1.x, q1.y), widened(q1.z, q1.w) };
+				f32x4_t part[4] = {};
+#pragma unroll
+				for (int k = 0; k < 4; k++) {
+#pragma unroll
+					for (int m = 0; m < 4; m++) {
+						part[m] = multiply<f16_t>(c[k], r[m][k], part[m]);
+					}
+				}
 #pragma unroll
 				for (int m = 0; m < 4; m++) {
-					const f32x4_t s = multiply8(a, b, r[m][0], r[m][1]);
 					f32x4_t &to = sums[m][j / G][j % G];
 #pragma unroll
 					for (int i = 0; i < 4; i++) {
-						to[i] = __builtin_fmaf(s[i], by[m][j / G], to[i]);
+						to[i] = __builtin_fmaf(part[m][i], by[m][j / G], to[i]);
 					}
 				}
 			}
@@ -184,9 +213,14 @@ int forward(const void *d_rows, uint64_t rows_pitch, int type, const int32_t *d_
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
+	const uint64_t bytes = (uint64_t)width * product_type_size(type);
+	const bool direct = in_chunks(d_rows, rows_pitch, bytes) && in_chunks(d_weight, weight_pitch, bytes) && expert_pitch % 16 == 0;
 	auto with = [&](auto element) {
 		using T = decltype(element);
-		auto kernel = bm == 256 ? expert_forward_kernel<T, 4, 2> : bm == 128 ? expert_forward_kernel<T, 2, 4> : expert_forward_kernel<T, 1, 4>;
+		auto kernel = direct ? (bm == 256 ? expert_forward_kernel<T, 4, 2, true>
+						: bm == 128 ? expert_forward_kernel<T, 2, 4, true> : expert_forward_kernel<T, 1, 4, true>)
+				     : (bm == 256 ? expert_forward_kernel<T, 4, 2, false>
+						: bm == 128 ? expert_forward_kernel<T, 2, 4, false> : expert_forward_kernel<T, 1, 4, false>);
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			launch_kernel(kernel, dim3(count), dim3(bm == 64 ? 256 : 512), 0, as_stream(stream), d_offset,
 				      static_cast<const uint8_t *>(d_rows), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, width, n,

@@ -162,6 +162,20 @@ template <typename T> __device__ __forceinline__ u32x4_t chunk_at(const uint8_t 
 	return v;
 }
 
+/* 16 bytes for each lane of the wavefront from the buffer to LDS, at `lds` and 16 more for each lane; zeros from beyond the buffer */
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t buffer, uint32_t offset, uint8_t *lds)
+{
+	__builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_void_t *)lds, 16, (int)offset, 0, 0, 0);
+}
+
+/* `left` bytes from p on, as far as 31 bits count */
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const uint8_t *p, int64_t left)
+{
+	const int n = left <= 0 ? 0 : left < 0x7fffffff ? (int)left : 0x7fffffff;
+	return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, n, 0x00020000);
+}
+constexpr uint32_t kBeyond = 0x80000000u; /* of any buffer */
+
 /*
  * ROWS rows of an operand whose rows run along the summed axis.  base: the first row's start; rows of them are there, each of `bytes`;
  * what is not there is zeros.
@@ -189,6 +203,18 @@ template <typename T, uint32_t ROWS, uint32_t THREADS> struct along_t {
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
 			*reinterpret_cast<u32x4_t *>(lds + (t * THREADS + threadIdx.x) * 16) = held[t];
+		}
+	}
+	/* Both at once, past the registers: rows in whole chunks (in_chunks) */
+	__device__ __forceinline__ void fill(uint32_t step, uint8_t *lds) const
+	{
+		const int64_t at = (int64_t)step * kStepBytes;
+		const auto buffer = buffer_at(base + at, rows ? (int64_t)((rows - 1) * pitch) + bytes - at : 0);
+		const uint32_t row = threadIdx.x / 8, chunk = (threadIdx.x & 7u) ^ (row & 7u), wave = uniform(threadIdx.x >> 6);
+		const uint32_t beyond = at + chunk * 16 < bytes ? 0 : kBeyond;
+#pragma unroll
+		for (uint32_t t = 0; t < kChunks; t++) {
+			to_lds(buffer, ((t * kRowsOfRound + row) * (uint32_t)pitch + chunk * 16) | beyond, lds + (t * THREADS + wave * 64) * 16);
 		}
 	}
 };
@@ -237,6 +263,17 @@ template <typename T, uint32_t W, uint32_t THREADS> struct across_t {
 			*reinterpret_cast<u32x4_t *>(lds + (t * THREADS + threadIdx.x) * 16) = held[t];
 		}
 	}
+	__device__ __forceinline__ void fill(uint32_t step, uint8_t *lds) const
+	{
+		const int64_t at = (int64_t)step * kStepRows * (int64_t)pitch;
+		const auto buffer = buffer_at(base + at, rows ? (int64_t)((rows - 1) * pitch) + bytes - at : 0);
+		const uint32_t wave = uniform(threadIdx.x >> 6);
+#pragma unroll
+		for (uint32_t t = 0; t < kChunks; t++) {
+			const uint32_t slot = t * THREADS + threadIdx.x, k = slot / kOfRow, chunk = (slot % kOfRow) ^ across_slot<W>(k);
+			to_lds(buffer, (k * (uint32_t)pitch + chunk * 16) | (chunk * 16 < bytes ? 0 : kBeyond), lds + (t * THREADS + wave * 64) * 16);
+		}
+	}
 };
 
 /* The columns of `across` that a lane feeds to a matrix instruction: eight of the summed axis in four bytes-of-two each twice */
@@ -272,14 +309,13 @@ template <typename T> __device__ __forceinline__ f32x4_t multiply(u32x4_t column
 	}
 }
 
-/* The same for 128 values of e4m3: both operands take the summed axis in the same order, whichever that is */
-__device__ __forceinline__ f32x4_t multiply8(u32x4_t columns0, u32x4_t columns1, u32x4_t rows0, u32x4_t rows1)
+/* Eight values of e4m3 as float16, which holds each of them */
+__device__ __forceinline__ u32x4_t widened(uint32_t a, uint32_t b)
 {
-	struct pair_t {
-		u32x4_t a, b;
-	};
-	const i32x8_t c = __builtin_bit_cast(i32x8_t, pair_t{ columns0, columns1 }), r = __builtin_bit_cast(i32x8_t, pair_t{ rows0, rows1 });
-	return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(c, r, f32x4_t{ 0, 0, 0, 0 }, 0, 0, 0, 127, 0, 127); /* both scales 2^0 */
+	const auto w0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false), w1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
+	const auto w2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false), w3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
+	return u32x4_t{ __builtin_bit_cast(uint32_t, w0), __builtin_bit_cast(uint32_t, w1), __builtin_bit_cast(uint32_t, w2),
+			__builtin_bit_cast(uint32_t, w3) };
 }
 
 /* ---- sums ----------------------------------------------------------------------------------------------------- */
@@ -287,48 +323,54 @@ __device__ __forceinline__ f32x4_t multiply8(u32x4_t columns0, u32x4_t columns1,
 /*
  * A tile's sums by rows: finish(row of the tile, columns of part 0, of part 1, what load(row) gave), four neighbouring columns of both
  * parts in a lane, from column 4 (lane % 32) of the part on; half a wavefront has a row, so that what is read and written of it is one
- * piece.  The sums go through LDS, a quarter of the rows at a time: 2 to 3 hundredths of the tile's time at 4096 summed, for
- * epilogues of a twentieth of the registers that whole columns in a lane would take.
+ * piece.  The sums go through LDS, half of the rows at a time, so that one loop does for all of them: unrolled over the registers the
+ * same epilogue was 200 KB of instructions.
  */
 template <uint32_t WM, uint32_t WN, typename Load, typename Finish>
 __device__ __forceinline__ void for_rows(const f32x4_t (&sums)[4][2][8 / WN], uint8_t *lds, Load load, Finish finish)
 {
-	constexpr uint32_t G = 8 / WN, kRows = WM * 16, kTurns = kRows / (WM * WN) / 2;
+	constexpr uint32_t G = 8 / WN, kTurns = 16 / WN; /* of WM * 32 rows, two to each of WM * WN wavefronts */
 	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-	__syncthreads(); /* the tiles have been read */
-	auto quarter = [&](auto which) __attribute__((always_inline)) {
-		constexpr uint32_t m = decltype(which)::value;
-		uint8_t *const buffer = lds + (m & 1u) * kRows * 1024;
-		decltype(load(0u)) in[kTurns];
-		uint32_t at[kTurns], row[kTurns];
+#pragma unroll 1
+	for (uint32_t half = 0; half < 2; half++) {
+		/* rows 32 half + [0, 32) of each 64 */
+		auto place = [&](uint32_t turn) { return (wave * kTurns + turn) * 2 + (lane >> 5); };
+		auto row_of = [&](uint32_t at) { return at / 32 * 64 + half * 32 + at % 32; };
+		auto in = load(row_of(place(0)));
+		__syncthreads(); /* the tiles, or the half before, have been read */
+		auto put = [&](uint32_t m, const f32x4_t(&from)[2][G]) {
+			const uint32_t r = wm * 32 + m * 16 + (lane & 15u);
 #pragma unroll
-		for (uint32_t i = 0; i < kTurns; i++) {
-			at[i] = (wave * kTurns + i) * 2 + (lane >> 5);
-			row[i] = at[i] / 16 * 64 + m * 16 + at[i] % 16;
-			in[i] = load(row[i]);
-		}
+			for (uint32_t p = 0; p < 2; p++) {
 #pragma unroll
-		for (uint32_t p = 0; p < 2; p++) {
-#pragma unroll
-			for (uint32_t j = 0; j < G; j++) {
-				const uint32_t r = wm * 16 + (lane & 15u), chunk = p * 32 + (wn * G + j) * 4 + (lane >> 4);
-				*reinterpret_cast<f32x4_t *>(buffer + r * 1024 + ((chunk ^ (r & 15u)) << 4)) = sums[m][p][j];
+				for (uint32_t j = 0; j < G; j++) {
+					const uint32_t chunk = p * 32 + (wn * G + j) * 4 + (lane >> 4);
+					*reinterpret_cast<f32x4_t *>(lds + r * 1024 + ((chunk ^ (r & 15u)) << 4)) = from[p][j];
+				}
 			}
+		};
+		if (half == 0) {
+			put(0, sums[0]);
+			put(1, sums[1]);
+		} else {
+			put(0, sums[2]);
+			put(1, sums[3]);
 		}
-		__syncthreads(); /* and the other buffer's readers are past it */
-#pragma unroll
-		for (uint32_t i = 0; i < kTurns; i++) {
-			const uint8_t *const from = buffer + at[i] * 1024;
-			const uint32_t chunk = (lane & 31u) ^ (at[i] & 15u);
+		__syncthreads();
+#pragma unroll 1
+		for (uint32_t turn = 0; turn < kTurns; turn++) {
+			const uint32_t at = place(turn);
+			const auto now = in;
+			if (turn + 1 < kTurns) {
+				in = load(row_of(place(turn + 1)));
+			}
+			const uint8_t *const from = lds + at * 1024;
+			const uint32_t chunk = (lane & 31u) ^ (at & 15u);
 			const f32x4_t a = *reinterpret_cast<const f32x4_t *>(from + (chunk << 4));
 			const f32x4_t b = *reinterpret_cast<const f32x4_t *>(from + ((chunk + 32) << 4));
-			finish(row[i], a, b, in[i]);
+			finish(row_of(at), a, b, now);
 		}
-	};
-	quarter(std::integral_constant<uint32_t, 0>{});
-	quarter(std::integral_constant<uint32_t, 1>{});
-	quarter(std::integral_constant<uint32_t, 2>{});
-	quarter(std::integral_constant<uint32_t, 3>{});
+	}
 }
 
 /* Where the columns of a matrix of 16-bit, float32 or e4m3 values are read and written; none: p NULL */

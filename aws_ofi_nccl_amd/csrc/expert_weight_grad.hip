@@ -19,7 +19,7 @@ template <typename T> constexpr uint32_t kTwoOnes = 0x3f803f80u; /* bfloat16 */
 template <> constexpr uint32_t kTwoOnes<f16_t> = 0x3c003c00u;
 
 /* rows of the result: m (dout's columns); columns: n (x's) */
-template <typename T, uint32_t WM, uint32_t WN>
+template <typename T, uint32_t WM, uint32_t WN, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const int32_t *offset, const uint8_t *dout, const uint8_t *x,
 									  uint32_t max_rows, uint32_t m_width, uint32_t n_width,
 									  uint32_t m_tiles, uint32_t n_tiles, uint32_t tiles, uint32_t first_tile,
@@ -63,18 +63,29 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const 
 	const across_frag_t<BM> row_frag(lane);
 	const across_frag_t<BN> column_frag(lane);
 	const uint32_t steps = (hi - lo + kStepRows - 1) / kStepRows;
-	if (steps) {
+	if (DIRECT && steps) {
+		rows.fill(0, lds);
+		columns.fill(0, lds + rows_tile::kBytes);
+	} else if (steps) {
 		rows.load(0);
 		columns.load(0);
 	}
 	for (uint32_t step = 0; step < steps; step++) {
 		uint8_t *const now = lds + (step & 1u) * kTile, *const now_columns = now + rows_tile::kBytes;
-		rows.store(now);
-		columns.store(now_columns);
-		__syncthreads(); /* the other tile's readers are past it, too */
+		if (!DIRECT) {
+			rows.store(now);
+			columns.store(now_columns);
+		}
+		__syncthreads(); /* this tile is there, and the other one's readers are past it */
 		if (step + 1 < steps) {
-			rows.load(step + 1);
-			columns.load(step + 1);
+			uint8_t *const next = lds + ((step + 1) & 1u) * kTile;
+			if (DIRECT) {
+				rows.fill(step + 1, next);
+				columns.fill(step + 1, next + rows_tile::kBytes);
+			} else {
+				rows.load(step + 1);
+				columns.load(step + 1);
+			}
 		}
 #pragma unroll
 		for (uint32_t half = 0; half < 2; half++) {
@@ -178,6 +189,7 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
+	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * out_width) && in_chunks(d_rows, rows_pitch, 2ull * width);
 	weight_grad_t o = {};
 	o.out = { static_cast<uint8_t *>(d_dweight), dweight_pitch, dweight_type, nullptr, 0 };
 	o.add = { static_cast<uint8_t *>(const_cast<void *>(d_add)), dweight_pitch, dweight_type, nullptr, 0 };
@@ -186,7 +198,8 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	o.dbias = d_dbias;
 	auto with = [&](auto element) {
 		using T = decltype(element);
-		auto kernel = wide ? expert_weight_grad_kernel<T, 4, 2> : expert_weight_grad_kernel<T, 2, 4>;
+		auto kernel = direct ? (wide ? expert_weight_grad_kernel<T, 4, 2, true> : expert_weight_grad_kernel<T, 2, 4, true>)
+				     : (wide ? expert_weight_grad_kernel<T, 4, 2, false> : expert_weight_grad_kernel<T, 2, 4, false>);
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset, static_cast<const uint8_t *>(d_dout),
 				      static_cast<const uint8_t *>(d_rows), max_rows, out_width, width, m_tiles, n_tiles, (uint32_t)tiles, first,
