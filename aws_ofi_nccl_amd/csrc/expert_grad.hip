@@ -18,13 +18,13 @@ struct backward_t {
 };
 
 /* k: the product's outputs, n: its columns */
-template <typename T, uint32_t WM, uint32_t WN, bool HIDDEN, bool DIRECT>
+template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool HIDDEN, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int32_t *offset, const uint8_t *dout, const uint8_t *w,
 								       uint32_t n_experts, uint32_t max_rows, uint32_t k, uint32_t n,
 								       uint32_t n_tiles, uint32_t first_tile, uint64_t dout_pitch,
 								       uint64_t w_pitch, uint64_t expert_pitch, backward_t o)
 {
-	constexpr uint32_t BM = 64 * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
+	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
 	using rows_tile = along_t<T, BM, THREADS>;
 	using columns_tile = across_t<T, BN, THREADS>;
 	constexpr uint32_t kTile = rows_tile::kBytes + columns_tile::kBytes;
@@ -39,65 +39,38 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int
 	rows_tile rows = { dout + tile.from * dout_pitch, dout_pitch, tile.rows, (int64_t)k * 2 };
 	columns_tile columns = { w + tile.expert * expert_pitch + c0 * 2, w_pitch, k, (int64_t)there * 2 };
 
-	f32x4_t sums[4][2][G];
+	f32x4_t sums[MF][2][G];
 #pragma unroll
-	for (int m = 0; m < 4; m++) {
+	for (int m = 0; m < (int)MF; m++) {
 #pragma unroll
 		for (int j = 0; j < (int)(2 * G); j++) {
 			sums[m][j / G][j % G] = f32x4_t{ 0, 0, 0, 0 };
 		}
 	}
-	const along_frag_t row_frag(wm * 64, lane);
-	const across_frag_t<BN> column_frag(lane);
-	const uint32_t steps = (k + kStepRows - 1) / kStepRows;
-	if (DIRECT) {
-		rows.fill(0, lds);
-		columns.fill(0, lds + rows_tile::kBytes);
-	} else {
-		rows.load(0);
-		columns.load(0);
-	}
-	for (uint32_t step = 0; step < steps; step++) {
-		uint8_t *const now = lds + (step & 1u) * kTile, *const now_columns = now + rows_tile::kBytes;
-		if (!DIRECT) {
-			rows.store(now);
-			columns.store(now_columns);
-		}
-		__syncthreads(); /* this tile is there, and the other one's readers are past it */
-		if (step + 1 < steps) {
-			uint8_t *const next = lds + ((step + 1) & 1u) * kTile;
-			if (DIRECT) {
-				rows.fill(step + 1, next);
-				columns.fill(step + 1, next + rows_tile::kBytes);
-			} else {
-				rows.load(step + 1);
-				columns.load(step + 1);
-			}
-		}
-#pragma unroll
-		for (uint32_t half = 0; half < 2; half++) {
-			u32x4_t r[4];
-#pragma unroll
-			for (int m = 0; m < 4; m++) {
-				r[m] = row_frag.get(now, m, half);
-			}
-#pragma unroll
-			for (int j = 0; j < (int)(2 * G); j++) {
-				const u32x4_t c = column_frag.get(now_columns, j / G * kBlock + wn * 16 * G + j % G * 16, half);
-#pragma unroll
-				for (int m = 0; m < 4; m++) {
-					sums[m][j / G][j % G] = multiply<T>(c, r[m], sums[m][j / G][j % G]);
-				}
-			}
-		}
-	}
+	const along_frag_t row_frag(wm * 16 * MF, lane);
+	const across_frag_t<BN> column_frag(wn * 16 * G, lane);
+	sum_steps<T, DIRECT>(
+		sums, (k + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
+		[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
+			rows.fill(step, to);
+			columns.fill(step, to + rows_tile::kBytes);
+		},
+		[&](uint32_t step) __attribute__((always_inline)) {
+			rows.load(step);
+			columns.load(step);
+		},
+		[&](uint8_t *to) __attribute__((always_inline)) {
+			rows.store(to);
+			columns.store(to + rows_tile::kBytes);
+		},
+		[](const u32x4_t(&)[MF]) {});
 
 	const uint32_t c = (lane & 31u) * 4, blocks = blocks_of(n), block = c0 / kBlock;
 	const uint32_t left[2] = { c < there ? there - c : 0, c + kBlock < there ? there - c - kBlock : 0 };
 	struct in_t {
 		f32x4_t g[2], u[2]; /* what was kept, or what is added */
 	};
-	for_rows<WM, WN>(
+	for_rows<WM, WN, MF>(
 		sums, lds,
 		[&](uint32_t r) {
 			in_t in = {};
@@ -164,13 +137,14 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * k) && in_chunks(d_weight, weight_pitch, 2ull * n) && expert_pitch % 16 == 0;
 	auto with = [&](auto element) {
 		using T = decltype(element);
-		auto kernel =
-			direct ? (bm == 256 ? expert_backward_kernel<T, 4, 2, HIDDEN, true>
-					    : bm == 128 ? expert_backward_kernel<T, 2, 4, HIDDEN, true> : expert_backward_kernel<T, 1, 4, HIDDEN, true>)
-			       : (bm == 256 ? expert_backward_kernel<T, 4, 2, HIDDEN, false>
-					    : bm == 128 ? expert_backward_kernel<T, 2, 4, HIDDEN, false> : expert_backward_kernel<T, 1, 4, HIDDEN, false>);
+		auto kernel = direct ? (bm == 256 ? expert_backward_kernel<T, 4, 2, 4, HIDDEN, true>
+						: bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, true>
+							    : expert_backward_kernel<T, 1, 8, 4, HIDDEN, true>)
+				     : (bm == 256 ? expert_backward_kernel<T, 4, 2, 4, HIDDEN, false>
+						: bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, false>
+							    : expert_backward_kernel<T, 1, 8, 4, HIDDEN, false>);
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
-			launch_kernel(kernel, dim3(count), dim3(bm == 64 ? 256 : 512), 0, as_stream(stream), d_offset,
+			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset,
 				      static_cast<const uint8_t *>(d_dout), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, k, n,
 				      n_tiles, first, dout_pitch, weight_pitch, expert_pitch, o);
 		});

@@ -18,13 +18,13 @@ struct forward_t {
 	bool gated;
 };
 
-template <typename T, uint32_t WM, uint32_t WN, bool DIRECT>
+template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int32_t *offset, const uint8_t *x, const uint8_t *w, uint32_t n_experts,
 								      uint32_t max_rows, uint32_t width, uint32_t n, uint32_t n_tiles,
 								      uint32_t first_tile, uint64_t x_pitch, uint64_t w_pitch,
 								      uint64_t expert_pitch, forward_t o)
 {
-	constexpr uint32_t BM = 64 * WM, THREADS = 64 * WM * WN, G = 8 / WN;
+	constexpr uint32_t BM = 16 * MF * WM, THREADS = 64 * WM * WN, G = 8 / WN;
 	constexpr bool SCALED = sizeof(T) == 1;
 	using rows_tile = along_t<T, BM, THREADS>;
 	using part_tile = along_t<T, kBlock, THREADS>;
@@ -45,115 +45,100 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 	part_tile part0 = { weights + c0 * w_pitch, w_pitch, there0, bytes };
 	part_tile part1 = { weights + (there1 ? (o.gated ? (uint64_t)n : 0) + c1 : 0) * w_pitch, w_pitch, there1, bytes };
 
-	f32x4_t sums[4][2][G];
+	f32x4_t sums[MF][2][G];
 #pragma unroll
-	for (int m = 0; m < 4; m++) {
+	for (int m = 0; m < (int)MF; m++) {
 #pragma unroll
 		for (int j = 0; j < (int)(2 * G); j++) {
 			sums[m][j / G][j % G] = f32x4_t{ 0, 0, 0, 0 };
 		}
 	}
-	const along_frag_t row_frag(wm * 64, lane), column_frag(wn * 16 * G, lane);
+	const along_frag_t row_frag(wm * 16 * MF, lane), column_frag(wn * 16 * G, lane);
 	const uint32_t steps = (width + kStepOf<T> - 1) / kStepOf<T>;
-	/* 8-bit rows: a lane's row of each of its four groups */
-	const float *row_scale[4], *weight_scale[2];
-	if constexpr (SCALED) {
+	auto fill = [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
+		rows.fill(step, to);
+		part0.fill(step, to + rows_tile::kBytes);
+		part1.fill(step, to + rows_tile::kBytes + part_tile::kBytes);
+	};
+	auto load = [&](uint32_t step) __attribute__((always_inline)) {
+		rows.load(step);
+		part0.load(step);
+		part1.load(step);
+	};
+	auto store = [&](uint8_t *to) __attribute__((always_inline)) {
+		rows.store(to);
+		part0.store(to + rows_tile::kBytes);
+		part1.store(to + rows_tile::kBytes + part_tile::kBytes);
+	};
+	if constexpr (!SCALED) {
+		sum_steps<T, DIRECT>(sums, steps, lds, kTile, rows_tile::kBytes, row_frag, column_frag, fill, load, store,
+				     [](const u32x4_t(&)[MF]) {});
+	} else {
+		/* a lane's row of each of its groups */
+		const float *row_scale[MF], *weight_scale[2];
 		const uint32_t k_blocks = blocks_of(width), n_blocks = blocks_of(n);
 		const float *of_expert = o.weight_scale + (uint64_t)tile.expert * (o.gated ? 2 : 1) * n_blocks * k_blocks;
 		weight_scale[0] = of_expert + (uint64_t)(c0 / kBlock) * k_blocks;
 		weight_scale[1] = there1 ? of_expert + (uint64_t)((o.gated ? n_blocks : 0) + c1 / kBlock) * k_blocks : weight_scale[0];
 #pragma unroll
-		for (int m = 0; m < 4; m++) {
-			const uint32_t r = wm * 64 + m * 16 + (lane & 15u);
+		for (int m = 0; m < (int)MF; m++) {
+			const uint32_t r = (wm * MF + m) * 16 + (lane & 15u);
 			row_scale[m] = row_at(o.scale, o.scale_pitch, tile.from + (r < tile.rows ? r : tile.rows - 1));
 		}
-	}
-	auto fill = [&](uint32_t step) {
-		uint8_t *const to = lds + (step & 1u) * kTile;
-		rows.fill(step, to);
-		part0.fill(step, to + rows_tile::kBytes);
-		part1.fill(step, to + rows_tile::kBytes + part_tile::kBytes);
-	};
-	auto load = [&](uint32_t step) {
-		rows.load(step);
-		part0.load(step);
-		part1.load(step);
-	};
-	if (DIRECT) {
-		fill(0);
-	} else {
-		load(0);
-	}
-	for (uint32_t step = 0; step < steps; step++) {
-		uint8_t *const now = lds + (step & 1u) * kTile, *const columns0 = now + rows_tile::kBytes;
-		uint8_t *const columns1 = columns0 + part_tile::kBytes;
-		if (!DIRECT) {
-			rows.store(now);
-			part0.store(columns0);
-			part1.store(columns1);
+		if (DIRECT) {
+			fill(0, lds);
+		} else {
+			load(0);
 		}
-		__syncthreads(); /* this tile is there, and the other one's readers are past it */
-		if (step + 1 < steps) {
+		for (uint32_t step = 0; step < steps; step++) {
+			uint8_t *const now = lds + (step & 1u) * kTile;
 			if (DIRECT) {
-				fill(step + 1);
+				landed();
 			} else {
-				load(step + 1);
+				store(now);
 			}
-		}
-		if constexpr (SCALED) {
-			float by[4][2];
+			__syncthreads(); /* this tile is there, and the other one's readers are past it */
+			if (step + 1 < steps) {
+				if (DIRECT) {
+					fill(step + 1, lds + (~step & 1u) * kTile);
+				} else {
+					load(step + 1);
+				}
+			}
+			float by[MF][2];
+			u32x4_t r[MF][4];
 #pragma unroll
-			for (int m = 0; m < 4; m++) {
+			for (int m = 0; m < (int)MF; m++) {
 				const float s = row_scale[m][step];
 				by[m][0] = s * weight_scale[0][step];
 				by[m][1] = s * weight_scale[1][step];
-			}
-			u32x4_t r[4][4];
-#pragma unroll
-			for (int m = 0; m < 4; m++) {
 #pragma unroll
 				for (uint32_t half = 0; half < 2; half++) {
-					const u32x4_t q = row_frag.get(now, m, half);
+					const u32x4_t q = row_frag.get(now, m * 16, half);
 					r[m][2 * half] = widened(q.x, q.y);
 					r[m][2 * half + 1] = widened(q.z, q.w);
 				}
 			}
 #pragma unroll
 			for (int j = 0; j < (int)(2 * G); j++) {
-				const uint8_t *const columns = j < (int)G ? columns0 : columns1;
-				const u32x4_t q0 = column_frag.get(columns, j % G, 0), q1 = column_frag.get(columns, j % G, 1);
+				const uint8_t *const columns = now + rows_tile::kBytes;
+				const u32x4_t q0 = column_frag.get(columns, j / G * kBlock + j % G * 16, 0);
+				const u32x4_t q1 = column_frag.get(columns, j / G * kBlock + j % G * 16, 1);
 				const u32x4_t c[4] = { widened(q0.x, q0.y), widened(q0.z, q0.w), widened(q1.x, q1.y), widened(q1.z, q1.w) };
-				f32x4_t part[4] = {};
+				f32x4_t part[MF] = {};
 #pragma unroll
 				for (int k = 0; k < 4; k++) {
 #pragma unroll
-					for (int m = 0; m < 4; m++) {
+					for (int m = 0; m < (int)MF; m++) {
 						part[m] = multiply<f16_t>(c[k], r[m][k], part[m]);
 					}
 				}
 #pragma unroll
-				for (int m = 0; m < 4; m++) {
+				for (int m = 0; m < (int)MF; m++) {
 					f32x4_t &to = sums[m][j / G][j % G];
 #pragma unroll
 					for (int i = 0; i < 4; i++) {
 						to[i] = __builtin_fmaf(part[m][i], by[m][j / G], to[i]);
-					}
-				}
-			}
-		} else {
-#pragma unroll
-			for (uint32_t half = 0; half < 2; half++) {
-				u32x4_t r[4];
-#pragma unroll
-				for (int m = 0; m < 4; m++) {
-					r[m] = row_frag.get(now, m, half);
-				}
-#pragma unroll
-				for (int j = 0; j < (int)(2 * G); j++) {
-					const u32x4_t c = column_frag.get(j < (int)G ? columns0 : columns1, j % G, half);
-#pragma unroll
-					for (int m = 0; m < 4; m++) {
-						sums[m][j / G][j % G] = multiply<T>(c, r[m], sums[m][j / G][j % G]);
 					}
 				}
 			}
@@ -170,7 +155,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 	struct in_t {
 		f32x4_t add0, add1;
 	};
-	for_rows<WM, WN>(
+	for_rows<WM, WN, MF>(
 		sums, lds,
 		[&](uint32_t r) {
 			in_t in = {};
@@ -217,12 +202,12 @@ int forward(const void *d_rows, uint64_t rows_pitch, int type, const int32_t *d_
 	const bool direct = in_chunks(d_rows, rows_pitch, bytes) && in_chunks(d_weight, weight_pitch, bytes) && expert_pitch % 16 == 0;
 	auto with = [&](auto element) {
 		using T = decltype(element);
-		auto kernel = direct ? (bm == 256 ? expert_forward_kernel<T, 4, 2, true>
-						: bm == 128 ? expert_forward_kernel<T, 2, 4, true> : expert_forward_kernel<T, 1, 4, true>)
-				     : (bm == 256 ? expert_forward_kernel<T, 4, 2, false>
-						: bm == 128 ? expert_forward_kernel<T, 2, 4, false> : expert_forward_kernel<T, 1, 4, false>);
+		auto kernel = direct ? (bm == 256 ? expert_forward_kernel<T, 4, 2, 4, true>
+						: bm == 128 ? expert_forward_kernel<T, 2, 4, 4, true> : expert_forward_kernel<T, 1, 8, 4, true>)
+				     : (bm == 256 ? expert_forward_kernel<T, 4, 2, 4, false>
+						: bm == 128 ? expert_forward_kernel<T, 2, 4, 4, false> : expert_forward_kernel<T, 1, 8, 4, false>);
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
-			launch_kernel(kernel, dim3(count), dim3(bm == 64 ? 256 : 512), 0, as_stream(stream), d_offset,
+			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset,
 				      static_cast<const uint8_t *>(d_rows), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, width, n,
 				      n_tiles, first, rows_pitch, weight_pitch, expert_pitch, o);
 		});

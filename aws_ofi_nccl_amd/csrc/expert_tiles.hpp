@@ -162,18 +162,21 @@ template <typename T> __device__ __forceinline__ u32x4_t chunk_at(const uint8_t 
 	return v;
 }
 
-/* 16 bytes for each lane of the wavefront from the buffer to LDS, at `lds` and 16 more for each lane; zeros from beyond the buffer */
-__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t buffer, uint32_t offset, uint8_t *lds)
+/*
+ * 16 bytes for each lane of the wavefront from a buffer of `bytes` at p, to LDS at `lds` (of the wavefront) and 16 more for each lane;
+ * zeros from beyond the buffer.  Written as the instruction, because the compiler waits for the builtin's bytes before the next
+ * exchanging read of LDS, whichever part of it that reads: the wait is landed()'s.
+ */
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void to_lds(const uint8_t *p, int bytes, uint32_t offset, uint8_t *lds)
 {
-	__builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_void_t *)lds, 16, (int)offset, 0, 0, 0);
+	const uint64_t at = reinterpret_cast<uint64_t>(p);
+	const i32x4_t buffer = { (int)uniform((uint32_t)at), (int)uniform((uint32_t)(at >> 32) & 0xffffu), (int)uniform((uint32_t)bytes), 0x00020000 };
+	const uint32_t to = uniform((uint32_t)reinterpret_cast<uintptr_t>((lds_void_t *)lds));
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory");
 }
-
-/* `left` bytes from p on, as far as 31 bits count */
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const uint8_t *p, int64_t left)
-{
-	const int n = left <= 0 ? 0 : left < 0x7fffffff ? (int)left : 0x7fffffff;
-	return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, n, 0x00020000);
-}
+/* All of the wavefront's to_lds have landed */
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 constexpr uint32_t kBeyond = 0x80000000u; /* of any buffer */
 
 /*
@@ -205,31 +208,34 @@ template <typename T, uint32_t ROWS, uint32_t THREADS> struct along_t {
 			*reinterpret_cast<u32x4_t *>(lds + (t * THREADS + threadIdx.x) * 16) = held[t];
 		}
 	}
-	/* Both at once, past the registers: rows in whole chunks (in_chunks) */
+	/* Both at once, past the registers: rows in whole chunks (in_chunks), so that a tile is within 31 bits */
 	__device__ __forceinline__ void fill(uint32_t step, uint8_t *lds) const
 	{
-		const int64_t at = (int64_t)step * kStepBytes;
-		const auto buffer = buffer_at(base + at, rows ? (int64_t)((rows - 1) * pitch) + bytes - at : 0);
 		const uint32_t row = threadIdx.x / 8, chunk = (threadIdx.x & 7u) ^ (row & 7u), wave = uniform(threadIdx.x >> 6);
-		const uint32_t beyond = at + chunk * 16 < bytes ? 0 : kBeyond;
+		const uint32_t at = step * kStepBytes, apart = (uint32_t)pitch * kRowsOfRound;
+		const uint32_t place = (row * (uint32_t)pitch + chunk * 16) | (at + chunk * 16 < (uint32_t)bytes ? 0 : kBeyond);
+		const int left = rows ? (int)((rows - 1) * (uint32_t)pitch + (uint32_t)bytes) - (int)at : 0;
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
-			to_lds(buffer, ((t * kRowsOfRound + row) * (uint32_t)pitch + chunk * 16) | beyond, lds + (t * THREADS + wave * 64) * 16);
+			const int n = left - (int)(t * apart);
+			to_lds(base + at + (uint64_t)(t * apart), n > 0 ? n : 0, place, lds + (t * THREADS + wave * 64) * 16);
 		}
 	}
 };
 
-/* The rows of `along` that a lane feeds to a matrix instruction: 32 bytes of each, in two halves of 16 */
+/* The rows of `along` that a lane feeds to a matrix instruction: 16 bytes of each half of a step */
 struct along_frag_t {
-	uint32_t at;
+	static constexpr int kReads = 1;
+	uint32_t at[2];
 	__device__ __forceinline__ along_frag_t(uint32_t first_row, uint32_t lane)
-		: at((first_row + (lane & 15u)) * kStepBytes + (((lane >> 4) ^ (lane & 7u)) << 4))
 	{
+		at[0] = (first_row + (lane & 15u)) * kStepBytes + (((lane >> 4) ^ (lane & 7u)) << 4);
+		at[1] = at[0] ^ 64u;
 	}
-	/* group: of 16 rows; half: of the step */
-	__device__ __forceinline__ u32x4_t get(const uint8_t *lds, uint32_t group, uint32_t half) const
+	/* row: the first of 16, behind first_row */
+	__device__ __forceinline__ u32x4_t get(const uint8_t *lds, uint32_t row, uint32_t half) const
 	{
-		return *reinterpret_cast<const u32x4_t *>(lds + ((at + group * 16 * kStepBytes) ^ (half << 6)));
+		return *reinterpret_cast<const u32x4_t *>(lds + at[half] + row * kStepBytes);
 	}
 };
 
@@ -265,33 +271,42 @@ template <typename T, uint32_t W, uint32_t THREADS> struct across_t {
 	}
 	__device__ __forceinline__ void fill(uint32_t step, uint8_t *lds) const
 	{
-		const int64_t at = (int64_t)step * kStepRows * (int64_t)pitch;
-		const auto buffer = buffer_at(base + at, rows ? (int64_t)((rows - 1) * pitch) + bytes - at : 0);
-		const uint32_t wave = uniform(threadIdx.x >> 6);
+		constexpr uint32_t kRowsOfRound = THREADS / kOfRow;
+		const uint64_t at = (uint64_t)step * kStepRows * pitch;
+		const int64_t left = rows ? (int64_t)((rows - 1) * pitch + bytes - at) : 0;
+		const uint32_t apart = (uint32_t)pitch * kRowsOfRound, row = threadIdx.x / kOfRow, wave = uniform(threadIdx.x >> 6);
+		const int some = left <= 0 ? 0 : left < 0x7fffffff ? (int)left : 0x7fffffff;
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
-			const uint32_t slot = t * THREADS + threadIdx.x, k = slot / kOfRow, chunk = (slot % kOfRow) ^ across_slot<W>(k);
-			to_lds(buffer, (k * (uint32_t)pitch + chunk * 16) | (chunk * 16 < bytes ? 0 : kBeyond), lds + (t * THREADS + wave * 64) * 16);
+			const uint32_t chunk = (threadIdx.x % kOfRow) ^ across_slot<W>(t * kRowsOfRound + row);
+			const uint32_t place = (row * (uint32_t)pitch + chunk * 16) | (chunk * 16 < (uint32_t)bytes ? 0 : kBeyond);
+			const int n = some - (int)(t * apart);
+			to_lds(base + at + (uint64_t)(t * apart), n > 0 ? n : 0, place, lds + (t * THREADS + wave * 64) * 16);
 		}
 	}
 };
 
-/* The columns of `across` that a lane feeds to a matrix instruction: eight of the summed axis in four bytes-of-two each twice */
+/* The columns of `across` that a lane feeds to a matrix instruction: eight of the summed axis, four at a time */
 template <uint32_t W> struct across_frag_t {
-	uint32_t row, swizzle, low;
-	__device__ __forceinline__ across_frag_t(uint32_t lane)
+	static constexpr int kReads = 2;
+	uint32_t at[4]; /* of the first four groups of 16 columns; the others are a multiple of 128 bytes or flip bits of these */
+	uint32_t first;
+	__device__ __forceinline__ across_frag_t(uint32_t first_column, uint32_t lane)
 	{
 		const uint32_t k = (lane >> 4) * 8 + ((lane & 15u) >> 2);
-		row = k * W * 2 + (lane & 1u) * 8;
-		swizzle = across_slot<W>(k);
-		low = (lane & 3u) >> 1;
+		first = first_column;
+#pragma unroll
+		for (uint32_t g = 0; g < 4; g++) {
+			at[g] = k * W * 2 + (lane & 1u) * 8 + ((((first_column / 8 + 2 * g) ^ across_slot<W>(k)) + ((lane & 3u) >> 1)) << 4);
+		}
 	}
-	/* column: the first of 16 */
+	/* column: the first of 16, behind first_column */
 	__device__ __forceinline__ u32x4_t get(uint8_t *lds, uint32_t column, uint32_t half) const
 	{
-		const uint32_t at = row + (((column / 8 ^ swizzle) + low) << 4) + half * 32 * W * 2;
-		const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(lds + at));
-		const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(lds + at + 4 * W * 2));
+		/* groups four on flip the bit above, which first_column (a multiple of 128 where there are more than four) has not set */
+		uint8_t *const p = lds + ((at[column / 16 & 3u] ^ (column & 64u ? 128u : 0u)) + (column & 128u ? 256u : 0u)) + half * 32 * W * 2;
+		const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)p);
+		const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(p + 4 * W * 2));
 		const u32x2_t lo = __builtin_bit_cast(u32x2_t, a), hi = __builtin_bit_cast(u32x2_t, b);
 		return u32x4_t{ lo.x, lo.y, hi.x, hi.y };
 	}
@@ -318,6 +333,91 @@ __device__ __forceinline__ u32x4_t widened(uint32_t a, uint32_t b)
 			__builtin_bit_cast(uint32_t, w3) };
 }
 
+/*
+ * sums[m][p][j] += all steps.  Fragments of half a step are read while the other half's are multiplied.  When all of a step's are in
+ * registers, a barrier: the next step's tile is there (it was asked for a step before), and this one's place is free for the step
+ * after that.  fill: both operands' tiles of a step to LDS; or load: to registers, and store: from there.
+ * Fills behind the last step write zeros.
+ */
+template <typename T, bool DIRECT, uint32_t MF, uint32_t G, typename RowFrag, typename ColumnFrag, typename Fill, typename Load, typename Store,
+	  typename Also>
+__device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], uint32_t steps, uint8_t *lds, uint32_t tile_bytes, uint32_t rows_bytes,
+					  const RowFrag &row_frag, const ColumnFrag &column_frag, Fill fill, Load load, Store store, Also also)
+{
+	u32x4_t r[2][MF], c[2][2 * G];
+	auto read = [&](uint8_t *tile, uint32_t half, u32x4_t(&rows)[MF], u32x4_t(&columns)[2 * G]) __attribute__((always_inline)) {
+#pragma unroll
+		for (uint32_t m = 0; m < MF; m++) {
+			rows[m] = row_frag.get(tile, m * 16, half);
+		}
+#pragma unroll
+		for (uint32_t j = 0; j < 2 * G; j++) {
+			columns[j] = column_frag.get(tile + rows_bytes, j / G * kBlock + j % G * 16, half);
+		}
+	};
+	auto mul = [&](const u32x4_t(&rows)[MF], const u32x4_t(&columns)[2 * G]) __attribute__((always_inline)) {
+#pragma unroll
+		for (uint32_t j = 0; j < 2 * G; j++) {
+#pragma unroll
+			for (uint32_t m = 0; m < MF; m++) {
+				sums[m][j / G][j % G] = multiply<T>(columns[j], rows[m], sums[m][j / G][j % G]);
+			}
+		}
+		also(rows);
+	};
+	/* reads of LDS in pairs of matrix instructions, so that they are done when their half begins */
+	auto spread = [&]() __attribute__((always_inline)) {
+		constexpr int kReads = MF * RowFrag::kReads + 2 * G * ColumnFrag::kReads, kPairs = MF * G;
+		constexpr int kEach = (kReads + kPairs - 1) / kPairs;
+#pragma unroll
+		for (int i = 0; i < kPairs; i++) {
+			__builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+			__builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+		}
+		__builtin_amdgcn_sched_barrier(0);
+	};
+	if (steps == 0) {
+		return;
+	}
+	if (DIRECT) {
+		fill(0, lds);
+		landed();
+		__syncthreads();
+		fill(1, lds + tile_bytes);
+	} else {
+		load(0);
+		store(lds);
+		__syncthreads();
+		load(1);
+	}
+	read(lds, 0, r[0], c[0]);
+	for (uint32_t step = 0; step < steps; step++) {
+		uint8_t *const now = lds + (step & 1u) * tile_bytes, *const next = lds + (~step & 1u) * tile_bytes;
+		read(now, 1, r[1], c[1]);
+		mul(r[0], c[0]);
+		spread();
+		if (DIRECT) {
+			landed();
+		} else {
+			store(next);
+		}
+		__syncthreads();
+		__builtin_amdgcn_sched_barrier(0);
+		if (DIRECT) {
+			fill(step + 2, now);
+		} else {
+			load(step + 2);
+		}
+		__builtin_amdgcn_sched_barrier(0);
+		read(next, 0, r[0], c[0]);
+		mul(r[1], c[1]);
+		spread();
+	}
+	if (DIRECT) {
+		landed(); /* what follows writes there */
+	}
+}
+
 /* ---- sums ----------------------------------------------------------------------------------------------------- */
 
 /*
@@ -326,20 +426,20 @@ __device__ __forceinline__ u32x4_t widened(uint32_t a, uint32_t b)
  * piece.  The sums go through LDS, half of the rows at a time, so that one loop does for all of them: unrolled over the registers the
  * same epilogue was 200 KB of instructions.
  */
-template <uint32_t WM, uint32_t WN, typename Load, typename Finish>
-__device__ __forceinline__ void for_rows(const f32x4_t (&sums)[4][2][8 / WN], uint8_t *lds, Load load, Finish finish)
+template <uint32_t WM, uint32_t WN, uint32_t MF, typename Load, typename Finish>
+__device__ __forceinline__ void for_rows(const f32x4_t (&sums)[MF][2][8 / WN], uint8_t *lds, Load load, Finish finish)
 {
-	constexpr uint32_t G = 8 / WN, kTurns = 16 / WN; /* of WM * 32 rows, two to each of WM * WN wavefronts */
+	constexpr uint32_t G = 8 / WN, kOfWave = MF * 8; /* rows of half a wavefront's tile */
+	constexpr uint32_t kTurns = kOfWave / WN / 2;    /* of WM * kOfWave rows, two to each of WM * WN wavefronts */
 	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
 #pragma unroll 1
 	for (uint32_t half = 0; half < 2; half++) {
-		/* rows 32 half + [0, 32) of each 64 */
 		auto place = [&](uint32_t turn) { return (wave * kTurns + turn) * 2 + (lane >> 5); };
-		auto row_of = [&](uint32_t at) { return at / 32 * 64 + half * 32 + at % 32; };
+		auto row_of = [&](uint32_t at) { return at / kOfWave * 2 * kOfWave + half * kOfWave + at % kOfWave; };
 		auto in = load(row_of(place(0)));
 		__syncthreads(); /* the tiles, or the half before, have been read */
-		auto put = [&](uint32_t m, const f32x4_t(&from)[2][G]) {
-			const uint32_t r = wm * 32 + m * 16 + (lane & 15u);
+		auto put = [&](uint32_t m, const f32x4_t(&from)[2][G]) __attribute__((always_inline)) {
+			const uint32_t r = wm * kOfWave + m * 16 + (lane & 15u);
 #pragma unroll
 			for (uint32_t p = 0; p < 2; p++) {
 #pragma unroll
@@ -350,11 +450,15 @@ __device__ __forceinline__ void for_rows(const f32x4_t (&sums)[4][2][8 / WN], ui
 			}
 		};
 		if (half == 0) {
-			put(0, sums[0]);
-			put(1, sums[1]);
+#pragma unroll
+			for (uint32_t m = 0; m < MF / 2; m++) {
+				put(m, sums[m]);
+			}
 		} else {
-			put(0, sums[2]);
-			put(1, sums[3]);
+#pragma unroll
+			for (uint32_t m = 0; m < MF / 2; m++) {
+				put(m, sums[MF / 2 + m]);
+			}
 		}
 		__syncthreads();
 #pragma unroll 1

@@ -19,13 +19,13 @@ template <typename T> constexpr uint32_t kTwoOnes = 0x3f803f80u; /* bfloat16 */
 template <> constexpr uint32_t kTwoOnes<f16_t> = 0x3c003c00u;
 
 /* rows of the result: m (dout's columns); columns: n (x's) */
-template <typename T, uint32_t WM, uint32_t WN, bool DIRECT>
+template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const int32_t *offset, const uint8_t *dout, const uint8_t *x,
 									  uint32_t max_rows, uint32_t m_width, uint32_t n_width,
 									  uint32_t m_tiles, uint32_t n_tiles, uint32_t tiles, uint32_t first_tile,
 									  uint64_t dout_pitch, uint64_t x_pitch, weight_grad_t o)
 {
-	constexpr uint32_t BM = 64 * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
+	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
 	using rows_tile = across_t<T, BM, THREADS>;
 	using columns_tile = across_t<T, BN, THREADS>;
 	constexpr uint32_t kTile = rows_tile::kBytes + columns_tile::kBytes;
@@ -49,73 +49,52 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const 
 	const uint32_t m_there = m_width - m0 < BM ? m_width - m0 : BM, n_there = n_width - n0 < BN ? n_width - n0 : BN;
 	rows_tile rows = { dout + lo * dout_pitch + m0 * 2, dout_pitch, hi - lo, (int64_t)m_there * 2 };
 	columns_tile columns = { x + lo * x_pitch + n0 * 2, x_pitch, hi - lo, (int64_t)n_there * 2 };
-	const bool with_bias = o.dbias && n0 == 0 && wn == 0;
+	const bool with_bias = o.dbias && n0 == 0; /* of one column tile, in a loop of its own */
 
-	f32x4_t sums[4][2][G], bias[4];
+	f32x4_t sums[MF][2][G], bias[MF];
 #pragma unroll
-	for (int m = 0; m < 4; m++) {
+	for (int m = 0; m < (int)MF; m++) {
 		bias[m] = f32x4_t{ 0, 0, 0, 0 };
 #pragma unroll
 		for (int j = 0; j < (int)(2 * G); j++) {
 			sums[m][j / G][j % G] = f32x4_t{ 0, 0, 0, 0 };
 		}
 	}
-	const across_frag_t<BM> row_frag(lane);
-	const across_frag_t<BN> column_frag(lane);
-	const uint32_t steps = (hi - lo + kStepRows - 1) / kStepRows;
-	if (DIRECT && steps) {
-		rows.fill(0, lds);
-		columns.fill(0, lds + rows_tile::kBytes);
-	} else if (steps) {
-		rows.load(0);
-		columns.load(0);
-	}
-	for (uint32_t step = 0; step < steps; step++) {
-		uint8_t *const now = lds + (step & 1u) * kTile, *const now_columns = now + rows_tile::kBytes;
-		if (!DIRECT) {
-			rows.store(now);
-			columns.store(now_columns);
-		}
-		__syncthreads(); /* this tile is there, and the other one's readers are past it */
-		if (step + 1 < steps) {
-			uint8_t *const next = lds + ((step + 1) & 1u) * kTile;
-			if (DIRECT) {
-				rows.fill(step + 1, next);
-				columns.fill(step + 1, next + rows_tile::kBytes);
-			} else {
-				rows.load(step + 1);
-				columns.load(step + 1);
+	const across_frag_t<BM> row_frag(wm * 16 * MF, lane);
+	const across_frag_t<BN> column_frag(wn * 16 * G, lane);
+	auto sum = [&](auto also) __attribute__((always_inline)) {
+		sum_steps<T, DIRECT>(
+			sums, (hi - lo + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
+			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
+				rows.fill(step, to);
+				columns.fill(step, to + rows_tile::kBytes);
+			},
+			[&](uint32_t step) __attribute__((always_inline)) {
+				rows.load(step);
+				columns.load(step);
+			},
+			[&](uint8_t *to) __attribute__((always_inline)) {
+				rows.store(to);
+				columns.store(to + rows_tile::kBytes);
+			},
+			also);
+	};
+	if (with_bias) {
+		sum([&](const u32x4_t(&r)[MF]) __attribute__((always_inline)) {
+			const u32x4_t ones = { kTwoOnes<T>, kTwoOnes<T>, kTwoOnes<T>, kTwoOnes<T> };
+#pragma unroll
+			for (int m = 0; m < (int)MF; m++) {
+				bias[m] = multiply<T>(ones, r[m], bias[m]);
 			}
-		}
-#pragma unroll
-		for (uint32_t half = 0; half < 2; half++) {
-			u32x4_t r[4];
-#pragma unroll
-			for (int m = 0; m < 4; m++) {
-				r[m] = row_frag.get(now, wm * 64 + m * 16, half);
-			}
-			if (with_bias) {
-				const u32x4_t ones = { kTwoOnes<T>, kTwoOnes<T>, kTwoOnes<T>, kTwoOnes<T> };
-#pragma unroll
-				for (int m = 0; m < 4; m++) {
-					bias[m] = multiply<T>(ones, r[m], bias[m]);
-				}
-			}
-#pragma unroll
-			for (int j = 0; j < (int)(2 * G); j++) {
-				const u32x4_t c = column_frag.get(now_columns, j / G * kBlock + wn * 16 * G + j % G * 16, half);
-#pragma unroll
-				for (int m = 0; m < 4; m++) {
-					sums[m][j / G][j % G] = multiply<T>(c, r[m], sums[m][j / G][j % G]);
-				}
-			}
-		}
+		});
+	} else {
+		sum([](const u32x4_t(&)[MF]) {});
 	}
 
-	if (with_bias && lane < 16) {
+	if (with_bias && wn == 0 && lane < 16) {
 #pragma unroll
-		for (int m = 0; m < 4; m++) {
-			const uint32_t r = wm * 64 + m * 16 + lane;
+		for (int m = 0; m < (int)MF; m++) {
+			const uint32_t r = (wm * MF + m) * 16 + lane;
 			if (r < m_there) {
 				const uint64_t i = (uint64_t)expert * m_width + m0 + r;
 				o.dbias[i] = bias[m][0] + (o.bias_add ? o.bias_add[i] : 0.0f);
@@ -129,7 +108,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const 
 	struct in_t {
 		f32x4_t was[2];
 	};
-	for_rows<WM, WN>(
+	for_rows<WM, WN, MF>(
 		sums, lds,
 		[&](uint32_t r) {
 			in_t in = {};
@@ -198,8 +177,8 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	o.dbias = d_dbias;
 	auto with = [&](auto element) {
 		using T = decltype(element);
-		auto kernel = direct ? (wide ? expert_weight_grad_kernel<T, 4, 2, true> : expert_weight_grad_kernel<T, 2, 4, true>)
-				     : (wide ? expert_weight_grad_kernel<T, 4, 2, false> : expert_weight_grad_kernel<T, 2, 4, false>);
+		auto kernel = direct ? (wide ? expert_weight_grad_kernel<T, 4, 2, 4, true> : expert_weight_grad_kernel<T, 2, 4, 4, true>)
+				     : (wide ? expert_weight_grad_kernel<T, 4, 2, 4, false> : expert_weight_grad_kernel<T, 2, 4, 4, false>);
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset, static_cast<const uint8_t *>(d_dout),
 				      static_cast<const uint8_t *>(d_rows), max_rows, out_width, width, m_tiles, n_tiles, (uint32_t)tiles, first,
