@@ -50,7 +50,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int
 	const along_frag_t row_frag(wm * 16 * MF, lane);
 	const across_frag_t<BN> column_frag(wn * 16 * G, lane);
 	sum_steps<T, DIRECT>(
-		sums, (k + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
+		sums, wm * 16 * MF < tile.rows, (k + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
 		[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
 			rows.fill(step, to);
 			columns.fill(step, to + rows_tile::kBytes);
@@ -65,10 +65,10 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int
 		},
 		[](const u32x4_t(&)[MF]) {});
 
-	const uint32_t c = (lane & 31u) * 4, blocks = blocks_of(n), block = c0 / kBlock;
+	const uint32_t c = (lane & 15u) * 8, blocks = blocks_of(n), block = c0 / kBlock;
 	const uint32_t left[2] = { c < there ? there - c : 0, c + kBlock < there ? there - c - kBlock : 0 };
 	struct in_t {
-		f32x4_t g[2], u[2]; /* what was kept, or what is added */
+		eight_t g[2], u[2]; /* what was kept, or what is added */
 	};
 	for_rows<WM, WN, MF>(
 		sums, lds,
@@ -80,38 +80,42 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int
 				const uint32_t column = c0 + p * kBlock + c;
 				if (r < tile.rows && left[p]) {
 					if (!HIDDEN && o.add.p) {
-						in.g[p] = read_values(o.add, row, column, left[p], 0);
+						in.g[p] = load_eight(o.add, row, column, left[p], 0);
 					} else if (HIDDEN) {
-						in.g[p] = read_values(o.saved, row, column, left[p], block + p);
+						in.g[p] = load_eight(o.saved, row, column, left[p], block + p);
 						if (o.gated) {
-							in.u[p] = read_values(o.saved, row, (uint64_t)n + column, left[p], blocks + block + p);
+							in.u[p] = load_eight(o.saved, row, (uint64_t)n + column, left[p], blocks + block + p);
 						}
 					}
 				}
 			}
 			return in;
 		},
-		[&](uint32_t r, f32x4_t a, f32x4_t b, const in_t &in) {
+		[&](uint32_t r, f32x8_t a, f32x8_t b, const in_t &in) {
 			const uint64_t row = tile.from + r;
 #pragma unroll
 			for (int p = 0; p < 2; p++) {
 				const uint32_t column = c0 + p * kBlock + c;
-				f32x4_t v = p ? b : a, u = in.u[p], dg, h;
+				f32x8_t v = p ? b : a;
 				if (r >= tile.rows || left[p] == 0) {
 					continue;
 				}
 				if constexpr (HIDDEN) {
+					f32x8_t g = values_of(in.g[p], o.saved.type), u = {}, h;
+					if (o.gated) {
+						u = values_of(in.u[p], o.saved.type);
+					}
 					with_activation(o.activation, [&](auto activation) {
 #pragma unroll
-						for (int i = 0; i < 4; i++) {
+						for (int i = 0; i < 8; i++) {
 							float value, slope;
-							activated_with_slope<decltype(activation)::value>(in.g[p][i], value, slope);
-							dg[i] = o.gated ? v[i] * u[i] * slope : v[i] * slope;
+							activated_with_slope<decltype(activation)::value>(g[i], value, slope);
+							g[i] = o.gated ? v[i] * u[i] * slope : v[i] * slope;
 							h[i] = o.gated ? value * u[i] : value;
 							v[i] *= value;
 						}
 					});
-					write_values(o.dsaved, row, column, left[p], dg);
+					write_values(o.dsaved, row, column, left[p], g);
 					if (o.gated) {
 						write_values(o.dsaved, row, (uint64_t)n + column, left[p], v);
 					}
@@ -119,7 +123,10 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int
 						write_values(o.hidden, row, column, left[p], h);
 					}
 				} else {
-					write_values(o.out, row, column, left[p], v + in.g[p]);
+					if (o.add.p) {
+						v += values_of(in.g[p], o.add.type);
+					}
+					write_values(o.out, row, column, left[p], v);
 				}
 			}
 		});
@@ -129,20 +136,19 @@ template <bool HIDDEN>
 int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows,
 	     const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t k, uint32_t n, const backward_t &o, void *stream)
 {
-	const uint32_t bm = row_tile_for(max_rows, n_experts), n_tiles = (n + 2 * kBlock - 1) / (2 * kBlock);
+	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * k) && in_chunks(d_weight, weight_pitch, 2ull * n) && expert_pitch % 16 == 0;
+	const uint32_t bm = row_tile_for(max_rows, n_experts, direct), n_tiles = (n + 2 * kBlock - 1) / (2 * kBlock);
 	const uint64_t tiles = most_row_tiles(max_rows, n_experts, bm) * n_tiles;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
-	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * k) && in_chunks(d_weight, weight_pitch, 2ull * n) && expert_pitch % 16 == 0;
 	auto with = [&](auto element) {
 		using T = decltype(element);
 		auto kernel = direct ? (bm == 256 ? expert_backward_kernel<T, 4, 2, 4, HIDDEN, true>
 						: bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, true>
 							    : expert_backward_kernel<T, 1, 8, 4, HIDDEN, true>)
-				     : (bm == 256 ? expert_backward_kernel<T, 4, 2, 4, HIDDEN, false>
-						: bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, false>
-							    : expert_backward_kernel<T, 1, 8, 4, HIDDEN, false>);
+				     : bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, false>
+						 : expert_backward_kernel<T, 1, 8, 4, HIDDEN, false>;
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset,
 				      static_cast<const uint8_t *>(d_dout), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, k, n,

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 		part1.store(to + rows_tile::kBytes + part_tile::kBytes);
 	};
 	if constexpr (!SCALED) {
-		sum_steps<T, DIRECT>(sums, steps, lds, kTile, rows_tile::kBytes, row_frag, column_frag, fill, load, store,
+		sum_steps<T, DIRECT>(sums, wm * 16 * MF < tile.rows, steps, lds, kTile, rows_tile::kBytes, row_frag, column_frag, fill, load, store,
 				     [](const u32x4_t(&)[MF]) {});
 	} else {
 		/* a lane's row of each of its groups */
@@ -145,38 +145,45 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 		}
 	}
 
-	const uint32_t c = (lane & 31u) * 4, blocks = blocks_of(n), block0 = c0 / kBlock, block1 = c1 / kBlock;
+	const uint32_t c = (lane & 15u) * 8, blocks = blocks_of(n), block0 = c0 / kBlock, block1 = c1 / kBlock;
 	const uint32_t left0 = c < there0 ? there0 - c : 0, left1 = c < there1 ? there1 - c : 0;
-	f32x4_t bias0 = { 0, 0, 0, 0 }, bias1 = { 0, 0, 0, 0 };
+	f32x8_t bias0 = {}, bias1 = {};
 	if (o.bias.p) {
-		bias0 = read_values(o.bias, 0, (uint64_t)tile.expert * n + c0 + c, left0, 0);
-		bias1 = read_values(o.bias, 0, (uint64_t)tile.expert * n + c1 + c, left1, 0);
+		auto bias_at = [&](uint32_t column, uint32_t left) {
+			const uint64_t at = (uint64_t)tile.expert * n + column;
+			return o.bias.type == OFI_AMD_FLOAT32 ? read_floats(o.bias.p + at * 4, left)
+							      : values_of(load_eight(o.bias, 0, at, left, 0), o.bias.type);
+		};
+		bias0 = bias_at(c0 + c, left0);
+		bias1 = bias_at(c1 + c, left1);
 	}
 	struct in_t {
-		f32x4_t add0, add1;
+		eight_t add0, add1;
 	};
 	for_rows<WM, WN, MF>(
 		sums, lds,
 		[&](uint32_t r) {
 			in_t in = {};
 			if (o.residual.p && r < tile.rows) {
-				in.add0 = read_values(o.residual, tile.from + r, c0 + c, left0, 0);
-				in.add1 = read_values(o.residual, tile.from + r, c1 + c, left1, 0);
+				in.add0 = load_eight(o.residual, tile.from + r, c0 + c, left0, 0);
+				in.add1 = load_eight(o.residual, tile.from + r, c1 + c, left1, 0);
 			}
 			return in;
 		},
-		[&](uint32_t r, f32x4_t a, f32x4_t b, const in_t &in) {
+		[&](uint32_t r, f32x8_t a, f32x8_t b, const in_t &in) {
 			const uint64_t row = tile.from + r;
 			const bool write = r < tile.rows;
-			a += bias0;
-			b += bias1;
+			if (o.bias.p) {
+				a += bias0;
+				b += bias1;
+			}
 			if (o.saved.p) {
 				write_any(o.saved, row, c0 + c, left0, block0, a, write);
 				write_any(o.saved, row, (o.gated ? (uint64_t)n : 0) + c1 + c, left1, (o.gated ? blocks : 0) + block1, b, write);
 			}
 			with_activation(o.activation, [&](auto activation) {
 #pragma unroll
-				for (int i = 0; i < 4; i++) {
+				for (int i = 0; i < 8; i++) {
 					a[i] = activated<decltype(activation)::value>(a[i]);
 					b[i] = o.gated ? b[i] : activated<decltype(activation)::value>(b[i]);
 				}
@@ -184,28 +191,32 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 			if (o.gated) {
 				a *= b;
 			} else {
-				write_any(o.out, row, c1 + c, left1, block1, b + in.add1, write);
+				if (o.residual.p) {
+					a += values_of(in.add0, o.residual.type);
+					b += values_of(in.add1, o.residual.type);
+				}
+				write_any(o.out, row, c1 + c, left1, block1, b, write);
 			}
-			write_any(o.out, row, c0 + c, left0, block0, a + in.add0, write);
+			write_any(o.out, row, c0 + c, left0, block0, a, write);
 		});
 }
 
 int forward(const void *d_rows, uint64_t rows_pitch, int type, const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows,
 	    const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t width, uint32_t n, const forward_t &o, void *stream)
 {
-	const uint32_t bm = row_tile_for(max_rows, n_experts), n_tiles = (n + (o.gated ? kBlock : 2 * kBlock) - 1) / (o.gated ? kBlock : 2 * kBlock);
+	const uint64_t bytes = (uint64_t)width * product_type_size(type);
+	const bool direct = in_chunks(d_rows, rows_pitch, bytes) && in_chunks(d_weight, weight_pitch, bytes) && expert_pitch % 16 == 0;
+	const uint32_t bm = row_tile_for(max_rows, n_experts, direct);
+	const uint32_t n_tiles = (n + (o.gated ? kBlock : 2 * kBlock) - 1) / (o.gated ? kBlock : 2 * kBlock);
 	const uint64_t tiles = most_row_tiles(max_rows, n_experts, bm) * n_tiles;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
-	const uint64_t bytes = (uint64_t)width * product_type_size(type);
-	const bool direct = in_chunks(d_rows, rows_pitch, bytes) && in_chunks(d_weight, weight_pitch, bytes) && expert_pitch % 16 == 0;
 	auto with = [&](auto element) {
 		using T = decltype(element);
 		auto kernel = direct ? (bm == 256 ? expert_forward_kernel<T, 4, 2, 4, true>
 						: bm == 128 ? expert_forward_kernel<T, 2, 4, 4, true> : expert_forward_kernel<T, 1, 8, 4, true>)
-				     : (bm == 256 ? expert_forward_kernel<T, 4, 2, 4, false>
-						: bm == 128 ? expert_forward_kernel<T, 2, 4, 4, false> : expert_forward_kernel<T, 1, 8, 4, false>);
+				     : bm == 128 ? expert_forward_kernel<T, 2, 4, 4, false> : expert_forward_kernel<T, 1, 8, 4, false>;
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset,
 				      static_cast<const uint8_t *>(d_rows), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, width, n,

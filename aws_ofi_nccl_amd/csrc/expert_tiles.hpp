@@ -29,6 +29,7 @@ struct e4m3_t {
 };
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x8_t __attribute__((ext_vector_type(8)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -337,11 +338,12 @@ __device__ __forceinline__ u32x4_t widened(uint32_t a, uint32_t b)
  * sums[m][p][j] += all steps.  Fragments of half a step are read while the other half's are multiplied.  When all of a step's are in
  * registers, a barrier: the next step's tile is there (it was asked for a step before), and this one's place is free for the step
  * after that.  fill: both operands' tiles of a step to LDS; or load: to registers, and store: from there.
- * Fills behind the last step write zeros.
+ * Fills behind the last step write zeros.  busy: whether the wavefront has rows; the matrix cores are another's where it has none, so
+ * that an expert's last tile costs the quarters of it that there are.
  */
 template <typename T, bool DIRECT, uint32_t MF, uint32_t G, typename RowFrag, typename ColumnFrag, typename Fill, typename Load, typename Store,
 	  typename Also>
-__device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], uint32_t steps, uint8_t *lds, uint32_t tile_bytes, uint32_t rows_bytes,
+__device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, uint32_t steps, uint8_t *lds, uint32_t tile_bytes, uint32_t rows_bytes,
 					  const RowFrag &row_frag, const ColumnFrag &column_frag, Fill fill, Load load, Store store, Also also)
 {
 	u32x4_t r[2][MF], c[2][2 * G];
@@ -390,28 +392,42 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], uint32_t st
 		__syncthreads();
 		load(1);
 	}
-	read(lds, 0, r[0], c[0]);
-	for (uint32_t step = 0; step < steps; step++) {
-		uint8_t *const now = lds + (step & 1u) * tile_bytes, *const next = lds + (~step & 1u) * tile_bytes;
-		read(now, 1, r[1], c[1]);
-		mul(r[0], c[0]);
-		spread();
-		if (DIRECT) {
-			landed();
-		} else {
-			store(next);
+	auto loop = [&](auto has_rows) __attribute__((always_inline)) {
+		constexpr bool kBusy = decltype(has_rows)::value;
+		if (kBusy) {
+			read(lds, 0, r[0], c[0]);
 		}
-		__syncthreads();
-		__builtin_amdgcn_sched_barrier(0);
-		if (DIRECT) {
-			fill(step + 2, now);
-		} else {
-			load(step + 2);
+		for (uint32_t step = 0; step < steps; step++) {
+			uint8_t *const now = lds + (step & 1u) * tile_bytes, *const next = lds + (~step & 1u) * tile_bytes;
+			if (kBusy) {
+				read(now, 1, r[1], c[1]);
+				mul(r[0], c[0]);
+				spread();
+			}
+			if (DIRECT) {
+				landed();
+			} else {
+				store(next);
+			}
+			__syncthreads();
+			__builtin_amdgcn_sched_barrier(0);
+			if (DIRECT) {
+				fill(step + 2, now);
+			} else {
+				load(step + 2);
+			}
+			__builtin_amdgcn_sched_barrier(0);
+			if (kBusy) {
+				read(next, 0, r[0], c[0]);
+				mul(r[1], c[1]);
+				spread();
+			}
 		}
-		__builtin_amdgcn_sched_barrier(0);
-		read(next, 0, r[0], c[0]);
-		mul(r[1], c[1]);
-		spread();
+	};
+	if (busy) { /* of the whole wavefront; both loops meet the same barriers */
+		loop(std::true_type{});
+	} else {
+		loop(std::false_type{});
 	}
 	if (DIRECT) {
 		landed(); /* what follows writes there */
@@ -421,22 +437,28 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], uint32_t st
 /* ---- sums ----------------------------------------------------------------------------------------------------- */
 
 /*
- * A tile's sums by rows: finish(row of the tile, columns of part 0, of part 1, what load(row) gave), four neighbouring columns of both
- * parts in a lane, from column 4 (lane % 32) of the part on; half a wavefront has a row, so that what is read and written of it is one
- * piece.  The sums go through LDS, half of the rows at a time, so that one loop does for all of them: unrolled over the registers the
- * same epilogue was 200 KB of instructions.
+ * A tile's sums by rows: finish(row of the tile, columns of part 0, of part 1, what load(row) gave), eight neighbouring columns of both
+ * parts in a lane, from column 8 (lane % 16) of the part on; a quarter of a wavefront has a row, so that what is read and written of
+ * it is one piece, and a block of 128 columns is sixteen neighbouring lanes.  The sums go through LDS, half of the rows at a time, so that
+ * one loop does for all of them (unrolled over the registers the same epilogue was 200 KB of instructions).  What is loaded is
+ * asked for two turns ahead: a CU then has 64 KB of float32 on its way.
  */
 template <uint32_t WM, uint32_t WN, uint32_t MF, typename Load, typename Finish>
 __device__ __forceinline__ void for_rows(const f32x4_t (&sums)[MF][2][8 / WN], uint8_t *lds, Load load, Finish finish)
 {
 	constexpr uint32_t G = 8 / WN, kOfWave = MF * 8; /* rows of half a wavefront's tile */
-	constexpr uint32_t kTurns = kOfWave / WN / 2;    /* of WM * kOfWave rows, two to each of WM * WN wavefronts */
+	constexpr uint32_t kTurns = kOfWave / WN / 4;    /* of WM * kOfWave rows, four to each of WM * WN wavefronts */
+	constexpr uint32_t kAhead = kTurns < 2 ? 1 : 2;
 	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
 #pragma unroll 1
 	for (uint32_t half = 0; half < 2; half++) {
-		auto place = [&](uint32_t turn) { return (wave * kTurns + turn) * 2 + (lane >> 5); };
+		auto place = [&](uint32_t turn) { return (wave * kTurns + turn) * 4 + (lane >> 4); };
 		auto row_of = [&](uint32_t at) { return at / kOfWave * 2 * kOfWave + half * kOfWave + at % kOfWave; };
-		auto in = load(row_of(place(0)));
+		decltype(load(0u)) in[kAhead];
+#pragma unroll
+		for (uint32_t i = 0; i < kAhead; i++) {
+			in[i] = load(row_of(place(i)));
+		}
 		__syncthreads(); /* the tiles, or the half before, have been read */
 		auto put = [&](uint32_t m, const f32x4_t(&from)[2][G]) __attribute__((always_inline)) {
 			const uint32_t r = wm * kOfWave + m * 16 + (lane & 15u);
@@ -462,22 +484,26 @@ __device__ __forceinline__ void for_rows(const f32x4_t (&sums)[MF][2][8 / WN], u
 		}
 		__syncthreads();
 #pragma unroll 1
-		for (uint32_t turn = 0; turn < kTurns; turn++) {
-			const uint32_t at = place(turn);
-			const auto now = in;
-			if (turn + 1 < kTurns) {
-				in = load(row_of(place(turn + 1)));
+		for (uint32_t turn = 0; turn < kTurns; turn += kAhead) {
+#pragma unroll
+			for (uint32_t i = 0; i < kAhead; i++) {
+				const uint32_t at = place(turn + i);
+				const auto now = in[i];
+				if (turn + i + kAhead < kTurns) {
+					in[i] = load(row_of(place(turn + i + kAhead)));
+				}
+				const uint8_t *const from = lds + at * 1024;
+				const uint32_t swizzle = at & 15u, chunk = (lane & 15u) * 2;
+				auto get = [&](uint32_t c) { return *reinterpret_cast<const f32x4_t *>(from + ((c ^ swizzle) << 4)); };
+				const f32x4_t a0 = get(chunk), a1 = get(chunk + 1), b0 = get(chunk + 32), b1 = get(chunk + 33);
+				finish(row_of(at), __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7),
+				       __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7), now);
 			}
-			const uint8_t *const from = lds + at * 1024;
-			const uint32_t chunk = (lane & 31u) ^ (at & 15u);
-			const f32x4_t a = *reinterpret_cast<const f32x4_t *>(from + (chunk << 4));
-			const f32x4_t b = *reinterpret_cast<const f32x4_t *>(from + ((chunk + 32) << 4));
-			finish(row_of(at), a, b, now);
 		}
 	}
 }
 
-/* Where the columns of a matrix of 16-bit, float32 or e4m3 values are read and written; none: p NULL */
+/* A matrix of 16-bit, float32 or e4m3 values; none: p NULL */
 struct matrix_t {
 	uint8_t *p;
 	uint64_t pitch;
@@ -486,62 +512,77 @@ struct matrix_t {
 	uint64_t scale_pitch;
 };
 
-/* Four values of a row from p on, of which `left` are there; zeros for the others */
-template <typename T> __device__ __forceinline__ f32x4_t read_as(const uint8_t *p, uint32_t left)
+/* `left` of V values at p, as words; zeros for the others */
+template <typename U, uint32_t V, typename W> __device__ __forceinline__ void read_words(const uint8_t *p, uint32_t left, W &w)
 {
-	f32x4_t v = { 0, 0, 0, 0 };
-	if (left >= 4) {
-		v = __builtin_convertvector(*reinterpret_cast<const typename piece_t<T, 4>::anywhere *>(p), f32x4_t);
+	typedef U any_t __attribute__((ext_vector_type(V), aligned(sizeof(U))));
+	static_assert(sizeof(any_t) <= sizeof(W), "room");
+	if (left >= V) {
+		const any_t all = *reinterpret_cast<const any_t *>(p);
+		__builtin_memcpy(&w, &all, sizeof(all));
 	} else {
+		any_t some = {};
 #pragma unroll
-		for (uint32_t i = 0; i < 3; i++) {
+		for (uint32_t i = 0; i < V - 1; i++) {
 			if (i < left) {
-				v[i] = (float)reinterpret_cast<const T *>(p)[i];
+				some[i] = reinterpret_cast<const U *>(p)[i];
 			}
 		}
+		__builtin_memcpy(&w, &some, sizeof(some));
 	}
+}
+
+/* Eight values of a 16-bit or 8-bit type as they lie in memory, and the scale of those of 8 bits */
+struct eight_t {
+	u32x4_t words;
+	float scale;
+};
+/* block: of the columns, for the scale */
+__device__ __forceinline__ eight_t load_eight(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block)
+{
+	eight_t e = {};
+	const uint8_t *const p = m.p + row * m.pitch;
+	if (m.type == OFI_AMD_E4M3) {
+		e.scale = row_at(m.scale, m.scale_pitch, row)[block];
+		read_words<uint8_t, 8>(p + column, left, e.words);
+	} else {
+		read_words<uint16_t, 8>(p + column * 2, left, e.words);
+	}
+	return e;
+}
+template <typename T> __device__ __forceinline__ f32x8_t floats_of(u32x4_t w)
+{
+	return __builtin_convertvector(__builtin_bit_cast(raw_t<T, 8>, w), f32x8_t);
+}
+__device__ __forceinline__ f32x8_t values_of(const eight_t &e, int type)
+{
+	if (type == OFI_AMD_BFLOAT16) {
+		return floats_of<bf16_t>(e.words);
+	}
+	if (type == OFI_AMD_FLOAT16) {
+		return floats_of<f16_t>(e.words);
+	}
+	const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)e.words.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)e.words.x, true);
+	const auto c = __builtin_amdgcn_cvt_pk_f32_fp8((int)e.words.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)e.words.y, true);
+	return f32x8_t{ a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1] } * e.scale;
+}
+
+__device__ __forceinline__ f32x8_t read_floats(const uint8_t *p, uint32_t left)
+{
+	f32x8_t v;
+	read_words<float, 8>(p, left, v);
 	return v;
 }
 
-__device__ __forceinline__ f32x4_t read_e4m3(const uint8_t *p, uint32_t left, float scale)
+/* Each value is rounded to the type once, to nearest even */
+template <typename T> __device__ __forceinline__ void write_as(uint8_t *p, uint32_t left, f32x8_t v)
 {
-	typedef uint32_t any4_t __attribute__((aligned(1)));
-	uint32_t w = 0;
-	if (left >= 4) {
-		w = *reinterpret_cast<const any4_t *>(p);
+	const auto r = __builtin_convertvector(v, raw_t<T, 8>);
+	if (left >= 8) {
+		*reinterpret_cast<typename piece_t<T, 8>::anywhere *>(p) = r;
 	} else {
 #pragma unroll
-		for (uint32_t i = 0; i < 3; i++) {
-			if (i < left) {
-				w |= (uint32_t)p[i] << (8 * i);
-			}
-		}
-	}
-	const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-	return f32x4_t{ a[0], a[1], b[0], b[1] } * scale;
-}
-
-/* block: of the columns, for their scale */
-__device__ __forceinline__ f32x4_t read_values(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block)
-{
-	const uint8_t *p = m.p + row * m.pitch;
-	switch (m.type) {
-	case OFI_AMD_BFLOAT16: return read_as<bf16_t>(p + column * 2, left);
-	case OFI_AMD_FLOAT16: return read_as<f16_t>(p + column * 2, left);
-	case OFI_AMD_FLOAT32: return read_as<float>(p + column * 4, left);
-	default: return read_e4m3(p + column, left, row_at(m.scale, m.scale_pitch, row)[block]);
-	}
-}
-
-/* Each value is rounded to the matrix's type once, to nearest even */
-template <typename T> __device__ __forceinline__ void write_as(uint8_t *p, uint32_t left, f32x4_t v)
-{
-	const auto r = __builtin_convertvector(v, raw_t<T, 4>);
-	if (left >= 4) {
-		*reinterpret_cast<typename piece_t<T, 4>::anywhere *>(p) = r;
-	} else {
-#pragma unroll
-		for (uint32_t i = 0; i < 3; i++) {
+		for (uint32_t i = 0; i < 7; i++) {
 			if (i < left) {
 				reinterpret_cast<T *>(p)[i] = r[i];
 			}
@@ -549,9 +590,9 @@ template <typename T> __device__ __forceinline__ void write_as(uint8_t *p, uint3
 	}
 }
 
-__device__ __forceinline__ void write_values(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, f32x4_t v)
+__device__ __forceinline__ void write_values(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, f32x8_t v)
 {
-	uint8_t *p = m.p + row * m.pitch;
+	uint8_t *const p = m.p + row * m.pitch;
 	switch (m.type) {
 	case OFI_AMD_BFLOAT16: write_as<bf16_t>(p + column * 2, left, v); break;
 	case OFI_AMD_FLOAT16: write_as<f16_t>(p + column * 2, left, v); break;
@@ -559,42 +600,46 @@ __device__ __forceinline__ void write_values(const matrix_t &m, uint64_t row, ui
 	}
 }
 
-/* A block of 128 columns of a row, which the 32 lanes of half a wavefront hold: values divided by their scale as the norms divide
- * them (with a division's rounding, then rounded to e4m3), and the scale.  All 32 lanes call; `write`: whether the row is there. */
-__device__ __forceinline__ void write_block(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block, f32x4_t v, bool write)
+/* A block of 128 columns of a row, which sixteen lanes hold: values divided by their scale as the norms divide them (with a
+ * division's rounding, then rounded to e4m3), and the scale.  All sixteen call; `write`: whether the row is there. */
+__device__ __forceinline__ void write_block(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block, f32x8_t v, bool write)
 {
 	uint32_t most = 0;
 #pragma unroll
-	for (uint32_t i = 0; i < 4; i++) {
+	for (uint32_t i = 0; i < 8; i++) {
 		const uint32_t bits = i < left ? abs_bits(v[i]) : 0u;
 		most = bits > most ? bits : most;
 	}
-	const float scale = scale_of(max_bits_over<32>(most));
-	const divisor_t by = divisor_of(scale);
-	const int low = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[0], by), quotient(v[1], by), 0, false);
-	const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[2], by), quotient(v[3], by), low, true);
+	const float scale = scale_of(max_bits_over<16>(most));
 	if (!write || left == 0) {
 		return;
 	}
-	if ((threadIdx.x & 31u) == 0) {
+	const divisor_t by = divisor_of(scale);
+	typedef uint32_t any8_t __attribute__((ext_vector_type(2), aligned(1)));
+	any8_t w;
+#pragma unroll
+	for (int i = 0; i < 2; i++) {
+		const int low = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[4 * i], by), quotient(v[4 * i + 1], by), 0, false);
+		w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[4 * i + 2], by), quotient(v[4 * i + 3], by), low, true);
+	}
+	if ((threadIdx.x & 15u) == 0) {
 		row_at(m.scale, m.scale_pitch, row)[block] = scale;
 	}
-	typedef uint32_t any4_t __attribute__((aligned(1)));
-	uint8_t *p = m.p + row * m.pitch + column;
-	if (left >= 4) {
-		*reinterpret_cast<any4_t *>(p) = w;
+	uint8_t *const p = m.p + row * m.pitch + column;
+	if (left >= 8) {
+		*reinterpret_cast<any8_t *>(p) = w;
 	} else {
 #pragma unroll
-		for (uint32_t i = 0; i < 3; i++) {
+		for (uint32_t i = 0; i < 7; i++) {
 			if (i < left) {
-				p[i] = (uint8_t)(w >> (8 * i));
+				p[i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
 			}
 		}
 	}
 }
 
-/* The same to 16-bit types without blocks */
-__device__ __forceinline__ void write_any(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block, f32x4_t v, bool write)
+/* As e4m3 with the block's scale, or in 16 bits */
+__device__ __forceinline__ void write_any(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block, f32x8_t v, bool write)
 {
 	if (m.type == OFI_AMD_E4M3) {
 		write_block(m, row, column, left, block, v, write);
@@ -726,11 +771,11 @@ inline uint64_t most_row_tiles(uint32_t max_rows, uint32_t n_experts, uint32_t b
 	return (max_rows - parts) / bm + parts;
 }
 
-/* Row tiles of 256, 128 or 64: as many as there are rows for */
-inline uint32_t row_tile_for(uint32_t max_rows, uint32_t n_experts)
+/* Row tiles of 256, 128 or 64: as many as there are rows for.  256 with rows that come through registers would not fit them. */
+inline uint32_t row_tile_for(uint32_t max_rows, uint32_t n_experts, bool direct)
 {
 	const uint32_t of_expert = (max_rows + n_experts - 1) / n_experts;
-	return of_expert > 128 ? 256 : of_expert > 64 ? 128 : 64;
+	return of_expert > 128 && direct ? 256 : of_expert > 64 ? 128 : 64;
 }
 
 inline bool activation_ok(int a) { return a == OFI_AMD_NO_ACTIVATION || a == OFI_AMD_RELU || a == OFI_AMD_SILU || a == OFI_AMD_GELU; }

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const 
 	const across_frag_t<BN> column_frag(wn * 16 * G, lane);
 	auto sum = [&](auto also) __attribute__((always_inline)) {
 		sum_steps<T, DIRECT>(
-			sums, (hi - lo + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
+			sums, wm * 16 * MF < m_there, (hi - lo + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
 			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
 				rows.fill(step, to);
 				columns.fill(step, to + rows_tile::kBytes);
@@ -103,10 +103,10 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const 
 	}
 	const matrix_t out = { o.out.p + expert * o.expert_pitch, o.out.pitch, o.out.type, nullptr, 0 };
 	const matrix_t add = { o.add.p ? o.add.p + expert * o.expert_pitch : nullptr, o.add.pitch, o.add.type, nullptr, 0 };
-	const uint32_t c = (lane & 31u) * 4;
+	const uint32_t c = (lane & 15u) * 8;
 	const uint32_t left[2] = { c < n_there ? n_there - c : 0, c + kBlock < n_there ? n_there - c - kBlock : 0 };
 	struct in_t {
-		f32x4_t was[2];
+		f32x8_t was[2]; /* float32, or eight values of 16 bits */
 	};
 	for_rows<WM, WN, MF>(
 		sums, lds,
@@ -115,16 +115,26 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const 
 #pragma unroll
 			for (int p = 0; p < 2; p++) {
 				if (add.p && r < m_there && left[p]) {
-					in.was[p] = read_values(add, m0 + r, n0 + p * kBlock + c, left[p], 0);
+					const uint64_t column = n0 + p * kBlock + c;
+					if (add.type == OFI_AMD_FLOAT32) {
+						in.was[p] = read_floats(add.p + (m0 + r) * add.pitch + column * 4, left[p]);
+					} else {
+						in.was[p].lo = __builtin_bit_cast(f32x4_t, load_eight(add, m0 + r, column, left[p], 0).words);
+					}
 				}
 			}
 			return in;
 		},
-		[&](uint32_t r, f32x4_t a, f32x4_t b, const in_t &in) {
+		[&](uint32_t r, f32x8_t a, f32x8_t b, const in_t &in) {
 #pragma unroll
 			for (int p = 0; p < 2; p++) {
+				f32x8_t v = p ? b : a;
 				if (r < m_there && left[p]) {
-					write_values(out, m0 + r, n0 + p * kBlock + c, left[p], (p ? b : a) + in.was[p]);
+					if (add.p) {
+						const f32x4_t low = in.was[p].lo;
+						v += add.type == OFI_AMD_FLOAT32 ? in.was[p] : floats_of<T>(__builtin_bit_cast(u32x4_t, low));
+					}
+					write_values(out, m0 + r, n0 + p * kBlock + c, left[p], v);
 				}
 			}
 		});
@@ -162,13 +172,13 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	}
 	/* tiles of 256 x 256 where they are enough for the GPU, else of 128 x 256 */
 	const uint32_t n_tiles = (width + 255) / 256;
-	const bool wide = (uint64_t)n_experts * ((out_width + 255) / 256) * n_tiles >= 256;
+	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * out_width) && in_chunks(d_rows, rows_pitch, 2ull * width);
+	const bool wide = direct && (uint64_t)n_experts * ((out_width + 255) / 256) * n_tiles >= 256;
 	const uint32_t bm = wide ? 256 : 128, m_tiles = (out_width + bm - 1) / bm;
 	const uint64_t tiles = (uint64_t)n_experts * m_tiles * n_tiles;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
-	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * out_width) && in_chunks(d_rows, rows_pitch, 2ull * width);
 	weight_grad_t o = {};
 	o.out = { static_cast<uint8_t *>(d_dweight), dweight_pitch, dweight_type, nullptr, 0 };
 	o.add = { static_cast<uint8_t *>(const_cast<void *>(d_add)), dweight_pitch, dweight_type, nullptr, 0 };
@@ -178,7 +188,7 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	auto with = [&](auto element) {
 		using T = decltype(element);
 		auto kernel = direct ? (wide ? expert_weight_grad_kernel<T, 4, 2, 4, true> : expert_weight_grad_kernel<T, 2, 4, 4, true>)
-				     : (wide ? expert_weight_grad_kernel<T, 4, 2, 4, false> : expert_weight_grad_kernel<T, 2, 4, 4, false>);
+				     : expert_weight_grad_kernel<T, 2, 4, 4, false>;
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset, static_cast<const uint8_t *>(d_dout),
 				      static_cast<const uint8_t *>(d_rows), max_rows, out_width, width, m_tiles, n_tiles, (uint32_t)tiles, first,
