@@ -27,8 +27,9 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int
 	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
 	using rows_tile = along_t<T, BM, THREADS>;
 	using columns_tile = across_t<T, BN, THREADS>;
-	constexpr uint32_t kTile = rows_tile::kBytes + columns_tile::kBytes;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kTile];
+	constexpr uint32_t kTile = rows_tile::kBytes + columns_tile::kBytes, kFills = rows_tile::kChunks + columns_tile::kChunks;
+	constexpr uint32_t kStages = DIRECT && WM < 4 ? 3 : 2;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * kTile];
 
 	const tile_t tile = tile_of<BM>(offset, n_experts, max_rows, n_tiles, first_tile + blockIdx.x);
 	if (!tile.any) {
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int
 	}
 	const along_frag_t row_frag(wm * 16 * MF, lane);
 	const across_frag_t<BN> column_frag(wn * 16 * G, lane);
-	sum_steps<T, DIRECT>(
+	sum_steps<T, DIRECT, kStages, kFills>(
 		sums, wm * 16 * MF < tile.rows, (k + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
 		[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
 			rows.fill(step, to);
@@ -137,7 +138,7 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 	     const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t k, uint32_t n, const backward_t &o, void *stream)
 {
 	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * k) && in_chunks(d_weight, weight_pitch, 2ull * n) && expert_pitch % 16 == 0;
-	const uint32_t bm = row_tile_for(max_rows, n_experts, direct), n_tiles = (n + 2 * kBlock - 1) / (2 * kBlock);
+	const uint32_t n_tiles = (n + 2 * kBlock - 1) / (2 * kBlock), bm = row_tile_for(max_rows, n_experts, n_tiles, direct);
 	const uint64_t tiles = most_row_tiles(max_rows, n_experts, bm) * n_tiles;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;

@@ -5,18 +5,10 @@
  * x and the weights run along the summed axis.  Rows of e4m3 and their weights have a scale for every 128 of it, which are what one
  * step sums: a step's sums are multiplied by both scales in 32 bits and added.
  */
-#include "expert_tiles.hpp"
+#include "expert_forward.hpp"
 
 namespace ofi_amd {
 namespace {
-
-struct forward_t {
-	const float *scale, *weight_scale;
-	uint64_t scale_pitch;
-	matrix_t bias, residual, out, saved;
-	int activation;
-	bool gated;
-};
 
 template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int32_t *offset, const uint8_t *x, const uint8_t *w, uint32_t n_experts,
@@ -28,8 +20,9 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 	constexpr bool SCALED = sizeof(T) == 1;
 	using rows_tile = along_t<T, BM, THREADS>;
 	using part_tile = along_t<T, kBlock, THREADS>;
-	constexpr uint32_t kTile = rows_tile::kBytes + 2 * part_tile::kBytes;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kTile];
+	constexpr uint32_t kTile = rows_tile::kBytes + 2 * part_tile::kBytes, kFills = rows_tile::kChunks + 2 * part_tile::kChunks;
+	constexpr uint32_t kStages = DIRECT && !SCALED && WM < 4 ? 3 : 2;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * kTile];
 
 	const tile_t tile = tile_of<BM>(offset, n_experts, max_rows, n_tiles, first_tile + blockIdx.x);
 	if (!tile.any) {
@@ -71,7 +64,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 		part1.store(to + rows_tile::kBytes + part_tile::kBytes);
 	};
 	if constexpr (!SCALED) {
-		sum_steps<T, DIRECT>(sums, wm * 16 * MF < tile.rows, steps, lds, kTile, rows_tile::kBytes, row_frag, column_frag, fill, load, store,
+		sum_steps<T, DIRECT, kStages, kFills>(sums, wm * 16 * MF < tile.rows, steps, lds, kTile, rows_tile::kBytes, row_frag, column_frag, fill, load, store,
 				     [](const u32x4_t(&)[MF]) {});
 	} else {
 		/* a lane's row of each of its groups */
@@ -93,7 +86,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 		for (uint32_t step = 0; step < steps; step++) {
 			uint8_t *const now = lds + (step & 1u) * kTile;
 			if (DIRECT) {
-				landed();
+				landed<0>();
 			} else {
 				store(now);
 			}
@@ -145,69 +138,23 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int3
 		}
 	}
 
-	const uint32_t c = (lane & 15u) * 8, blocks = blocks_of(n), block0 = c0 / kBlock, block1 = c1 / kBlock;
-	const uint32_t left0 = c < there0 ? there0 - c : 0, left1 = c < there1 ? there1 - c : 0;
-	f32x8_t bias0 = {}, bias1 = {};
-	if (o.bias.p) {
-		auto bias_at = [&](uint32_t column, uint32_t left) {
-			const uint64_t at = (uint64_t)tile.expert * n + column;
-			return o.bias.type == OFI_AMD_FLOAT32 ? read_floats(o.bias.p + at * 4, left)
-							      : values_of(load_eight(o.bias, 0, at, left, 0), o.bias.type);
-		};
-		bias0 = bias_at(c0 + c, left0);
-		bias1 = bias_at(c1 + c, left1);
-	}
-	struct in_t {
-		eight_t add0, add1;
-	};
+	const forward_rows_t out(o, tile, n, c0, c1, kBlock, (lane & 15u) * 8);
 	for_rows<WM, WN, MF>(
-		sums, lds,
-		[&](uint32_t r) {
-			in_t in = {};
-			if (o.residual.p && r < tile.rows) {
-				in.add0 = load_eight(o.residual, tile.from + r, c0 + c, left0, 0);
-				in.add1 = load_eight(o.residual, tile.from + r, c1 + c, left1, 0);
-			}
-			return in;
-		},
-		[&](uint32_t r, f32x8_t a, f32x8_t b, const in_t &in) {
-			const uint64_t row = tile.from + r;
-			const bool write = r < tile.rows;
-			if (o.bias.p) {
-				a += bias0;
-				b += bias1;
-			}
-			if (o.saved.p) {
-				write_any(o.saved, row, c0 + c, left0, block0, a, write);
-				write_any(o.saved, row, (o.gated ? (uint64_t)n : 0) + c1 + c, left1, (o.gated ? blocks : 0) + block1, b, write);
-			}
-			with_activation(o.activation, [&](auto activation) {
-#pragma unroll
-				for (int i = 0; i < 8; i++) {
-					a[i] = activated<decltype(activation)::value>(a[i]);
-					b[i] = o.gated ? b[i] : activated<decltype(activation)::value>(b[i]);
-				}
-			});
-			if (o.gated) {
-				a *= b;
-			} else {
-				if (o.residual.p) {
-					a += values_of(in.add0, o.residual.type);
-					b += values_of(in.add1, o.residual.type);
-				}
-				write_any(o.out, row, c1 + c, left1, block1, b, write);
-			}
-			write_any(o.out, row, c0 + c, left0, block0, a, write);
-		});
+		sums, lds, [&](uint32_t r) { return out.load(r); },
+		[&](uint32_t r, f32x8_t a, f32x8_t b, const forward_rows_t::in_t &in) { out.finish(r, a, b, in); });
 }
+
 
 int forward(const void *d_rows, uint64_t rows_pitch, int type, const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows,
 	    const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t width, uint32_t n, const forward_t &o, void *stream)
 {
 	const uint64_t bytes = (uint64_t)width * product_type_size(type);
 	const bool direct = in_chunks(d_rows, rows_pitch, bytes) && in_chunks(d_weight, weight_pitch, bytes) && expert_pitch % 16 == 0;
-	const uint32_t bm = row_tile_for(max_rows, n_experts, direct);
 	const uint32_t n_tiles = (n + (o.gated ? kBlock : 2 * kBlock) - 1) / (o.gated ? kBlock : 2 * kBlock);
+	const uint32_t bm = row_tile_for(max_rows, n_experts, n_tiles, direct);
+	if (forward_is_few(max_rows, n_experts, n_tiles)) {
+		return forward_few(d_rows, rows_pitch, type, d_offset, n_experts, max_rows, d_weight, weight_pitch, expert_pitch, width, n, o, stream);
+	}
 	const uint64_t tiles = most_row_tiles(max_rows, n_experts, bm) * n_tiles;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;

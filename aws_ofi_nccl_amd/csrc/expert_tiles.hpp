@@ -41,6 +41,7 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 constexpr uint32_t kBlock = 128;       /* columns that share a scale, and columns of a part */
 constexpr uint32_t kStepBytes = 128;   /* of a row along the summed axis, in a step */
 constexpr uint32_t kStepRows = 64;     /* rows across it */
+constexpr uint32_t kComputeUnits = 256;
 constexpr uint32_t kMostExperts = 1024, kMostExpertWidth = 1u << 20;
 
 template <typename T> constexpr uint32_t kStepOf = kStepBytes / sizeof(T); /* elements of the summed axis in a step */
@@ -176,8 +177,25 @@ __device__ __forceinline__ void to_lds(const uint8_t *p, int bytes, uint32_t off
 	const uint32_t to = uniform((uint32_t)reinterpret_cast<uintptr_t>((lds_void_t *)lds));
 	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory");
 }
-/* All of the wavefront's to_lds have landed */
-__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+/* All but the last N of the wavefront's to_lds have landed */
+template <uint32_t N> __device__ __forceinline__ void landed()
+{
+	static_assert(N < 64, "the counter has six bits");
+	asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+/* A barrier at which every wavefront's reads of LDS are done.  What to_lds has on its way stays on its way (__syncthreads would wait for
+ * it); what comes through registers is stored by then. */
+template <bool DIRECT> __device__ __forceinline__ void workgroup_meets()
+{
+	if (DIRECT) {
+		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+		__builtin_amdgcn_s_barrier();
+		asm volatile("" ::: "memory");
+	} else {
+		__syncthreads();
+	}
+	__builtin_amdgcn_sched_barrier(0);
+}
 constexpr uint32_t kBeyond = 0x80000000u; /* of any buffer */
 
 /*
@@ -336,16 +354,18 @@ __device__ __forceinline__ u32x4_t widened(uint32_t a, uint32_t b)
 
 /*
  * sums[m][p][j] += all steps.  Fragments of half a step are read while the other half's are multiplied.  When all of a step's are in
- * registers, a barrier: the next step's tile is there (it was asked for a step before), and this one's place is free for the step
- * after that.  fill: both operands' tiles of a step to LDS; or load: to registers, and store: from there.
- * Fills behind the last step write zeros.  busy: whether the wavefront has rows; the matrix cores are another's where it has none, so
- * that an expert's last tile costs the quarters of it that there are.
+ * registers, a barrier: the next step's tile is there (it was asked for STAGES - 1 steps before), and this one's place is free for the
+ * step STAGES on.  fill: both operands' tiles of a step to LDS, kFills instructions of a wavefront; or (not DIRECT, two stages) load: to
+ * registers, and store: from there.  Fills behind the last step write zeros.  busy: whether the wavefront has rows; the matrix
+ * cores are another's where it has none, so that an expert's last tile costs the quarters of it that there are.
  */
-template <typename T, bool DIRECT, uint32_t MF, uint32_t G, typename RowFrag, typename ColumnFrag, typename Fill, typename Load, typename Store,
-	  typename Also>
-__device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, uint32_t steps, uint8_t *lds, uint32_t tile_bytes, uint32_t rows_bytes,
-					  const RowFrag &row_frag, const ColumnFrag &column_frag, Fill fill, Load load, Store store, Also also)
+template <typename T, bool DIRECT, uint32_t STAGES, uint32_t FILLS, uint32_t MF, uint32_t G, typename RowFrag, typename ColumnFrag, typename Fill,
+	  typename Load, typename Store, typename Also>
+__device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, uint32_t steps, uint8_t *lds, uint32_t tile_bytes,
+					  uint32_t rows_bytes, const RowFrag &row_frag, const ColumnFrag &column_frag, Fill fill, Load load, Store store,
+					  Also also)
 {
+	static_assert(DIRECT || STAGES == 2, "what comes through registers has two stages");
 	u32x4_t r[2][MF], c[2][2 * G];
 	auto read = [&](uint8_t *tile, uint32_t half, u32x4_t(&rows)[MF], u32x4_t(&columns)[2 * G]) __attribute__((always_inline)) {
 #pragma unroll
@@ -382,10 +402,12 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 		return;
 	}
 	if (DIRECT) {
-		fill(0, lds);
-		landed();
+#pragma unroll
+		for (uint32_t s = 0; s < STAGES; s++) {
+			fill(s, lds + s * tile_bytes);
+		}
+		landed<(STAGES - 1) * FILLS>();
 		__syncthreads();
-		fill(1, lds + tile_bytes);
 	} else {
 		load(0);
 		store(lds);
@@ -394,25 +416,27 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 	}
 	auto loop = [&](auto has_rows) __attribute__((always_inline)) {
 		constexpr bool kBusy = decltype(has_rows)::value;
+		uint32_t at = 0;
 		if (kBusy) {
 			read(lds, 0, r[0], c[0]);
 		}
 		for (uint32_t step = 0; step < steps; step++) {
-			uint8_t *const now = lds + (step & 1u) * tile_bytes, *const next = lds + (~step & 1u) * tile_bytes;
+			uint8_t *const now = lds + at;
+			at = at + tile_bytes < STAGES * tile_bytes ? at + tile_bytes : 0;
+			uint8_t *const next = lds + at;
 			if (kBusy) {
 				read(now, 1, r[1], c[1]);
 				mul(r[0], c[0]);
 				spread();
 			}
 			if (DIRECT) {
-				landed();
+				landed<(STAGES - 2) * FILLS>();
 			} else {
 				store(next);
 			}
-			__syncthreads();
-			__builtin_amdgcn_sched_barrier(0);
+			workgroup_meets<DIRECT>();
 			if (DIRECT) {
-				fill(step + 2, now);
+				fill(step + STAGES, now);
 			} else {
 				load(step + 2);
 			}
@@ -430,7 +454,7 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 		loop(std::false_type{});
 	}
 	if (DIRECT) {
-		landed(); /* what follows writes there */
+		landed<0>(); /* what follows writes there */
 	}
 }
 
@@ -771,11 +795,15 @@ inline uint64_t most_row_tiles(uint32_t max_rows, uint32_t n_experts, uint32_t b
 	return (max_rows - parts) / bm + parts;
 }
 
-/* Row tiles of 256, 128 or 64: as many as there are rows for.  256 with rows that come through registers would not fit them. */
-inline uint32_t row_tile_for(uint32_t max_rows, uint32_t n_experts, bool direct)
+/* Row tiles of 256, 128 or 64: the largest that the experts' rows fill and of which there are enough for the GPU.  256 with rows that
+ * come through registers would not fit them. */
+inline uint32_t row_tile_for(uint32_t max_rows, uint32_t n_experts, uint32_t n_tiles, bool direct)
 {
-	const uint32_t of_expert = (max_rows + n_experts - 1) / n_experts;
-	return of_expert > 128 && direct ? 256 : of_expert > 64 ? 128 : 64;
+	const uint32_t experts = n_experts < max_rows ? n_experts : max_rows, of_expert = (max_rows + experts - 1) / experts;
+	auto fits = [&](uint32_t bm) {
+		return of_expert > bm / 2 && (uint64_t)experts * ((of_expert + bm - 1) / bm) * n_tiles >= kComputeUnits;
+	};
+	return direct && fits(256) ? 256 : fits(128) ? 128 : 64;
 }
 
 inline bool activation_ok(int a) { return a == OFI_AMD_NO_ACTIVATION || a == OFI_AMD_RELU || a == OFI_AMD_SILU || a == OFI_AMD_GELU; }

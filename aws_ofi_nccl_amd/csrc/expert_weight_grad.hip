@@ -28,8 +28,9 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const 
 	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
 	using rows_tile = across_t<T, BM, THREADS>;
 	using columns_tile = across_t<T, BN, THREADS>;
-	constexpr uint32_t kTile = rows_tile::kBytes + columns_tile::kBytes;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kTile];
+	constexpr uint32_t kTile = rows_tile::kBytes + columns_tile::kBytes, kFills = rows_tile::kChunks + columns_tile::kChunks;
+	constexpr uint32_t kStages = DIRECT && WM < 4 ? 3 : 2;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * kTile];
 
 	/* an eighth of the tiles in one piece for each XCD; in an expert, bands of eight row tiles */
 	const uint32_t id = first_tile + blockIdx.x, share = (tiles + 7) / 8, at = (id & 7u) * share + (id >> 3);
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const 
 	const across_frag_t<BM> row_frag(wm * 16 * MF, lane);
 	const across_frag_t<BN> column_frag(wn * 16 * G, lane);
 	auto sum = [&](auto also) __attribute__((always_inline)) {
-		sum_steps<T, DIRECT>(
+		sum_steps<T, DIRECT, kStages, kFills>(
 			sums, wm * 16 * MF < m_there, (hi - lo + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
 			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
 				rows.fill(step, to);
