@@ -22,7 +22,9 @@ __global__ __launch_bounds__(64 * CG * KS, MB == 1 ? 4 : 2) void expert_few_kern
 	constexpr bool SCALED = sizeof(T) == 1;
 	__shared__ __attribute__((aligned(16))) float part[KS][BM][2][PART];
 
-	const tile_t tile = tile_of<BM>(offset, n_experts, max_rows, n_tiles, first_tile + blockIdx.x);
+	__shared__ uint32_t known[4][64];
+	const rows_t of = { offset, n_experts, max_rows, n_tiles };
+	const tile_t tile = find_tile<BM>(of, count_tiles<BM>(of, known), first_tile + blockIdx.x, known);
 	if (!tile.any) {
 		return;
 	}
@@ -166,18 +168,18 @@ __global__ __launch_bounds__(64 * CG * KS, MB == 1 ? 4 : 2) void expert_few_kern
 		}
 	}
 	__syncthreads();
+	const forward_tile_t place = { tile.from, tile.rows, c0, c1, n - c0 < PART ? n - c0 : PART, c1 >= n ? 0 : n - c1 < PART ? n - c1 : PART, n, tile.expert };
 	constexpr uint32_t kOfRow = PART / 8; /* lanes that have a row */
 	for (uint32_t r = threadIdx.x / kOfRow; r < BM; r += 64 * CG * KS / kOfRow) {
 		const uint32_t c = threadIdx.x % kOfRow * 8;
-		const forward_rows_t out(o, tile, n, c0, c1, PART, c);
-		const auto in = out.load(r);
+		const forward_in_t in = forward_load<false>(o, place, r, c);
 		f32x8_t a = {}, b = {};
 #pragma unroll
 		for (uint32_t s = 0; s < KS; s++) {
 			a += *reinterpret_cast<const f32x8_t *>(&part[s][r][0][c]);
 			b += *reinterpret_cast<const f32x8_t *>(&part[s][r][1][c]);
 		}
-		out.finish(r, a, b, in);
+		forward_finish<false>(o, place, r, c, a, b, in);
 	}
 }
 

@@ -17,75 +17,73 @@ struct forward_t {
 	bool gated;
 };
 
-struct forward_rows_t {
-	struct in_t {
-		eight_t add0, add1;
-	};
-	const forward_t &o;
-	uint64_t from, n;
-	uint32_t rows, column0, column1, left0, left1, block0, block1, blocks;
-	f32x8_t bias0, bias1;
+/* A tile of both parts of a forward product, the same for all lanes: its rows from `from` on, the parts' columns from c0 and c1 on, of which
+ * there0 and there1 are there; n: columns of the matrix */
+struct forward_tile_t {
+	uint64_t from;
+	uint32_t rows, c0, c1, there0, there1, n, expert;
+};
+struct forward_in_t {
+	eight_t add0, add1;
+};
 
-	/* c0, c1: the parts' first columns, each of `part` columns at most; c: the lane's first in them */
-	__device__ __forceinline__ forward_rows_t(const forward_t &with, const tile_t &tile, uint32_t width, uint32_t c0, uint32_t c1, uint32_t part,
-						  uint32_t c)
-		: o(with), from(tile.from), n(width), rows(tile.rows), column0(c0 + c), column1(c1 + c), block0(c0 / kBlock), block1(c1 / kBlock),
-		  blocks(blocks_of(width)), bias0{}, bias1{}
-	{
-		const uint32_t end0 = c0 + part < width ? c0 + part : width, end1 = c1 + part < width ? c1 + part : width;
-		left0 = column0 < end0 ? end0 - column0 : 0;
-		left1 = column1 < end1 ? end1 - column1 : 0;
-		if (o.bias.p) {
-			auto bias_at = [&](uint32_t column, uint32_t left) {
-				const uint64_t at = (uint64_t)tile.expert * n + column;
-				return o.bias.type == OFI_AMD_FLOAT32 ? read_floats(o.bias.p + at * 4, left)
-								      : values_of(load_eight(o.bias, 0, at, left, 0), o.bias.type);
-			};
-			bias0 = bias_at(column0, left0);
-			bias1 = bias_at(column1, left1);
-		}
+__device__ __forceinline__ uint32_t left_of(uint32_t there, uint32_t c) { return c < there ? there - c : 0u; }
+
+/* c: the lane's first column in its part */
+template <bool WHOLE> __device__ __forceinline__ forward_in_t forward_load(const forward_t &o, forward_tile_t t, uint32_t r, uint32_t c)
+{
+	forward_in_t in = {};
+	if (o.residual.p && (WHOLE || r < t.rows)) {
+		in.add0 = load_eight(o.residual, t.from + r, t.c0 + c, WHOLE ? 8 : left_of(t.there0, c), 0);
+		in.add1 = load_eight(o.residual, t.from + r, t.c1 + c, WHOLE ? 8 : left_of(t.there1, c), 0);
 	}
-	__device__ __forceinline__ in_t load(uint32_t r) const
-	{
-		in_t in = {};
-		if (o.residual.p && r < rows) {
-			in.add0 = load_eight(o.residual, from + r, column0, left0, 0);
-			in.add1 = load_eight(o.residual, from + r, column1, left1, 0);
-		}
-		return in;
+	return in;
+}
+
+__device__ __forceinline__ f32x8_t bias_at(const matrix_t &bias, uint64_t at, uint32_t left)
+{
+	return bias.type == OFI_AMD_FLOAT32 ? read_floats(bias.p + at * 4, left) : values_of(load_eight(bias, 0, at, left, 0), bias.type);
+}
+
+/* All sixteen lanes of a block call */
+template <bool WHOLE>
+__device__ __forceinline__ void forward_finish(const forward_t &o, forward_tile_t t, uint32_t r, uint32_t c, f32x8_t a, f32x8_t b,
+					       const forward_in_t &in)
+{
+	const uint32_t left0 = WHOLE ? 8 : left_of(t.there0, c), left1 = WHOLE ? 8 : left_of(t.there1, c), blocks = blocks_of(t.n);
+	const uint32_t block0 = t.c0 / kBlock, block1 = t.c1 / kBlock;
+	if (o.bias.p) { /* out of the caches: held, it would be sixteen registers of the whole epilogue */
+		const uint64_t at = (uint64_t)t.expert * t.n + c;
+		a += bias_at(o.bias, at + t.c0, left0);
+		b += bias_at(o.bias, at + t.c1, left1);
 	}
-	/* All sixteen lanes of a block call */
-	__device__ __forceinline__ void finish(uint32_t r, f32x8_t a, f32x8_t b, const in_t &in) const
-	{
-		const uint64_t row = from + r;
-		const bool write = r < rows;
-		if (o.bias.p) {
-			a += bias0;
-			b += bias1;
-		}
-		if (o.saved.p) {
-			write_any(o.saved, row, column0, left0, block0, a, write);
-			write_any(o.saved, row, (o.gated ? n : 0) + column1, left1, (o.gated ? blocks : 0) + block1, b, write);
-		}
-		with_activation(o.activation, [&](auto activation) {
+	if (o.saved.p) {
+		write_row<WHOLE>(o.saved, t.from, t.c0 + c, block0, r, t.rows, left0, a);
+		write_row<WHOLE>(o.saved, t.from, (o.gated ? (uint64_t)t.n : 0) + t.c1 + c, (o.gated ? blocks : 0) + block1, r, t.rows, left1, b);
+	}
+	if (o.gated) {
+		with_activation(o.activation, [&](auto activation) __attribute__((always_inline)) {
+#pragma unroll
+			for (int i = 0; i < 8; i++) {
+				a[i] = activated<decltype(activation)::value>(a[i]) * b[i];
+			}
+		});
+	} else {
+		with_activation(o.activation, [&](auto activation) __attribute__((always_inline)) {
 #pragma unroll
 			for (int i = 0; i < 8; i++) {
 				a[i] = activated<decltype(activation)::value>(a[i]);
-				b[i] = o.gated ? b[i] : activated<decltype(activation)::value>(b[i]);
+				b[i] = activated<decltype(activation)::value>(b[i]);
 			}
 		});
-		if (o.gated) {
-			a *= b;
-		} else {
-			if (o.residual.p) {
-				a += values_of(in.add0, o.residual.type);
-				b += values_of(in.add1, o.residual.type);
-			}
-			write_any(o.out, row, column1, left1, block1, b, write);
+		if (o.residual.p) {
+			a += values_of(in.add0, o.residual.type);
+			b += values_of(in.add1, o.residual.type);
 		}
-		write_any(o.out, row, column0, left0, block0, a, write);
+		write_row<WHOLE>(o.out, t.from, t.c1 + c, block1, r, t.rows, left1, b);
 	}
-};
+	write_row<WHOLE>(o.out, t.from, t.c0 + c, block0, r, t.rows, left0, a);
+}
 
 /* Few rows an expert: expert_few.hip.  Few are up to 8, and up to 64 where tiles of 64 x 256 would leave compute units without any.
  * Both sides, us (width 4096 to 2048 in 8 bits, 32 experts): 128 rows 98 in streams and 127 in tiles, 256 rows 115 and 136, 512 183 and

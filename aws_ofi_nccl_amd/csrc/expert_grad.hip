@@ -18,116 +18,144 @@ struct backward_t {
 };
 
 /* k: the product's outputs, n: its columns */
+struct backward_args_t {
+	rows_t of;
+	const uint8_t *dout, *w;
+	uint64_t dout_pitch, w_pitch, expert_pitch;
+	uint32_t k, n, first_tile;
+	backward_t o;
+};
+
+/* A tile, the same for all lanes: its rows from `from` on, `there` columns from c0 on of n */
+struct backward_tile_t {
+	uint64_t from;
+	uint32_t rows, c0, there, n;
+};
+
+template <typename T, uint32_t BM, uint32_t THREADS> struct backward_operands_t {
+	along_t<T, BM, THREADS> rows;
+	across_t<T, 2 * kBlock, THREADS> columns;
+	backward_tile_t place;
+	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kBytes = kRowsBytes + decltype(columns)::kBytes;
+	static constexpr uint32_t kFills = decltype(rows)::kChunks + decltype(columns)::kChunks;
+
+	__device__ __forceinline__ void set(const backward_args_t *a, const tile_t &tile)
+	{
+		const uint32_t n = a->n, c0 = tile.nt * 2 * kBlock, there = n - c0 < 2 * kBlock ? n - c0 : 2 * kBlock;
+		place = { tile.from, tile.rows, c0, there, n };
+		rows.set(a->dout + tile.from * a->dout_pitch, a->dout_pitch, tile.rows, (int64_t)a->k * 2);
+		columns.set(a->w + tile.expert * a->expert_pitch + c0 * 2, a->w_pitch, a->k, (int64_t)there * 2);
+	}
+	__device__ __forceinline__ void load(uint32_t step)
+	{
+		rows.load(step);
+		columns.load(step);
+	}
+	__device__ __forceinline__ void store(uint32_t step, uint8_t *to) const
+	{
+		rows.store(step, to);
+		columns.store(step, to + kRowsBytes);
+	}
+	__device__ __forceinline__ void fill(uint32_t step, uint8_t *to) const
+	{
+		rows.fill(step, to);
+		columns.fill(step, to + kRowsBytes);
+	}
+};
+
 template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool HIDDEN, bool DIRECT>
-__global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(const int32_t *offset, const uint8_t *dout, const uint8_t *w,
-								       uint32_t n_experts, uint32_t max_rows, uint32_t k, uint32_t n,
-								       uint32_t n_tiles, uint32_t first_tile, uint64_t dout_pitch,
-								       uint64_t w_pitch, uint64_t expert_pitch, backward_t o)
+__global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(backward_args_t)
 {
 	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
-	using rows_tile = along_t<T, BM, THREADS>;
-	using columns_tile = across_t<T, BN, THREADS>;
-	constexpr uint32_t kTile = rows_tile::kBytes + columns_tile::kBytes, kFills = rows_tile::kChunks + columns_tile::kChunks;
+	using operands_t = backward_operands_t<T, BM, THREADS>;
 	constexpr uint32_t kStages = DIRECT && WM < 4 ? 3 : 2;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * kTile];
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * operands_t::kBytes];
+	__shared__ uint32_t known[4][64];
 
-	const tile_t tile = tile_of<BM>(offset, n_experts, max_rows, n_tiles, first_tile + blockIdx.x);
-	if (!tile.any) {
-		return;
+	operands_t of;
+	uint32_t steps;
+	{
+		const backward_args_t *const a = argument<backward_args_t>();
+		steps = (a->k + kStepRows - 1) / kStepRows;
+		const tile_t tile = find_tile<BM>(a->of, count_tiles<BM>(a->of, known), a->first_tile + blockIdx.x, known);
+		if (!tile.any) {
+			return;
+		}
+		of.set(a, tile);
 	}
 	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-	const uint32_t c0 = tile.nt * BN, there = n - c0 < BN ? n - c0 : BN;
-	rows_tile rows = { dout + tile.from * dout_pitch, dout_pitch, tile.rows, (int64_t)k * 2 };
-	columns_tile columns = { w + tile.expert * expert_pitch + c0 * 2, w_pitch, k, (int64_t)there * 2 };
+	f32x4_t sums[MF][2][G] = {};
+	sum_steps<T, DIRECT, kStages, operands_t::kFills>(
+		sums, wm * 16 * MF < of.place.rows, steps, lds, operands_t::kBytes, operands_t::kRowsBytes, along_frag_t(wm * 16 * MF, lane),
+		across_frag_t<BN>(wn * 16 * G, lane), [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.fill(step, to); },
+		[&](uint32_t step) __attribute__((always_inline)) { of.load(step); },
+		[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.store(step, to); }, [](const u32x4_t(&)[MF]) {});
 
-	f32x4_t sums[MF][2][G];
-#pragma unroll
-	for (int m = 0; m < (int)MF; m++) {
-#pragma unroll
-		for (int j = 0; j < (int)(2 * G); j++) {
-			sums[m][j / G][j % G] = f32x4_t{ 0, 0, 0, 0 };
-		}
-	}
-	const along_frag_t row_frag(wm * 16 * MF, lane);
-	const across_frag_t<BN> column_frag(wn * 16 * G, lane);
-	sum_steps<T, DIRECT, kStages, kFills>(
-		sums, wm * 16 * MF < tile.rows, (k + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
-		[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
-			rows.fill(step, to);
-			columns.fill(step, to + rows_tile::kBytes);
-		},
-		[&](uint32_t step) __attribute__((always_inline)) {
-			rows.load(step);
-			columns.load(step);
-		},
-		[&](uint8_t *to) __attribute__((always_inline)) {
-			rows.store(to);
-			columns.store(to + rows_tile::kBytes);
-		},
-		[](const u32x4_t(&)[MF]) {});
-
-	const uint32_t c = (lane & 15u) * 8, blocks = blocks_of(n), block = c0 / kBlock;
-	const uint32_t left[2] = { c < there ? there - c : 0, c + kBlock < there ? there - c - kBlock : 0 };
 	struct in_t {
 		eight_t g[2], u[2]; /* what was kept, or what is added */
 	};
-	for_rows<WM, WN, MF>(
-		sums, lds,
-		[&](uint32_t r) {
+	const backward_tile_t place = of.place;
+	auto left_at = [&](uint32_t column) { return column < place.there ? place.there - column : 0u; };
+	for_rows<WM, WN, MF, false>(
+		sums, lds, place.rows == BM && place.there == BN,
+		[&](auto all, uint32_t r, uint32_t part_lane) __attribute__((always_inline)) {
+			constexpr bool WHOLE = decltype(all)::value;
+			const backward_t &o = argument<backward_args_t>()->o;
 			in_t in = {};
-			const uint64_t row = tile.from + r;
+			const uint32_t c = part_lane * 8, block = place.c0 / kBlock;
+			const uint64_t row = place.from + r;
 #pragma unroll
 			for (int p = 0; p < 2; p++) {
-				const uint32_t column = c0 + p * kBlock + c;
-				if (r < tile.rows && left[p]) {
+				const uint32_t column = place.c0 + p * kBlock + c, some = WHOLE ? 8 : left_at(p * kBlock + c);
+				if (WHOLE || (r < place.rows && some)) {
 					if (!HIDDEN && o.add.p) {
-						in.g[p] = load_eight(o.add, row, column, left[p], 0);
+						in.g[p] = load_eight(o.add, row, column, some, 0);
 					} else if (HIDDEN) {
-						in.g[p] = load_eight(o.saved, row, column, left[p], block + p);
+						in.g[p] = load_eight(o.saved, row, column, some, block + p);
 						if (o.gated) {
-							in.u[p] = load_eight(o.saved, row, (uint64_t)n + column, left[p], blocks + block + p);
+							in.u[p] = load_eight(o.saved, row, (uint64_t)place.n + column, some, blocks_of(place.n) + block + p);
 						}
 					}
 				}
 			}
 			return in;
 		},
-		[&](uint32_t r, f32x8_t a, f32x8_t b, const in_t &in) {
-			const uint64_t row = tile.from + r;
+		[&](auto all, uint32_t r, uint32_t part_lane, f32x8_t p0, f32x8_t p1, const in_t &in) __attribute__((always_inline)) {
+			constexpr bool WHOLE = decltype(all)::value;
+			const backward_t &o = argument<backward_args_t>()->o;
+			const uint32_t c = part_lane * 8;
 #pragma unroll
 			for (int p = 0; p < 2; p++) {
-				const uint32_t column = c0 + p * kBlock + c;
-				f32x8_t v = p ? b : a;
-				if (r >= tile.rows || left[p] == 0) {
-					continue;
-				}
+				const uint64_t column = place.c0 + p * kBlock + c;
+				const uint32_t left = WHOLE ? 8 : left_at(p * kBlock + c);
+				f32x8_t v = p ? p1 : p0;
 				if constexpr (HIDDEN) {
-					f32x8_t g = values_of(in.g[p], o.saved.type), u = {}, h;
+					f32x8_t g = values_of(in.g[p], o.saved.type), h = { 1, 1, 1, 1, 1, 1, 1, 1 };
 					if (o.gated) {
-						u = values_of(in.u[p], o.saved.type);
+						h = values_of(in.u[p], o.saved.type);
 					}
-					with_activation(o.activation, [&](auto activation) {
+					with_activation(o.activation, [&](auto activation) __attribute__((always_inline)) {
 #pragma unroll
 						for (int i = 0; i < 8; i++) {
 							float value, slope;
 							activated_with_slope<decltype(activation)::value>(g[i], value, slope);
-							g[i] = o.gated ? v[i] * u[i] * slope : v[i] * slope;
-							h[i] = o.gated ? value * u[i] : value;
+							g[i] = v[i] * h[i] * slope;
+							h[i] *= value;
 							v[i] *= value;
 						}
 					});
-					write_values(o.dsaved, row, column, left[p], g);
+					write_row<WHOLE>(o.dsaved, place.from, column, 0, r, place.rows, left, g);
 					if (o.gated) {
-						write_values(o.dsaved, row, (uint64_t)n + column, left[p], v);
+						write_row<WHOLE>(o.dsaved, place.from, (uint64_t)place.n + column, 0, r, place.rows, left, v);
 					}
 					if (o.hidden.p) {
-						write_values(o.hidden, row, column, left[p], h);
+						write_row<WHOLE>(o.hidden, place.from, column, 0, r, place.rows, left, h);
 					}
 				} else {
 					if (o.add.p) {
 						v += values_of(in.g[p], o.add.type);
 					}
-					write_values(o.out, row, column, left[p], v);
+					write_row<WHOLE>(o.out, place.from, column, 0, r, place.rows, left, v);
 				}
 			}
 		});
@@ -143,6 +171,8 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
+	backward_args_t args = { { d_offset, n_experts, max_rows, n_tiles }, static_cast<const uint8_t *>(d_dout), static_cast<const uint8_t *>(d_weight),
+				 dout_pitch, weight_pitch, expert_pitch, k, n, 0, o };
 	auto with = [&](auto element) {
 		using T = decltype(element);
 		auto kernel = direct ? (bm == 256 ? expert_backward_kernel<T, 4, 2, 4, HIDDEN, true>
@@ -151,9 +181,8 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 				     : bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, false>
 						 : expert_backward_kernel<T, 1, 8, 4, HIDDEN, false>;
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
-			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset,
-				      static_cast<const uint8_t *>(d_dout), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, k, n,
-				      n_tiles, first, dout_pitch, weight_pitch, expert_pitch, o);
+			args.first_tile = first;
+			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {

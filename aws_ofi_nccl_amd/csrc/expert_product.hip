@@ -10,140 +10,176 @@
 namespace ofi_amd {
 namespace {
 
-template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT>
-__global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(const int32_t *offset, const uint8_t *x, const uint8_t *w, uint32_t n_experts,
-								      uint32_t max_rows, uint32_t width, uint32_t n, uint32_t n_tiles,
-								      uint32_t first_tile, uint64_t x_pitch, uint64_t w_pitch,
-								      uint64_t expert_pitch, forward_t o)
-{
-	constexpr uint32_t BM = 16 * MF * WM, THREADS = 64 * WM * WN, G = 8 / WN;
-	constexpr bool SCALED = sizeof(T) == 1;
-	using rows_tile = along_t<T, BM, THREADS>;
-	using part_tile = along_t<T, kBlock, THREADS>;
-	constexpr uint32_t kTile = rows_tile::kBytes + 2 * part_tile::kBytes, kFills = rows_tile::kChunks + 2 * part_tile::kChunks;
-	constexpr uint32_t kStages = DIRECT && !SCALED && WM < 4 ? 3 : 2;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * kTile];
+struct forward_args_t {
+	rows_t of;
+	const uint8_t *x, *w;
+	uint64_t x_pitch, w_pitch, expert_pitch;
+	uint32_t width, n, first_tile;
+	forward_t o;
+};
 
-	const tile_t tile = tile_of<BM>(offset, n_experts, max_rows, n_tiles, first_tile + blockIdx.x);
-	if (!tile.any) {
-		return;
-	}
-	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-	/* column 0 of both parts, in the matrix of n columns; a gated block's parts are n rows of weights apart */
-	const uint32_t c0 = tile.nt * (o.gated ? kBlock : 2 * kBlock), c1 = o.gated ? c0 : c0 + kBlock;
-	const uint32_t there0 = n - c0 < kBlock ? n - c0 : kBlock, there1 = c1 >= n ? 0 : n - c1 < kBlock ? n - c1 : kBlock;
-	const uint8_t *const weights = w + tile.expert * expert_pitch;
-	const int64_t bytes = (int64_t)width * sizeof(T);
-	rows_tile rows = { x + tile.from * x_pitch, x_pitch, tile.rows, bytes };
-	part_tile part0 = { weights + c0 * w_pitch, w_pitch, there0, bytes };
-	part_tile part1 = { weights + (there1 ? (o.gated ? (uint64_t)n : 0) + c1 : 0) * w_pitch, w_pitch, there1, bytes };
+template <typename T, uint32_t BM, uint32_t THREADS> struct forward_operands_t {
+	along_t<T, BM, THREADS> rows;
+	along_t<T, kBlock, THREADS> part0, part1;
+	forward_tile_t place;
+	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kPartBytes = decltype(part0)::kBytes, kBytes = kRowsBytes + 2 * kPartBytes;
+	static constexpr uint32_t kFills = decltype(rows)::kChunks + 2 * decltype(part0)::kChunks;
 
-	f32x4_t sums[MF][2][G];
-#pragma unroll
-	for (int m = 0; m < (int)MF; m++) {
-#pragma unroll
-		for (int j = 0; j < (int)(2 * G); j++) {
-			sums[m][j / G][j % G] = f32x4_t{ 0, 0, 0, 0 };
-		}
+	/* direct: a part without columns is not read; else the first column stands for them */
+	__device__ __forceinline__ void set(const forward_args_t *a, const tile_t &tile, bool direct)
+	{
+		const bool gated = a->o.gated;
+		const uint32_t n = a->n, c0 = tile.nt * (gated ? kBlock : 2 * kBlock), c1 = gated ? c0 : c0 + kBlock;
+		const uint32_t there0 = n - c0 < kBlock ? n - c0 : kBlock, there1 = c1 >= n ? 0 : n - c1 < kBlock ? n - c1 : kBlock;
+		const uint8_t *const weights = a->w + tile.expert * a->expert_pitch;
+		const int64_t bytes = (int64_t)a->width * sizeof(T);
+		place = { tile.from, tile.rows, c0, c1, there0, there1, n, tile.expert };
+		rows.set(a->x + tile.from * a->x_pitch, a->x_pitch, tile.rows, bytes);
+		part0.set(weights + c0 * a->w_pitch, a->w_pitch, there0, bytes);
+		part1.set(weights + (there1 ? (gated ? (uint64_t)n : 0) + c1 : 0) * a->w_pitch, a->w_pitch, there1 || direct ? there1 : 1, bytes);
 	}
-	const along_frag_t row_frag(wm * 16 * MF, lane), column_frag(wn * 16 * G, lane);
-	const uint32_t steps = (width + kStepOf<T> - 1) / kStepOf<T>;
-	auto fill = [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
-		rows.fill(step, to);
-		part0.fill(step, to + rows_tile::kBytes);
-		part1.fill(step, to + rows_tile::kBytes + part_tile::kBytes);
-	};
-	auto load = [&](uint32_t step) __attribute__((always_inline)) {
+	__device__ __forceinline__ void load(uint32_t step)
+	{
 		rows.load(step);
 		part0.load(step);
 		part1.load(step);
-	};
-	auto store = [&](uint8_t *to) __attribute__((always_inline)) {
-		rows.store(to);
-		part0.store(to + rows_tile::kBytes);
-		part1.store(to + rows_tile::kBytes + part_tile::kBytes);
-	};
-	if constexpr (!SCALED) {
-		sum_steps<T, DIRECT, kStages, kFills>(sums, wm * 16 * MF < tile.rows, steps, lds, kTile, rows_tile::kBytes, row_frag, column_frag, fill, load, store,
-				     [](const u32x4_t(&)[MF]) {});
+	}
+	__device__ __forceinline__ void store(uint32_t step, uint8_t *to) const
+	{
+		rows.store(step, to);
+		part0.store(step, to + kRowsBytes);
+		part1.store(step, to + kRowsBytes + kPartBytes);
+	}
+	__device__ __forceinline__ void fill(uint32_t step, uint8_t *to) const
+	{
+		rows.fill(step, to);
+		part0.fill(step, to + kRowsBytes);
+		part1.fill(step, to + kRowsBytes + kPartBytes);
+	}
+};
+
+/* sums += all steps of 8-bit rows, each with its scales: sum_steps without fragments on their way, for want of registers */
+template <uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT, typename Operands>
+__device__ __forceinline__ void sum_scaled_steps(f32x4_t (&sums)[MF][2][8 / WN], uint32_t steps, uint8_t *lds, Operands &of)
+{
+	constexpr uint32_t G = 8 / WN;
+	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+	const along_frag_t row_frag(wm * 16 * MF, lane), column_frag(wn * 16 * G, lane);
+	const forward_args_t *const a = argument<forward_args_t>();
+	const forward_tile_t &place = of.place;
+	/* the scales of a lane's row of each of its groups, and of the parts' weights */
+	const float *row_scale[MF], *weight_scale[2];
+	const uint32_t k_blocks = blocks_of(a->width), n_blocks = blocks_of(place.n);
+	const float *const of_expert = a->o.weight_scale + (uint64_t)place.expert * (a->o.gated ? 2 : 1) * n_blocks * k_blocks;
+	weight_scale[0] = of_expert + (uint64_t)(place.c0 / kBlock) * k_blocks;
+	weight_scale[1] = place.there1 ? of_expert + (uint64_t)((a->o.gated ? n_blocks : 0) + place.c1 / kBlock) * k_blocks : weight_scale[0];
+#pragma unroll
+	for (int m = 0; m < (int)MF; m++) {
+		const uint32_t r = (wm * MF + m) * 16 + (lane & 15u);
+		row_scale[m] = row_at(a->o.scale, a->o.scale_pitch, place.from + (r < place.rows ? r : place.rows - 1));
+	}
+	if (DIRECT) {
+		of.fill(0, lds);
 	} else {
-		/* a lane's row of each of its groups */
-		const float *row_scale[MF], *weight_scale[2];
-		const uint32_t k_blocks = blocks_of(width), n_blocks = blocks_of(n);
-		const float *of_expert = o.weight_scale + (uint64_t)tile.expert * (o.gated ? 2 : 1) * n_blocks * k_blocks;
-		weight_scale[0] = of_expert + (uint64_t)(c0 / kBlock) * k_blocks;
-		weight_scale[1] = there1 ? of_expert + (uint64_t)((o.gated ? n_blocks : 0) + c1 / kBlock) * k_blocks : weight_scale[0];
+		of.load(0);
+	}
+	for (uint32_t step = 0; step < steps; step++) {
+		uint8_t *const now = lds + (step & 1u) * Operands::kBytes;
+		if (DIRECT) {
+			landed<0>();
+		} else {
+			of.store(step, now);
+		}
+		workgroup_meets<DIRECT>(); /* this tile is there, and the other one's readers are past it */
+		if (step + 1 < steps) {
+			if (DIRECT) {
+				of.fill(step + 1, lds + (~step & 1u) * Operands::kBytes);
+			} else {
+				of.load(step + 1);
+			}
+		}
+		float by[MF][2];
+		u32x4_t r[MF][4];
 #pragma unroll
 		for (int m = 0; m < (int)MF; m++) {
-			const uint32_t r = (wm * MF + m) * 16 + (lane & 15u);
-			row_scale[m] = row_at(o.scale, o.scale_pitch, tile.from + (r < tile.rows ? r : tile.rows - 1));
+			const float s = row_scale[m][step];
+			by[m][0] = s * weight_scale[0][step];
+			by[m][1] = s * weight_scale[1][step];
+#pragma unroll
+			for (uint32_t half = 0; half < 2; half++) {
+				const u32x4_t q = row_frag.get(now, m * 16, half);
+				r[m][2 * half] = widened(q.x, q.y);
+				r[m][2 * half + 1] = widened(q.z, q.w);
+			}
 		}
-		if (DIRECT) {
-			fill(0, lds);
-		} else {
-			load(0);
-		}
-		for (uint32_t step = 0; step < steps; step++) {
-			uint8_t *const now = lds + (step & 1u) * kTile;
-			if (DIRECT) {
-				landed<0>();
-			} else {
-				store(now);
-			}
-			__syncthreads(); /* this tile is there, and the other one's readers are past it */
-			if (step + 1 < steps) {
-				if (DIRECT) {
-					fill(step + 1, lds + (~step & 1u) * kTile);
-				} else {
-					load(step + 1);
-				}
-			}
-			float by[MF][2];
-			u32x4_t r[MF][4];
 #pragma unroll
-			for (int m = 0; m < (int)MF; m++) {
-				const float s = row_scale[m][step];
-				by[m][0] = s * weight_scale[0][step];
-				by[m][1] = s * weight_scale[1][step];
+		for (int j = 0; j < (int)(2 * G); j++) {
+			const uint8_t *const columns = now + Operands::kRowsBytes;
+			const u32x4_t q0 = column_frag.get(columns, j / G * kBlock + j % G * 16, 0);
+			const u32x4_t q1 = column_frag.get(columns, j / G * kBlock + j % G * 16, 1);
+			const u32x4_t c[4] = { widened(q0.x, q0.y), widened(q0.z, q0.w), widened(q1.x, q1.y), widened(q1.z, q1.w) };
+			f32x4_t part[MF] = {};
 #pragma unroll
-				for (uint32_t half = 0; half < 2; half++) {
-					const u32x4_t q = row_frag.get(now, m * 16, half);
-					r[m][2 * half] = widened(q.x, q.y);
-					r[m][2 * half + 1] = widened(q.z, q.w);
-				}
-			}
-#pragma unroll
-			for (int j = 0; j < (int)(2 * G); j++) {
-				const uint8_t *const columns = now + rows_tile::kBytes;
-				const u32x4_t q0 = column_frag.get(columns, j / G * kBlock + j % G * 16, 0);
-				const u32x4_t q1 = column_frag.get(columns, j / G * kBlock + j % G * 16, 1);
-				const u32x4_t c[4] = { widened(q0.x, q0.y), widened(q0.z, q0.w), widened(q1.x, q1.y), widened(q1.z, q1.w) };
-				f32x4_t part[MF] = {};
-#pragma unroll
-				for (int k = 0; k < 4; k++) {
-#pragma unroll
-					for (int m = 0; m < (int)MF; m++) {
-						part[m] = multiply<f16_t>(c[k], r[m][k], part[m]);
-					}
-				}
+			for (int k = 0; k < 4; k++) {
 #pragma unroll
 				for (int m = 0; m < (int)MF; m++) {
-					f32x4_t &to = sums[m][j / G][j % G];
+					part[m] = multiply<f16_t>(c[k], r[m][k], part[m]);
+				}
+			}
 #pragma unroll
-					for (int i = 0; i < 4; i++) {
-						to[i] = __builtin_fmaf(part[m][i], by[m][j / G], to[i]);
-					}
+			for (int m = 0; m < (int)MF; m++) {
+				f32x4_t &to = sums[m][j / G][j % G];
+#pragma unroll
+				for (int i = 0; i < 4; i++) {
+					to[i] = __builtin_fmaf(part[m][i], by[m][j / G], to[i]);
 				}
 			}
 		}
 	}
-
-	const forward_rows_t out(o, tile, n, c0, c1, kBlock, (lane & 15u) * 8);
-	for_rows<WM, WN, MF>(
-		sums, lds, [&](uint32_t r) { return out.load(r); },
-		[&](uint32_t r, f32x8_t a, f32x8_t b, const forward_rows_t::in_t &in) { out.finish(r, a, b, in); });
 }
 
+template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT>
+__global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(forward_args_t)
+{
+	constexpr uint32_t BM = 16 * MF * WM, THREADS = 64 * WM * WN, G = 8 / WN;
+	constexpr bool SCALED = sizeof(T) == 1;
+	using operands_t = forward_operands_t<T, BM, THREADS>;
+	constexpr uint32_t kStages = DIRECT && !SCALED && WM < 4 ? 3 : 2;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * operands_t::kBytes];
+	__shared__ uint32_t known[4][64];
+
+	operands_t of;
+	uint32_t steps;
+	{
+		const forward_args_t *const a = argument<forward_args_t>();
+		steps = (a->width + kStepOf<T> - 1) / kStepOf<T>;
+		const tile_t tile = find_tile<BM>(a->of, count_tiles<BM>(a->of, known), a->first_tile + blockIdx.x, known);
+		if (!tile.any) {
+			return;
+		}
+		of.set(a, tile, DIRECT);
+	}
+	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+	f32x4_t sums[MF][2][G] = {};
+	if constexpr (SCALED) {
+		sum_scaled_steps<WM, WN, MF, DIRECT>(sums, steps, lds, of);
+	} else {
+		sum_steps<T, DIRECT, kStages, operands_t::kFills>(
+			sums, wm * 16 * MF < of.place.rows, steps, lds, operands_t::kBytes, operands_t::kRowsBytes, along_frag_t(wm * 16 * MF, lane),
+			along_frag_t(wn * 16 * G, lane), [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.fill(step, to); },
+			[&](uint32_t step) __attribute__((always_inline)) { of.load(step); },
+			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.store(step, to); }, [](const u32x4_t(&)[MF]) {});
+	}
+	const forward_tile_t place = of.place;
+	for_rows<WM, WN, MF, false>(
+		sums, lds, place.rows == BM && place.there0 == kBlock && place.there1 == kBlock,
+		[&](auto all, uint32_t r, uint32_t part_lane) __attribute__((always_inline)) {
+			return forward_load<decltype(all)::value>(argument<forward_args_t>()->o, place, r, part_lane * 8);
+		},
+		[&](auto all, uint32_t r, uint32_t part_lane, f32x8_t p0, f32x8_t p1, const forward_in_t &in) __attribute__((always_inline)) {
+			forward_finish<decltype(all)::value>(argument<forward_args_t>()->o, place, r, part_lane * 8, p0, p1, in);
+		});
+}
 
 int forward(const void *d_rows, uint64_t rows_pitch, int type, const int32_t *d_offset, uint32_t n_experts, uint32_t max_rows,
 	    const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t width, uint32_t n, const forward_t &o, void *stream)
@@ -159,15 +195,16 @@ int forward(const void *d_rows, uint64_t rows_pitch, int type, const int32_t *d_
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
+	forward_args_t args = { { d_offset, n_experts, max_rows, n_tiles }, static_cast<const uint8_t *>(d_rows), static_cast<const uint8_t *>(d_weight),
+				rows_pitch, weight_pitch, expert_pitch, width, n, 0, o };
 	auto with = [&](auto element) {
 		using T = decltype(element);
 		auto kernel = direct ? (bm == 256 ? expert_forward_kernel<T, 4, 2, 4, true>
 						: bm == 128 ? expert_forward_kernel<T, 2, 4, 4, true> : expert_forward_kernel<T, 1, 8, 4, true>)
 				     : bm == 128 ? expert_forward_kernel<T, 2, 4, 4, false> : expert_forward_kernel<T, 1, 8, 4, false>;
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
-			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset,
-				      static_cast<const uint8_t *>(d_rows), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, width, n,
-				      n_tiles, first, rows_pitch, weight_pitch, expert_pitch, o);
+			args.first_tile = first;
+			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {

@@ -50,7 +50,7 @@ __host__ __device__ inline uint32_t blocks_of(uint32_t width) { return (width + 
 
 /* ---- rows of experts ---------------------------------------------------------------------------------------- */
 
-/* first: the expert's first row; from: the tile's, rows: those it has; nt: which of the column tiles */
+/* from: the tile's first row, rows: those it has; nt: which of the column tiles */
 struct tile_t {
 	uint32_t expert, from, rows, nt;
 	bool any;
@@ -79,65 +79,89 @@ __device__ __forceinline__ uint32_t running_sum(uint32_t v, uint32_t lane)
 }
 
 /*
- * The tile that workgroup `id` of the launch takes.  Tiles are numbered expert by expert, an expert's in bands of eight row tiles, a
- * band's column by column: what an XCD's 32 compute units work on at once is about eight row tiles by four column tiles, which its L2
- * holds a step of.  Workgroups go to the eight XCDs in turn, so each XCD gets an eighth of the numbers in one piece.
+ * The tiles of a launch.  They are numbered expert by expert, an expert's in bands of eight row tiles, a band's column by column: what an
+ * XCD's 32 compute units work on at once is about eight row tiles by four column tiles, which its L2 holds a step of.  Workgroups go to
+ * the eight XCDs in turn, so each XCD gets an eighth of the numbers in one piece.  Each lane has one of 64 experts.
+ * All wavefronts of the workgroup call.
  */
-template <uint32_t BM>
-__device__ __forceinline__ tile_t tile_of(const int32_t *offset, uint32_t n_experts, uint32_t max_rows, uint32_t n_tiles, uint32_t id)
+struct rows_t {
+	const int32_t *offset;
+	uint32_t n_experts, max_rows, n_tiles;
+};
+
+/* Experts e to e + 63, behind `before` row tiles: the row tiles behind them.  What the lanes found is kept in four words of each in LDS, so
+ * that it holds no registers meanwhile; every wavefront keeps the same words. */
+template <uint32_t BM> __device__ __forceinline__ uint32_t look_at_experts(rows_t rows, uint32_t e, uint32_t before, uint32_t (*kept)[64])
 {
 	const uint32_t lane = threadIdx.x & 63u;
-	uint32_t total = 0, at = 0, e0 = 0, lo = 0, hi = 0, before = 0, mine = 0;
-	for (e0 = 0; e0 < n_experts; e0 += 64) {
-		lo = hi = 0;
-		if (e0 + lane < n_experts) {
-			run_of(offset, e0 + lane, max_rows, lo, hi);
-		}
-		mine = (hi - lo + BM - 1) / BM;
-		const uint32_t sum = running_sum(mine, lane);
-		before = total + sum - mine;
-		total += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+	uint32_t lo = 0, hi = 0;
+	if (e + lane < rows.n_experts) {
+		run_of(rows.offset, e + lane, rows.max_rows, lo, hi);
 	}
+	const uint32_t mine = (hi - lo + BM - 1) / BM, sum = running_sum(mine, lane);
+	kept[0][lane] = lo;
+	kept[1][lane] = hi;
+	kept[2][lane] = mine;
+	kept[3][lane] = before + sum - mine;
+	return before + (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+}
+
+/* The row tiles of all experts */
+template <uint32_t BM> __device__ __forceinline__ uint32_t count_tiles(rows_t rows, uint32_t (*kept)[64])
+{
+	uint32_t total = 0;
+	for (uint32_t e = 0; e < rows.n_experts; e += 64) {
+		total = look_at_experts<BM>(rows, e, total, kept);
+	}
+	return total;
+}
+
+/* The tile of workgroup `id` */
+template <uint32_t BM> __device__ __forceinline__ tile_t find_tile(rows_t rows, uint32_t total, uint32_t id, uint32_t (*kept)[64])
+{
 	tile_t t = {};
-	const uint32_t tiles = total * n_tiles, share = (tiles + 7) / 8;
-	at = (id & 7u) * share + (id >> 3);
+	const uint32_t n_tiles = rows.n_tiles, tiles = total * n_tiles, share = (tiles + 7) / 8;
+	uint32_t at = uniform((id & 7u) * share + (id >> 3));
 	if ((id >> 3) >= share || at >= tiles) {
 		return t;
 	}
-	if (n_experts > 64) { /* the lanes know the last experts: again, up to the one that has the tile */
-		uint32_t sums = 0;
-		for (e0 = 0; e0 < n_experts; e0 += 64) {
-			lo = hi = 0;
-			if (e0 + lane < n_experts) {
-				run_of(offset, e0 + lane, max_rows, lo, hi);
-			}
-			mine = (hi - lo + BM - 1) / BM;
-			const uint32_t sum = running_sum(mine, lane);
-			before = sums + sum - mine;
-			sums += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
-			if (at < sums * n_tiles) {
-				break;
-			}
+	uint32_t first = 0;
+	if (rows.n_experts > 64) { /* the words are of others: again, up to the one that has the tile */
+		__syncthreads();   /* which no wavefront still needs */
+		uint32_t seen = look_at_experts<BM>(rows, 0, 0, kept);
+		while (first + 64 < rows.n_experts && at >= seen * n_tiles) {
+			first += 64;
+			seen = look_at_experts<BM>(rows, first, seen, kept);
 		}
-	} else {
-		e0 = 0;
 	}
+	const uint32_t lane = threadIdx.x & 63u, lo = kept[0][lane], hi = kept[1][lane], mine = kept[2][lane], before = kept[3][lane];
 	const uint64_t has = __ballot(mine != 0 && at >= before * n_tiles && at < (before + mine) * n_tiles);
 	if (!has) {
 		return t;
 	}
 	const int who = (int)__builtin_ctzll(has);
-	const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)lo, who), end = (uint32_t)__builtin_amdgcn_readlane((int)hi, who);
+	const uint32_t begin = (uint32_t)__builtin_amdgcn_readlane((int)lo, who), end = (uint32_t)__builtin_amdgcn_readlane((int)hi, who);
 	const uint32_t row_tiles = (uint32_t)__builtin_amdgcn_readlane((int)mine, who);
-	at = uniform(at) - (uint32_t)__builtin_amdgcn_readlane((int)before, who) * n_tiles;
+	at -= (uint32_t)__builtin_amdgcn_readlane((int)before, who) * n_tiles;
 	const uint32_t band = at / (8 * n_tiles), in_band = at - band * 8 * n_tiles;
 	const uint32_t height = row_tiles - band * 8 < 8 ? row_tiles - band * 8 : 8;
-	t.expert = e0 + (uint32_t)who;
+	t.expert = first + (uint32_t)who;
 	t.nt = in_band / height;
-	t.from = first + (band * 8 + in_band % height) * BM;
+	t.from = begin + (band * 8 + in_band - t.nt * height) * BM;
 	t.rows = end - t.from < BM ? end - t.from : BM;
 	t.any = true;
 	return t;
+}
+
+/*
+ * The kernel's argument, a single A.  Each call is another pointer to the compiler: what one part of a kernel needs of it is loaded there, and
+ * does not lie in scalar registers from the beginning on (200 of them were spilled into the registers of the sums).
+ */
+template <typename A> __device__ __forceinline__ const A *argument()
+{
+	auto p = __builtin_amdgcn_kernarg_segment_ptr();
+	asm volatile("" : "+s"(p));
+	return (const A *)p;
 }
 
 /* ---- operands ----------------------------------------------------------------------------------------------- */
@@ -198,9 +222,18 @@ template <bool DIRECT> __device__ __forceinline__ void workgroup_meets()
 }
 constexpr uint32_t kBeyond = 0x80000000u; /* of any buffer */
 
+/* The chunk whose last `over` bytes lie behind the row, read as the 16 bytes that end with it: its own bytes, and zeros */
+__device__ __forceinline__ u32x4_t shifted(u32x4_t v, uint32_t over)
+{
+	const uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
+	const uint32_t bits = 8 * over;
+	const uint64_t low = bits >= 64 ? hi >> (bits - 64) : bits ? lo >> bits | hi << (64 - bits) : lo, high = bits >= 64 ? 0 : hi >> bits;
+	return u32x4_t{ (uint32_t)low, (uint32_t)(low >> 32), (uint32_t)high, (uint32_t)(high >> 32) };
+}
+
 /*
  * ROWS rows of an operand whose rows run along the summed axis.  base: the first row's start; rows of them are there, each of `bytes`;
- * what is not there is zeros.
+ * what is not there of the summed axis is zeros.
  */
 template <typename T, uint32_t ROWS, uint32_t THREADS> struct along_t {
 	static constexpr uint32_t kChunks = ROWS * 8 / THREADS, kRowsOfRound = THREADS / 8, kBytes = ROWS * kStepBytes;
@@ -210,6 +243,15 @@ template <typename T, uint32_t ROWS, uint32_t THREADS> struct along_t {
 	int64_t bytes;
 	u32x4_t held[kChunks];
 
+	__device__ __forceinline__ void set(const uint8_t *p, uint64_t apart, uint32_t n, int64_t size)
+	{
+		base = p;
+		pitch = apart;
+		rows = n;
+		bytes = size;
+	}
+	/* Rows that are not there are read as the last that is (no result of theirs is written), chunks behind the row as its last 16 bytes: no load
+	 * is conditional where a row has 16 bytes */
 	__device__ __forceinline__ void load(uint32_t step)
 	{
 		const uint32_t row = threadIdx.x / 8, chunk = (threadIdx.x & 7u) ^ (row & 7u);
@@ -217,14 +259,23 @@ template <typename T, uint32_t ROWS, uint32_t THREADS> struct along_t {
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
 			const uint32_t r = t * kRowsOfRound + row;
-			held[t] = chunk_at<T>(base + (uint64_t)(r < rows ? r : 0) * pitch + at, r < rows ? bytes - at : 0);
+			const uint8_t *const p = base + (uint64_t)(r < rows ? r : rows - 1) * pitch;
+			held[t] = bytes >= 16 ? *reinterpret_cast<const any16_t *>(p + (at + 16 <= bytes ? at : bytes - 16)) : chunk_at<T>(p + at, bytes - at);
 		}
 	}
-	__device__ __forceinline__ void store(uint8_t *lds) const
+	__device__ __forceinline__ void store(uint32_t step, uint8_t *lds) const
 	{
+		const uint32_t row = threadIdx.x / 8, chunk = (threadIdx.x & 7u) ^ (row & 7u);
+		const int64_t at = (int64_t)step * kStepBytes + chunk * 16;
+		const bool rest = (int64_t)(step + 1) * kStepBytes > bytes && bytes >= 16;
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
-			*reinterpret_cast<u32x4_t *>(lds + (t * THREADS + threadIdx.x) * 16) = held[t];
+			u32x4_t v = held[t];
+			if (rest) { /* of all rows alike */
+				const u32x4_t s = shifted(v, (uint32_t)(16 - bytes % 16) % 16);
+				v = at + 16 <= bytes ? v : at < bytes ? s : u32x4_t{ 0, 0, 0, 0 };
+			}
+			*reinterpret_cast<u32x4_t *>(lds + (t * THREADS + threadIdx.x) * 16) = v;
 		}
 	}
 	/* Both at once, past the registers: rows in whole chunks (in_chunks), so that a tile is within 31 bits */
@@ -233,7 +284,7 @@ template <typename T, uint32_t ROWS, uint32_t THREADS> struct along_t {
 		const uint32_t row = threadIdx.x / 8, chunk = (threadIdx.x & 7u) ^ (row & 7u), wave = uniform(threadIdx.x >> 6);
 		const uint32_t at = step * kStepBytes, apart = (uint32_t)pitch * kRowsOfRound;
 		const uint32_t place = (row * (uint32_t)pitch + chunk * 16) | (at + chunk * 16 < (uint32_t)bytes ? 0 : kBeyond);
-		const int left = rows ? (int)((rows - 1) * (uint32_t)pitch + (uint32_t)bytes) - (int)at : 0;
+		const int left = (int)((rows - 1) * (uint32_t)pitch + (uint32_t)bytes) - (int)at - (rows ? 0 : 0x40000000); /* no rows: nothing */
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
 			const int n = left - (int)(t * apart);
@@ -272,27 +323,47 @@ template <typename T, uint32_t W, uint32_t THREADS> struct across_t {
 	int64_t bytes;  /* of the columns there are, at most W's */
 	u32x4_t held[kChunks];
 
+	__device__ __forceinline__ void set(const uint8_t *p, uint64_t apart, uint32_t n, int64_t size)
+	{
+		base = p;
+		pitch = apart;
+		rows = n;
+		bytes = size;
+	}
 	__device__ __forceinline__ void load(uint32_t step)
 	{
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
 			const uint32_t slot = t * THREADS + threadIdx.x, k = slot / kOfRow, r = step * kStepRows + k;
-			const uint32_t chunk = (slot % kOfRow) ^ across_slot<W>(k);
-			held[t] = chunk_at<T>(base + (uint64_t)(r < rows ? r : 0) * pitch + chunk * 16, r < rows ? bytes - (int64_t)chunk * 16 : 0);
+			const int64_t at = (slot % kOfRow ^ across_slot<W>(k)) * 16;
+			const uint8_t *const p = base + (uint64_t)(r < rows ? r : rows - 1) * pitch;
+			held[t] = bytes >= 16 ? *reinterpret_cast<const any16_t *>(p + (at + 16 <= bytes ? at : bytes - 16)) : chunk_at<T>(p + at, bytes - at);
 		}
 	}
-	__device__ __forceinline__ void store(uint8_t *lds) const
+	__device__ __forceinline__ void store(uint32_t step, uint8_t *lds) const
 	{
+		const uint32_t over = (uint32_t)(16 - bytes % 16) % 16;
+		const bool some = over && bytes >= 16, rest = (step + 1) * kStepRows > rows;
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
-			*reinterpret_cast<u32x4_t *>(lds + (t * THREADS + threadIdx.x) * 16) = held[t];
+			const uint32_t slot = t * THREADS + threadIdx.x, k = slot / kOfRow, r = step * kStepRows + k;
+			u32x4_t v = held[t];
+			if (some) {
+				const int64_t at = (slot % kOfRow ^ across_slot<W>(k)) * 16;
+				const u32x4_t s = shifted(v, over);
+				v = at < bytes && at + 16 > bytes ? s : v;
+			}
+			if (rest) {
+				v = r < rows ? v : u32x4_t{ 0, 0, 0, 0 };
+			}
+			*reinterpret_cast<u32x4_t *>(lds + (t * THREADS + threadIdx.x) * 16) = v;
 		}
 	}
 	__device__ __forceinline__ void fill(uint32_t step, uint8_t *lds) const
 	{
 		constexpr uint32_t kRowsOfRound = THREADS / kOfRow;
 		const uint64_t at = (uint64_t)step * kStepRows * pitch;
-		const int64_t left = rows ? (int64_t)((rows - 1) * pitch + bytes - at) : 0;
+		const int64_t left = (int64_t)((rows - 1) * pitch + bytes - at) - (rows ? 0 : 1ll << 60); /* no rows: nothing */
 		const uint32_t apart = (uint32_t)pitch * kRowsOfRound, row = threadIdx.x / kOfRow, wave = uniform(threadIdx.x >> 6);
 		const int some = left <= 0 ? 0 : left < 0x7fffffff ? (int)left : 0x7fffffff;
 #pragma unroll
@@ -407,10 +478,10 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 			fill(s, lds + s * tile_bytes);
 		}
 		landed<(STAGES - 1) * FILLS>();
-		__syncthreads();
+		workgroup_meets<true>();
 	} else {
 		load(0);
-		store(lds);
+		store(0, lds);
 		__syncthreads();
 		load(1);
 	}
@@ -432,7 +503,7 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 			if (DIRECT) {
 				landed<(STAGES - 2) * FILLS>();
 			} else {
-				store(next);
+				store(step + 1, next);
 			}
 			workgroup_meets<DIRECT>();
 			if (DIRECT) {
@@ -460,69 +531,90 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 
 /* ---- sums ----------------------------------------------------------------------------------------------------- */
 
-/*
- * A tile's sums by rows: finish(row of the tile, columns of part 0, of part 1, what load(row) gave), eight neighbouring columns of both
- * parts in a lane, from column 8 (lane % 16) of the part on; a quarter of a wavefront has a row, so that what is read and written of
- * it is one piece, and a block of 128 columns is sixteen neighbouring lanes.  The sums go through LDS, half of the rows at a time, so that
- * one loop does for all of them (unrolled over the registers the same epilogue was 200 KB of instructions).  What is loaded is
- * asked for two turns ahead: a CU then has 64 KB of float32 on its way.
- */
-template <uint32_t WM, uint32_t WN, uint32_t MF, typename Load, typename Finish>
-__device__ __forceinline__ void for_rows(const f32x4_t (&sums)[MF][2][8 / WN], uint8_t *lds, Load load, Finish finish)
+/* The value, but not to be computed with outside of the loop: what would be there for every matrix that a loop might write takes the
+ * registers of a tile's sums */
+__device__ __forceinline__ uint32_t in_loop(uint32_t v)
 {
-	constexpr uint32_t G = 8 / WN, kOfWave = MF * 8; /* rows of half a wavefront's tile */
-	constexpr uint32_t kTurns = kOfWave / WN / 4;    /* of WM * kOfWave rows, four to each of WM * WN wavefronts */
-	constexpr uint32_t kAhead = kTurns < 2 ? 1 : 2;
+	asm volatile("" : "+v"(v));
+	return v;
+}
+
+/*
+ * A tile's sums by rows: finish(row of the tile, lane % 16, columns of part 0, of part 1, what load(row) gave), eight columns of both parts in a lane, a
+ * row in a quarter of a wavefront, so that what is read and written of it is one piece, and a block of 128 columns is sixteen
+ * neighbouring lanes.  They are columns 8 (lane % 16) on of the part, or with SPLIT 4 (lane % 16) and 64 + 4 (lane % 16) on, with which four
+ * bytes a column are whole lines.  The sums go through LDS, 64 rows of a tile of 256 at a time, so that one loop does for all of
+ * them (unrolled over the registers the same epilogue was 200 KB of instructions); what is loaded is asked for one such turn ahead.
+ * No barrier waits for what has been written.
+ * whole: all of the tile's rows and columns are there; load and finish get it as a constant and have no conditions then (with them, every
+ * eight values went through six branches: a tile of 256 x 256 with 1024 summed 40.4 us, without 37.4; 23 are the sums).
+ * One row after the other: two at once took the registers of the sums.
+ */
+template <uint32_t WM, uint32_t WN, uint32_t MF, bool SPLIT, typename Load, typename Finish>
+__device__ __forceinline__ void for_rows(const f32x4_t (&sums)[MF][2][8 / WN], uint8_t *lds, bool whole, Load load, Finish finish)
+{
+	static_assert(MF == 4, "four groups of rows");
+	constexpr uint32_t G = 8 / WN, kGroups = WM == 4 ? 1 : 2; /* groups of 16 rows of a wavefront in a turn */
+	constexpr uint32_t kRows = kGroups * 16, kLoops = 4 / kGroups, kTurns = kRows / WN / 4;
 	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-#pragma unroll 1
-	for (uint32_t half = 0; half < 2; half++) {
-		auto place = [&](uint32_t turn) { return (wave * kTurns + turn) * 4 + (lane >> 4); };
-		auto row_of = [&](uint32_t at) { return at / kOfWave * 2 * kOfWave + half * kOfWave + at % kOfWave; };
-		decltype(load(0u)) in[kAhead];
+	auto place = [&](uint32_t turn) { return (wave * kTurns + turn) * 4 + (lane >> 4); };
+	auto row_of = [&](uint32_t loop, uint32_t at) { return at / kRows * 64 + loop * kRows + at % kRows; };
+	using in_t = decltype(load(std::true_type{}, 0u, 0u));
+	in_t in[kTurns];
+	auto load_all = [&](uint32_t loop) __attribute__((always_inline)) {
 #pragma unroll
-		for (uint32_t i = 0; i < kAhead; i++) {
-			in[i] = load(row_of(place(i)));
+		for (uint32_t i = 0; i < kTurns; i++) {
+			const uint32_t part_lane = in_loop(lane & 15u);
+			in[i] = whole ? load(std::true_type{}, row_of(loop, place(i)), part_lane) : load(std::false_type{}, row_of(loop, place(i)), part_lane);
 		}
-		__syncthreads(); /* the tiles, or the half before, have been read */
-		auto put = [&](uint32_t m, const f32x4_t(&from)[2][G]) __attribute__((always_inline)) {
-			const uint32_t r = wm * kOfWave + m * 16 + (lane & 15u);
+	};
+	load_all(0);
+	auto put = [&](uint32_t m, const f32x4_t(&from)[2][G]) __attribute__((always_inline)) {
+		const uint32_t r = wm * kRows + m * 16 + (lane & 15u);
 #pragma unroll
-			for (uint32_t p = 0; p < 2; p++) {
+		for (uint32_t p = 0; p < 2; p++) {
 #pragma unroll
-				for (uint32_t j = 0; j < G; j++) {
-					const uint32_t chunk = p * 32 + (wn * G + j) * 4 + (lane >> 4);
-					*reinterpret_cast<f32x4_t *>(lds + r * 1024 + ((chunk ^ (r & 15u)) << 4)) = from[p][j];
-				}
+			for (uint32_t j = 0; j < G; j++) {
+				const uint32_t chunk = p * 32 + (wn * G + j) * 4 + (lane >> 4);
+				*reinterpret_cast<f32x4_t *>(lds + r * 1024 + ((chunk ^ (r & 15u)) << 4)) = from[p][j];
 			}
-		};
-		if (half == 0) {
-#pragma unroll
-			for (uint32_t m = 0; m < MF / 2; m++) {
-				put(m, sums[m]);
+		}
+	};
+#pragma unroll 1
+	for (uint32_t loop = 0; loop < kLoops; loop++) {
+		workgroup_meets<true>(); /* the tiles, or the rows before, have been read */
+		if (kGroups == 1) {
+			switch (loop) {
+			case 0: put(0, sums[0]); break;
+			case 1: put(0, sums[1]); break;
+			case 2: put(0, sums[2]); break;
+			default: put(0, sums[3]);
 			}
+		} else if (loop == 0) {
+			put(0, sums[0]);
+			put(1, sums[1]);
 		} else {
-#pragma unroll
-			for (uint32_t m = 0; m < MF / 2; m++) {
-				put(m, sums[MF / 2 + m]);
-			}
+			put(0, sums[2]);
+			put(1, sums[3]);
 		}
-		__syncthreads();
-#pragma unroll 1
-		for (uint32_t turn = 0; turn < kTurns; turn += kAhead) {
+		workgroup_meets<true>();
 #pragma unroll
-			for (uint32_t i = 0; i < kAhead; i++) {
-				const uint32_t at = place(turn + i);
-				const auto now = in[i];
-				if (turn + i + kAhead < kTurns) {
-					in[i] = load(row_of(place(turn + i + kAhead)));
-				}
-				const uint8_t *const from = lds + at * 1024;
-				const uint32_t swizzle = at & 15u, chunk = (lane & 15u) * 2;
-				auto get = [&](uint32_t c) { return *reinterpret_cast<const f32x4_t *>(from + ((c ^ swizzle) << 4)); };
-				const f32x4_t a0 = get(chunk), a1 = get(chunk + 1), b0 = get(chunk + 32), b1 = get(chunk + 33);
-				finish(row_of(at), __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7),
-				       __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7), now);
+		for (uint32_t i = 0; i < kTurns; i++) {
+			const uint32_t at = place(i);
+			const uint8_t *const from = lds + at * 1024;
+			const uint32_t swizzle = at & 15u, chunk = SPLIT ? lane & 15u : (lane & 15u) * 2, other = SPLIT ? chunk + 16 : chunk + 1;
+			auto get = [&](uint32_t c) { return *reinterpret_cast<const f32x4_t *>(from + ((c ^ swizzle) << 4)); };
+			const f32x4_t a0 = get(chunk), a1 = get(other), b0 = get(chunk + 32), b1 = get(other + 32);
+			const f32x8_t a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+			if (whole) {
+				finish(std::true_type{}, row_of(loop, at), in_loop(lane & 15u), a, b, in[i]);
+			} else {
+				finish(std::false_type{}, row_of(loop, at), in_loop(lane & 15u), a, b, in[i]);
 			}
+			__builtin_amdgcn_sched_barrier(0);
+		}
+		if (loop + 1 < kLoops) {
+			load_all(loop + 1);
 		}
 	}
 }
@@ -614,30 +706,75 @@ template <typename T> __device__ __forceinline__ void write_as(uint8_t *p, uint3
 	}
 }
 
-__device__ __forceinline__ void write_values(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, f32x8_t v)
+/* Four values of a row of 16 bits or float32, of which `left` are there: zeros for the others */
+template <typename T> __device__ __forceinline__ f32x4_t four_at(const uint8_t *p, uint32_t left)
 {
-	uint8_t *const p = m.p + row * m.pitch;
-	switch (m.type) {
-	case OFI_AMD_BFLOAT16: write_as<bf16_t>(p + column * 2, left, v); break;
-	case OFI_AMD_FLOAT16: write_as<f16_t>(p + column * 2, left, v); break;
-	default: write_as<float>(p + column * 4, left, v);
+	raw_t<T, 4> r = {};
+	if (left >= 4) {
+		r = *reinterpret_cast<const typename piece_t<T, 4>::anywhere *>(p);
+	} else {
+#pragma unroll
+		for (uint32_t i = 0; i < 3; i++) {
+			if (i < left) {
+				r[i] = reinterpret_cast<const T *>(p)[i];
+			}
+		}
+	}
+	return __builtin_convertvector(r, f32x4_t);
+}
+__device__ __forceinline__ f32x4_t read_four(int type, const uint8_t *p, uint64_t column, uint32_t left)
+{
+	switch (type) {
+	case OFI_AMD_BFLOAT16: return four_at<bf16_t>(p + column * 2, left);
+	case OFI_AMD_FLOAT16: return four_at<f16_t>(p + column * 2, left);
+	default: return four_at<float>(p + column * 4, left);
+	}
+}
+template <typename T> __device__ __forceinline__ void write_four_as(uint8_t *p, uint32_t left, f32x4_t v)
+{
+	const auto r = __builtin_convertvector(v, raw_t<T, 4>);
+	if (left >= 4) {
+		*reinterpret_cast<typename piece_t<T, 4>::anywhere *>(p) = r;
+	} else {
+#pragma unroll
+		for (uint32_t i = 0; i < 3; i++) {
+			if (i < left) {
+				reinterpret_cast<T *>(p)[i] = r[i];
+			}
+		}
+	}
+}
+__device__ __forceinline__ void write_four(int type, uint8_t *p, uint64_t column, uint32_t left, f32x4_t v)
+{
+	switch (type) {
+	case OFI_AMD_BFLOAT16: write_four_as<bf16_t>(p + column * 2, left, v); break;
+	case OFI_AMD_FLOAT16: write_four_as<f16_t>(p + column * 2, left, v); break;
+	default: write_four_as<float>(p + column * 4, left, v);
 	}
 }
 
-/* A block of 128 columns of a row, which sixteen lanes hold: values divided by their scale as the norms divide them (with a
- * division's rounding, then rounded to e4m3), and the scale.  All sixteen call; `write`: whether the row is there. */
-__device__ __forceinline__ void write_block(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block, f32x8_t v, bool write)
+/* Eight columns of the row that is `row` behind `from`, if it is one of the rows there are, as far as columns are left; WHOLE: both are */
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void write_row_as(const matrix_t &m, uint64_t from, uint64_t column, uint32_t row, uint32_t rows, uint32_t left, f32x8_t v)
+{
+	if (WHOLE || (row < rows && left)) {
+		write_as<T>(m.p + from * m.pitch + column * sizeof(T) + row * m.pitch, WHOLE ? 8 : left, v);
+	}
+}
+
+/* A block of 128 columns of a row, which sixteen lanes hold: values divided by their scale as the norms divide them (with a division's
+ * rounding, then rounded to e4m3), and the scale.  All sixteen call. */
+template <bool WHOLE>
+__device__ __forceinline__ void write_block(const matrix_t &m, uint64_t from, uint64_t column, uint32_t block, uint32_t row, uint32_t rows, uint32_t left,
+					    f32x8_t v)
 {
 	uint32_t most = 0;
 #pragma unroll
 	for (uint32_t i = 0; i < 8; i++) {
-		const uint32_t bits = i < left ? abs_bits(v[i]) : 0u;
+		const uint32_t bits = WHOLE || i < left ? abs_bits(v[i]) : 0u;
 		most = bits > most ? bits : most;
 	}
 	const float scale = scale_of(max_bits_over<16>(most));
-	if (!write || left == 0) {
-		return;
-	}
 	const divisor_t by = divisor_of(scale);
 	typedef uint32_t any8_t __attribute__((ext_vector_type(2), aligned(1)));
 	any8_t w;
@@ -646,29 +783,35 @@ __device__ __forceinline__ void write_block(const matrix_t &m, uint64_t row, uin
 		const int low = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[4 * i], by), quotient(v[4 * i + 1], by), 0, false);
 		w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[4 * i + 2], by), quotient(v[4 * i + 3], by), low, true);
 	}
-	if ((threadIdx.x & 15u) == 0) {
-		row_at(m.scale, m.scale_pitch, row)[block] = scale;
-	}
-	uint8_t *const p = m.p + row * m.pitch + column;
-	if (left >= 8) {
-		*reinterpret_cast<any8_t *>(p) = w;
-	} else {
+	if (WHOLE || (row < rows && left)) {
+		if ((threadIdx.x & 15u) == 0) {
+			row_at(m.scale, m.scale_pitch, from + row)[block] = scale;
+		}
+		uint8_t *const at = m.p + from * m.pitch + column + row * m.pitch;
+		if (WHOLE || left >= 8) {
+			*reinterpret_cast<any8_t *>(at) = w;
+		} else {
 #pragma unroll
-		for (uint32_t i = 0; i < 7; i++) {
-			if (i < left) {
-				p[i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+			for (uint32_t i = 0; i < 7; i++) {
+				if (i < left) {
+					at[i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+				}
 			}
 		}
 	}
 }
 
-/* As e4m3 with the block's scale, or in 16 bits */
-__device__ __forceinline__ void write_any(const matrix_t &m, uint64_t row, uint64_t column, uint32_t left, uint32_t block, f32x8_t v, bool write)
+/* block: that of the columns */
+template <bool WHOLE>
+__device__ __forceinline__ void write_row(const matrix_t &m, uint64_t from, uint64_t column, uint32_t block, uint32_t row, uint32_t rows, uint32_t left,
+					  f32x8_t v)
 {
 	if (m.type == OFI_AMD_E4M3) {
-		write_block(m, row, column, left, block, v, write);
-	} else if (write && left) {
-		write_values(m, row, column, left, v);
+		write_block<WHOLE>(m, from, column, block, row, rows, left, v);
+	} else if (m.type == OFI_AMD_BFLOAT16) {
+		write_row_as<WHOLE, bf16_t>(m, from, column, row, rows, left, v);
+	} else {
+		write_row_as<WHOLE, f16_t>(m, from, column, row, rows, left, v);
 	}
 }
 

@@ -8,7 +8,12 @@
 namespace ofi_amd {
 namespace {
 
-struct weight_grad_t {
+struct weight_grad_args_t {
+	const int32_t *offset;
+	const uint8_t *dout, *x;
+	uint64_t dout_pitch, x_pitch;
+	uint32_t max_rows, m, n; /* rows of the result are dout's columns, m of them; its columns are x's */
+	uint32_t n_experts, m_tiles, n_tiles, first_tile;
 	matrix_t add, out;
 	uint64_t expert_pitch; /* of both */
 	const float *bias_add;
@@ -18,69 +23,85 @@ struct weight_grad_t {
 template <typename T> constexpr uint32_t kTwoOnes = 0x3f803f80u; /* bfloat16 */
 template <> constexpr uint32_t kTwoOnes<f16_t> = 0x3c003c00u;
 
-/* rows of the result: m (dout's columns); columns: n (x's) */
-template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT>
-__global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const int32_t *offset, const uint8_t *dout, const uint8_t *x,
-									  uint32_t max_rows, uint32_t m_width, uint32_t n_width,
-									  uint32_t m_tiles, uint32_t n_tiles, uint32_t tiles, uint32_t first_tile,
-									  uint64_t dout_pitch, uint64_t x_pitch, weight_grad_t o)
-{
-	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
-	using rows_tile = across_t<T, BM, THREADS>;
-	using columns_tile = across_t<T, BN, THREADS>;
-	constexpr uint32_t kTile = rows_tile::kBytes + columns_tile::kBytes, kFills = rows_tile::kChunks + columns_tile::kChunks;
-	constexpr uint32_t kStages = DIRECT && WM < 4 ? 3 : 2;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * kTile];
+/* A tile, the same for all lanes */
+struct weight_tile_t {
+	uint32_t expert, m0, n0, m_there, n_there, summed;
+	bool bias; /* of one column tile, in a loop of its own */
+};
 
-	/* an eighth of the tiles in one piece for each XCD; in an expert, bands of eight row tiles */
-	const uint32_t id = first_tile + blockIdx.x, share = (tiles + 7) / 8, at = (id & 7u) * share + (id >> 3);
-	if ((id >> 3) >= share || at >= tiles) {
-		return;
+template <typename T, uint32_t BM, uint32_t THREADS> struct weight_operands_t {
+	static constexpr uint32_t BN = 2 * kBlock;
+	across_t<T, BM, THREADS> rows;
+	across_t<T, BN, THREADS> columns;
+	weight_tile_t place;
+	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kBytes = kRowsBytes + decltype(columns)::kBytes;
+	static constexpr uint32_t kFills = decltype(rows)::kChunks + decltype(columns)::kChunks;
+
+	/* Workgroups go to the eight XCDs in turn: each XCD has an eighth of every expert's tiles, in one piece, as the experts have unlike numbers of
+	 * rows to sum (with whole experts to an XCD 2003 us for 32,768 rows of 32 experts).  In an expert, bands of eight row tiles.  False: `id` has none */
+	__device__ __forceinline__ bool set(const weight_grad_args_t *a, uint32_t id)
+	{
+		const uint32_t n_tiles = a->n_tiles, m_tiles = a->m_tiles, share = (m_tiles * n_tiles + 7) / 8, at = id >> 3, expert = at / share;
+		const uint32_t in_expert = (id & 7u) * share + at - expert * share;
+		if (expert >= a->n_experts || in_expert >= m_tiles * n_tiles) {
+			return false;
+		}
+		const uint32_t band = in_expert / (8 * n_tiles), in_band = in_expert - band * 8 * n_tiles;
+		const uint32_t height = m_tiles - band * 8 < 8 ? m_tiles - band * 8 : 8, nt = in_band / height;
+		const uint32_t m0 = (band * 8 + in_band - nt * height) * BM, n0 = nt * BN;
+		uint32_t lo, hi;
+		run_of(a->offset, expert, a->max_rows, lo, hi);
+		lo = uniform(lo);
+		hi = uniform(hi);
+		place = { expert, m0, n0, a->m - m0 < BM ? a->m - m0 : BM, a->n - n0 < BN ? a->n - n0 : BN, hi - lo, a->dbias && n0 == 0 };
+		rows.set(a->dout + lo * a->dout_pitch + m0 * 2, a->dout_pitch, hi - lo, (int64_t)place.m_there * 2);
+		columns.set(a->x + lo * a->x_pitch + n0 * 2, a->x_pitch, hi - lo, (int64_t)place.n_there * 2);
+		return true;
 	}
-	const uint32_t expert = at / (m_tiles * n_tiles), in_expert = at % (m_tiles * n_tiles);
-	const uint32_t band = in_expert / (8 * n_tiles), in_band = in_expert - band * 8 * n_tiles;
-	const uint32_t height = m_tiles - band * 8 < 8 ? m_tiles - band * 8 : 8;
-	const uint32_t m0 = (band * 8 + in_band % height) * BM, n0 = in_band / height * BN;
-	uint32_t lo, hi;
-	run_of(offset, expert, max_rows, lo, hi);
-	lo = uniform(lo);
-	hi = uniform(hi);
+	__device__ __forceinline__ void load(uint32_t step)
+	{
+		rows.load(step);
+		columns.load(step);
+	}
+	__device__ __forceinline__ void store(uint32_t step, uint8_t *to) const
+	{
+		rows.store(step, to);
+		columns.store(step, to + kRowsBytes);
+	}
+	__device__ __forceinline__ void fill(uint32_t step, uint8_t *to) const
+	{
+		rows.fill(step, to);
+		columns.fill(step, to + kRowsBytes);
+	}
+};
 
-	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-	const uint32_t m_there = m_width - m0 < BM ? m_width - m0 : BM, n_there = n_width - n0 < BN ? n_width - n0 : BN;
-	rows_tile rows = { dout + lo * dout_pitch + m0 * 2, dout_pitch, hi - lo, (int64_t)m_there * 2 };
-	columns_tile columns = { x + lo * x_pitch + n0 * 2, x_pitch, hi - lo, (int64_t)n_there * 2 };
-	const bool with_bias = o.dbias && n0 == 0; /* of one column tile, in a loop of its own */
+template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT>
+__global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(weight_grad_args_t)
+{
+	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN, kStages = 2;
+	using operands_t = weight_operands_t<T, BM, THREADS>;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * operands_t::kBytes];
 
-	f32x4_t sums[MF][2][G], bias[MF];
-#pragma unroll
-	for (int m = 0; m < (int)MF; m++) {
-		bias[m] = f32x4_t{ 0, 0, 0, 0 };
-#pragma unroll
-		for (int j = 0; j < (int)(2 * G); j++) {
-			sums[m][j / G][j % G] = f32x4_t{ 0, 0, 0, 0 };
+	operands_t of;
+	{
+		const weight_grad_args_t *const a = argument<weight_grad_args_t>();
+		if (!of.set(a, a->first_tile + blockIdx.x)) {
+			return;
 		}
 	}
-	const across_frag_t<BM> row_frag(wm * 16 * MF, lane);
-	const across_frag_t<BN> column_frag(wn * 16 * G, lane);
+	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+	const weight_tile_t place = of.place;
+	f32x4_t sums[MF][2][G] = {};
 	auto sum = [&](auto also) __attribute__((always_inline)) {
-		sum_steps<T, DIRECT, kStages, kFills>(
-			sums, wm * 16 * MF < m_there, (hi - lo + kStepRows - 1) / kStepRows, lds, kTile, rows_tile::kBytes, row_frag, column_frag,
-			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) {
-				rows.fill(step, to);
-				columns.fill(step, to + rows_tile::kBytes);
-			},
-			[&](uint32_t step) __attribute__((always_inline)) {
-				rows.load(step);
-				columns.load(step);
-			},
-			[&](uint8_t *to) __attribute__((always_inline)) {
-				rows.store(to);
-				columns.store(to + rows_tile::kBytes);
-			},
-			also);
+		sum_steps<T, DIRECT, kStages, operands_t::kFills>(
+			sums, wm * 16 * MF < place.m_there, (place.summed + kStepRows - 1) / kStepRows, lds, operands_t::kBytes, operands_t::kRowsBytes,
+			across_frag_t<BM>(wm * 16 * MF, lane), across_frag_t<BN>(wn * 16 * G, lane),
+			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.fill(step, to); },
+			[&](uint32_t step) __attribute__((always_inline)) { of.load(step); },
+			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.store(step, to); }, also);
 	};
-	if (with_bias) {
+	if (place.bias) {
+		f32x4_t bias[MF] = {};
 		sum([&](const u32x4_t(&r)[MF]) __attribute__((always_inline)) {
 			const u32x4_t ones = { kTwoOnes<T>, kTwoOnes<T>, kTwoOnes<T>, kTwoOnes<T> };
 #pragma unroll
@@ -88,54 +109,52 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(const 
 				bias[m] = multiply<T>(ones, r[m], bias[m]);
 			}
 		});
+		const weight_grad_args_t *const a = argument<weight_grad_args_t>();
+		if (wn == 0 && lane < 16) {
+#pragma unroll
+			for (int m = 0; m < (int)MF; m++) {
+				const uint32_t r = (wm * MF + m) * 16 + lane;
+				if (r < place.m_there) {
+					const uint64_t i = (uint64_t)place.expert * a->m + place.m0 + r;
+					a->dbias[i] = bias[m][0] + (a->bias_add ? a->bias_add[i] : 0.0f);
+				}
+			}
+		}
 	} else {
 		sum([](const u32x4_t(&)[MF]) {});
 	}
 
-	if (with_bias && wn == 0 && lane < 16) {
-#pragma unroll
-		for (int m = 0; m < (int)MF; m++) {
-			const uint32_t r = (wm * MF + m) * 16 + lane;
-			if (r < m_there) {
-				const uint64_t i = (uint64_t)expert * m_width + m0 + r;
-				o.dbias[i] = bias[m][0] + (o.bias_add ? o.bias_add[i] : 0.0f);
-			}
-		}
-	}
-	const matrix_t out = { o.out.p + expert * o.expert_pitch, o.out.pitch, o.out.type, nullptr, 0 };
-	const matrix_t add = { o.add.p ? o.add.p + expert * o.expert_pitch : nullptr, o.add.pitch, o.add.type, nullptr, 0 };
-	const uint32_t c = (lane & 15u) * 8;
-	const uint32_t left[2] = { c < n_there ? n_there - c : 0, c + kBlock < n_there ? n_there - c - kBlock : 0 };
 	struct in_t {
-		f32x8_t was[2]; /* float32, or eight values of 16 bits */
+		f32x4_t was[4];
 	};
-	for_rows<WM, WN, MF>(
-		sums, lds,
-		[&](uint32_t r) {
+	auto left = [&](uint32_t column) { return column < place.n_there ? place.n_there - column : 0u; };
+	/* a lane's columns of each part: four, and four 64 further */
+	for_rows<WM, WN, MF, true>(
+		sums, lds, place.m_there == BM && place.n_there == BN,
+		[&](auto all, uint32_t r, uint32_t part_lane) __attribute__((always_inline)) {
+			constexpr bool WHOLE = decltype(all)::value;
+			const weight_grad_args_t *const a = argument<weight_grad_args_t>();
+			const uint32_t c = part_lane * 4;
 			in_t in = {};
+			if (a->add.p && (WHOLE || r < place.m_there)) {
+				const uint8_t *const p = a->add.p + place.expert * a->expert_pitch + (uint64_t)(place.m0 + r) * a->add.pitch;
 #pragma unroll
-			for (int p = 0; p < 2; p++) {
-				if (add.p && r < m_there && left[p]) {
-					const uint64_t column = n0 + p * kBlock + c;
-					if (add.type == OFI_AMD_FLOAT32) {
-						in.was[p] = read_floats(add.p + (m0 + r) * add.pitch + column * 4, left[p]);
-					} else {
-						in.was[p].lo = __builtin_bit_cast(f32x4_t, load_eight(add, m0 + r, column, left[p], 0).words);
-					}
+				for (uint32_t i = 0; i < 4; i++) {
+					in.was[i] = read_four(a->add.type, p, place.n0 + i * 64 + c, WHOLE ? 4 : left(i * 64 + c));
 				}
 			}
 			return in;
 		},
-		[&](uint32_t r, f32x8_t a, f32x8_t b, const in_t &in) {
+		[&](auto all, uint32_t r, uint32_t part_lane, f32x8_t p0, f32x8_t p1, const in_t &in) __attribute__((always_inline)) {
+			constexpr bool WHOLE = decltype(all)::value;
+			const weight_grad_args_t *const a = argument<weight_grad_args_t>();
+			const uint32_t c = part_lane * 4;
+			if (WHOLE || r < place.m_there) {
+				uint8_t *const p = a->out.p + place.expert * a->expert_pitch + (uint64_t)(place.m0 + r) * a->out.pitch;
 #pragma unroll
-			for (int p = 0; p < 2; p++) {
-				f32x8_t v = p ? b : a;
-				if (r < m_there && left[p]) {
-					if (add.p) {
-						const f32x4_t low = in.was[p].lo;
-						v += add.type == OFI_AMD_FLOAT32 ? in.was[p] : floats_of<T>(__builtin_bit_cast(u32x4_t, low));
-					}
-					write_values(out, m0 + r, n0 + p * kBlock + c, left[p], v);
+				for (uint32_t i = 0; i < 4; i++) {
+					const f32x4_t v = i == 0 ? p0.lo : i == 1 ? p0.hi : i == 2 ? p1.lo : p1.hi;
+					write_four(a->out.type, p, place.n0 + i * 64 + c, WHOLE ? 4 : left(i * 64 + c), v + in.was[i]);
 				}
 			}
 		});
@@ -171,29 +190,26 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	    (reinterpret_cast<uintptr_t>(d_add) % size) || ((reinterpret_cast<uintptr_t>(d_dbias) | reinterpret_cast<uintptr_t>(d_bias_add)) & 3u)) {
 		return -EINVAL;
 	}
-	/* tiles of 256 x 256 where they are enough for the GPU, else of 128 x 256 */
+	/* tiles of 256 x 256 where they are enough for the GPU and the experts have rows to sum, else of 128 x 256 */
 	const uint32_t n_tiles = (width + 255) / 256;
 	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * out_width) && in_chunks(d_rows, rows_pitch, 2ull * width);
-	const bool wide = direct && (uint64_t)n_experts * ((out_width + 255) / 256) * n_tiles >= 256;
+	const bool wide = direct && (uint64_t)n_experts * ((out_width + 255) / 256) * n_tiles >= kComputeUnits;
 	const uint32_t bm = wide ? 256 : 128, m_tiles = (out_width + bm - 1) / bm;
-	const uint64_t tiles = (uint64_t)n_experts * m_tiles * n_tiles;
+	const uint64_t tiles = (uint64_t)n_experts * (((uint64_t)m_tiles * n_tiles + 7) / 8) * 8;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
-	weight_grad_t o = {};
-	o.out = { static_cast<uint8_t *>(d_dweight), dweight_pitch, dweight_type, nullptr, 0 };
-	o.add = { static_cast<uint8_t *>(const_cast<void *>(d_add)), dweight_pitch, dweight_type, nullptr, 0 };
-	o.expert_pitch = expert_pitch;
-	o.bias_add = d_bias_add;
-	o.dbias = d_dbias;
+	const matrix_t out = { static_cast<uint8_t *>(d_dweight), dweight_pitch, dweight_type, nullptr, 0 };
+	const matrix_t add = { static_cast<uint8_t *>(const_cast<void *>(d_add)), dweight_pitch, dweight_type, nullptr, 0 };
+	weight_grad_args_t args = { d_offset, static_cast<const uint8_t *>(d_dout), static_cast<const uint8_t *>(d_rows), dout_pitch, rows_pitch, max_rows,
+				    out_width, width, n_experts, m_tiles, n_tiles, 0, add, out, expert_pitch, d_bias_add, d_dbias };
 	auto with = [&](auto element) {
 		using T = decltype(element);
 		auto kernel = direct ? (wide ? expert_weight_grad_kernel<T, 4, 2, 4, true> : expert_weight_grad_kernel<T, 2, 4, 4, true>)
 				     : expert_weight_grad_kernel<T, 2, 4, 4, false>;
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
-			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), d_offset, static_cast<const uint8_t *>(d_dout),
-				      static_cast<const uint8_t *>(d_rows), max_rows, out_width, width, m_tiles, n_tiles, (uint32_t)tiles, first,
-				      dout_pitch, rows_pitch, o);
+			args.first_tile = first;
+			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {
