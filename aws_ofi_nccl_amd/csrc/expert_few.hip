@@ -22,9 +22,7 @@ __global__ __launch_bounds__(64 * CG * KS, MB == 1 ? 4 : 2) void expert_few_kern
 	constexpr bool SCALED = sizeof(T) == 1;
 	__shared__ __attribute__((aligned(16))) float part[KS][BM][2][PART];
 
-	__shared__ uint32_t known[4][64];
-	const rows_t of = { offset, n_experts, max_rows, n_tiles };
-	const tile_t tile = find_tile<BM>(of, count_tiles<BM>(of, known), first_tile + blockIdx.x, known);
+	const tile_t tile = find_tile<BM>({ offset, n_experts, max_rows, n_tiles }, first_tile + blockIdx.x);
 	if (!tile.any) {
 		return;
 	}

@@ -70,14 +70,13 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(backward_
 	using operands_t = backward_operands_t<T, BM, THREADS>;
 	constexpr uint32_t kStages = DIRECT && WM < 4 ? 3 : 2;
 	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * operands_t::kBytes];
-	__shared__ uint32_t known[4][64];
 
 	operands_t of;
 	uint32_t steps;
 	{
 		const backward_args_t *const a = argument<backward_args_t>();
 		steps = (a->k + kStepRows - 1) / kStepRows;
-		const tile_t tile = find_tile<BM>(a->of, count_tiles<BM>(a->of, known), a->first_tile + blockIdx.x, known);
+		const tile_t tile = find_tile<BM>(a->of, a->first_tile + blockIdx.x);
 		if (!tile.any) {
 			return;
 		}

@@ -82,67 +82,61 @@ __device__ __forceinline__ uint32_t running_sum(uint32_t v, uint32_t lane)
  * The tiles of a launch.  They are numbered expert by expert, an expert's in bands of eight row tiles, a band's column by column: what an
  * XCD's 32 compute units work on at once is about eight row tiles by four column tiles, which its L2 holds a step of.  Workgroups go to
  * the eight XCDs in turn, so each XCD gets an eighth of the numbers in one piece.  Each lane has one of 64 experts.
- * All wavefronts of the workgroup call.
  */
 struct rows_t {
 	const int32_t *offset;
 	uint32_t n_experts, max_rows, n_tiles;
 };
 
-/* Experts e to e + 63, behind `before` row tiles: the row tiles behind them.  What the lanes found is kept in four words of each in LDS, so
- * that it holds no registers meanwhile; every wavefront keeps the same words. */
-template <uint32_t BM> __device__ __forceinline__ uint32_t look_at_experts(rows_t rows, uint32_t e, uint32_t before, uint32_t (*kept)[64])
+/* Of one of 64 experts, in a lane: its rows, its row tiles, and those of the experts before it */
+struct seen_t {
+	uint32_t lo, hi, mine, before;
+};
+
+/* Experts e to e + 63, behind `before` row tiles, which is then all up to them */
+template <uint32_t BM> __device__ __forceinline__ seen_t look_at_experts(rows_t rows, uint32_t e, uint32_t &before)
 {
 	const uint32_t lane = threadIdx.x & 63u;
-	uint32_t lo = 0, hi = 0;
+	seen_t s = {};
 	if (e + lane < rows.n_experts) {
-		run_of(rows.offset, e + lane, rows.max_rows, lo, hi);
+		run_of(rows.offset, e + lane, rows.max_rows, s.lo, s.hi);
 	}
-	const uint32_t mine = (hi - lo + BM - 1) / BM, sum = running_sum(mine, lane);
-	kept[0][lane] = lo;
-	kept[1][lane] = hi;
-	kept[2][lane] = mine;
-	kept[3][lane] = before + sum - mine;
-	return before + (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
-}
-
-/* The row tiles of all experts */
-template <uint32_t BM> __device__ __forceinline__ uint32_t count_tiles(rows_t rows, uint32_t (*kept)[64])
-{
-	uint32_t total = 0;
-	for (uint32_t e = 0; e < rows.n_experts; e += 64) {
-		total = look_at_experts<BM>(rows, e, total, kept);
-	}
-	return total;
+	s.mine = (s.hi - s.lo + BM - 1) / BM;
+	const uint32_t sum = running_sum(s.mine, lane);
+	s.before = before + sum - s.mine;
+	before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+	return s;
 }
 
 /* The tile of workgroup `id` */
-template <uint32_t BM> __device__ __forceinline__ tile_t find_tile(rows_t rows, uint32_t total, uint32_t id, uint32_t (*kept)[64])
+template <uint32_t BM> __device__ __forceinline__ tile_t find_tile(rows_t rows, uint32_t id)
 {
 	tile_t t = {};
+	uint32_t total = 0, first = 0;
+	seen_t seen = look_at_experts<BM>(rows, 0, total);
+	for (uint32_t e = 64; e < rows.n_experts; e += 64) {
+		(void)look_at_experts<BM>(rows, e, total);
+	}
 	const uint32_t n_tiles = rows.n_tiles, tiles = total * n_tiles, share = (tiles + 7) / 8;
 	uint32_t at = uniform((id & 7u) * share + (id >> 3));
 	if ((id >> 3) >= share || at >= tiles) {
 		return t;
 	}
-	uint32_t first = 0;
-	if (rows.n_experts > 64) { /* the words are of others: again, up to the one that has the tile */
-		__syncthreads();   /* which no wavefront still needs */
-		uint32_t seen = look_at_experts<BM>(rows, 0, 0, kept);
-		while (first + 64 < rows.n_experts && at >= seen * n_tiles) {
-			first += 64;
-			seen = look_at_experts<BM>(rows, first, seen, kept);
+	if (rows.n_experts > 64) { /* again, up to the expert that has the tile */
+		uint32_t before = 0;
+		for (uint32_t e = 0; e < rows.n_experts && at >= before * n_tiles; e += 64) {
+			first = e;
+			seen = look_at_experts<BM>(rows, e, before);
 		}
 	}
-	const uint32_t lane = threadIdx.x & 63u, lo = kept[0][lane], hi = kept[1][lane], mine = kept[2][lane], before = kept[3][lane];
-	const uint64_t has = __ballot(mine != 0 && at >= before * n_tiles && at < (before + mine) * n_tiles);
+	const uint64_t has = __ballot(seen.mine != 0 && at >= seen.before * n_tiles && at < (seen.before + seen.mine) * n_tiles);
 	if (!has) {
 		return t;
 	}
 	const int who = (int)__builtin_ctzll(has);
-	const uint32_t begin = (uint32_t)__builtin_amdgcn_readlane((int)lo, who), end = (uint32_t)__builtin_amdgcn_readlane((int)hi, who);
-	const uint32_t row_tiles = (uint32_t)__builtin_amdgcn_readlane((int)mine, who);
-	at -= (uint32_t)__builtin_amdgcn_readlane((int)before, who) * n_tiles;
+	const uint32_t begin = (uint32_t)__builtin_amdgcn_readlane((int)seen.lo, who), end = (uint32_t)__builtin_amdgcn_readlane((int)seen.hi, who);
+	const uint32_t row_tiles = (uint32_t)__builtin_amdgcn_readlane((int)seen.mine, who);
+	at -= (uint32_t)__builtin_amdgcn_readlane((int)seen.before, who) * n_tiles;
 	const uint32_t band = at / (8 * n_tiles), in_band = at - band * 8 * n_tiles;
 	const uint32_t height = row_tiles - band * 8 < 8 ? row_tiles - band * 8 : 8;
 	t.expert = first + (uint32_t)who;
