@@ -554,15 +554,11 @@ __device__ __forceinline__ void for_rows(const f32x4_t (&sums)[MF][2][8 / WN], u
 	auto place = [&](uint32_t turn) { return (wave * kTurns + turn) * 4 + (lane >> 4); };
 	auto row_of = [&](uint32_t loop, uint32_t at) { return at / kRows * 64 + loop * kRows + at % kRows; };
 	using in_t = decltype(load(std::true_type{}, 0u, 0u));
-	in_t in[kTurns];
-	auto load_all = [&](uint32_t loop) __attribute__((always_inline)) {
-#pragma unroll
-		for (uint32_t i = 0; i < kTurns; i++) {
-			const uint32_t part_lane = in_loop(lane & 15u);
-			in[i] = whole ? load(std::true_type{}, row_of(loop, place(i)), part_lane) : load(std::false_type{}, row_of(loop, place(i)), part_lane);
-		}
+	auto ask = [&](uint32_t loop, uint32_t turn) __attribute__((always_inline)) {
+		const uint32_t r = row_of(loop, place(turn)), part_lane = in_loop(lane & 15u);
+		return whole ? load(std::true_type{}, r, part_lane) : load(std::false_type{}, r, part_lane);
 	};
-	load_all(0);
+	in_t in = ask(0, 0);
 	auto put = [&](uint32_t m, const f32x4_t(&from)[2][G]) __attribute__((always_inline)) {
 		const uint32_t r = wm * kRows + m * 16 + (lane & 15u);
 #pragma unroll
@@ -600,15 +596,18 @@ __device__ __forceinline__ void for_rows(const f32x4_t (&sums)[MF][2][8 / WN], u
 			auto get = [&](uint32_t c) { return *reinterpret_cast<const f32x4_t *>(from + ((c ^ swizzle) << 4)); };
 			const f32x4_t a0 = get(chunk), a1 = get(other), b0 = get(chunk + 32), b1 = get(other + 32);
 			const f32x8_t a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+			const in_t now = in;
+			if (i + 1 < kTurns) {
+				in = ask(loop, i + 1);
+			} else if (loop + 1 < kLoops) {
+				in = ask(loop + 1, 0);
+			}
 			if (whole) {
-				finish(std::true_type{}, row_of(loop, at), in_loop(lane & 15u), a, b, in[i]);
+				finish(std::true_type{}, row_of(loop, at), in_loop(lane & 15u), a, b, now);
 			} else {
-				finish(std::false_type{}, row_of(loop, at), in_loop(lane & 15u), a, b, in[i]);
+				finish(std::false_type{}, row_of(loop, at), in_loop(lane & 15u), a, b, now);
 			}
 			__builtin_amdgcn_sched_barrier(0);
-		}
-		if (loop + 1 < kLoops) {
-			load_all(loop + 1);
 		}
 	}
 }
