@@ -78,6 +78,16 @@ __device__ __forceinline__ void sum_scaled_steps(f32x4_t (&sums)[MF][2][8 / WN],
 		const uint32_t r = (wm * MF + m) * 16 + (lane & 15u);
 		row_scale[m] = row_at(a->o.scale, a->o.scale_pitch, place.from + (r < place.rows ? r : place.rows - 1));
 	}
+	float row_next[MF], weight_next[2];
+	auto scales_of = [&](uint32_t step) __attribute__((always_inline)) {
+#pragma unroll
+		for (int m = 0; m < (int)MF; m++) {
+			row_next[m] = row_scale[m][step];
+		}
+		weight_next[0] = weight_scale[0][step];
+		weight_next[1] = weight_scale[1][step];
+	};
+	scales_of(0);
 	if (DIRECT) {
 		of.fill(0, lds);
 	} else {
@@ -90,21 +100,25 @@ __device__ __forceinline__ void sum_scaled_steps(f32x4_t (&sums)[MF][2][8 / WN],
 		} else {
 			of.store(step, now);
 		}
+		/* the scales came with the tile; taken here, where nothing is on its way, as waiting for them later would wait for the next tile */
+		float by[MF][2];
+#pragma unroll
+		for (int m = 0; m < (int)MF; m++) {
+			by[m][0] = row_next[m] * weight_next[0];
+			by[m][1] = row_next[m] * weight_next[1];
+		}
 		workgroup_meets<DIRECT>(); /* this tile is there, and the other one's readers are past it */
 		if (step + 1 < steps) {
+			scales_of(step + 1);
 			if (DIRECT) {
 				of.fill(step + 1, lds + (~step & 1u) * Operands::kBytes);
 			} else {
 				of.load(step + 1);
 			}
 		}
-		float by[MF][2];
 		u32x4_t r[MF][4];
 #pragma unroll
 		for (int m = 0; m < (int)MF; m++) {
-			const float s = row_scale[m][step];
-			by[m][0] = s * weight_scale[0][step];
-			by[m][1] = s * weight_scale[1][step];
 #pragma unroll
 			for (uint32_t half = 0; half < 2; half++) {
 				const u32x4_t q = row_frag.get(now, m * 16, half);
