@@ -21,9 +21,13 @@ struct forward_args_t {
 template <typename T, uint32_t BM, uint32_t THREADS> struct forward_operands_t {
 	along_t<T, BM, THREADS> rows;
 	along_t<T, kBlock, THREADS> part0, part1;
+	const uint8_t *scale; /* of the first row, for 8-bit ones: one word of each row in a step */
+	uint32_t scale_pitch;
 	forward_tile_t place;
-	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kPartBytes = decltype(part0)::kBytes, kBytes = kRowsBytes + 2 * kPartBytes;
-	static constexpr uint32_t kFills = decltype(rows)::kChunks + 2 * decltype(part0)::kChunks;
+	static constexpr bool kScaled = sizeof(T) == 1;
+	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kPartBytes = decltype(part0)::kBytes, kScalesAt = kRowsBytes + 2 * kPartBytes;
+	static constexpr uint32_t kBytes = kScalesAt + (kScaled ? BM * 4 : 0);
+	static constexpr uint32_t kFills = decltype(rows)::kChunks + 2 * decltype(part0)::kChunks + (kScaled ? 1 : 0);
 
 	/* direct: a part without columns is not read; else the first column stands for them */
 	__device__ __forceinline__ void set(const forward_args_t *a, const tile_t &tile, bool direct)
@@ -36,6 +40,10 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct forward_operands_t {
 		place = { tile.from, tile.rows, c0, c1, there0, there1, n, tile.expert };
 		rows.set(a->x + tile.from * a->x_pitch, a->x_pitch, tile.rows, bytes);
 		part0.set(weights + c0 * a->w_pitch, a->w_pitch, there0, bytes);
+		if (kScaled) {
+			scale = reinterpret_cast<const uint8_t *>(row_at(a->o.scale, a->o.scale_pitch, tile.from));
+			scale_pitch = (uint32_t)a->o.scale_pitch;
+		}
 		part1.set(weights + (there1 ? (gated ? (uint64_t)n : 0) + c1 : 0) * a->w_pitch, a->w_pitch, there1 || direct ? there1 : 1, bytes);
 	}
 	__device__ __forceinline__ void load(uint32_t step)
@@ -55,11 +63,17 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct forward_operands_t {
 		rows.fill(step, to);
 		part0.fill(step, to + kRowsBytes);
 		part1.fill(step, to + kRowsBytes + kPartBytes);
+		if (kScaled) { /* every wavefront has one, so that all count alike: they are as many times BM / 64 */
+			const uint32_t some = uniform(threadIdx.x >> 6) % (BM / 64) * 64, r = some + (threadIdx.x & 63u);
+			const int bytes = (int)((place.rows - 1) * scale_pitch) + 4;
+			words_to_lds(scale + step * 4, step * kStepBytes < (uint32_t)rows.bytes ? bytes : 0, r * scale_pitch, to + kScalesAt + some * 4);
+		}
 	}
 };
 
-/* sums += all steps of 8-bit rows, each with its scales: sum_steps without fragments on their way, for want of registers */
-template <uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT, typename Operands>
+/* sums += all steps of 8-bit rows, each with its scales: sum_steps without fragments on their way, for want of registers.  The rows' scales come
+ * with the tile, so that no load of a lane's own is waited for, which would wait for the tiles on their way. */
+template <uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT, uint32_t STAGES, typename Operands>
 __device__ __forceinline__ void sum_scaled_steps(f32x4_t (&sums)[MF][2][8 / WN], uint32_t steps, uint8_t *lds, Operands &of)
 {
 	constexpr uint32_t G = 8 / WN;
@@ -67,54 +81,61 @@ __device__ __forceinline__ void sum_scaled_steps(f32x4_t (&sums)[MF][2][8 / WN],
 	const along_frag_t row_frag(wm * 16 * MF, lane), column_frag(wn * 16 * G, lane);
 	const forward_args_t *const a = argument<forward_args_t>();
 	const forward_tile_t &place = of.place;
-	/* the scales of a lane's row of each of its groups, and of the parts' weights */
 	const float *row_scale[MF], *weight_scale[2];
 	const uint32_t k_blocks = blocks_of(a->width), n_blocks = blocks_of(place.n);
 	const float *const of_expert = a->o.weight_scale + (uint64_t)place.expert * (a->o.gated ? 2 : 1) * n_blocks * k_blocks;
 	weight_scale[0] = of_expert + (uint64_t)(place.c0 / kBlock) * k_blocks;
 	weight_scale[1] = place.there1 ? of_expert + (uint64_t)((a->o.gated ? n_blocks : 0) + place.c1 / kBlock) * k_blocks : weight_scale[0];
-#pragma unroll
-	for (int m = 0; m < (int)MF; m++) {
-		const uint32_t r = (wm * MF + m) * 16 + (lane & 15u);
-		row_scale[m] = row_at(a->o.scale, a->o.scale_pitch, place.from + (r < place.rows ? r : place.rows - 1));
-	}
 	float row_next[MF], weight_next[2];
 	auto scales_of = [&](uint32_t step) __attribute__((always_inline)) {
+		if (!DIRECT) {
 #pragma unroll
-		for (int m = 0; m < (int)MF; m++) {
-			row_next[m] = row_scale[m][step];
+			for (int m = 0; m < (int)MF; m++) {
+				row_next[m] = row_scale[m][step];
+			}
 		}
 		weight_next[0] = weight_scale[0][step];
 		weight_next[1] = weight_scale[1][step];
 	};
-	scales_of(0);
 	if (DIRECT) {
-		of.fill(0, lds);
+#pragma unroll
+		for (uint32_t s = 0; s + 1 < STAGES; s++) {
+			of.fill(s, lds + s * Operands::kBytes);
+		}
 	} else {
+#pragma unroll
+		for (int m = 0; m < (int)MF; m++) {
+			const uint32_t r = (wm * MF + m) * 16 + (lane & 15u);
+			row_scale[m] = row_at(a->o.scale, a->o.scale_pitch, place.from + (r < place.rows ? r : place.rows - 1));
+		}
 		of.load(0);
 	}
+	scales_of(0);
+	uint32_t at = 0;
 	for (uint32_t step = 0; step < steps; step++) {
-		uint8_t *const now = lds + (step & 1u) * Operands::kBytes;
+		uint8_t *const now = lds + at, *const last = lds + (at ? at - Operands::kBytes : (STAGES - 1) * Operands::kBytes);
+		at = at + Operands::kBytes < STAGES * Operands::kBytes ? at + Operands::kBytes : 0;
 		if (DIRECT) {
-			landed<0>();
+			landed<(STAGES - 2) * Operands::kFills>();
 		} else {
 			of.store(step, now);
 		}
-		/* the scales came with the tile; taken here, where nothing is on its way, as waiting for them later would wait for the next tile */
+		workgroup_meets<DIRECT>(); /* this tile is there, and the last one's readers are past it */
 		float by[MF][2];
 #pragma unroll
 		for (int m = 0; m < (int)MF; m++) {
-			by[m][0] = row_next[m] * weight_next[0];
-			by[m][1] = row_next[m] * weight_next[1];
+			const float s = DIRECT ? reinterpret_cast<const float *>(now + Operands::kScalesAt)[(wm * MF + m) * 16 + (lane & 15u)] : row_next[m];
+			by[m][0] = s * weight_next[0];
+			by[m][1] = s * weight_next[1];
 		}
-		workgroup_meets<DIRECT>(); /* this tile is there, and the other one's readers are past it */
 		if (step + 1 < steps) {
 			scales_of(step + 1);
-			if (DIRECT) {
-				of.fill(step + 1, lds + (~step & 1u) * Operands::kBytes);
-			} else {
+			if (!DIRECT) {
 				of.load(step + 1);
 			}
+		}
+		if (DIRECT) {
+			of.fill(step + STAGES - 1, last);
 		}
 		u32x4_t r[MF][4];
 #pragma unroll
@@ -150,6 +171,9 @@ __device__ __forceinline__ void sum_scaled_steps(f32x4_t (&sums)[MF][2][8 / WN],
 			}
 		}
 	}
+	if (DIRECT) {
+		landed<0>(); /* what follows writes there */
+	}
 }
 
 template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT>
@@ -158,7 +182,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(forward_ar
 	constexpr uint32_t BM = 16 * MF * WM, THREADS = 64 * WM * WN, G = 8 / WN;
 	constexpr bool SCALED = sizeof(T) == 1;
 	using operands_t = forward_operands_t<T, BM, THREADS>;
-	constexpr uint32_t kStages = DIRECT && !SCALED && WM < 4 ? 3 : 2;
+	constexpr uint32_t kStages = DIRECT && WM < 4 ? 3 : 2;
 	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * operands_t::kBytes];
 
 	operands_t of;
@@ -175,7 +199,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_forward_kernel(forward_ar
 	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
 	f32x4_t sums[MF][2][G] = {};
 	if constexpr (SCALED) {
-		sum_scaled_steps<WM, WN, MF, DIRECT>(sums, steps, lds, of);
+		sum_scaled_steps<WM, WN, MF, DIRECT, kStages>(sums, steps, lds, of);
 	} else {
 		sum_steps<T, DIRECT, kStages, operands_t::kFills>(
 			sums, wm * 16 * MF < of.place.rows, steps, lds, operands_t::kBytes, operands_t::kRowsBytes, along_frag_t(wm * 16 * MF, lane),
@@ -198,7 +222,8 @@ int forward(const void *d_rows, uint64_t rows_pitch, int type, const int32_t *d_
 	    const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t width, uint32_t n, const forward_t &o, void *stream)
 {
 	const uint64_t bytes = (uint64_t)width * product_type_size(type);
-	const bool direct = in_chunks(d_rows, rows_pitch, bytes) && in_chunks(d_weight, weight_pitch, bytes) && expert_pitch % 16 == 0;
+	const bool direct = in_chunks(d_rows, rows_pitch, bytes) && in_chunks(d_weight, weight_pitch, bytes) && expert_pitch % 16 == 0 &&
+			    (type != OFI_AMD_E4M3 || o.scale_pitch <= kMostPitch);
 	const uint32_t n_tiles = (n + (o.gated ? kBlock : 2 * kBlock) - 1) / (o.gated ? kBlock : 2 * kBlock);
 	const uint32_t bm = row_tile_for(max_rows, n_experts, n_tiles, direct);
 	if (forward_is_few(max_rows, n_experts, n_tiles)) {

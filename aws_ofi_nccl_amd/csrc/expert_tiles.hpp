@@ -195,6 +195,14 @@ __device__ __forceinline__ void to_lds(const uint8_t *p, int bytes, uint32_t off
 	const uint32_t to = uniform((uint32_t)reinterpret_cast<uintptr_t>((lds_void_t *)lds));
 	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory");
 }
+/* The same of 4 bytes for each lane */
+__device__ __forceinline__ void words_to_lds(const uint8_t *p, int bytes, uint32_t offset, uint8_t *lds)
+{
+	const uint64_t at = reinterpret_cast<uint64_t>(p);
+	const i32x4_t buffer = { (int)uniform((uint32_t)at), (int)uniform((uint32_t)(at >> 32) & 0xffffu), (int)uniform((uint32_t)bytes), 0x00020000 };
+	const uint32_t to = uniform((uint32_t)reinterpret_cast<uintptr_t>((lds_void_t *)lds));
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory");
+}
 /* All but the last N of the wavefront's to_lds have landed */
 template <uint32_t N> __device__ __forceinline__ void landed()
 {
@@ -907,10 +915,12 @@ inline bool stack_ok(const void *p, uint64_t pitch, uint64_t expert_pitch, uint3
 
 inline bool scales_ok(const void *p, uint64_t pitch, uint64_t n, uint32_t blocks) { return rows_ok(p, pitch, n, 4ull * blocks, 4); }
 
+constexpr uint32_t kMostPitch = 1u << 22;
+
 /* Rows of `bytes` that whole chunks of 16 bytes make up, and that start on them, a tile of 256 rows within 31 bits */
 inline bool in_chunks(const void *p, uint64_t pitch, uint64_t bytes)
 {
-	return ((reinterpret_cast<uintptr_t>(p) | pitch | bytes) & 15u) == 0 && pitch <= (1u << 22);
+	return ((reinterpret_cast<uintptr_t>(p) | pitch | bytes) & 15u) == 0 && pitch <= kMostPitch;
 }
 
 constexpr uint32_t kTilesOfLaunch = 1u << 22; /* with 512 lanes each within the 32 bits of a launch's size */
