@@ -2,12 +2,13 @@
 the results fetched back, weighted sums -- and the gradients of all of it: those of the rows are put to their ranks and the
 experts' fetched back the same way.
 
-    python -m aws_ofi_nccl_amd.expert_exchange [--tokens 512] [--width 1024] [--experts 16] [--top-k 4] [--ranks 4]
+    python -m aws_ofi_nccl_amd.expert_exchange [--tokens 512] [--width 1024] [--experts 16] [--top-k 4] [--ranks 4] [--gated 8]
 
 The operators are the library's (`ofi_amd_rms_norm`, `ofi_amd_token_dispatch`, `ofi_amd_token_combine` and their
-gradients).  The exchange goes through `ofi_amd_rma_iput` / `_iputSignal` / `_iget` over the device fabric: the ranks are
+gradients).  With --gated the experts are the library's too: gated blocks and the product behind them (`ofi_amd_expert_*`),
+which keep what their activations were taken of in 8 or 16 bits, and whose weights get gradients.  The exchange goes through `ofi_amd_rma_iput` / `_iputSignal` / `_iget` over the device fabric: the ranks are
 windows of this process on one GPU, and what a rank gets is the run of sorted rows of its experts, whose place and length are
-two of the offsets.  The experts themselves, and a check of everything against the formulas, are plain torch.
+two of the offsets.  Other experts, and a check of everything against the formulas, are plain torch.
 """
 import argparse
 import ctypes
@@ -133,6 +134,56 @@ def experts_of(rows, up, down):
     return torch.nn.functional.silu(rows @ up) @ down
 
 
+class GatedExperts:
+    """Gated blocks in bfloat16: silu(x G^T) * (x U^T), then W2.  w1: [experts, 2 * inner, width], the rows of G first; w2: [experts, width, inner].
+    kept: 8 or 16, the bits of a checkpoint."""
+
+    def __init__(self, w1, w2, kept):
+        self.w1, self.w2, self.kept = w1, w2, kept
+        self.experts, self.width, self.inner = w2.shape
+        self.dw1, self.dw2 = torch.zeros_like(w1, dtype=torch.float32), torch.zeros_like(w2, dtype=torch.float32)
+
+    def formula(self, rows, e):
+        both = rows @ self.w1[e].to(rows.dtype).t()
+        return (torch.nn.functional.silu(both[:, :self.inner]) * both[:, self.inner:]) @ self.w2[e].to(rows.dtype).t()
+
+    def _stack(self, w, first):
+        return w[first].data_ptr(), w.stride(1) * w.element_size(), w.stride(0) * w.element_size()
+
+    def forward(self, lib, x, offset, first, last, result):
+        """Experts first to last on their rows of x; x and result have all sorted rows' places, offset all experts'."""
+        n, inner = x.shape[0], self.inner
+        kept = torch.float8_e4m3fn if self.kept == 8 else torch.bfloat16
+        code = _m.E4M3 if self.kept == 8 else _m.BFLOAT16
+        h = torch.empty(n, inner, dtype=torch.bfloat16, device="cuda")
+        saved = torch.empty(n, 2 * inner, dtype=kept, device="cuda")
+        scale = torch.empty(n, 2 * -(-inner // GROUP), device="cuda")
+        rows = _ptr(offset[first:]), last - first, n
+        _m.check(lib.ofi_amd_expert_gated(*_rows(x), None, 0, _m.BFLOAT16, *rows, *self._stack(self.w1, first), None, self.width, inner, _m.SILU,
+                                          *_rows(h), _m.BFLOAT16, None, 0, *_rows(saved), code, *_rows(scale), _stream()), "expert_gated")
+        _m.check(lib.ofi_amd_expert_product(*_rows(h), None, 0, _m.BFLOAT16, *rows, *self._stack(self.w2, first), None, inner, self.width, None, 0,
+                                            _m.NO_ACTIVATION, None, 0, *_rows(result), _m.BFLOAT16, None, 0, None, 0, 0, None, 0, _stream()),
+                 "expert_product")
+        return x, saved, scale, code
+
+    def backward(self, lib, kept, offset, first, last, result):
+        """result holds the gradients of the results and takes those of the rows; the weights' are left in dw1 and dw2."""
+        x, saved, scale, code = kept
+        n, inner, width = x.shape[0], self.inner, self.width
+        hidden = torch.empty(n, inner, dtype=torch.bfloat16, device="cuda")
+        dsaved = torch.empty(n, 2 * inner, dtype=torch.bfloat16, device="cuda")
+        rows = _ptr(offset[first:]), last - first, n
+        _m.check(lib.ofi_amd_expert_hidden_grad(*_rows(result), _m.BFLOAT16, *rows, *self._stack(self.w2, first), width, inner, 1, _m.SILU,
+                                                *_rows(saved), code, *_rows(scale), *_rows(dsaved), *_rows(hidden), _stream()),
+                 "expert_hidden_grad")
+        _m.check(lib.ofi_amd_expert_weight_grad(*_rows(result), *_rows(hidden), _m.BFLOAT16, *rows, inner, width, None,
+                                                *self._stack(self.dw2, first), _m.FLOAT32, None, None, _stream()), "expert_weight_grad")
+        _m.check(lib.ofi_amd_expert_rows_grad(*_rows(dsaved), _m.BFLOAT16, *rows, *self._stack(self.w1, first), width, 2 * inner, None, 0,
+                                              *_rows(result), _stream()), "expert_rows_grad")
+        _m.check(lib.ofi_amd_expert_weight_grad(*_rows(dsaved), *_rows(x), _m.BFLOAT16, *rows, width, 2 * inner, None,
+                                                *self._stack(self.dw1, first), _m.FLOAT32, None, None, _stream()), "expert_weight_grad")
+
+
 def fetch_results(link, runs, width):
     """Every rank's run of bfloat16 rows from its window into the same place of the own one."""
     torch.cuda.synchronize()
@@ -142,10 +193,10 @@ def fetch_results(link, runs, width):
     link.finish()
 
 
-def layer(lib, link, x, residual, gain, ids, weight, up, down, dout=None):
-    """The layer's output (and with dout the gradients), through the library and the link."""
+def layer(lib, link, x, residual, gain, ids, weight, up, down, dout=None, gated=None):
+    """The layer's output (and with dout the gradients), through the library and the link.  gated: GatedExperts in the place of up and down."""
     tokens, width = x.shape
-    top_k, experts, ranks = ids.shape[1], up.shape[0], link.ranks
+    top_k, experts, ranks = ids.shape[1], gated.experts if gated else up.shape[0], link.ranks
     pairs, groups, own = tokens * top_k, -(-width // GROUP), link.own
     total, rstd = torch.empty_like(x), torch.empty(tokens, device="cuda")
     q = torch.empty(tokens, width, dtype=torch.float8_e4m3fn, device="cuda")
@@ -167,8 +218,14 @@ def layer(lib, link, x, residual, gain, ids, weight, up, down, dout=None):
             link.put(r, own.scale_at + lo * groups * 4, (hi - lo) * groups * 4)
             link.put_signal(r, lo * width, (hi - lo) * width)
     link.finish()
-    places = [(r, first[e], first[e + 1]) for r in range(ranks) for e in range(bound[r], bound[r + 1])]
-    inputs, outputs = [], []
+    places = [(r, first[e], first[e + 1]) for r in range(ranks) for e in range(bound[r], bound[r + 1])] if gated is None else []
+    inputs, outputs, kept = [], [], []
+    if gated is not None:
+        for r, w in enumerate(link.windows):
+            lo, hi = runs[r]
+            rows = torch.zeros(pairs, width, dtype=torch.bfloat16, device="cuda")
+            rows[lo:hi] = dequantised(w.q[lo:hi], w.scale[lo:hi], width)
+            kept.append(gated.forward(lib, rows, offset, bound[r], bound[r + 1], w.result))
     for e, (r, lo, hi) in enumerate(places):          # each rank's own work, on what has arrived in its window
         w = link.windows[r]
         rows = dequantised(w.q[lo:hi], w.scale[lo:hi], width)
@@ -192,6 +249,8 @@ def layer(lib, link, x, residual, gain, ids, weight, up, down, dout=None):
         if hi > lo:
             link.put_signal(r, own.result_at + lo * width * 2, (hi - lo) * width * 2)
     link.finish()
+    for r in range(len(kept)):
+        gated.backward(lib, kept[r], offset, bound[r], bound[r + 1], link.windows[r].result)
     for (r, lo, hi), rows, y in zip(places, inputs, outputs):
         if hi > lo:                                   # the experts' own gradient
             result = link.windows[r].result[lo:hi]
@@ -208,8 +267,12 @@ def layer(lib, link, x, residual, gain, ids, weight, up, down, dout=None):
     return got
 
 
-def plain(got, x, residual, gain, ids, weight, up, down, dout):
+def plain(got, x, residual, gain, ids, weight, up, down, dout, gated=None):
     """The same by torch alone in 64 bits, from the 8-bit rows that the layer sent: their rounding is passed through by gradients."""
+    if gated is not None:
+        w1, w2 = (v.double().requires_grad_(True) for v in (gated.w1, gated.w2))
+        wide = GatedExperts(w1, w2, gated.kept)
+        up = w1
     width = x.shape[1]
     s = (x.double() + residual.double()).requires_grad_(True)
     g, w = gain.double().requires_grad_(True), weight.double().requires_grad_(True)
@@ -221,17 +284,19 @@ def plain(got, x, residual, gain, ids, weight, up, down, dout):
         y = torch.zeros_like(s)
         for e in range(up.shape[0]):
             here = torch.nonzero(ids[:, k] == e)[:, 0]
-            y = y.index_add(0, here, experts_of(n[here], up[e].double(), down[e].double()))
+            y = y.index_add(0, here, experts_of(n[here], up[e].double(), down[e].double()) if gated is None else wide.formula(n[here], e))
         out = out + w[:, k, None] * y
-    ds, dg, dw = torch.autograd.grad(out, (s, g, w), dout.double())
+    ds, dg, dw, *of_experts = torch.autograd.grad(out, (s, g, w) + (() if gated is None else (w1, w2)), dout.double())
     normed = (s / torch.sqrt((s * s).mean(dim=1, keepdim=True) + EPS) * g).detach()
-    return dict(out=out.detach(), dx=ds, dgain=dg, dweight=dw, sent_off=((sent - normed).norm() / normed.norm()).item())
+    want = dict(out=out.detach(), dx=ds, dgain=dg, dweight=dw, sent_off=((sent - normed).norm() / normed.norm()).item())
+    return want if gated is None else dict(want, dw1=of_experts[0], dw2=of_experts[1])
 
 
 def main(argv=None):
     ap = argparse.ArgumentParser(prog="expert_exchange", description=__doc__.splitlines()[0])
     for name, value in (("tokens", 512), ("width", 1024), ("experts", 16), ("top-k", 4), ("ranks", 4), ("inner", 256), ("seed", 1)):
         ap.add_argument("--" + name, type=int, default=value)
+    ap.add_argument("--gated", type=int, choices=(8, 16), help="gated experts by the library, with checkpoints of so many bits")
     args = ap.parse_args(argv)
     if not (args.tokens > 0 and args.width > 0 and 0 < args.ranks <= args.experts and 0 < args.top_k <= args.experts and args.inner > 0):
         ap.error("sizes are positive, ranks and top-k at most as many as experts")
@@ -246,25 +311,35 @@ def main(argv=None):
     weight = torch.softmax(top, dim=1).contiguous()
     up = normal(args.experts, args.width, args.inner) / args.width ** 0.5
     down = normal(args.experts, args.inner, args.width) / args.inner ** 0.5
+    gated = None
+    if args.gated:
+        w1 = (normal(args.experts, 2 * args.inner, args.width) / args.width ** 0.5).to(torch.bfloat16)
+        gated = GatedExperts(w1, (normal(args.experts, args.width, args.inner) / args.inner ** 0.5).to(torch.bfloat16), args.gated)
     link = Link(lib, args.ranks, args.tokens * args.top_k, args.width)
     try:
         for _ in range(2):
             began = time.perf_counter()
-            got = layer(lib, link, x, residual, gain, ids, weight, up, down, dout)
+            got = layer(lib, link, x, residual, gain, ids, weight, up, down, dout, gated)
             torch.cuda.synchronize()
             took = time.perf_counter() - began
         arrived = link.counters.cpu().tolist()
     finally:
         link.close()
-    want = plain(got, x, residual, gain, ids, weight, up, down, dout)
-    off = {k: ((got[k].double() - want[k]).norm() / want[k].norm()).item() for k in ("out", "dx", "dgain", "dweight")}
+    want = plain(got, x, residual, gain, ids, weight, up, down, dout, gated)
+    names = ("out", "dx", "dgain", "dweight")
+    if gated is not None:
+        got.update(dw1=gated.dw1, dw2=gated.dw2)
+        names += ("dw1", "dw2")
+    off = {k: ((got[k].double() - want[k]).norm() / want[k].norm()).item() for k in names}
     print("%d tokens x %d choices -> %d rows to %d ranks, signals %s, forward and backward %.2f ms" % (
         args.tokens, args.top_k, got["first"][-1], args.ranks, arrived, took * 1e3))
     print("off from the formulas in 64 bits: " + ", ".join("%s %.2g" % kv for kv in off.items()) +
           "; 8-bit rows off from the norm: %.2g" % want["sent_off"])
     # two layers, each with a signal forward and one backward to every rank that has rows;
     # bfloat16 results: a rounding (2^-8 of a value at most) of each of the few tensors on the way; e4m3: half a step of 2^-4
-    ok = all(v < 0.015 for v in off.values()) and want["sent_off"] < 0.04 and all(
+    # what 8-bit checkpoints were rounded by, two factors of up to 2^-4 each, the gradients behind them have too
+    rough = {k: 0.0625 if args.gated == 8 and k in ("dx", "dgain", "dw1", "dw2") else 0.015 for k in names}
+    ok = all(v < rough[k] for k, v in off.items()) and want["sent_off"] < 0.04 and all(
         n == (4 if hi > lo else 0) for n, (lo, hi) in zip(arrived, got["runs"]))
     print("ok" if ok else "DIFFERS")
     return 0 if ok else 1
