@@ -707,50 +707,24 @@ template <typename T> __device__ __forceinline__ void write_as(uint8_t *p, uint3
 	}
 }
 
-/* Four values of a row of 16 bits or float32, of which `left` are there: zeros for the others */
-template <typename T> __device__ __forceinline__ f32x4_t four_at(const uint8_t *p, uint32_t left)
+/* `left` of four values at p: zeros for the others */
+__device__ __forceinline__ f32x4_t read_four(const float *p, uint32_t left)
 {
-	raw_t<T, 4> r = {};
+	f32x4_t v;
+	read_words<float, 4>(reinterpret_cast<const uint8_t *>(p), left, v);
+	return v;
+}
+__device__ __forceinline__ void write_four(float *p, uint32_t left, f32x4_t v)
+{
 	if (left >= 4) {
-		r = *reinterpret_cast<const typename piece_t<T, 4>::anywhere *>(p);
+		*reinterpret_cast<piece_t<float, 4>::anywhere *>(p) = v;
 	} else {
 #pragma unroll
 		for (uint32_t i = 0; i < 3; i++) {
 			if (i < left) {
-				r[i] = reinterpret_cast<const T *>(p)[i];
+				p[i] = v[i];
 			}
 		}
-	}
-	return __builtin_convertvector(r, f32x4_t);
-}
-__device__ __forceinline__ f32x4_t read_four(int type, const uint8_t *p, uint64_t column, uint32_t left)
-{
-	switch (type) {
-	case OFI_AMD_BFLOAT16: return four_at<bf16_t>(p + column * 2, left);
-	case OFI_AMD_FLOAT16: return four_at<f16_t>(p + column * 2, left);
-	default: return four_at<float>(p + column * 4, left);
-	}
-}
-template <typename T> __device__ __forceinline__ void write_four_as(uint8_t *p, uint32_t left, f32x4_t v)
-{
-	const auto r = __builtin_convertvector(v, raw_t<T, 4>);
-	if (left >= 4) {
-		*reinterpret_cast<typename piece_t<T, 4>::anywhere *>(p) = r;
-	} else {
-#pragma unroll
-		for (uint32_t i = 0; i < 3; i++) {
-			if (i < left) {
-				reinterpret_cast<T *>(p)[i] = r[i];
-			}
-		}
-	}
-}
-__device__ __forceinline__ void write_four(int type, uint8_t *p, uint64_t column, uint32_t left, f32x4_t v)
-{
-	switch (type) {
-	case OFI_AMD_BFLOAT16: write_four_as<bf16_t>(p + column * 2, left, v); break;
-	case OFI_AMD_FLOAT16: write_four_as<f16_t>(p + column * 2, left, v); break;
-	default: write_four_as<float>(p + column * 4, left, v);
 	}
 }
 

@@ -75,7 +75,8 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct weight_operands_t {
 	}
 };
 
-template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT>
+/* F32: float32 out, else T */
+template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT, bool F32>
 __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(weight_grad_args_t)
 {
 	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN, kStages = 2;
@@ -124,23 +125,33 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(weight
 		sum([](const u32x4_t(&)[MF]) {});
 	}
 
+	/* a lane's columns of each part: of float32 four, and four 64 further, so that sixteen lanes have 256 bytes of a row both times; of 16 bits eight */
 	struct in_t {
-		f32x4_t was[4];
+		eight_t eight[F32 ? 1 : 2];
+		f32x4_t four[F32 ? 4 : 1];
 	};
-	auto left = [&](uint32_t column) { return column < place.n_there ? place.n_there - column : 0u; };
-	/* a lane's columns of each part: four, and four 64 further */
-	for_rows<WM, WN, MF, true>(
+	auto left_of = [&](uint32_t column) { return column < place.n_there ? place.n_there - column : 0u; };
+	for_rows<WM, WN, MF, F32>(
 		sums, lds, place.m_there == BM && place.n_there == BN,
 		[&](auto all, uint32_t r, uint32_t part_lane) __attribute__((always_inline)) {
 			constexpr bool WHOLE = decltype(all)::value;
 			const weight_grad_args_t *const a = argument<weight_grad_args_t>();
-			const uint32_t c = part_lane * 4;
 			in_t in = {};
 			if (a->add.p && (WHOLE || r < place.m_there)) {
-				const uint8_t *const p = a->add.p + place.expert * a->expert_pitch + (uint64_t)(place.m0 + r) * a->add.pitch;
+				const matrix_t add = { a->add.p + place.expert * a->expert_pitch, a->add.pitch, a->add.type, nullptr, 0 };
+				if constexpr (F32) {
+					const float *const p = reinterpret_cast<const float *>(add.p + (uint64_t)(place.m0 + r) * add.pitch);
 #pragma unroll
-				for (uint32_t i = 0; i < 4; i++) {
-					in.was[i] = read_four(a->add.type, p, place.n0 + i * 64 + c, WHOLE ? 4 : left(i * 64 + c));
+					for (uint32_t i = 0; i < 4; i++) {
+						const uint32_t c = i * 64 + part_lane * 4;
+						in.four[i] = read_four(p + place.n0 + c, WHOLE ? 4 : left_of(c));
+					}
+				} else {
+#pragma unroll
+					for (uint32_t i = 0; i < 2; i++) {
+						const uint32_t c = i * kBlock + part_lane * 8;
+						in.eight[i] = load_eight(add, place.m0 + r, place.n0 + c, WHOLE ? 8 : left_of(c), 0);
+					}
 				}
 			}
 			return in;
@@ -148,13 +159,26 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(weight
 		[&](auto all, uint32_t r, uint32_t part_lane, f32x8_t p0, f32x8_t p1, const in_t &in) __attribute__((always_inline)) {
 			constexpr bool WHOLE = decltype(all)::value;
 			const weight_grad_args_t *const a = argument<weight_grad_args_t>();
-			const uint32_t c = part_lane * 4;
-			if (WHOLE || r < place.m_there) {
-				uint8_t *const p = a->out.p + place.expert * a->expert_pitch + (uint64_t)(place.m0 + r) * a->out.pitch;
+			const matrix_t out = { a->out.p + place.expert * a->expert_pitch, a->out.pitch, a->out.type, nullptr, 0 };
+			if constexpr (F32) {
+				if (WHOLE || r < place.m_there) {
+					float *const p = reinterpret_cast<float *>(out.p + (uint64_t)(place.m0 + r) * out.pitch);
 #pragma unroll
-				for (uint32_t i = 0; i < 4; i++) {
-					const f32x4_t v = i == 0 ? p0.lo : i == 1 ? p0.hi : i == 2 ? p1.lo : p1.hi;
-					write_four(a->out.type, p, place.n0 + i * 64 + c, WHOLE ? 4 : left(i * 64 + c), v + in.was[i]);
+					for (uint32_t i = 0; i < 4; i++) {
+						const f32x4_t v = i == 0 ? p0.lo : i == 1 ? p0.hi : i == 2 ? p1.lo : p1.hi;
+						const uint32_t c = i * 64 + part_lane * 4;
+						write_four(p + place.n0 + c, WHOLE ? 4 : left_of(c), v + in.four[i]);
+					}
+				}
+			} else {
+#pragma unroll
+				for (uint32_t i = 0; i < 2; i++) {
+					const uint32_t c = i * kBlock + part_lane * 8;
+					f32x8_t v = i ? p1 : p0;
+					if (a->add.p) {
+						v += floats_of<T>(in.eight[i].words);
+					}
+					write_row_as<WHOLE, T>(out, place.m0, place.n0 + c, r, place.m_there, WHOLE ? 8 : left_of(c), v);
 				}
 			}
 		});
@@ -205,8 +229,12 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 				    out_width, width, n_experts, m_tiles, n_tiles, 0, add, out, expert_pitch, d_bias_add, d_dbias };
 	auto with = [&](auto element) {
 		using T = decltype(element);
-		auto kernel = direct ? (wide ? expert_weight_grad_kernel<T, 4, 2, 4, true> : expert_weight_grad_kernel<T, 2, 4, 4, true>)
-				     : expert_weight_grad_kernel<T, 2, 4, 4, false>;
+		auto of = [&](auto f32) {
+			constexpr bool F = decltype(f32)::value;
+			return direct ? (wide ? expert_weight_grad_kernel<T, 4, 2, 4, true, F> : expert_weight_grad_kernel<T, 2, 4, 4, true, F>)
+				      : expert_weight_grad_kernel<T, 2, 4, 4, false, F>;
+		};
+		auto kernel = dweight_type == OFI_AMD_FLOAT32 ? of(std::true_type{}) : of(std::false_type{});
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			args.first_tile = first;
 			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), args);
