@@ -35,6 +35,7 @@ struct backward_tile_t {
 template <typename T, uint32_t BM, uint32_t THREADS> struct backward_operands_t {
 	along_t<T, BM, THREADS> rows;
 	across_t<T, 2 * kBlock, THREADS> columns;
+	across_t<T, 2 * kBlock, THREADS, kStepRows / 2> halves;
 	backward_tile_t place;
 	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kBytes = kRowsBytes + decltype(columns)::kBytes;
 	static constexpr uint32_t kFills = decltype(rows)::kChunks + decltype(columns)::kChunks;
@@ -45,6 +46,7 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct backward_operands_t 
 		place = { tile.from, tile.rows, c0, there, n };
 		rows.set(a->dout + tile.from * a->dout_pitch, a->dout_pitch, tile.rows, (int64_t)a->k * 2);
 		columns.set(a->w + tile.expert * a->expert_pitch + c0 * 2, a->w_pitch, a->k, (int64_t)there * 2);
+		halves.set(a->w + tile.expert * a->expert_pitch + c0 * 2, a->w_pitch, a->k, (int64_t)there * 2);
 	}
 	__device__ __forceinline__ void load(uint32_t step)
 	{
@@ -64,12 +66,14 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct backward_operands_t 
 };
 
 template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool HIDDEN, bool DIRECT>
-__global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(backward_args_t)
+__global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void expert_backward_kernel(backward_args_t)
 {
 	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
 	using operands_t = backward_operands_t<T, BM, THREADS>;
 	constexpr uint32_t kStages = DIRECT && WM < 4 ? 3 : 2;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * operands_t::kBytes];
+	constexpr bool PAIR = WM * WN == 4;
+	constexpr uint32_t kHalfBytes = BN * kStepRows;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[PAIR ? 2 * operands_t::kRowsBytes + 3 * kHalfBytes : kStages * operands_t::kBytes];
 
 	operands_t of;
 	uint32_t steps;
@@ -84,6 +88,13 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_backward_kernel(backward_
 	}
 	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
 	f32x4_t sums[MF][2][G] = {};
+	if constexpr (PAIR) {
+		sum_halves<T, decltype(of.rows)::kChunks, decltype(of.halves)::kChunks, operands_t::kRowsBytes, kHalfBytes>(
+			sums, wm * 16 * MF < of.place.rows, steps, lds, along_frag_t(wm * 16 * MF, lane), across_frag_t<BN>(wn * 16 * G, lane),
+			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.rows.fill(step, to); },
+			[&](uint32_t half, uint8_t *to) __attribute__((always_inline)) { of.halves.fill(half, to); },
+			[](const u32x4_t(&)[MF]) {});
+	} else
 	sum_steps<T, DIRECT, kStages, operands_t::kFills>(
 		sums, wm * 16 * MF < of.place.rows, steps, lds, operands_t::kBytes, operands_t::kRowsBytes, along_frag_t(wm * 16 * MF, lane),
 		across_frag_t<BN>(wn * 16 * G, lane), [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.fill(step, to); },
@@ -166,7 +177,7 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 {
 	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * k) && in_chunks(d_weight, weight_pitch, 2ull * n) && expert_pitch % 16 == 0;
 	const uint32_t n_tiles = (n + 2 * kBlock - 1) / (2 * kBlock), bm = row_tile_for(max_rows, n_experts, n_tiles, direct);
-	const uint64_t tiles = most_row_tiles(max_rows, n_experts, bm) * n_tiles;
+	const uint64_t tiles = most_row_tiles(max_rows, n_experts, bm == 256 ? 128 : bm) * n_tiles;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
@@ -174,14 +185,14 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 				 dout_pitch, weight_pitch, expert_pitch, k, n, 0, o };
 	auto with = [&](auto element) {
 		using T = decltype(element);
-		auto kernel = direct ? (bm == 256 ? expert_backward_kernel<T, 4, 2, 4, HIDDEN, true>
+		auto kernel = direct ? (bm == 256 ? expert_backward_kernel<T, 2, 2, 4, HIDDEN, true>
 						: bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, true>
 							    : expert_backward_kernel<T, 1, 8, 4, HIDDEN, true>)
 				     : bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, false>
 						 : expert_backward_kernel<T, 1, 8, 4, HIDDEN, false>;
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			args.first_tile = first;
-			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), args);
+			launch_kernel(kernel, dim3(count), dim3(bm == 256 ? 256 : 512), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {

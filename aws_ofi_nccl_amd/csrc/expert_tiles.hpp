@@ -317,8 +317,8 @@ template <uint32_t W> __device__ __forceinline__ uint32_t across_slot(uint32_t k
 }
 
 /* W columns of an operand whose rows run across the summed axis; two-byte elements.  base: column 0 of the first row */
-template <typename T, uint32_t W, uint32_t THREADS> struct across_t {
-	static constexpr uint32_t kOfRow = W / 8, kChunks = kStepRows * kOfRow / THREADS, kBytes = kStepRows * W * 2;
+template <typename T, uint32_t W, uint32_t THREADS, uint32_t ROWS = kStepRows> struct across_t {
+	static constexpr uint32_t kOfRow = W / 8, kChunks = ROWS * kOfRow / THREADS, kBytes = ROWS * W * 2;
 	const uint8_t *base;
 	uint64_t pitch;
 	uint32_t rows;  /* of the summed axis */
@@ -336,7 +336,7 @@ template <typename T, uint32_t W, uint32_t THREADS> struct across_t {
 	{
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
-			const uint32_t slot = t * THREADS + threadIdx.x, k = slot / kOfRow, r = step * kStepRows + k;
+			const uint32_t slot = t * THREADS + threadIdx.x, k = slot / kOfRow, r = step * ROWS + k;
 			const int64_t at = (slot % kOfRow ^ across_slot<W>(k)) * 16;
 			const uint8_t *const p = base + (uint64_t)(r < rows ? r : rows - 1) * pitch;
 			held[t] = bytes >= 16 ? *reinterpret_cast<const any16_t *>(p + (at + 16 <= bytes ? at : bytes - 16)) : chunk_at<T>(p + at, bytes - at);
@@ -345,10 +345,10 @@ template <typename T, uint32_t W, uint32_t THREADS> struct across_t {
 	__device__ __forceinline__ void store(uint32_t step, uint8_t *lds) const
 	{
 		const uint32_t over = (uint32_t)(16 - bytes % 16) % 16;
-		const bool some = over && bytes >= 16, rest = (step + 1) * kStepRows > rows;
+		const bool some = over && bytes >= 16, rest = (step + 1) * ROWS > rows;
 #pragma unroll
 		for (uint32_t t = 0; t < kChunks; t++) {
-			const uint32_t slot = t * THREADS + threadIdx.x, k = slot / kOfRow, r = step * kStepRows + k;
+			const uint32_t slot = t * THREADS + threadIdx.x, k = slot / kOfRow, r = step * ROWS + k;
 			u32x4_t v = held[t];
 			if (some) {
 				const int64_t at = (slot % kOfRow ^ across_slot<W>(k)) * 16;
@@ -364,7 +364,7 @@ template <typename T, uint32_t W, uint32_t THREADS> struct across_t {
 	__device__ __forceinline__ void fill(uint32_t step, uint8_t *lds) const
 	{
 		constexpr uint32_t kRowsOfRound = THREADS / kOfRow;
-		const uint64_t at = (uint64_t)step * kStepRows * pitch;
+		const uint64_t at = (uint64_t)step * ROWS * pitch;
 		const int64_t left = (int64_t)((rows - 1) * pitch + bytes - at) - (rows ? 0 : 1ll << 60); /* no rows: nothing */
 		const uint32_t apart = (uint32_t)pitch * kRowsOfRound, row = threadIdx.x / kOfRow, wave = uniform(threadIdx.x >> 6);
 		const int some = left <= 0 ? 0 : left < 0x7fffffff ? (int)left : 0x7fffffff;
@@ -425,6 +425,18 @@ __device__ __forceinline__ u32x4_t widened(uint32_t a, uint32_t b)
 			__builtin_bit_cast(uint32_t, w3) };
 }
 
+/* READS of LDS among PAIRS pairs of matrix instructions, so that they are done when their half begins */
+template <int READS, int PAIRS> __device__ __forceinline__ void spread_reads()
+{
+	constexpr int kEach = (READS + PAIRS - 1) / PAIRS;
+#pragma unroll
+	for (int i = 0; i < PAIRS; i++) {
+		__builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+		__builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+	}
+	__builtin_amdgcn_sched_barrier(0);
+}
+
 /*
  * sums[m][p][j] += all steps.  Fragments of half a step are read while the other half's are multiplied.  When all of a step's are in
  * registers, a barrier: the next step's tile is there (it was asked for STAGES - 1 steps before), and this one's place is free for the
@@ -460,17 +472,7 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 		}
 		also(rows);
 	};
-	/* reads of LDS in pairs of matrix instructions, so that they are done when their half begins */
-	auto spread = [&]() __attribute__((always_inline)) {
-		constexpr int kReads = MF * RowFrag::kReads + 2 * G * ColumnFrag::kReads, kPairs = MF * G;
-		constexpr int kEach = (kReads + kPairs - 1) / kPairs;
-#pragma unroll
-		for (int i = 0; i < kPairs; i++) {
-			__builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
-			__builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-		}
-		__builtin_amdgcn_sched_barrier(0);
-	};
+	auto spread = [&]() __attribute__((always_inline)) { spread_reads<MF * RowFrag::kReads + 2 * G * ColumnFrag::kReads, MF * G>(); };
 	if (steps == 0) {
 		return;
 	}
@@ -529,6 +531,94 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 	if (DIRECT) {
 		landed<0>(); /* what follows writes there */
 	}
+}
+
+/*
+ * The same for workgroups of four wavefronts, of which a compute unit has two: while one is at its beginning, its epilogue or a barrier, the other
+ * multiplies.  Each has 80 KB of LDS: the rows' tiles of two steps, and the columns' of three halves of a step.  They come that many steps and halves
+ * before they are read.
+ */
+template <typename T, uint32_t ROW_FILLS, uint32_t COLUMN_FILLS, uint32_t ROWS_BYTES, uint32_t HALF_BYTES, uint32_t MF, uint32_t G, typename RowFrag,
+	  typename ColumnFrag, typename FillRows, typename FillColumns, typename Also>
+__device__ __forceinline__ void sum_halves(f32x4_t (&sums)[MF][2][G], bool busy, uint32_t steps, uint8_t *lds, const RowFrag &row_frag,
+					   const ColumnFrag &column_frag, FillRows fill_rows, FillColumns fill_columns, Also also)
+{
+	u32x4_t r[2][MF], c[2][2 * G];
+	auto read = [&](uint8_t *rows, uint8_t *columns, uint32_t half) __attribute__((always_inline)) {
+#pragma unroll
+		for (uint32_t m = 0; m < MF; m++) {
+			r[half][m] = row_frag.get(rows, m * 16, half);
+		}
+#pragma unroll
+		for (uint32_t j = 0; j < 2 * G; j++) {
+			c[half][j] = column_frag.get(columns, j / G * kBlock + j % G * 16, 0);
+		}
+	};
+	auto mul = [&](uint32_t half) __attribute__((always_inline)) {
+#pragma unroll
+		for (uint32_t j = 0; j < 2 * G; j++) {
+#pragma unroll
+			for (uint32_t m = 0; m < MF; m++) {
+				sums[m][j / G][j % G] = multiply<T>(c[half][j], r[half][m], sums[m][j / G][j % G]);
+			}
+		}
+		also(r[half]);
+		spread_reads<MF * RowFrag::kReads + 2 * G * ColumnFrag::kReads, MF * G>();
+	};
+	if (steps == 0) {
+		return;
+	}
+	uint8_t *rows = lds, *next_rows = lds + ROWS_BYTES;
+	uint8_t *now = lds + 2 * ROWS_BYTES, *next = now + HALF_BYTES, *third = next + HALF_BYTES;
+	fill_rows(0, rows);
+	fill_columns(0, now);
+	fill_columns(1, next);
+	fill_rows(1, next_rows);
+	fill_columns(2, third);
+	landed<ROW_FILLS + 2 * COLUMN_FILLS>();
+	workgroup_meets<true>();
+	auto loop = [&](auto has_rows) __attribute__((always_inline)) {
+		constexpr bool kBusy = decltype(has_rows)::value;
+		auto turn = [&]() __attribute__((always_inline)) {
+			uint8_t *const done = now;
+			now = next;
+			next = third;
+			third = done;
+		};
+		if (kBusy) {
+			read(rows, now, 0);
+		}
+		for (uint32_t step = 0; step < steps; step++) {
+			landed<ROW_FILLS + COLUMN_FILLS>(); /* the columns' second half */
+			workgroup_meets<true>();
+			turn();
+			fill_columns(2 * step + 3, third);
+			__builtin_amdgcn_sched_barrier(0);
+			if (kBusy) {
+				read(rows, now, 1);
+				mul(0);
+			}
+			landed<COLUMN_FILLS>(); /* the next step's rows and first half */
+			workgroup_meets<true>();
+			turn();
+			fill_rows(step + 2, rows);
+			fill_columns(2 * step + 4, third);
+			uint8_t *const done = rows;
+			rows = next_rows;
+			next_rows = done;
+			__builtin_amdgcn_sched_barrier(0);
+			if (kBusy) {
+				read(rows, now, 0);
+				mul(1);
+			}
+		}
+	};
+	if (busy) {
+		loop(std::true_type{});
+	} else {
+		loop(std::false_type{});
+	}
+	landed<0>();
 }
 
 /* ---- sums ----------------------------------------------------------------------------------------------------- */

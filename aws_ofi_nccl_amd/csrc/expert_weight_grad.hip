@@ -33,6 +33,7 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct weight_operands_t {
 	static constexpr uint32_t BN = 2 * kBlock;
 	across_t<T, BM, THREADS> rows;
 	across_t<T, BN, THREADS> columns;
+	across_t<T, 2 * kBlock, THREADS, kStepRows / 2> halves;
 	weight_tile_t place;
 	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kBytes = kRowsBytes + decltype(columns)::kBytes;
 	static constexpr uint32_t kFills = decltype(rows)::kChunks + decltype(columns)::kChunks;
@@ -56,6 +57,7 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct weight_operands_t {
 		place = { expert, m0, n0, a->m - m0 < BM ? a->m - m0 : BM, a->n - n0 < BN ? a->n - n0 : BN, hi - lo, a->dbias && n0 == 0 };
 		rows.set(a->dout + lo * a->dout_pitch + m0 * 2, a->dout_pitch, hi - lo, (int64_t)place.m_there * 2);
 		columns.set(a->x + lo * a->x_pitch + n0 * 2, a->x_pitch, hi - lo, (int64_t)place.n_there * 2);
+		halves.set(a->x + lo * a->x_pitch + n0 * 2, a->x_pitch, hi - lo, (int64_t)place.n_there * 2);
 		return true;
 	}
 	__device__ __forceinline__ void load(uint32_t step)
@@ -77,11 +79,13 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct weight_operands_t {
 
 /* F32: float32 out, else T */
 template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT, bool F32>
-__global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(weight_grad_args_t)
+__global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void expert_weight_grad_kernel(weight_grad_args_t)
 {
 	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN, kStages = 2;
 	using operands_t = weight_operands_t<T, BM, THREADS>;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * operands_t::kBytes];
+	constexpr bool PAIR = WM * WN == 4;
+	constexpr uint32_t kHalfBytes = BN * kStepRows;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[PAIR ? 2 * operands_t::kRowsBytes + 3 * kHalfBytes : kStages * operands_t::kBytes];
 
 	operands_t of;
 	{
@@ -94,6 +98,12 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_weight_grad_kernel(weight
 	const weight_tile_t place = of.place;
 	f32x4_t sums[MF][2][G] = {};
 	auto sum = [&](auto also) __attribute__((always_inline)) {
+		if constexpr (PAIR) {
+			sum_halves<T, decltype(of.rows)::kChunks, decltype(of.halves)::kChunks, operands_t::kRowsBytes, kHalfBytes>(
+				sums, wm * 16 * MF < place.m_there, (place.summed + kStepRows - 1) / kStepRows, lds, across_frag_t<BM>(wm * 16 * MF, lane),
+				across_frag_t<BN>(wn * 16 * G, lane), [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.rows.fill(step, to); },
+				[&](uint32_t half, uint8_t *to) __attribute__((always_inline)) { of.halves.fill(half, to); }, also);
+		} else
 		sum_steps<T, DIRECT, kStages, operands_t::kFills>(
 			sums, wm * 16 * MF < place.m_there, (place.summed + kStepRows - 1) / kStepRows, lds, operands_t::kBytes, operands_t::kRowsBytes,
 			across_frag_t<BM>(wm * 16 * MF, lane), across_frag_t<BN>(wn * 16 * G, lane),
@@ -218,7 +228,7 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	const uint32_t n_tiles = (width + 255) / 256;
 	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * out_width) && in_chunks(d_rows, rows_pitch, 2ull * width);
 	const bool wide = direct && (uint64_t)n_experts * ((out_width + 255) / 256) * n_tiles >= kComputeUnits;
-	const uint32_t bm = wide ? 256 : 128, m_tiles = (out_width + bm - 1) / bm;
+	const uint32_t bm = 128, m_tiles = (out_width + bm - 1) / bm;
 	const uint64_t tiles = (uint64_t)n_experts * (((uint64_t)m_tiles * n_tiles + 7) / 8) * 8;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
@@ -231,13 +241,13 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 		using T = decltype(element);
 		auto of = [&](auto f32) {
 			constexpr bool F = decltype(f32)::value;
-			return direct ? (wide ? expert_weight_grad_kernel<T, 4, 2, 4, true, F> : expert_weight_grad_kernel<T, 2, 4, 4, true, F>)
+			return direct ? (wide ? expert_weight_grad_kernel<T, 2, 2, 4, true, F> : expert_weight_grad_kernel<T, 2, 4, 4, true, F>)
 				      : expert_weight_grad_kernel<T, 2, 4, 4, false, F>;
 		};
 		auto kernel = dweight_type == OFI_AMD_FLOAT32 ? of(std::true_type{}) : of(std::false_type{});
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			args.first_tile = first;
-			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), args);
+			launch_kernel(kernel, dim3(count), dim3(wide ? 256 : 512), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {
