@@ -32,12 +32,12 @@ struct backward_tile_t {
 	uint32_t rows, c0, there, n;
 };
 
-template <typename T, uint32_t BM, uint32_t THREADS> struct backward_operands_t {
+/* COLUMN_ROWS: of the summed axis in a tile of the columns, a step's or half a step's */
+template <typename T, uint32_t BM, uint32_t THREADS, uint32_t COLUMN_ROWS> struct backward_operands_t {
 	along_t<T, BM, THREADS> rows;
-	across_t<T, 2 * kBlock, THREADS> columns;
-	across_t<T, 2 * kBlock, THREADS, kStepRows / 2> halves;
+	across_t<T, 2 * kBlock, THREADS, COLUMN_ROWS> columns;
 	backward_tile_t place;
-	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kBytes = kRowsBytes + decltype(columns)::kBytes;
+	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kColumnsBytes = decltype(columns)::kBytes, kBytes = kRowsBytes + kColumnsBytes;
 	static constexpr uint32_t kFills = decltype(rows)::kChunks + decltype(columns)::kChunks;
 
 	__device__ __forceinline__ void set(const backward_args_t *a, const tile_t &tile)
@@ -46,7 +46,6 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct backward_operands_t 
 		place = { tile.from, tile.rows, c0, there, n };
 		rows.set(a->dout + tile.from * a->dout_pitch, a->dout_pitch, tile.rows, (int64_t)a->k * 2);
 		columns.set(a->w + tile.expert * a->expert_pitch + c0 * 2, a->w_pitch, a->k, (int64_t)there * 2);
-		halves.set(a->w + tile.expert * a->expert_pitch + c0 * 2, a->w_pitch, a->k, (int64_t)there * 2);
 	}
 	__device__ __forceinline__ void load(uint32_t step)
 	{
@@ -69,11 +68,10 @@ template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool HIDDEN, bool D
 __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void expert_backward_kernel(backward_args_t)
 {
 	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN;
-	using operands_t = backward_operands_t<T, BM, THREADS>;
-	constexpr uint32_t kStages = DIRECT && WM < 4 ? 3 : 2;
-	constexpr bool PAIR = WM * WN == 4;
-	constexpr uint32_t kHalfBytes = BN * kStepRows;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[PAIR ? 2 * operands_t::kRowsBytes + 3 * kHalfBytes : kStages * operands_t::kBytes];
+	constexpr bool PAIR = WM * WN == 4; /* of workgroups on a compute unit */
+	using operands_t = backward_operands_t<T, BM, THREADS, PAIR ? kStepRows / 2 : kStepRows>;
+	constexpr uint32_t kStages = DIRECT ? 3 : 2;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[PAIR ? 2 * operands_t::kRowsBytes + 3 * operands_t::kColumnsBytes : kStages * operands_t::kBytes];
 
 	operands_t of;
 	uint32_t steps;
@@ -89,17 +87,17 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void expert_bac
 	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
 	f32x4_t sums[MF][2][G] = {};
 	if constexpr (PAIR) {
-		sum_halves<T, decltype(of.rows)::kChunks, decltype(of.halves)::kChunks, operands_t::kRowsBytes, kHalfBytes>(
+		sum_halves<T, decltype(of.rows)::kChunks, decltype(of.columns)::kChunks, operands_t::kRowsBytes, operands_t::kColumnsBytes>(
 			sums, wm * 16 * MF < of.place.rows, steps, lds, along_frag_t(wm * 16 * MF, lane), across_frag_t<BN>(wn * 16 * G, lane),
 			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.rows.fill(step, to); },
-			[&](uint32_t half, uint8_t *to) __attribute__((always_inline)) { of.halves.fill(half, to); },
-			[](const u32x4_t(&)[MF]) {});
-	} else
-	sum_steps<T, DIRECT, kStages, operands_t::kFills>(
-		sums, wm * 16 * MF < of.place.rows, steps, lds, operands_t::kBytes, operands_t::kRowsBytes, along_frag_t(wm * 16 * MF, lane),
-		across_frag_t<BN>(wn * 16 * G, lane), [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.fill(step, to); },
-		[&](uint32_t step) __attribute__((always_inline)) { of.load(step); },
-		[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.store(step, to); }, [](const u32x4_t(&)[MF]) {});
+			[&](uint32_t half, uint8_t *to) __attribute__((always_inline)) { of.columns.fill(half, to); }, [](const u32x4_t(&)[MF]) {});
+	} else {
+		sum_steps<T, DIRECT, kStages, operands_t::kFills>(
+			sums, wm * 16 * MF < of.place.rows, steps, lds, operands_t::kBytes, operands_t::kRowsBytes, along_frag_t(wm * 16 * MF, lane),
+			across_frag_t<BN>(wn * 16 * G, lane), [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.fill(step, to); },
+			[&](uint32_t step) __attribute__((always_inline)) { of.load(step); },
+			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.store(step, to); }, [](const u32x4_t(&)[MF]) {});
+	}
 
 	struct in_t {
 		eight_t g[2], u[2]; /* what was kept, or what is added */
@@ -176,8 +174,10 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 	     const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t k, uint32_t n, const backward_t &o, void *stream)
 {
 	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * k) && in_chunks(d_weight, weight_pitch, 2ull * n) && expert_pitch % 16 == 0;
-	const uint32_t n_tiles = (n + 2 * kBlock - 1) / (2 * kBlock), bm = row_tile_for(max_rows, n_experts, n_tiles, direct);
-	const uint64_t tiles = most_row_tiles(max_rows, n_experts, bm == 256 ? 128 : bm) * n_tiles;
+	const uint32_t n_tiles = (n + 2 * kBlock - 1) / (2 * kBlock);
+	const bool pairs = direct && pairs_fit(max_rows, n_experts, n_tiles);
+	const uint32_t bm = pairs ? 128 : row_tile_for(max_rows, n_experts, n_tiles, false);
+	const uint64_t tiles = most_row_tiles(max_rows, n_experts, bm) * n_tiles;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
 	}
@@ -185,14 +185,14 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 				 dout_pitch, weight_pitch, expert_pitch, k, n, 0, o };
 	auto with = [&](auto element) {
 		using T = decltype(element);
-		auto kernel = direct ? (bm == 256 ? expert_backward_kernel<T, 2, 2, 4, HIDDEN, true>
-						: bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, true>
+		auto kernel = direct ? (pairs ? expert_backward_kernel<T, 2, 2, 4, HIDDEN, true>
+						   : bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, true>
 							    : expert_backward_kernel<T, 1, 8, 4, HIDDEN, true>)
 				     : bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, false>
 						 : expert_backward_kernel<T, 1, 8, 4, HIDDEN, false>;
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			args.first_tile = first;
-			launch_kernel(kernel, dim3(count), dim3(bm == 256 ? 256 : 512), 0, as_stream(stream), args);
+			launch_kernel(kernel, dim3(count), dim3(pairs ? 256 : 512), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {

@@ -1005,15 +1005,32 @@ inline uint64_t most_row_tiles(uint32_t max_rows, uint32_t n_experts, uint32_t b
 	return (max_rows - parts) / bm + parts;
 }
 
+/* Experts that have rows, at most, and the rows of each if all have the same */
+inline void spread_of(uint32_t max_rows, uint32_t n_experts, uint32_t &experts, uint32_t &of_expert)
+{
+	experts = n_experts < max_rows ? n_experts : max_rows;
+	of_expert = (max_rows + experts - 1) / experts;
+}
+
 /* Row tiles of 256, 128 or 64: the largest that the experts' rows fill and of which there are enough for the GPU.  256 with rows that
  * come through registers would not fit them. */
-inline uint32_t row_tile_for(uint32_t max_rows, uint32_t n_experts, uint32_t n_tiles, bool direct)
+inline uint32_t row_tile_for(uint32_t max_rows, uint32_t n_experts, uint32_t n_tiles, bool most_is_256)
 {
-	const uint32_t experts = n_experts < max_rows ? n_experts : max_rows, of_expert = (max_rows + experts - 1) / experts;
+	uint32_t experts, of_expert;
+	spread_of(max_rows, n_experts, experts, of_expert);
 	auto fits = [&](uint32_t bm) {
 		return of_expert > bm / 2 && (uint64_t)experts * ((of_expert + bm - 1) / bm) * n_tiles >= kComputeUnits;
 	};
-	return direct && fits(256) ? 256 : fits(128) ? 128 : 64;
+	return most_is_256 && fits(256) ? 256 : fits(128) ? 128 : 64;
+}
+
+/* Whether row tiles of 128 are filled and enough for two workgroups on each compute unit (sum_halves): 12,288 rows of 64 experts, 2048 summed to
+ * 4096 columns 288 us, with one 302; 2048 rows of 16 are too few, and take 80 us in tiles of 64 */
+inline bool pairs_fit(uint32_t max_rows, uint32_t n_experts, uint32_t n_tiles)
+{
+	uint32_t experts, of_expert;
+	spread_of(max_rows, n_experts, experts, of_expert);
+	return of_expert > 64 && (uint64_t)experts * ((of_expert + 127) / 128) * n_tiles >= 2 * kComputeUnits;
 }
 
 inline bool activation_ok(int a) { return a == OFI_AMD_NO_ACTIVATION || a == OFI_AMD_RELU || a == OFI_AMD_SILU || a == OFI_AMD_GELU; }

@@ -29,13 +29,13 @@ struct weight_tile_t {
 	bool bias; /* of one column tile, in a loop of its own */
 };
 
-template <typename T, uint32_t BM, uint32_t THREADS> struct weight_operands_t {
+/* COLUMN_ROWS: of the summed axis in a tile of the columns, a step's or half a step's */
+template <typename T, uint32_t BM, uint32_t THREADS, uint32_t COLUMN_ROWS> struct weight_operands_t {
 	static constexpr uint32_t BN = 2 * kBlock;
 	across_t<T, BM, THREADS> rows;
-	across_t<T, BN, THREADS> columns;
-	across_t<T, 2 * kBlock, THREADS, kStepRows / 2> halves;
+	across_t<T, BN, THREADS, COLUMN_ROWS> columns;
 	weight_tile_t place;
-	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kBytes = kRowsBytes + decltype(columns)::kBytes;
+	static constexpr uint32_t kRowsBytes = decltype(rows)::kBytes, kColumnsBytes = decltype(columns)::kBytes, kBytes = kRowsBytes + kColumnsBytes;
 	static constexpr uint32_t kFills = decltype(rows)::kChunks + decltype(columns)::kChunks;
 
 	/* Workgroups go to the eight XCDs in turn: each XCD has an eighth of every expert's tiles, in one piece, as the experts have unlike numbers of
@@ -57,7 +57,6 @@ template <typename T, uint32_t BM, uint32_t THREADS> struct weight_operands_t {
 		place = { expert, m0, n0, a->m - m0 < BM ? a->m - m0 : BM, a->n - n0 < BN ? a->n - n0 : BN, hi - lo, a->dbias && n0 == 0 };
 		rows.set(a->dout + lo * a->dout_pitch + m0 * 2, a->dout_pitch, hi - lo, (int64_t)place.m_there * 2);
 		columns.set(a->x + lo * a->x_pitch + n0 * 2, a->x_pitch, hi - lo, (int64_t)place.n_there * 2);
-		halves.set(a->x + lo * a->x_pitch + n0 * 2, a->x_pitch, hi - lo, (int64_t)place.n_there * 2);
 		return true;
 	}
 	__device__ __forceinline__ void load(uint32_t step)
@@ -82,10 +81,9 @@ template <typename T, uint32_t WM, uint32_t WN, uint32_t MF, bool DIRECT, bool F
 __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void expert_weight_grad_kernel(weight_grad_args_t)
 {
 	constexpr uint32_t BM = 16 * MF * WM, BN = 2 * kBlock, THREADS = 64 * WM * WN, G = 8 / WN, kStages = 2;
-	using operands_t = weight_operands_t<T, BM, THREADS>;
-	constexpr bool PAIR = WM * WN == 4;
-	constexpr uint32_t kHalfBytes = BN * kStepRows;
-	__shared__ __attribute__((aligned(1024))) uint8_t lds[PAIR ? 2 * operands_t::kRowsBytes + 3 * kHalfBytes : kStages * operands_t::kBytes];
+	constexpr bool PAIR = WM * WN == 4; /* of workgroups on a compute unit */
+	using operands_t = weight_operands_t<T, BM, THREADS, PAIR ? kStepRows / 2 : kStepRows>;
+	__shared__ __attribute__((aligned(1024))) uint8_t lds[PAIR ? 2 * operands_t::kRowsBytes + 3 * operands_t::kColumnsBytes : kStages * operands_t::kBytes];
 
 	operands_t of;
 	{
@@ -96,20 +94,22 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void expert_wei
 	}
 	const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
 	const weight_tile_t place = of.place;
+	const uint32_t steps = (place.summed + kStepRows - 1) / kStepRows;
+	const bool busy = wm * 16 * MF < place.m_there;
 	f32x4_t sums[MF][2][G] = {};
 	auto sum = [&](auto also) __attribute__((always_inline)) {
 		if constexpr (PAIR) {
-			sum_halves<T, decltype(of.rows)::kChunks, decltype(of.halves)::kChunks, operands_t::kRowsBytes, kHalfBytes>(
-				sums, wm * 16 * MF < place.m_there, (place.summed + kStepRows - 1) / kStepRows, lds, across_frag_t<BM>(wm * 16 * MF, lane),
-				across_frag_t<BN>(wn * 16 * G, lane), [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.rows.fill(step, to); },
-				[&](uint32_t half, uint8_t *to) __attribute__((always_inline)) { of.halves.fill(half, to); }, also);
-		} else
-		sum_steps<T, DIRECT, kStages, operands_t::kFills>(
-			sums, wm * 16 * MF < place.m_there, (place.summed + kStepRows - 1) / kStepRows, lds, operands_t::kBytes, operands_t::kRowsBytes,
-			across_frag_t<BM>(wm * 16 * MF, lane), across_frag_t<BN>(wn * 16 * G, lane),
-			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.fill(step, to); },
-			[&](uint32_t step) __attribute__((always_inline)) { of.load(step); },
-			[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.store(step, to); }, also);
+			sum_halves<T, decltype(of.rows)::kChunks, decltype(of.columns)::kChunks, operands_t::kRowsBytes, operands_t::kColumnsBytes>(
+				sums, busy, steps, lds, across_frag_t<BM>(wm * 16 * MF, lane), across_frag_t<BN>(wn * 16 * G, lane),
+				[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.rows.fill(step, to); },
+				[&](uint32_t half, uint8_t *to) __attribute__((always_inline)) { of.columns.fill(half, to); }, also);
+		} else {
+			sum_steps<T, DIRECT, kStages, operands_t::kFills>(
+				sums, busy, steps, lds, operands_t::kBytes, operands_t::kRowsBytes, across_frag_t<BM>(wm * 16 * MF, lane),
+				across_frag_t<BN>(wn * 16 * G, lane), [&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.fill(step, to); },
+				[&](uint32_t step) __attribute__((always_inline)) { of.load(step); },
+				[&](uint32_t step, uint8_t *to) __attribute__((always_inline)) { of.store(step, to); }, also);
+		}
 	};
 	if (place.bias) {
 		f32x4_t bias[MF] = {};
@@ -224,11 +224,10 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	    (reinterpret_cast<uintptr_t>(d_add) % size) || ((reinterpret_cast<uintptr_t>(d_dbias) | reinterpret_cast<uintptr_t>(d_bias_add)) & 3u)) {
 		return -EINVAL;
 	}
-	/* tiles of 256 x 256 where they are enough for the GPU and the experts have rows to sum, else of 128 x 256 */
-	const uint32_t n_tiles = (width + 255) / 256;
+	/* tiles of 128 x 256, two workgroups to a compute unit where they are enough for that */
+	const uint32_t n_tiles = (width + 255) / 256, m_tiles = (out_width + 127) / 128;
 	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * out_width) && in_chunks(d_rows, rows_pitch, 2ull * width);
-	const bool wide = direct && (uint64_t)n_experts * ((out_width + 255) / 256) * n_tiles >= kComputeUnits;
-	const uint32_t bm = 128, m_tiles = (out_width + bm - 1) / bm;
+	const bool pairs = direct && (uint64_t)n_experts * m_tiles * n_tiles >= 2 * kComputeUnits;
 	const uint64_t tiles = (uint64_t)n_experts * (((uint64_t)m_tiles * n_tiles + 7) / 8) * 8;
 	if (tiles > 0x7fffffffull) {
 		return -E2BIG;
@@ -241,13 +240,13 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 		using T = decltype(element);
 		auto of = [&](auto f32) {
 			constexpr bool F = decltype(f32)::value;
-			return direct ? (wide ? expert_weight_grad_kernel<T, 2, 2, 4, true, F> : expert_weight_grad_kernel<T, 2, 4, 4, true, F>)
+			return direct ? (pairs ? expert_weight_grad_kernel<T, 2, 2, 4, true, F> : expert_weight_grad_kernel<T, 2, 4, 4, true, F>)
 				      : expert_weight_grad_kernel<T, 2, 4, 4, false, F>;
 		};
 		auto kernel = dweight_type == OFI_AMD_FLOAT32 ? of(std::true_type{}) : of(std::false_type{});
 		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
 			args.first_tile = first;
-			launch_kernel(kernel, dim3(count), dim3(wide ? 256 : 512), 0, as_stream(stream), args);
+			launch_kernel(kernel, dim3(count), dim3(pairs ? 256 : 512), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {
