@@ -39,11 +39,12 @@ template <typename T, uint32_t BM, uint32_t THREADS, uint32_t COLUMN_ROWS> struc
 	static constexpr uint32_t kFills = decltype(rows)::kChunks + decltype(columns)::kChunks;
 
 	/* Workgroups go to the eight XCDs in turn: each XCD has an eighth of every expert's tiles, in one piece, as the experts have unlike numbers of
-	 * rows to sum (with whole experts to an XCD 2003 us for 32,768 rows of 32 experts).  In an expert, bands of eight row tiles.  False: `id` has none */
+	 * rows to sum (with whole experts to an XCD 1662 us for 1412 of 32,768 rows of 32 experts); one on for each expert, as the last piece may be
+	 * short or none (777 x 1023 of 60 experts has seven: 74.6 us, so 61.7).  In an expert, bands of eight row tiles.  False: `id` has none */
 	__device__ __forceinline__ bool set(const weight_grad_args_t *a, uint32_t id)
 	{
 		const uint32_t n_tiles = a->n_tiles, m_tiles = a->m_tiles, share = (m_tiles * n_tiles + 7) / 8, at = id >> 3, expert = at / share;
-		const uint32_t in_expert = (id & 7u) * share + at - expert * share;
+		const uint32_t in_expert = ((id + expert) & 7u) * share + at - expert * share;
 		if (expert >= a->n_experts || in_expert >= m_tiles * n_tiles) {
 			return false;
 		}
