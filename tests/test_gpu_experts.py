@@ -62,7 +62,7 @@ def test_a_layer_of_one_expert(lib, gpu, rows, kind, bias_type):
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 def test_large_tiles(lib, gpu, kind):
-    """256 rows a tile: products of every kind over experts of some hundreds of rows."""
+    """The forward products' tiles of 256 rows; gradients over nearly as many."""
     counts = [700, 0, 513, 256, 1, 2000]
     check_gated(lib, counts, 264, 2176, kind, kind, "e4m3")
     check_product(lib, counts, 200, 4104, kind, a="gelu", bias_type=torch.float32, residual=True, saved_kind=kind)
@@ -71,6 +71,24 @@ def test_large_tiles(lib, gpu, kind):
     check_rows(lib, counts, 4104, 264, kind, added=True)
     check_weights(lib, counts, 1032, 2056, kind, "f32", added=True, bias=True)
     check_weights(lib, counts, 1032, 2056, kind, kind, bias=True)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("summed", [8, 40, 72, 136, 264])
+def test_tiles_in_pairs(lib, gpu, kind, summed):
+    """Gradients over 512 tiles of 128 rows and more, of which a compute unit has two: sums of half a step, an odd number of halves, several steps."""
+    counts = [700, 0, 513, 256, 1, 2000]  # 30 row tiles if they were alike, 18 column tiles
+    check_hidden(lib, counts, summed, 4480, kind, "e4m3")
+    check_hidden(lib, counts, summed, 4480, kind, kind, False, "gelu", with_hidden=False)
+    check_rows(lib, counts, 4480, summed, kind, added=True)
+
+
+@pytest.mark.parametrize("kind,out", [("bf16", "f32"), ("f16", "f32"), ("bf16", "bf16"), ("f16", "f16")])
+def test_weight_tiles_in_pairs(lib, gpu, kind, out):
+    """The same where the rows of an expert are summed: none, one, half a step and one more, several steps; the bias is of the first column tile."""
+    counts = [700, 0, 33, 64, 1, 65, 32, 129]  # 8 x 13 x 5 tiles
+    check_weights(lib, counts, 1032, 1560, kind, out, bias=True)
+    check_weights(lib, counts, 1280, 1664, kind, out, added=True, bias=True, in_place=True)
 
 
 def test_large_tiles_of_8_bits(lib, gpu):
