@@ -6,6 +6,9 @@
  * A wavefront has 16 columns of both parts (the gate's and the other's, or two neighbouring groups) and every KS-th step of 128 bytes of
  * their rows; what the KS have summed is added in LDS, in their order.  CG wavefronts side by side make a workgroup of 16 CG columns:
  * eight where a block of 128 shares an output's scale, else one, for as many workgroups as there can be.
+ * 8 rows of 8 of 32 experts in 8 bits: product of 2048 to 4096 17.5 us (3.9 TB/s of weights with the launch), gated 4096 to 2048 32 us (4.2 TB/s) into
+ * bfloat16 and 41 into 8 bits, as 16 blocks of 8 experts are half of the compute units; in bfloat16 31 and 55 us (4.3 and 4.9 TB/s).  128
+ * rows of all 32, gated, bfloat16: 176 us, 6.0 TB/s.
  */
 #include "expert_forward.hpp"
 

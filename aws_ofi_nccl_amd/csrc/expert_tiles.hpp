@@ -2,13 +2,13 @@
  * What the experts' products share: which rows of which expert a workgroup takes, how tiles of both operands come into LDS and
  * from there to the matrix cores, and how sums leave in rows.
  *
- * A workgroup of WM x WN wavefronts computes BM = 64 WM rows (of the result) by two parts of 128 columns: a part is the gate's or the
+ * A workgroup of WM x WN wavefronts computes 64 WM rows (of the result) by two parts of 128 columns: a part is the gate's or the
  * other projection's share of a gated block, or half of 256 neighbouring columns.  A wavefront has 64 rows and 128 / WN columns of both
  * parts, so that a gate's sums and those they are multiplied with lie in the same lane, and each part is one block of 128 columns that
  * shares an 8-bit scale.
  *
  * The summed axis is taken in steps: 128 bytes of a row where the operand's rows run along it ("along"), 64 rows where they run
- * across it ("across").  Two tiles of LDS take turns: while one is computed on, the other is filled.
+ * across it ("across").  Two or three tiles of LDS take turns: while one is computed on, the others are filled (sum_steps, sum_halves).
  *   along    16-byte chunk c of row r lies at slot c ^ (r & 7) of the row: eight rows' same chunk, which eight lanes read at once,
  *            are in eight different groups of banks
  *   across   row k's chunk c lies at slot c ^ 2 (k & 3 | (k >> 3 & 1) << 2): four rows' same 32 bytes, which sixteen lanes read and
@@ -535,8 +535,11 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 
 /*
  * The same for workgroups of four wavefronts, of which a compute unit has two: while one is at its beginning, its epilogue or a barrier, the other
- * multiplies.  Each has 80 KB of LDS: the rows' tiles of two steps, and the columns' of three halves of a step.  They come that many steps and halves
- * before they are read.
+ * multiplies.  Each has 80 KB of LDS: the rows' tiles of two steps, and the columns' of three halves of a step, asked for that long before they
+ * are read.  For columns across the summed axis, whose half a step is half of the rows; half of 128 bytes along it would be half a line.
+ * Tiles of 256 x 256, one to a compute unit, and these (32,768 rows of 32 experts; us): hidden_grad of 4096 to 2048 731 and 645, rows_grad of
+ * 4096 to 4096 1032 and 1010, weight_grad of 4096 x 4096 into float32 1545 and 1415.  With columns along the axis, three tiles of 128 columns and a
+ * step each for three halves, gated 4096 to 2048 took 1094 for 1086 and product 8192 x 4096 x 4096 295 for 277: those stay with sum_steps.
  */
 template <typename T, uint32_t ROW_FILLS, uint32_t COLUMN_FILLS, uint32_t ROWS_BYTES, uint32_t HALF_BYTES, uint32_t MF, uint32_t G, typename RowFrag,
 	  typename ColumnFrag, typename FillRows, typename FillColumns, typename Also>

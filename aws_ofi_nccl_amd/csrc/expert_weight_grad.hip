@@ -2,6 +2,9 @@
  * Gradients of the experts' weights and biases: dW_e = add + sum over the expert's rows of dy[r]^T x[r], db_e = add + sum of dy[r].
  * Both operands run across the summed axis, which is as long as the expert has rows; a workgroup sums all of it for one tile of
  * one expert's matrix, so that every sum runs in the rows' order.  The bias is the product with a column of ones.
+ * 32,768 rows of 32 experts, 4096 x 4096, bfloat16, us: bfloat16 out 1150 (956 TFLOP/s), float32 out 1270, float32 added to float32 1415 (4.8 GB at 3.4
+ * TB/s, 776 TFLOP/s): the matrix cores and, for float32, the memory's share that two workgroups on a compute unit do not hide.  1331 rows of 60
+ * experts, 777 x 1023: 62 us, of 776 x 1024 37, where most of a tile's time is its beginning and its epilogue.
  */
 #include "expert_tiles.hpp"
 

@@ -34,6 +34,11 @@ nothing else of interest, which keeps counter runs short.  The shapes:
   dispatch  <tokens>     rows of 8 KiB to 8 of 128 experts each (default 32,768)
   combine   <tokens>     8 rows of 8 KiB bfloat16 and an addend to a token, weighted (default 16,384)
   combine_grad <tokens>  the sum's gradients (default 16,384)
+  gated     <rows>       rows of 4096 sorted by 32 experts, chosen evenly at random, through gated blocks of 2048 columns, bfloat16 with a
+                         checkpoint of 8 bits (default 32,768 rows); gated8: rows, weights and output in 8 bits (default 16,384)
+  product   <rows>       the product behind them, 2048 to 4096 (default 32,768); product8: rows and weights in 8 bits (default 8)
+  hidden_grad, rows_grad, weight_grad <rows>  the gradients: of the block's hidden columns from the checkpoint of 8 bits; of rows of
+                         4096, summed over 4096; of weights of 4096 x 4096, added in float32 (default 32,768)
 """
 import argparse
 import ctypes
@@ -89,9 +94,70 @@ def token_step(m, lib, torch, kernel, tokens, stream):
                                                           width, bf16, *at(drows), dweight.data_ptr(), stream), "token_combine_grad")
 
 
+EXPERT_ROWS = {"gated": 32768, "gated8": 16384, "product": 32768, "product8": 8, "hidden_grad": 32768, "rows_grad": 32768, "weight_grad": 32768}
+
+
+def expert_step(m, lib, torch, kernel, rows, stream):
+    """One call of an experts' product on `rows` rows, as a function; everything it works on is kept by it."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(SEED)
+    experts, width, inner, bf16 = 32, 4096, 2048, m.BFLOAT16
+    of = torch.randint(0, experts, (rows,), generator=g, device="cuda")
+    offset = torch.cat([of.new_zeros(1), torch.bincount(of, minlength=experts).cumsum(0)]).to(torch.int32)
+    at = lambda t: (t.data_ptr(), t.stride(-2) * t.element_size())
+    weights = lambda t: (t.data_ptr(), t.stride(1) * t.element_size(), t.stride(0) * t.element_size())
+    empty = lambda *size, dtype=torch.bfloat16: torch.empty(*size, dtype=dtype, device="cuda")
+
+    def values(*size, eight=False, scale=1.0):
+        """bfloat16, or 8 bits and their scales: of rows for 128 columns, of matrices for blocks of 128 x 128"""
+        v = torch.empty(*size, dtype=torch.bfloat16, device="cuda")
+        for piece in v if len(size) == 3 else [v]:
+            piece.copy_(torch.randn(*piece.shape, generator=g, device="cuda") * scale)
+        if not eight:
+            return v
+        blocks = size[-1] // 128
+        scales = torch.full((size[0], size[1] // 128, blocks) if len(size) == 3 else (size[0], blocks), 1 / 64, device="cuda")
+        return (v.float() * 64).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8), scales
+
+    groups = lambda: (offset.data_ptr(), experts, rows)
+    none = (None, 0)
+    if kernel in ("gated", "gated8"):
+        eight = kernel == "gated8"
+        x, w = values(rows, width, eight=eight), values(experts, 2 * inner, width, eight=eight, scale=1 / 64)
+        if eight:
+            (x, x_scale), (w, w_scale) = x, w
+            out, out_scale = empty(rows, inner, dtype=torch.uint8), empty(rows, inner // 128, dtype=torch.float32)
+            return lambda: m.check(lib.ofi_amd_expert_gated(*at(x), *at(x_scale), m.E4M3, *groups(), *weights(w), w_scale.data_ptr(), width, inner,
+                                                            m.SILU, *at(out), m.E4M3, *at(out_scale), *none, 0, *none, stream), kernel)
+        out, saved, saved_scale = empty(rows, inner), empty(rows, 2 * inner, dtype=torch.uint8), empty(rows, 2 * inner // 128, dtype=torch.float32)
+        return lambda: m.check(lib.ofi_amd_expert_gated(*at(x), *none, bf16, *groups(), *weights(w), None, width, inner, m.SILU, *at(out), bf16,
+                                                        *none, *at(saved), m.E4M3, *at(saved_scale), stream), kernel)
+    if kernel in ("product", "product8"):
+        eight = kernel == "product8"
+        x, w, out = values(rows, inner, eight=eight), values(experts, width, inner, eight=eight, scale=1 / 64), empty(rows, width)
+        x_scale = w_scale = None
+        if eight:
+            (x, x_scale), (w, w_scale) = x, w
+        return lambda: m.check(lib.ofi_amd_expert_product(*at(x), *(at(x_scale) if eight else none), m.E4M3 if eight else bf16, *groups(), *weights(w),
+                                                          w_scale.data_ptr() if eight else None, inner, width, None, m.FLOAT32, m.NO_ACTIVATION,
+                                                          *none, *at(out), bf16, *none, *none, 0, *none, stream), kernel)
+    dout = values(rows, width)
+    if kernel == "hidden_grad":
+        w, (saved, scale) = values(experts, width, inner, scale=1 / 64), values(rows, 2 * inner, eight=True)
+        dsaved, hidden = empty(rows, 2 * inner), empty(rows, inner)
+        return lambda: m.check(lib.ofi_amd_expert_hidden_grad(*at(dout), bf16, *groups(), *weights(w), width, inner, 1, m.SILU, *at(saved), m.E4M3,
+                                                              *at(scale), *at(dsaved), *at(hidden), stream), kernel)
+    if kernel == "rows_grad":
+        w, drows = values(experts, width, width, scale=1 / 64), empty(rows, width)
+        return lambda: m.check(lib.ofi_amd_expert_rows_grad(*at(dout), bf16, *groups(), *weights(w), width, width, *none, *at(drows), stream), kernel)
+    x, dweight = values(rows, width), torch.zeros(experts, width, width, device="cuda")
+    return lambda: m.check(lib.ofi_amd_expert_weight_grad(*at(dout), *at(x), bf16, *groups(), width, width, dweight.data_ptr(), *weights(dweight),
+                                                          m.FLOAT32, None, None, stream), kernel)
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--kernel", required=True, choices=["bounce", "copy", "fill", "table", "striping", "model", "region", "eager"] + sorted(TOKEN_ROWS))
+    ap.add_argument("--kernel", required=True, choices=["bounce", "copy", "fill", "table", "striping", "model", "region", "eager"] + sorted(TOKEN_ROWS) + sorted(EXPERT_ROWS))
     ap.add_argument("--shape", default=None)
     ap.add_argument("--launches", type=int, default=30)
     ap.add_argument("--buffers", type=int, default=None,
@@ -164,6 +230,8 @@ def main():
         print("payload bytes per launch: %d, buffers: %d" % (w["src_bytes"], n))
     elif args.kernel in TOKEN_ROWS:
         step = token_step(m, lib, torch, args.kernel, int(args.shape or TOKEN_ROWS[args.kernel]), stream)
+    elif args.kernel in EXPERT_ROWS:
+        step = expert_step(m, lib, torch, args.kernel, int(args.shape or EXPERT_ROWS[args.kernel]), stream)
     elif args.kernel == "fill":
         d_fill = torch.empty(int(args.shape or "100") << 20, dtype=torch.uint8, device="cuda")
         step = lambda: d_fill.fill_(7)

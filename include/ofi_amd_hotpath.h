@@ -1106,7 +1106,7 @@ int ofi_amd_expert_product(const void *d_rows, uint64_t rows_pitch, const float 
  *   gated   dsaved = (dh * u * act'(g), dh * act(g)), 2 * inner columns;   hidden = act(g) * u
  *   else    dsaved = dh * act'(g), inner columns;                          hidden = act(g)
  * dsaved and hidden (or NULL: the block's output again, for the weights' gradient of the product, so that
- * it need not be kept) are of dout's type.  d_saved and d_dsaved do not overlap.
+ * it need not be kept) are of dout's type.  Neither overlaps d_saved or the other.
  */
 int ofi_amd_expert_hidden_grad(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d_offset, uint32_t n_experts,
 			       uint32_t max_rows, const void *d_weight, uint64_t weight_pitch, uint64_t expert_pitch, uint32_t width,
