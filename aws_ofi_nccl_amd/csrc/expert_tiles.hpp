@@ -785,11 +785,16 @@ __device__ __forceinline__ f32x8_t read_floats(const uint8_t *p, uint32_t left)
 }
 
 /* Each value is rounded to the type once, to nearest even */
-template <typename T> __device__ __forceinline__ void write_as(uint8_t *p, uint32_t left, f32x8_t v)
+template <typename T, bool STREAM = false> __device__ __forceinline__ void write_as(uint8_t *p, uint32_t left, f32x8_t v)
 {
 	const auto r = __builtin_convertvector(v, raw_t<T, 8>);
 	if (left >= 8) {
-		*reinterpret_cast<typename piece_t<T, 8>::anywhere *>(p) = r;
+		auto *const q = reinterpret_cast<typename piece_t<T, 8>::anywhere *>(p);
+		if (STREAM) {
+			__builtin_nontemporal_store(r, q);
+		} else {
+			*q = r;
+		}
 	} else {
 #pragma unroll
 		for (uint32_t i = 0; i < 7; i++) {
@@ -800,9 +805,12 @@ template <typename T> __device__ __forceinline__ void write_as(uint8_t *p, uint3
 	}
 }
 
-/* `left` of four values at p: zeros for the others */
+/* `left` of four values at p, which nothing reads again soon: zeros for the others */
 __device__ __forceinline__ f32x4_t read_four(const float *p, uint32_t left)
 {
+	if (left >= 4) {
+		return __builtin_nontemporal_load(reinterpret_cast<const piece_t<float, 4>::anywhere *>(p));
+	}
 	f32x4_t v;
 	read_words<float, 4>(reinterpret_cast<const uint8_t *>(p), left, v);
 	return v;
@@ -810,7 +818,7 @@ __device__ __forceinline__ f32x4_t read_four(const float *p, uint32_t left)
 __device__ __forceinline__ void write_four(float *p, uint32_t left, f32x4_t v)
 {
 	if (left >= 4) {
-		*reinterpret_cast<piece_t<float, 4>::anywhere *>(p) = v;
+		__builtin_nontemporal_store(v, reinterpret_cast<piece_t<float, 4>::anywhere *>(p));
 	} else {
 #pragma unroll
 		for (uint32_t i = 0; i < 3; i++) {
@@ -822,11 +830,11 @@ __device__ __forceinline__ void write_four(float *p, uint32_t left, f32x4_t v)
 }
 
 /* Eight columns of the row that is `row` behind `from`, if it is one of the rows there are, as far as columns are left; WHOLE: both are */
-template <bool WHOLE, typename T>
+template <bool WHOLE, typename T, bool STREAM = false>
 __device__ __forceinline__ void write_row_as(const matrix_t &m, uint64_t from, uint64_t column, uint32_t row, uint32_t rows, uint32_t left, f32x8_t v)
 {
 	if (WHOLE || (row < rows && left)) {
-		write_as<T>(m.p + from * m.pitch + column * sizeof(T) + row * m.pitch, WHOLE ? 8 : left, v);
+		write_as<T, STREAM>(m.p + from * m.pitch + column * sizeof(T) + row * m.pitch, WHOLE ? 8 : left, v);
 	}
 }
 

@@ -2,9 +2,9 @@
  * Gradients of the experts' weights and biases: dW_e = add + sum over the expert's rows of dy[r]^T x[r], db_e = add + sum of dy[r].
  * Both operands run across the summed axis, which is as long as the expert has rows; a workgroup sums all of it for one tile of
  * one expert's matrix, so that every sum runs in the rows' order.  The bias is the product with a column of ones.
- * 32,768 rows of 32 experts, 4096 x 4096, bfloat16, us: bfloat16 out 1150 (956 TFLOP/s), float32 out 1270, float32 added to float32 1415 (4.8 GB at 3.4
- * TB/s, 776 TFLOP/s): the matrix cores and, for float32, the memory's share that two workgroups on a compute unit do not hide.  1331 rows of 60
- * experts, 777 x 1023: 62 us, of 776 x 1024 37, where most of a tile's time is its beginning and its epilogue.
+ * 32,768 rows of 32 experts, 4096 x 4096, bfloat16, us: bfloat16 out 1170 (940 TFLOP/s), float32 out 1280, float32 added to float32 1390 (4.8 GB at 3.5
+ * TB/s, 790 TFLOP/s): the matrix cores and, for float32, the memory's share that two workgroups on a compute unit do not hide.  1331 rows of 60
+ * experts, 777 x 1023: 60 us, of 776 x 1024 33, where most of a tile's time is its beginning and its epilogue.
  */
 #include "expert_tiles.hpp"
 
@@ -139,7 +139,8 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void expert_wei
 		sum([](const u32x4_t(&)[MF]) {});
 	}
 
-	/* a lane's columns of each part: of float32 four, and four 64 further, so that sixteen lanes have 256 bytes of a row both times; of 16 bits eight */
+	/* Written past the caches, which are for the operands (float32 added to float32 1448 -> 1399 us, 776 x 1024 of 60 experts 36.3 -> 33.4).
+	 * A lane's columns of each part: of float32 four, and four 64 further, so that sixteen lanes have 256 bytes of a row both times; of 16 bits eight */
 	struct in_t {
 		eight_t eight[F32 ? 1 : 2];
 		f32x4_t four[F32 ? 4 : 1];
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void expert_wei
 					if (a->add.p) {
 						v += floats_of<T>(in.eight[i].words);
 					}
-					write_row_as<WHOLE, T>(out, place.m0, place.n0 + c, r, place.m_there, WHOLE ? 8 : left_of(c), v);
+					write_row_as<WHOLE, T, true>(out, place.m0, place.n0 + c, r, place.m_there, WHOLE ? 8 : left_of(c), v);
 				}
 			}
 		});
