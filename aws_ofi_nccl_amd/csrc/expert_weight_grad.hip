@@ -229,6 +229,10 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 	    (reinterpret_cast<uintptr_t>(d_add) % size) || ((reinterpret_cast<uintptr_t>(d_dbias) | reinterpret_cast<uintptr_t>(d_bias_add)) & 3u)) {
 		return -EINVAL;
 	}
+	if (max_rows == 1) { /* may be apart by anything; rows behind it have to lie behind its bytes, where zeros are read */
+		dout_pitch = 2ull * out_width;
+		rows_pitch = 2ull * width;
+	}
 	/* tiles of 128 x 256, two workgroups to a compute unit where they are enough for that */
 	const uint32_t n_tiles = (width + 255) / 256, m_tiles = (out_width + 127) / 128;
 	const bool direct = in_chunks(d_dout, dout_pitch, 2ull * out_width) && in_chunks(d_rows, rows_pitch, 2ull * width);

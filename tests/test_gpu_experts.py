@@ -2,7 +2,9 @@
 import pytest
 import torch
 
-from _experts import check_gated, check_hidden, check_product, check_rows, check_weights
+import _gpu
+import aws_ofi_nccl_amd as m
+from _experts import check_gated, check_hidden, check_product, check_rows, check_weights, gen, rnd
 from _rows import Rows
 
 pytestmark = pytest.mark.gpu
@@ -89,6 +91,20 @@ def test_weight_tiles_in_pairs(lib, gpu, kind, out):
     counts = [700, 0, 33, 64, 1, 65, 32, 129]  # 8 x 13 x 5 tiles
     check_weights(lib, counts, 1032, 1560, kind, out, bias=True)
     check_weights(lib, counts, 1280, 1664, kind, out, added=True, bias=True, in_place=True)
+
+
+@pytest.mark.parametrize("width,n", [(64, 64), (256, 264), (2048, 8192), (33, 65)])
+@pytest.mark.parametrize("pitch", [0, 16])
+def test_one_row_with_any_pitch(lib, gpu, width, n, pitch):
+    """A single row is summed once, whatever its pitch says of a next one."""
+    g = gen(width)
+    dout, x = (rnd(g, 1, k).to(torch.bfloat16) for k in (n, width))
+    dw, dbias = torch.full((n, width), 7.0, device="cuda"), torch.full((n,), 7.0, device="cuda")
+    assert lib.ofi_amd_expert_weight_grad(dout.data_ptr(), pitch, x.data_ptr(), pitch, m.BFLOAT16, None, 1, 1, width, n, None, dw.data_ptr(),
+                                          4 * width, 0, m.FLOAT32, None, dbias.data_ptr(), None) == 0
+    _gpu.sync()
+    assert torch.equal(dw, dout.float().t() * x.float())  # a product of two bfloat16 values is a float32 value
+    assert torch.equal(dbias, dout[0].float())
 
 
 def test_large_tiles_of_8_bits(lib, gpu):
