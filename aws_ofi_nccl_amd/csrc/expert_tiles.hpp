@@ -536,10 +536,11 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 /*
  * The same for workgroups of four wavefronts, of which a compute unit has two: while one is at its beginning, its epilogue or a barrier, the other
  * multiplies.  Each has 80 KB of LDS: the rows' tiles of two steps, and the columns' of three halves of a step, asked for that long before they
- * are read.  For columns across the summed axis, whose half a step is half of the rows; half of 128 bytes along it would be half a line.
+ * are read.  For columns across the summed axis, whose half a step is half of the rows.
  * Tiles of 256 x 256, one to a compute unit, and these (32,768 rows of 32 experts; us): hidden_grad of 4096 to 2048 731 and 645, rows_grad of
- * 4096 to 4096 1032 and 1010, weight_grad of 4096 x 4096 into float32 1545 and 1415.  With columns along the axis, three tiles of 128 columns and a
- * step each for three halves, gated 4096 to 2048 took 1094 for 1086 and product 8192 x 4096 x 4096 295 for 277: those stay with sum_steps.
+ * 4096 to 4096 1032 and 1010, weight_grad of 4096 x 4096 into float32 1545 and 1415.  Columns along the axis stay with sum_steps: half a step of
+ * them is half of a line (gated 4096 to 2048 1090 and 1145, product of 8192 rows 4096 x 4096 270 and 295), and units of 128 columns and a whole
+ * step instead, for which the rows are read from LDS twice, gain nothing (1086 and 1094, 277 and 295).
  */
 template <typename T, uint32_t ROW_FILLS, uint32_t COLUMN_FILLS, uint32_t ROWS_BYTES, uint32_t HALF_BYTES, uint32_t MF, uint32_t G, typename RowFrag,
 	  typename ColumnFrag, typename FillRows, typename FillColumns, typename Also>
