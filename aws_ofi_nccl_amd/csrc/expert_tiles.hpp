@@ -195,7 +195,7 @@ __device__ __forceinline__ void to_lds(const uint8_t *p, int bytes, uint32_t off
 	const uint64_t at = reinterpret_cast<uint64_t>(p);
 	const i32x4_t buffer = { (int)uniform((uint32_t)at), (int)uniform((uint32_t)(at >> 32) & 0xffffu), (int)uniform((uint32_t)bytes), 0x00020000 };
 	const uint32_t to = uniform((uint32_t)reinterpret_cast<uintptr_t>((lds_void_t *)lds));
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory");
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory", "m0");
 }
 /* The same of 4 bytes for each lane */
 __device__ __forceinline__ void words_to_lds(const uint8_t *p, int bytes, uint32_t offset, uint8_t *lds)
@@ -203,7 +203,7 @@ __device__ __forceinline__ void words_to_lds(const uint8_t *p, int bytes, uint32
 	const uint64_t at = reinterpret_cast<uint64_t>(p);
 	const i32x4_t buffer = { (int)uniform((uint32_t)at), (int)uniform((uint32_t)(at >> 32) & 0xffffu), (int)uniform((uint32_t)bytes), 0x00020000 };
 	const uint32_t to = uniform((uint32_t)reinterpret_cast<uintptr_t>((lds_void_t *)lds));
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory");
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory", "m0");
 }
 /* All but the last N of the wavefront's to_lds have landed */
 template <uint32_t N> __device__ __forceinline__ void landed()

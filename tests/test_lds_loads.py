@@ -68,3 +68,22 @@ def test_descriptors_are_there_when_a_load_to_lds_reads_them(name, tmp_path):
     found, loads = too_early(device_code(name, str(tmp_path)))
     assert not found, "%d of %d, the first: %s / %s" % (len(found), loads, *found[0])
     assert loads > 0 or name == "expert_few"
+
+
+def test_the_place_in_lds_is_set_for_each_load(tmp_path):
+    """M0, which has it, is the compiler's too: behind a load that sets it, the compiler's next one sets it anew."""
+    from aws_ofi_nccl_amd import build
+    if not os.path.exists(build.HIPCC):
+        pytest.skip("no compiler")
+    out = os.path.join(str(tmp_path), "places.s")
+    subprocess.run([build.HIPCC] + build.COMMON + ["-w", "--cuda-device-only", "-S", "-x", "hip",
+                                                   os.path.join(ROOT, "tests", "host", "lds_places_kernel.hip"), "-o", out], check=True)
+    with open(out) as f:
+        code = [line.split(";")[0].strip() for line in f]
+    set_since, loads = False, 0
+    for line in code:
+        set_since = set_since or line.startswith("s_mov_b32 m0,")
+        if line.startswith("buffer_load") and line.endswith(" lds"):
+            assert set_since, line
+            set_since, loads = False, loads + 1
+    assert loads == 5
