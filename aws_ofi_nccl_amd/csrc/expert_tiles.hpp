@@ -187,7 +187,7 @@ template <typename T> __device__ __forceinline__ u32x4_t chunk_at(const uint8_t 
  * zeros from beyond the buffer.  Written as the instruction, because the compiler waits for the builtin's bytes before the next
  * exchanging read of LDS, whichever part of it that reads: the wait is landed()'s.  What the compiler sees to in front of its own loads is done
  * here too: a scalar register that a vector instruction wrote (uniform(), or a spilled one's return) is not there for a load before five wait
- * states, which the move and s_nop 3 are, and M0 not before one.
+ * states, which s_nop 4 is, and M0, from which the place is taken, not before one.
  */
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void to_lds(const uint8_t *p, int bytes, uint32_t offset, uint8_t *lds)
@@ -195,7 +195,7 @@ __device__ __forceinline__ void to_lds(const uint8_t *p, int bytes, uint32_t off
 	const uint64_t at = reinterpret_cast<uint64_t>(p);
 	const i32x4_t buffer = { (int)uniform((uint32_t)at), (int)uniform((uint32_t)(at >> 32) & 0xffffu), (int)uniform((uint32_t)bytes), 0x00020000 };
 	const uint32_t to = uniform((uint32_t)reinterpret_cast<uintptr_t>((lds_void_t *)lds));
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory", "m0");
+	asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(to), "v"(offset), "s"(buffer) : "memory");
 }
 /* The same of 4 bytes for each lane */
 __device__ __forceinline__ void words_to_lds(const uint8_t *p, int bytes, uint32_t offset, uint8_t *lds)
@@ -203,7 +203,7 @@ __device__ __forceinline__ void words_to_lds(const uint8_t *p, int bytes, uint32
 	const uint64_t at = reinterpret_cast<uint64_t>(p);
 	const i32x4_t buffer = { (int)uniform((uint32_t)at), (int)uniform((uint32_t)(at >> 32) & 0xffffu), (int)uniform((uint32_t)bytes), 0x00020000 };
 	const uint32_t to = uniform((uint32_t)reinterpret_cast<uintptr_t>((lds_void_t *)lds));
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer) : "memory", "m0");
+	asm volatile("s_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"{m0}"(to), "v"(offset), "s"(buffer) : "memory");
 }
 /* All but the last N of the wavefront's to_lds have landed */
 template <uint32_t N> __device__ __forceinline__ void landed()

@@ -82,7 +82,7 @@ def test_the_place_in_lds_is_set_for_each_load(tmp_path):
         code = [line.split(";")[0].strip() for line in f]
     set_since, loads = False, 0
     for line in code:
-        set_since = set_since or line.startswith("s_mov_b32 m0,")
+        set_since = set_since or bool(re.match(r"s_\w+ m0,", line))
         if line.startswith("buffer_load") and line.endswith(" lds"):
             assert set_since, line
             set_since, loads = False, loads + 1
