@@ -85,11 +85,11 @@ template <typename T> struct as_declared { /* an argument is converted to the ke
  * 16,384 signals 13.1 both ways.  (From process to process such calls differ by up to 0.8.)  The error is the runtime's last
  * one, as with <<<>>>. */
 template <typename... P>
-inline void launch_kernel(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds_bytes, hipStream_t stream,
+inline bool launch_kernel(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds_bytes, hipStream_t stream,
 			  typename as_declared<P>::type... args)
 {
 	void *at[] = { const_cast<void *>(static_cast<const void *>(&args))... };
-	(void)hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, at, lds_bytes, stream);
+	return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, at, lds_bytes, stream) == hipSuccess;
 }
 
 enum : uint32_t {

@@ -201,10 +201,11 @@ int forward_few(const void *d_rows, uint64_t rows_pitch, int type, const int32_t
 		using T = decltype(element);
 		auto kernel = blocks ? (bm == 16 ? expert_few_kernel<T, 1, 8, 2> : bm == 32 ? expert_few_kernel<T, 2, 8, 1> : expert_few_kernel<T, 4, 8, 1>)
 				     : (bm == 16 ? expert_few_kernel<T, 1, 1, 8> : bm == 32 ? expert_few_kernel<T, 2, 1, 8> : expert_few_kernel<T, 4, 1, 8>);
-		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
-			launch_kernel(kernel, dim3(count), dim3(blocks && bm == 16 ? 1024 : 512), 0, as_stream(stream), d_offset,
-				      static_cast<const uint8_t *>(d_rows), static_cast<const uint8_t *>(d_weight), n_experts, max_rows, width, n,
-				      n_tiles, first, rows_pitch, weight_pitch, expert_pitch, o);
+		const uint32_t lanes = blocks && bm == 16 ? 1024 : 512;
+		launch_tiles(tiles, lanes, [&](uint32_t first, uint32_t count) {
+			return launch_kernel(kernel, dim3(count), dim3(lanes), 0, as_stream(stream), d_offset, static_cast<const uint8_t *>(d_rows),
+					     static_cast<const uint8_t *>(d_weight), n_experts, max_rows, width, n, n_tiles, first, rows_pitch,
+					     weight_pitch, expert_pitch, o);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {

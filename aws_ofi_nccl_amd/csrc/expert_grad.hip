@@ -194,9 +194,10 @@ int backward(const void *d_dout, uint64_t dout_pitch, int type, const int32_t *d
 							    : expert_backward_kernel<T, 1, 8, 4, HIDDEN, true>)
 				     : bm == 128 ? expert_backward_kernel<T, 2, 4, 4, HIDDEN, false>
 						 : expert_backward_kernel<T, 1, 8, 4, HIDDEN, false>;
-		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
+		const uint32_t lanes = pairs ? 256 : 512;
+		launch_tiles(tiles, lanes, [&](uint32_t first, uint32_t count) {
 			args.first_tile = first;
-			launch_kernel(kernel, dim3(count), dim3(pairs ? 256 : 512), 0, as_stream(stream), args);
+			return launch_kernel(kernel, dim3(count), dim3(lanes), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {

@@ -245,9 +245,9 @@ int forward(const void *d_rows, uint64_t rows_pitch, int type, const int32_t *d_
 		auto kernel = direct ? (bm == 256 ? expert_forward_kernel<T, 4, 2, 4, true>
 						: bm == 128 ? expert_forward_kernel<T, 2, 4, 4, true> : expert_forward_kernel<T, 1, 8, 4, true>)
 				     : bm == 128 ? expert_forward_kernel<T, 2, 4, 4, false> : expert_forward_kernel<T, 1, 8, 4, false>;
-		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
+		launch_tiles(tiles, 512, [&](uint32_t first, uint32_t count) {
 			args.first_tile = first;
-			launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), args);
+			return launch_kernel(kernel, dim3(count), dim3(512), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {

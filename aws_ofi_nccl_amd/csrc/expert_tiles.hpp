@@ -1001,14 +1001,18 @@ inline bool in_chunks(const void *p, uint64_t pitch, uint64_t bytes)
 	return ((reinterpret_cast<uintptr_t>(p) | pitch | bytes) & 15u) == 0 && pitch <= kMostPitch;
 }
 
-constexpr uint32_t kTilesOfLaunch = 1u << 22; /* with 512 lanes each within the 32 bits of a launch's size */
+constexpr uint32_t kLanesOfLaunch = 1u << 31; /* within the 32 bits of a launch's size */
 
-/* Calls launch(first tile, tiles) until all are launched; the tiles' number is a multiple of 8 */
-template <typename F> inline void launch_tiles(uint64_t tiles, F launch)
+/* Calls launch(first tile, tiles) until all are launched, or one was not, which hipGetLastError then tells; `lanes` (a power of 2) are a
+ * tile's, the tiles' number is a multiple of 8 */
+template <typename F> inline void launch_tiles(uint64_t tiles, uint32_t lanes, F launch)
 {
+	const uint64_t most = kLanesOfLaunch / lanes;
 	tiles = (tiles + 7) / 8 * 8;
-	for (uint64_t at = 0; at < tiles; at += kTilesOfLaunch) {
-		launch((uint32_t)at, (uint32_t)(tiles - at < kTilesOfLaunch ? tiles - at : kTilesOfLaunch));
+	for (uint64_t at = 0; at < tiles; at += most) {
+		if (!launch((uint32_t)at, (uint32_t)(tiles - at < most ? tiles - at : most))) {
+			return;
+		}
 	}
 }
 

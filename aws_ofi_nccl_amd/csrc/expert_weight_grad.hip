@@ -253,9 +253,10 @@ int ofi_amd_expert_weight_grad(const void *d_dout, uint64_t dout_pitch, const vo
 				      : expert_weight_grad_kernel<T, 2, 4, 4, false, F>;
 		};
 		auto kernel = dweight_type == OFI_AMD_FLOAT32 ? of(std::true_type{}) : of(std::false_type{});
-		launch_tiles(tiles, [&](uint32_t first, uint32_t count) {
+		const uint32_t lanes = pairs ? 256 : 512;
+		launch_tiles(tiles, lanes, [&](uint32_t first, uint32_t count) {
 			args.first_tile = first;
-			launch_kernel(kernel, dim3(count), dim3(pairs ? 256 : 512), 0, as_stream(stream), args);
+			return launch_kernel(kernel, dim3(count), dim3(lanes), 0, as_stream(stream), args);
 		});
 	};
 	if (type == OFI_AMD_BFLOAT16) {
