@@ -902,7 +902,10 @@ __device__ __forceinline__ float logistic(float v) { return __builtin_amdgcn_rcp
 /*
  * The normal distribution's share below v, and e^(-v^2/2).  Below 0 it is e^(-v^2/2) t P(t) with t = 1 / (1 + 0.45 |v| / sqrt 2): t P(t)
  * is half of e^(z^2) erfc(z), fitted over all z >= 0 (least squares in Chebyshev polynomials, weights drawn to the largest relative
- * errors), 3e-8 off at most; in 32 bits 5e-7 of the share, also where it is tiny.  About 20 operations.
+ * errors), 3e-8 off at most.  In 32 bits 4e-7 of the share near 0; where it is tiny the bell's exponent, rounded twice, is off by up to 1.1 v^2
+ * times 2^-24: 7e-7 of the share at v = -3, 2e-6 at -6, 4e-6 at -9, 7e-6 at -12 (bfloat16 rounds to 4e-3 of a value).
+ * Rounded exactly (six more operations) the bell is 1.2e-7 off everywhere, and 8192 rows of 4096 with bias, gelu and residual 258 us for 253.
+ * About 20 operations.
  */
 __device__ __forceinline__ float normal_share(float v, float &bell)
 {
