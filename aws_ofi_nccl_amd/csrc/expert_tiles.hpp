@@ -383,22 +383,19 @@ template <typename T, uint32_t W, uint32_t THREADS, uint32_t ROWS = kStepRows> s
 /* The columns of `across` that a lane feeds to a matrix instruction: eight of the summed axis, four at a time */
 template <uint32_t W> struct across_frag_t {
 	static constexpr int kReads = 2;
-	uint32_t at[4]; /* of the first four groups of 16 columns; the others are a multiple of 128 bytes or flip bits of these */
-	uint32_t first;
+	uint32_t at[4]; /* of four groups of 16 columns in a row; those of the other part are 256 bytes on */
 	__device__ __forceinline__ across_frag_t(uint32_t first_column, uint32_t lane)
 	{
 		const uint32_t k = (lane >> 4) * 8 + ((lane & 15u) >> 2);
-		first = first_column;
 #pragma unroll
 		for (uint32_t g = 0; g < 4; g++) {
 			at[g] = k * W * 2 + (lane & 1u) * 8 + ((((first_column / 8 + 2 * g) ^ across_slot<W>(k)) + ((lane & 3u) >> 1)) << 4);
 		}
 	}
-	/* column: the first of 16, behind first_column */
+	/* column: the first of 16, behind first_column: of the first four groups, or of those 128 columns on */
 	__device__ __forceinline__ u32x4_t get(uint8_t *lds, uint32_t column, uint32_t half) const
 	{
-		/* groups four on flip the bit above, which first_column (a multiple of 128 where there are more than four) has not set */
-		uint8_t *const p = lds + ((at[column / 16 & 3u] ^ (column & 64u ? 128u : 0u)) + (column & 128u ? 256u : 0u)) + half * 32 * W * 2;
+		uint8_t *const p = lds + at[column / 16 & 3u] + (column & 128u ? 256u : 0u) + half * 32 * W * 2;
 		const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)p);
 		const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(p + 4 * W * 2));
 		const u32x2_t lo = __builtin_bit_cast(u32x2_t, a), hi = __builtin_bit_cast(u32x2_t, b);
@@ -453,6 +450,7 @@ __device__ __forceinline__ void sum_steps(f32x4_t (&sums)[MF][2][G], bool busy, 
 					  Also also)
 {
 	static_assert(DIRECT || STAGES == 2, "what comes through registers has two stages");
+	static_assert(MF <= 4 && G <= 4, "groups of columns that a fragment has places for");
 	u32x4_t r[2][MF], c[2][2 * G];
 	auto read = [&](uint8_t *tile, uint32_t half, u32x4_t(&rows)[MF], u32x4_t(&columns)[2 * G]) __attribute__((always_inline)) {
 #pragma unroll
@@ -549,6 +547,7 @@ template <typename T, uint32_t ROW_FILLS, uint32_t COLUMN_FILLS, uint32_t ROWS_B
 __device__ __forceinline__ void sum_halves(f32x4_t (&sums)[MF][2][G], bool busy, uint32_t steps, uint8_t *lds, const RowFrag &row_frag,
 					   const ColumnFrag &column_frag, FillRows fill_rows, FillColumns fill_columns, Also also)
 {
+	static_assert(MF <= 4 && G <= 4, "groups of columns that a fragment has places for");
 	u32x4_t r[2][MF], c[2][2 * G];
 	auto read = [&](uint8_t *rows, uint8_t *columns, uint32_t half) __attribute__((always_inline)) {
 #pragma unroll
