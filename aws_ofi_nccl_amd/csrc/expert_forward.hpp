@@ -86,8 +86,10 @@ __device__ __forceinline__ void forward_finish(const forward_t &o, forward_tile_
 }
 
 /* Few rows an expert: expert_few.hip.  Few are up to 8, and up to 64 where tiles of 64 x 256 would leave compute units without any.
- * Both sides, us (width 4096 to 2048 in 8 bits, 32 experts): 128 rows 98 in streams and 127 in tiles, 256 rows 115 and 136, 512 183 and
- * 143; one expert of 4096 x 4096 in bfloat16: 1 row 12 and 46, 64 rows 25 and 49. */
+ * Both sides, us (width 4096 to 2048 in 8 bits into bfloat16, 32 experts): 128 rows 98-105 in streams and 127-129 in tiles, 256 rows 115 and 137,
+ * 512 183 and 138-143; into 8 bits, whose blocks of columns are workgroups of 128: 128 rows 115 and 130, 256 rows 161 and 138; one expert of
+ * 4096 x 4096 in bfloat16: 1 row 12 and 46, 64 rows 25 and 49.  What counts is the room for rows: 8 rows with room for 16,384 take 114 where
+ * those with room for 8 take 42. */
 inline bool forward_is_few(uint32_t max_rows, uint32_t n_experts, uint32_t n_tiles)
 {
 	const uint32_t experts = n_experts < max_rows ? n_experts : max_rows, of_expert = (max_rows + experts - 1) / experts;

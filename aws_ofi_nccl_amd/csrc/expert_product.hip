@@ -3,11 +3,11 @@
  *   gated      h = act(x G^T) (x U^T), both projections in one kernel, and what the activation was taken of kept for the way back
  *   product    y = act(x W^T + b) + r
  * x and the weights run along the summed axis.  Rows of e4m3 and their weights have a scale for every 128 of it, which are what one
- * step sums: a step's sums are multiplied by both scales in 32 bits and added.  Their products run as float16, which holds every e4m3 value: the 8-bit
- * matrix instructions keep sums of about 16 bits (1.4e-5 off where float16's are 1e-7), at 705 us for 635 below.
+ * step sums: a step's sums are multiplied by both scales in 32 bits and added.  Their products run as float16, which holds every e4m3 value: both 8-bit
+ * matrix instructions, of 32 and of 128 summed values, keep sums of about 16 bits (normal values: 1.5e-5 off, as float16 1e-8 to 8e-8).
  * Bound by the matrix cores: 32,768 rows of 32 experts, bfloat16, gated 4096 to 2048 with a checkpoint of 8 bits 1080 us (1,018 TFLOP/s), product 2048 to
  * 4096 575 us (956); one expert, 8192 rows, 4096 to 4096 with bias, gelu and residual 267 us (1,030); 16,384 rows in 8 bits, gated 4096 to 2048
- * into 8 bits 635 us (866).  A step of a tile of 256 x 256 is 1.6 us, 1,340 TFLOP/s; besides, a tile costs 11.5 us and an
+ * into 8 bits 612 us (898).  A step of a tile of 256 x 256 is 1.6 us, 1,340 TFLOP/s; besides, a tile costs 11.5 us and an
  * expert's last one may be part of one.
  */
 #include "expert_forward.hpp"

@@ -1054,8 +1054,11 @@ int ofi_amd_token_combine_grad(const void *d_dout, uint64_t dout_pitch, const vo
  *    Experts.  The rows of expert e are [d_offset[e], d_offset[e + 1]), as ofi_amd_token_dispatch leaves
  *    them; no other row is read or written.  d_offset NULL: one expert, which has all max_rows rows (an
  *    ordinary layer's product).  Offsets are taken within [0, max_rows] and have to grow; they stay on
- *    the GPU.  n_experts 1..1024, widths 1..2^20, max_rows < 2^31; -E2BIG beyond, or where a call has
- *    2^31 tiles of 64 rows and 128 columns or more.
+ *    the GPU.  n_experts 1..1024, widths 1..2^20, max_rows < 2^31; -E2BIG beyond, or where a call would
+ *    have 2^31 workgroups or more: tiles of 64 to 256 rows and 128 or 256 columns.
+ *    How many rows there are the host does not know, so a call is laid out for max_rows: room for many
+ *    more rows than there are costs time (8 rows of 32 experts through a gated block of 4096 to 2048
+ *    in 8 bits: 42 us, with room for 512 rows 50, for 16,384 114).  Give what a step can have at most.
  *    Weights are matrices of one row for each output, weight_pitch bytes from row to row and expert_pitch
  *    from expert to expert.
  *    Types are float16 or bfloat16 for rows and weights alike.  The forward products also take OCP e4m3
